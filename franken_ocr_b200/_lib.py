@@ -19,6 +19,7 @@ FOCR_E_ALLOC = -4
 FOCR_E_ROUTE = -5
 FOCR_E_TIMEOUT = -6
 FOCR_E_UNSUPPORTED = -7
+F32, F16, BF16 = 0, 1, 2
 MEM_HOST = 0
 MEM_DEVICE = 1
 
@@ -40,6 +41,8 @@ EXPORTS = [
     "focr_ep_experts", "focr_ep_combine", "focr_ep_decode", "focr_ep_status",
     "focr_decoder_create", "focr_decoder_destroy", "focr_decoder_prefill", "focr_decoder_generate",
     "focr_rms_norm_linear_i8", "focr_rope_ring_at",
+    "focr_paged_write", "focr_paged_attention_workspace", "focr_paged_attention",
+    "focr_paged_evict", "focr_beam_select_workspace", "focr_beam_select", "focr_beam_reorder",
 ]
 
 
@@ -99,6 +102,12 @@ class DecoderLayerWeights(C.Structure):
 class DecoderWeights(C.Structure):
     _fields_ = [("layers", C.POINTER(DecoderLayerWeights))] + [
         (n, vp) for n in ("final_norm", "lm_w", "lm_s", "embed")]
+
+
+class PagedCache(C.Structure):
+    _fields_ = [("k", vp), ("v", vp), ("table", vp), ("page_stride", sz), ("head_stride", sz),
+                ("table_stride", sz)] + [(n, C.c_uint32) for n in (
+                    "n_pages", "kv_heads", "page_size", "head_dim", "max_pages")] + [("dtype", i32)]
 
 
 lib.focr_last_error.restype = C.c_char_p
@@ -163,6 +172,15 @@ lib.focr_rope_apply_at.argtypes = [vp, sz, sz, vp, vp, vp, vp]
 lib.focr_ring_write.argtypes = [vp, vp, sz, sz, vp, vp, sz, vp, vp]
 lib.focr_add_rms_norm.argtypes = [vp, vp, sz, sz, vp, C.c_float, vp, vp, vp]
 lib.focr_attention_decode_at.argtypes = [vp, vp, vp, sz, sz, vp, vp, sz, sz, sz, vp, vp, vp]
+lib.focr_paged_write.argtypes = [vp, sz, vp, vp, i32, sz, sz, sz, vp, vp, vp]
+lib.focr_paged_attention_workspace.argtypes = [sz, sz, sz, sz, vp]
+lib.focr_paged_attention.argtypes = [vp, vp, i32, sz, sz, sz, vp, vp, sz, C.c_float, vp, sz, vp, sz,
+                                     sz, sz, vp, sz, vp]
+lib.focr_paged_evict.argtypes = [vp, sz, vp, vp, sz, sz, sz, vp, sz, sz, sz, sz, sz, vp, vp, vp, vp]
+lib.focr_beam_select_workspace.argtypes = [sz, sz, sz, sz, vp]
+lib.focr_beam_select.argtypes = [vp, i32, sz, sz, sz, sz, vp, vp, C.c_int32, sz, vp, vp, vp, vp, sz,
+                                 vp]
+lib.focr_beam_reorder.argtypes = [vp, sz, sz, sz, sz, vp, vp, vp, vp, vp, vp, sz, sz, sz, sz, vp, vp]
 STATE_POS, STATE_RING_LEN, STATE_RING_POS, STATE_SLOT, STATE_NEXT_POS, STATE_STEP = range(6)
 STATE_ERROR, STATE_WORDS = 6, 8
 

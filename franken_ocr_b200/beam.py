@@ -1,0 +1,110 @@
+"""Beam search beside the greedy ``argmax_row`` (sampler.rs:168-186):
+
+* ``beam_select`` -- the best continuations over beams and vocabulary, from the
+  lm-head's logits;
+* ``beam_reorder`` -- every beam gets its parent's paged cache.
+
+CUDA tensors on one device, torch's current stream; both can be captured.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from ._lib import check, lib
+from .paged import _On, _cache, _dtype, _need
+
+
+def beam_select(logits, scores, n: int | None = None, *, done=None, end_token: int = 1):
+    """From ``logits`` ``[batch, beams, vocab]`` (f32, f16 or bf16) and the beams'
+    cumulated log probabilities ``scores`` ``[batch, beams]`` f32: the ``n`` (by
+    default ``beams``) best continuations of every entry as ``(scores, parent,
+    token)``, each ``[batch, n]``, best first.
+
+    A candidate's score is ``scores[b, i] + log_softmax(logits[b, i])[t]``, held
+    in 64 bits for the ranking; equal ones go to the lower beam, then the larger
+    logit, then the lower token.  A beam with ``done[b, i]`` offers ``end_token``
+    alone with its score unchanged; -inf and NaN logits and beams with a score
+    that is not finite offer nothing.  Missing candidates: -inf, -1, -1."""
+    ctx = "beam_select"
+    if logits.dim() != 3:
+        raise ValueError(f"{ctx}: logits must be [batch, beams, vocab], not {tuple(logits.shape)}")
+    device = logits.device
+    if device.type != "cuda":
+        raise ValueError(f"{ctx}: logits must be a CUDA tensor, not on {device}")
+    code = _dtype(ctx, "logits", logits)
+    batch, beams, vocab = logits.shape
+    if logits.stride(2) != 1 or (batch > 1 and beams > 1 and logits.stride(0) != beams * logits.stride(1)):
+        raise ValueError(f"{ctx}: the rows of logits must be contiguous and evenly spaced")
+    _need(ctx, "scores", scores, torch.float32, (batch, beams), device)
+    if done is not None:
+        if done.dtype == torch.bool:
+            done = done.view(torch.uint8)
+        _need(ctx, "done", done, torch.uint8, (batch, beams), device)
+    if n is None:
+        n = beams
+    if n < 1:
+        raise ValueError(f"{ctx}: n must be positive")
+    out = torch.empty((batch, n), dtype=torch.float32, device=device)
+    parent = torch.empty((batch, n), dtype=torch.int32, device=device)
+    token = torch.empty((batch, n), dtype=torch.int32, device=device)
+    need = C.c_size_t()
+    check(lib.focr_beam_select_workspace(batch, beams, vocab, n, C.byref(need)))
+    with _On(device) as stream:
+        ws = torch.empty(need.value, dtype=torch.uint8, device=device)
+        check(lib.focr_beam_select(
+            logits.data_ptr(), code, batch, beams, vocab,
+            logits.stride(1) if beams > 1 else max(logits.stride(0), vocab), scores.data_ptr(),
+            None if done is None else done.data_ptr(), end_token, n, out.data_ptr(), parent.data_ptr(),
+            token.data_ptr(), ws.data_ptr(), need.value, stream))
+    return out, parent, token
+
+
+def beam_reorder(k_pages, v_pages, table, lens, parent, fresh, *, weights=None):
+    """Row ``i`` of entry ``b = i // beams`` becomes row ``b * beams + parent[b,
+    i % beams]`` of ``table`` ``[batch * beams, max_pages]``: full pages are
+    shared, the partly filled one is copied to page ``fresh[i]`` (which takes its
+    place also where it is still empty), in every layer of ``k_pages`` /
+    ``v_pages`` ``[layers, pages, kv_heads, page_size, head_dim]`` (or one layer,
+    without the first dimension).  ``weights`` ``[layers, rows, kv_heads, width]``
+    f32 (without the first dimension for one layer) follow.
+
+    Returns ``(table, lens, weights or None)``, new tensors.  A parent outside
+    ``[0, beams)`` leaves an empty row.  The fresh pages must differ from one
+    another and from every page the table uses."""
+    ctx = "beam_reorder"
+    layered = k_pages.dim() == 5
+    cache, device = _cache(ctx, k_pages, v_pages, table, 5 if layered else 4)
+    layers = k_pages.shape[0] if layered else 1
+    if parent.dim() != 2:
+        raise ValueError(f"{ctx}: parent must be [batch, beams], not {tuple(parent.shape)}")
+    batch, beams = parent.shape
+    rows, width = table.shape
+    if batch * beams != rows:
+        raise ValueError(f"{ctx}: table has {rows} rows for {batch} x {beams} beams")
+    _need(ctx, "parent", parent, torch.int32, (batch, beams), device)
+    _need(ctx, "lens", lens, torch.int32, (rows,), device)
+    _need(ctx, "fresh", fresh, torch.int32, (rows,), device)
+    w_out, span, w_layer, w_row, w_head = None, 0, 0, 0, 0
+    if weights is not None:
+        lead = (layers, rows, cache.kv_heads) if layered else (rows, cache.kv_heads)
+        if weights.dtype != torch.float32:
+            raise TypeError(f"{ctx}: weights must be torch.float32, not {weights.dtype}")
+        if weights.shape[:-1] != lead or weights.device != device:
+            raise ValueError(f"{ctx}: weights must be {list(lead)} + [width] on {device}, "
+                             f"not {tuple(weights.shape)} on {weights.device}")
+        if weights.stride(-1) != 1:
+            raise ValueError(f"{ctx}: the last dimension of weights must be contiguous")
+        span, w_row, w_head = weights.shape[-1], weights.stride(-3), weights.stride(-2)
+        w_layer = weights.stride(0) if layered else 0
+        w_out = torch.empty(weights.shape, dtype=torch.float32, device=device)
+    new_table = torch.empty((rows, width), dtype=torch.int32, device=device)
+    new_lens = torch.empty((rows,), dtype=torch.int32, device=device)
+    with _On(device) as stream:
+        check(lib.focr_beam_reorder(
+            C.byref(cache), layers, k_pages.stride(0) if layered else 0, batch, beams, lens.data_ptr(),
+            parent.data_ptr(), fresh.data_ptr(), new_table.data_ptr(), new_lens.data_ptr(),
+            None if weights is None else weights.data_ptr(), span, w_layer, w_row, w_head,
+            None if w_out is None else w_out.data_ptr(), stream))
+    return new_table, new_lens, w_out

@@ -493,6 +493,126 @@ int focr_decoder_prefill(focr_decoder *d, const float *embeds, size_t seq, float
 int focr_decoder_generate(focr_decoder *d, const float *embeds, size_t seq, size_t n_tokens,
                           int32_t *tokens, int mem, void *stream);
 
+/* ---- paged K/V cache and beams ------------------------------------------
+ * No counterpart in the reference, which decodes greedily over one dense cache
+ * per stream (BatchedRingCache, native_engine/rswa.rs:620-700): here many
+ * streams, and the beams of one stream, share one pool of pages.  Device
+ * pointers on the current device; every call only enqueues work on `stream`
+ * and can be captured.  Workspaces are the caller's, of the size the matching
+ * *_workspace call gives, 16-byte aligned; they need no initialisation and
+ * hold nothing between calls, and two calls that may run at the same time
+ * need two of them (two captured graphs too). */
+#define FOCR_F32 0
+#define FOCR_F16 1
+#define FOCR_BF16 2
+
+/* One layer's cache.  Position p of a row lies in page table[row][p /
+ * page_size], slot p % page_size; head h of page i at
+ * base + i * page_stride + h * head_stride, [page_size][head_dim] contiguous
+ * there; strides in elements, the same for k and v.  Page ids outside
+ * [0, n_pages) name no page: entries that no position below the row's length
+ * uses are never read.  head_dim * element size and both strides are
+ * multiples of 16 bytes, k and v 16-byte aligned, head_dim <= 256, and
+ * max_pages * page_size < 2^31. */
+typedef struct focr_paged_cache {
+    void *k, *v;
+    const int32_t *table; /* [rows][table_stride], max_pages entries used */
+    size_t page_stride, head_stride, table_stride;
+    uint32_t n_pages, kv_heads, page_size, head_dim, max_pages;
+    int32_t dtype; /* FOCR_F32, FOCR_F16 or FOCR_BF16 */
+} focr_paged_cache;
+
+/* Write `tokens` keys and values [tokens][kv_heads][head_dim] of `src_dtype`
+ * (tokens k_stride / v_stride elements apart) into the cache: token t goes to
+ * position pos[t] of table row row[t] (row NULL: t), rounded once to the
+ * cache's type.  row[t] < 0 is padding.  Padding, rows and positions outside
+ * the table, and pages outside the pool are skipped; nothing else is touched.
+ * Two tokens of a call must not name the same place.  The paged form of
+ * RingCache::record_prefill / write_decode_step (rswa.rs:389, :451-500). */
+int focr_paged_write(const focr_paged_cache *c, size_t rows, const void *k, const void *v,
+                     int src_dtype, size_t tokens, size_t k_stride, size_t v_stride,
+                     const int32_t *row, const int32_t *pos, void *stream);
+
+/* Attention of one new token per row: q, out [rows][q_heads][head_dim] of
+ * `q_dtype` (rows q_stride / out_stride elements apart); query head h reads
+ * kv head h / (q_heads / kv_heads).  Row r sees the positions j < lens[r]
+ * of its pages; with window > 0 only j < ref_lens[r] (NULL: 0) and
+ * j >= lens[r] - window, which is the R-SWA rule of decode_attention
+ * (rswa.rs:855-944).  out = softmax(scale * q.k) . v, all sums in f32, rounded
+ * once.  A row that sees nothing gives zeros; a row whose length passes
+ * max_pages * page_size (or weights_width), or one of whose pages is not in
+ * the pool, gives NaN.  K and V behind a row's length are never read.
+ *
+ * weights (may be NULL) [rows][kv_heads][weights_width] f32, strides in
+ * elements: weights[r][h][j] += the probabilities of position j over the query
+ * heads of h; entries of hidden positions, and of rows that give NaN, stay as
+ * they were.  Two rows of a call must not share weights.
+ * weights_width 0 for the workspace without weights. */
+int focr_paged_attention_workspace(size_t rows, size_t q_heads, size_t head_dim,
+                                   size_t weights_width, size_t *bytes);
+int focr_paged_attention(const focr_paged_cache *c, const void *q, int q_dtype, size_t rows,
+                         size_t q_heads, size_t q_stride, const int32_t *lens,
+                         const int32_t *ref_lens, size_t window, float scale, void *out,
+                         size_t out_stride, float *weights, size_t weights_width,
+                         size_t weights_row_stride, size_t weights_head_stride, void *workspace,
+                         size_t workspace_bytes, void *stream);
+
+/* Shrink rows to `budget` entries by accumulated attention weight.  A row of
+ * n <= budget entries keeps all; a longer one keeps its first `sink`, its last
+ * `recent` and, of the entries between, the budget - sink - recent with the
+ * largest weights[row][head][position] (equal weights: the lower position;
+ * NaN below every number).  Every kv head chooses for itself.  The kept
+ * entries move, in order, to positions 0.. of the row's new page list
+ * new_table [rows][new_table_stride] (new_pages entries used, new_pages *
+ * page_size >= budget): kept [rows][kv_heads][budget] gets their old
+ * positions (-1 behind the last), lens_out [rows] the new lengths, weights_out
+ * [rows][kv_heads][width] their weights with 0 behind them.
+ * The new pages must not be among the pages that any row of the call reads;
+ * the old pages are left as they were.  A length below 0, or past `width` or
+ * the table, counts as 0; entries on pages outside the pool are not copied. */
+int focr_paged_evict(const focr_paged_cache *c, size_t rows, const int32_t *lens,
+                     const float *weights, size_t width, size_t weights_row_stride,
+                     size_t weights_head_stride, const int32_t *new_table,
+                     size_t new_table_stride, size_t new_pages, size_t budget, size_t sink,
+                     size_t recent, int32_t *kept, int32_t *lens_out, float *weights_out,
+                     void *stream);
+
+/* Beam search's choice: from logits [batch][beams][vocab] (rows row_stride
+ * elements apart) and the beams' cumulated log probabilities scores
+ * [batch][beams], the n best continuations of every entry, ranked by
+ *   scores[b][i] + log softmax(logits[b][i])[t]
+ * in 64 bits; equal scores go to the lower beam, then the larger logit, then
+ * the lower token.  scores_out (rounded to f32), parent_out (the beam) and
+ * token_out are [batch][n].  NaN and -inf logits are no candidates and add
+ * nothing to a sum; +inf counts as the largest finite f32.  A beam with
+ * done[b][i] != 0 (done may be NULL) offers end_token alone, with its score as
+ * it is; a beam whose score is not finite offers nothing.  Where fewer than n
+ * candidates exist: score -inf, parent and token -1.  beams, n <= 64.
+ * Beside argmax_row (sampler.rs:168-186), which it equals for one beam, n = 1. */
+int focr_beam_select_workspace(size_t batch, size_t beams, size_t vocab, size_t n, size_t *bytes);
+int focr_beam_select(const void *logits, int dtype, size_t batch, size_t beams, size_t vocab,
+                     size_t row_stride, const float *scores, const uint8_t *done, int32_t end_token,
+                     size_t n, float *scores_out, int32_t *parent_out, int32_t *token_out,
+                     void *workspace, size_t workspace_bytes, void *stream);
+
+/* Give every beam its parent's cache: row i of entry b = i / beams becomes row
+ * b * beams + parent[i] of the table, in all `layers` (layer l's pages
+ * layer_stride elements behind layer l - 1's; one table for all).  Full pages
+ * are shared through table_out [rows][max_pages]; the parent's partly filled
+ * page is copied to page fresh[i], which also takes that place in table_out
+ * where nothing is copied, so every beam can go on writing.  lens_out [rows].
+ * Entries behind that page become -1.  weights [layers][rows][kv_heads][width]
+ * (may be NULL) follow into weights_out, contiguous, with 0 from the new
+ * length on.  A parent outside [0, beams) leaves an empty row.  The fresh pages
+ * must differ from one another and from every page the table uses.  The paged
+ * form of compacting BatchedRingCache slots (rswa.rs:620-700). */
+int focr_beam_reorder(const focr_paged_cache *c, size_t layers, size_t layer_stride,
+                      size_t batch, size_t beams, const int32_t *lens, const int32_t *parent,
+                      const int32_t *fresh, int32_t *table_out, int32_t *lens_out,
+                      const float *weights, size_t width, size_t weights_layer_stride,
+                      size_t weights_row_stride, size_t weights_head_stride, float *weights_out,
+                      void *stream);
+
 /* ---- device event trace (GPU counterpart of FOCR_PROFILE_DECODE,
  * native_engine/decoder.rs:986-1024) ------------------------------------
  * Register a device buffer of `capacity` 16-byte events {u32 tag, u32 phase,

@@ -1,0 +1,287 @@
+"""Beam selection and reordering on the GPU against their definitions in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from tests.paged_cases import DTYPES, Cache, select
+from tests.test_gpu_paged import same_bits, stale_memory  # noqa: F401
+
+pytestmark = [pytest.mark.gpu, pytest.mark.usefixtures("stale_memory")]
+
+
+def check_select(logits, scores, n, done=None, end=1, dev=None):
+    from franken_ocr_b200 import beam
+
+    x = logits.cuda() if dev is None else dev
+    got = beam.beam_select(x, scores.cuda(), n, done=None if done is None else done.cuda(), end_token=end)
+    score, parent, token = (t.cpu() for t in got)
+    for b, want in enumerate(select(logits, scores, n, done, end)):
+        for k in range(n):
+            if k >= len(want):
+                assert (float(score[b, k]), int(parent[b, k]), int(token[b, k])) == (-math.inf, -1, -1)
+                continue
+            s, i, t = want[k]
+            assert (int(parent[b, k]), int(token[b, k])) == (i, t), (b, k)
+            # one rounding to f32; the 64-bit sum's own error lies far below it
+            assert abs(float(score[b, k]) - s) <= 2.0 ** -24 * abs(s) * 1.001 + 1e-12 or math.isinf(float(score[b, k]))
+    return got
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("batch,beams,vocab,n", [(1, 1, 1, 1), (1, 1, 129280, 1), (2, 4, 1000, 4), (3, 5, 8193, 10),
+                                                 (1, 16, 32, 32), (2, 3, 5, 20), (1, 64, 700, 64), (5, 2, 50001, 3)])
+def test_select_matches_the_definition(cuda, dtype, batch, beams, vocab, n):
+    g = torch.Generator().manual_seed(vocab + n)
+    x = (torch.randn((batch, beams, vocab), generator=g) * 3).to(DTYPES[dtype])
+    check_select(x, torch.randn((batch, beams), generator=g) * 2 - 10, n)
+
+
+def test_select_equals_argmax_for_one_beam(cuda):
+    from franken_ocr_b200 import beam
+
+    x = torch.randn((6, 1, 4000), generator=torch.Generator().manual_seed(1)).half().cuda()
+    _, parent, token = beam.beam_select(x, torch.zeros((6, 1), device="cuda"))
+    assert token[:, 0].tolist() == x.float().cpu().argmax(-1)[:, 0].tolist() and bool((parent == 0).all())
+
+
+def test_select_ties_masks_and_values_that_are_no_numbers(cuda):
+    g = torch.Generator().manual_seed(3)
+    low = float(torch.finfo(torch.float32).min)
+    x = torch.randn((8, 4, 9000), generator=g)
+    x[0] = 0.0                                      # everything equal
+    x[1] = x[1].round()                             # many ties
+    x[2, :, :] = -math.inf                          # rows with nothing left
+    x[2, 1, 8999] = 1.0
+    x[3, 0] = low                                   # masked by the type's lowest value
+    x[3, 1, 1:] = low
+    x[4, :2] = math.nan
+    x[4, 2, ::3] = math.nan
+    x[5, 0, 17] = x[5, 0, 8500] = math.inf
+    x[6] = x[6, :1].expand(4, -1)                   # equal beams
+    x[7, 3, :] = 80.0 * (x[7, 3] > 3)               # a steep row
+    scores = torch.randn((8, 4), generator=g) - 5
+    scores[1] = scores[1, 0]
+    scores[6] = -1.5
+    scores[7, 1:3] = torch.tensor([-math.inf, math.nan])
+    scores[3, 2] = -1e9                             # a beam as good as dead
+    for n in (4, 8, 64):
+        check_select(x, scores, n)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_select_lowest_value_of_small_types(cuda, dtype):
+    t = DTYPES[dtype]
+    x = torch.full((2, 3, 500), torch.finfo(t).min, dtype=t)
+    x[0, 1, 77] = 2.0
+    x[1, 2, 5] = torch.finfo(t).max
+    check_select(x, torch.zeros((2, 3)) - 1, 6)
+
+
+def test_select_close_scores_of_different_beams(cuda):
+    """Scores that differ by less than f32 resolves are still ranked rightly."""
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn((1, 2, 30000), generator=g) * 2
+    p = torch.log_softmax(x.double(), -1).amax(-1)[0]
+    scores = torch.tensor([[-40.0, 0.0]])
+    for step in (-1, 1):
+        scores[0, 1] = torch.nextafter((scores[0, 0].double() + p[0] - p[1]).float(), torch.tensor(step * 1e9))
+        check_select(x, scores, 4)
+
+
+@pytest.mark.parametrize("kind", ["bool", "uint8"])
+def test_select_ended_beams(cuda, kind):
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn((4, 3, 600), generator=g)
+    done = torch.tensor([[0, 1, 0], [1, 1, 1], [0, 0, 0], [1, 0, 1]]).to(getattr(torch, kind))
+    x[3, 0] = math.nan                               # an ended beam's logits do not matter
+    scores = torch.randn((4, 3), generator=g) - 3
+    scores[0, 1] = 0.0
+    for n in (1, 3, 7):
+        check_select(x, scores, n, done, end=37)
+
+
+def test_select_strided_and_unaligned_rows(cuda):
+    g = torch.Generator().manual_seed(6)
+    for dtype in DTYPES.values():
+        wide = torch.randn((2, 3, 5011), generator=g).to(dtype)
+        dev = wide.cuda()
+        check_select(wide[:, :, 5:5008], torch.zeros((2, 3)), 5, dev=dev[:, :, 5:5008])
+        one = torch.randn((4, 1, 333), generator=g).to(dtype)
+        check_select(one, torch.zeros((4, 1)), 2)
+        # one beam an entry, entries apart
+        apart = torch.randn((4, 3, 333), generator=g).to(dtype)
+        check_select(apart[:, 1:2], torch.zeros((4, 1)), 2, dev=apart.cuda()[:, 1:2])
+
+
+def test_select_in_a_graph_and_twice_the_same(cuda):
+    from franken_ocr_b200 import beam
+
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn((3, 4, 20000), generator=g).cuda()
+    s = torch.randn((3, 4), generator=g).cuda()
+    want = beam.beam_select(x, s, 8)
+    graph = torch.cuda.CUDAGraph()
+    held = x.clone()
+    with torch.cuda.graph(graph):
+        got = beam.beam_select(held, s, 8)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(same_bits(a, b) for a, b in zip(got, want))
+    held.mul_(-1)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(same_bits(a, b) for a, b in zip(got, beam.beam_select(held, s, 8)))
+
+
+# ---- reordering -----------------------------------------------------------------
+
+def reorder_case(layers, batch, beams, lens, heads, page, dim, dtype, seed, width=None):
+    rows = batch * beams
+    c = Cache([lens[i // beams] for i in range(rows)], heads, page, dim, dtype, seed=seed, spare=rows,
+              capacity=max(lens) + 2 * page)
+    g = torch.Generator().manual_seed(seed + 1)
+    k = torch.stack([c.k] + [torch.randn(c.k.shape, generator=g).to(dtype) for _ in range(layers - 1)])
+    v = torch.stack([c.v] + [torch.randn(c.k.shape, generator=g).to(dtype) for _ in range(layers - 1)])
+    parent = torch.randint(0, beams, (batch, beams), generator=g, dtype=torch.int32)
+    w = None if width is None else torch.rand((layers, rows, heads, width), generator=g)
+    return c, k, v, parent, w
+
+
+def check_reorder(c, k, v, parent, w, flat=False):
+    from franken_ocr_b200 import beam
+
+    batch, beams = parent.shape
+    fresh = torch.tensor(c.spare, dtype=torch.int32)
+    kd, vd = k.cuda(), v.cuda()
+    wd = None if w is None else w.cuda()
+    args = (kd[0], vd[0]) if flat else (kd, vd)
+    table, lens, wo = beam.beam_reorder(*args, c.table.cuda(), c.lens.cuda(), parent.cuda(), fresh.cuda(),
+                                        weights=None if wd is None else wd[0] if flat else wd)
+    want = torch.full_like(c.table, -1)
+    k, v = k.clone(), v.clone()
+    ww = None if w is None else torch.zeros_like(w)
+    new = []
+    for i in range(batch * beams):
+        p = int(parent[i // beams, i % beams])
+        src = i // beams * beams + p
+        n = int(c.lens[src]) if 0 <= p < beams else 0
+        full, rest = divmod(n, c.page)
+        new.append(n)
+        if n:
+            want[i, :full] = c.table[src, :full]
+        want[i, full] = fresh[i]
+        if rest:
+            at = int(c.table[src, full])
+            k[:, int(fresh[i]), :, :rest] = k[:, at, :, :rest]
+            v[:, int(fresh[i]), :, :rest] = v[:, at, :, :rest]
+        if w is not None and n:
+            ww[:, i, :, :n] = w[:, src, :, :n]
+    assert torch.equal(table.cpu(), want) and lens.tolist() == new
+    assert same_bits(kd, k) and same_bits(vd, v)
+    if w is not None:
+        assert same_bits(wo, ww[0] if flat else ww)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("layers,batch,beams,lens,heads,page,dim,width", [
+    (12, 1, 4, [37], 10, 16, 128, None), (1, 3, 2, [16, 0, 31], 2, 16, 64, 40), (2, 2, 5, [1, 50], 3, 7, 80, 55),
+    (3, 1, 1, [9], 1, 1, 64, 9), (2, 2, 8, [63, 64], 1, 64, 256, None)])
+def test_reorder_matches_the_definition(cuda, dtype, layers, batch, beams, lens, heads, page, dim, width):
+    check_reorder(*reorder_case(layers, batch, beams, lens, heads, page, dim, DTYPES[dtype], seed=dim, width=width))
+
+
+def test_reorder_one_layer_without_its_dimension_and_parents_out_of_range(cuda):
+    case = reorder_case(1, 3, 4, [20, 33, 5], 2, 16, 64, torch.float32, seed=3, width=64)
+    check_reorder(*case, flat=True)
+    case[3][0] = torch.tensor([-1, 4, 100, 2])
+    check_reorder(*case)
+
+
+def test_reorder_skips_pages_outside_the_pool(cuda):
+    from franken_ocr_b200 import beam
+
+    c, k, v, parent, _ = reorder_case(2, 1, 3, [20], 2, 16, 64, torch.float32, seed=4)
+    kd, vd = k.cuda(), v.cuda()
+    fresh = torch.tensor([c.k.shape[0], -1, c.spare[0]], dtype=torch.int32, device="cuda")
+    table = c.table.cuda()
+    table[int(parent[0, 2]), 1] = -9
+    beam.beam_reorder(kd, vd, table, c.lens.cuda(), parent.cuda(), fresh)
+    assert same_bits(kd, k) and same_bits(vd, v)
+
+
+# ---- together -------------------------------------------------------------------------
+
+def test_beams_over_a_paged_cache_as_they_are_used(cuda):
+    """Prompt, then steps of select, reorder, write and attend, and an eviction on
+    the way: the cache and the outputs follow a dense 64-bit copy per beam."""
+    from franken_ocr_b200 import beam, paged
+
+    g = torch.Generator().manual_seed(11)
+    batch, beams, heads, group, dim, page, vocab = 2, 3, 2, 2, 64, 8, 300
+    rows, prompt, steps, budget = batch * beams, [21, 9], 14, 16
+    width = 8
+    pages = batch * width + rows * 2 * (steps + 2) + rows * 4
+    pool_k = torch.full((pages, heads, page, dim), math.nan, device="cuda")
+    pool_v = pool_k.clone()
+    free = torch.randperm(pages, generator=g).tolist()
+    # every beam of an entry starts on the same prompt pages
+    table = torch.full((rows, width), -1, dtype=torch.int32)
+    lens = torch.tensor([prompt[i // beams] for i in range(rows)], dtype=torch.int32)
+    dense = [None] * rows
+    for b in range(batch):
+        own = [free.pop() for _ in range(-(-prompt[b] // page))]
+        k = torch.randn((prompt[b], heads, dim), generator=g)
+        v = torch.randn((prompt[b], heads, dim), generator=g)
+        for i in range(b * beams, (b + 1) * beams):
+            table[i, :len(own)] = torch.tensor(own, dtype=torch.int32)
+            dense[i] = (k.clone(), v.clone(), torch.zeros((heads, prompt[b]), dtype=torch.float64))
+        first = torch.full((prompt[b],), b * beams, dtype=torch.int32).cuda()
+        paged.paged_write(k.cuda(), v.cuda(), pool_k, pool_v, table.cuda(),
+                          torch.arange(prompt[b], dtype=torch.int32).cuda(), row=first)
+    table, lens = table.cuda(), lens.cuda()
+    w = torch.zeros((rows, heads, width * page), device="cuda")
+    scores = torch.full((batch, beams), -math.inf, device="cuda")
+    scores[:, 0] = 0.0
+    for step in range(steps):
+        logits = torch.randn((batch, beams, vocab), generator=g) * 2
+        old = scores.cpu()
+        scores, parent, token = beam.beam_select(logits.cuda(), scores)
+        for b, want in enumerate(select(logits, old, beams)):
+            assert [(i, t) for _, i, t in want] == list(zip(parent[b].tolist(), token[b].tolist()))
+        fresh = torch.tensor([free.pop() for _ in range(rows)], dtype=torch.int32).cuda()
+        table, lens, w = beam.beam_reorder(pool_k, pool_v, table, lens, parent, fresh, weights=w)
+        source = [i // beams * beams + p for i, p in enumerate(parent.view(-1).tolist())]
+        dense = [tuple(x.clone() for x in dense[s]) for s in source]
+        k, v = torch.randn((rows, heads, dim), generator=g), torch.randn((rows, heads, dim), generator=g)
+        paged.paged_write(k.cuda(), v.cuda(), pool_k, pool_v, table, lens)
+        lens += 1
+        q = torch.randn((rows, heads * group, dim), generator=g)
+        out = paged.paged_attention(q.cuda(), pool_k, pool_v, table, lens, weights=w).cpu().double()
+        for i in range(rows):
+            dk, dv = torch.cat([dense[i][0], k[i:i + 1]]), torch.cat([dense[i][1], v[i:i + 1]])
+            dw = torch.cat([dense[i][2], torch.zeros((heads, 1), dtype=torch.float64)], 1)
+            for h in range(heads):
+                p = torch.softmax(q[i, h * group:(h + 1) * group].double() @ dk[:, h].double().T / 8, -1)
+                # ~40 entries, scores below 2^5: a few hundred units of 2^-24 of values below 2^2
+                assert torch.allclose(out[i, h * group:(h + 1) * group], p @ dv[:, h].double(), rtol=0, atol=1e-4)
+                dw[h] += p.sum(0)
+            dense[i] = (dk, dv, dw)
+        if step == 6:
+            n = lens.tolist()
+            into = torch.tensor([free.pop() for _ in range(rows * (budget // page))], dtype=torch.int32)
+            small = torch.full((rows, width), -1, dtype=torch.int32)
+            small[:, :budget // page] = into.view(rows, -1)
+            small = small.cuda()
+            kept, lens, w = paged.paged_evict(pool_k, pool_v, table, lens, w, small, budget, sink=1, recent=4)
+            table = small
+            for i in range(rows):
+                pick = kept[i].cpu().long()
+                live = min(n[i], budget)
+                pick = pick[:, :live]
+                dk = torch.stack([dense[i][0][pick[h], h] for h in range(heads)], 1)
+                dv = torch.stack([dense[i][1][pick[h], h] for h in range(heads)], 1)
+                dense[i] = (dk, dv, dense[i][2].gather(1, pick))
+                assert pick[:, 0].tolist() == [0] * heads and pick[:, -1].tolist() == [n[i] - 1] * heads
+    assert torch.allclose(w[0, :, :int(lens[0])].cpu().double(), dense[0][2], rtol=0, atol=1e-4)

@@ -1,0 +1,410 @@
+"""The paged K/V cache on the GPU against plain 64-bit forms: writes into pages,
+attention of one token over them, and eviction by accumulated weight."""
+import math
+
+import pytest
+import torch
+
+from tests.paged_cases import DTYPES, HALF_STEP, Cache, attention, evict_kept, visible
+
+pytestmark = [pytest.mark.gpu, pytest.mark.usefixtures("stale_memory")]
+
+
+@pytest.fixture
+def stale_memory(cuda):
+    """Workspaces and outputs come from memory that holds NaN (and indexes far
+    out of range): nothing may go by what a buffer held before."""
+    held = [torch.full((n,), math.nan, device="cuda") for n in (1 << 7, 1 << 12, 1 << 17, 1 << 22, 1 << 24)]
+    del held
+
+
+def same_bits(a, b):
+    kind = {4: torch.int32, 2: torch.int16}[a.element_size()]
+    return torch.equal(a.contiguous().cpu().view(kind), b.contiguous().cpu().view(kind))
+
+
+# ---- write -----------------------------------------------------------------
+
+@pytest.mark.parametrize("src", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("pool", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,page,dim,strided", [(10, 16, 128, False), (1, 1, 64, False), (3, 7, 80, True),
+                                                    (2, 24, 256, True)])
+def test_write_rounds_once_and_touches_nothing_else(cuda, src, pool, heads, page, dim, strided):
+    from franken_ocr_b200 import paged
+
+    lens = [5, 0, 3 * page + 2, 1]
+    c = Cache([3 * page + 2] * 4, heads, page, dim, DTYPES[pool], seed=dim, strided=strided)
+    kp, vp, table = c.cuda()
+    row = torch.tensor([r for r, n in enumerate(lens) for _ in range(n)] + [-1, -1], dtype=torch.int32)
+    pos = torch.tensor([p for n in lens for p in range(n)] + [0, 1], dtype=torch.int32)
+    mix = torch.randperm(len(row), generator=torch.Generator().manual_seed(1))
+    row, pos = row[mix], pos[mix]
+    g = torch.Generator().manual_seed(2)
+    k = torch.randn((len(row), heads, dim), generator=g).to(DTYPES[src])
+    v = torch.randn((len(row), heads, dim), generator=g).to(DTYPES[src])
+    paged.paged_write(k.cuda(), v.cuda(), kp, vp, table, pos.cuda(), row=row.cuda())
+    for t in range(len(row)):
+        r, p = int(row[t]), int(pos[t])
+        if r >= 0:
+            at = int(c.table[r, p // page])
+            c.k[at, :, p % page] = k[t].to(c.dtype)
+            c.v[at, :, p % page] = v[t].to(c.dtype)
+    assert same_bits(kp, c.k) and same_bits(vp, c.v)
+
+
+def test_write_from_a_fused_projection_and_unaligned_rows(cuda):
+    """k and v as slices of one [tokens, q|k|v] buffer, on and off 16-byte boundaries."""
+    from franken_ocr_b200 import paged
+
+    heads, dim, page = 3, 64, 16
+    for shift in (0, 1):
+        c = Cache([20] * 5, heads, page, dim, torch.bfloat16, seed=3)
+        kp, vp, table = c.cuda()
+        qkv = torch.randn((5, 3 * heads * dim + shift), generator=torch.Generator().manual_seed(4))
+        dev = qkv.cuda()
+        part = [dev[:, shift + i * heads * dim:shift + (i + 1) * heads * dim].view(5, heads, dim) for i in (1, 2)]
+        pos = torch.tensor([0, 15, 16, 19, 7], dtype=torch.int32)
+        paged.paged_write(part[0], part[1], kp, vp, table, pos.cuda())
+        for r in range(5):
+            at, s = int(c.table[r, int(pos[r]) // page]), int(pos[r]) % page
+            c.k[at, :, s] = qkv[r, shift + heads * dim:shift + 2 * heads * dim].view(heads, dim).to(c.dtype)
+            c.v[at, :, s] = qkv[r, shift + 2 * heads * dim:].view(heads, dim).to(c.dtype)
+        assert same_bits(kp, c.k) and same_bits(vp, c.v)
+
+
+def test_write_skips_what_is_out_of_range(cuda):
+    from franken_ocr_b200 import paged
+
+    c = Cache([16, 16], 2, 8, 64, torch.float32, seed=5)
+    kp, vp, table = c.cuda()
+    table[1, 0], table[1, 1] = c.k.shape[0], -1
+    row = torch.tensor([-5, 2, 0, 0, 1, 1], dtype=torch.int32, device="cuda")
+    pos = torch.tensor([0, 0, -1, 16, 3, 9], dtype=torch.int32, device="cuda")
+    x = torch.ones((6, 2, 64), device="cuda")
+    paged.paged_write(x, x, kp, vp, table, pos, row=row)
+    assert same_bits(kp, c.k) and same_bits(vp, c.v)
+    paged.paged_write(x[:0], x[:0], kp, vp, table, pos[:0], row=row[:0])
+    assert same_bits(kp, c.k)
+
+
+# ---- attention ----------------------------------------------------------------
+
+def check_attention(c, q, lens, refs=None, window=0, weights=False, scale=None, width=None, dev=None):
+    from franken_ocr_b200 import paged
+
+    kp, vp, table = dev or c.cuda()
+    rows = len(lens)
+    dl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    dr = None if refs is None else torch.tensor(refs, dtype=torch.int32, device="cuda")
+    w = w0 = None
+    if weights:
+        w0 = torch.rand((rows, c.heads, width or c.width * c.page), generator=torch.Generator().manual_seed(8))
+        w = w0.cuda()
+    used = 1 / math.sqrt(c.dim) if scale is None else scale
+    want, probs, bound = attention(c, q, lens, used, refs, window)
+    got = paged.paged_attention(q.cuda(), kp, vp, table, dl, ref_lens=dr, window=window, weights=w, scale=scale)
+    assert got.dtype == q.dtype and got.shape == q.shape
+    off = (got.cpu().double() - want).abs()
+    assert bool((off <= bound).all()), f"off by {float((off / bound).max())} bounds"
+    if weights:
+        group = q.shape[1] // c.heads
+        rest = torch.ones_like(w0, dtype=torch.bool)
+        gw = w.cpu()
+        for (r, h), (at, p) in probs.items():
+            rest[r, h, at] = False
+            new = gw[r, h, at].double() - w0[r, h, at].double()
+            # bound of a probability (as in `attention`), the group's sum, the add's rounding
+            tol = group * (bound_of_p(c, q, r, h, at, used, group)) * p + 2.0 ** -24 * (w0[r, h, at] + p + 1)
+            assert bool(((new - p).abs() <= tol).all())
+        assert torch.equal(gw[rest], w0[rest])
+    return got
+
+
+def bound_of_p(c, q, r, h, at, scale, group):
+    qs = q[r, h * group:(h + 1) * group].double()
+    k = c.row(r, at)[h]
+    s = (scale * qs @ k.T).abs()
+    ds = float((scale * qs.abs() @ k.abs().T).max()) * (c.dim + 2) * 2.0 ** -24
+    return 2 * ds + 2 * (len(at) + 16) * 2.0 ** -24 + 2.0 ** -21 + float(s.max()) * 2.0 ** -22
+
+
+@pytest.mark.parametrize("q_type,pool", [(a, b) for a in DTYPES for b in DTYPES])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attention_types(cuda, q_type, pool, dim):
+    lens = [1, 2, 0, 63, 64, 65, 257]
+    c = Cache(lens, 2, 16, dim, DTYPES[pool], seed=dim)
+    q = torch.randn((len(lens), 2, dim), generator=torch.Generator().manual_seed(1)).to(DTYPES[q_type])
+    check_attention(c, q, lens)
+
+
+@pytest.mark.parametrize("group", [1, 2, 3, 4, 5, 7, 8, 9, 16, 17, 33])
+@pytest.mark.parametrize("q_type,pool", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16"), ("f16", "f16")])
+def test_attention_head_groups_with_weights(cuda, group, q_type, pool):
+    lens = [130, 1, 0, 77]
+    c = Cache(lens, 3, 16, 128, DTYPES[pool], seed=group)
+    q = torch.randn((4, 3 * group, 128), generator=torch.Generator().manual_seed(group)).to(DTYPES[q_type])
+    check_attention(c, q, lens, weights=True)
+
+
+@pytest.mark.parametrize("dim,pool", [(8, "bf16"), (16, "f32"), (72, "f16"), (80, "bf16"), (96, "f32"), (4, "f32"),
+                                      (100, "f32"), (136, "bf16"), (192, "f16"), (200, "f32"), (248, "f16")])
+@pytest.mark.parametrize("group", [1, 6])
+def test_attention_odd_dims(cuda, dim, pool, group):
+    lens = [31, 100]
+    c = Cache(lens, 2, 8, dim, DTYPES[pool], seed=dim)
+    for q_type in ("f32", pool):
+        q = torch.randn((2, 2 * group, dim), generator=torch.Generator().manual_seed(dim)).to(DTYPES[q_type])
+        check_attention(c, q, lens, weights=True)
+
+
+@pytest.mark.parametrize("page", [1, 3, 8, 24, 100, 256])
+@pytest.mark.parametrize("pool,group", [("f32", 1), ("bf16", 8)])
+def test_attention_pages_that_end_inside_a_tile(cuda, page, pool, group):
+    lens = [1, page, page + 1, 5 * page - 1, 300]
+    c = Cache(lens, 2, page, 64, DTYPES[pool], seed=page, strided=True)
+    q = torch.randn((5, 2 * group, 64), generator=torch.Generator().manual_seed(page)).to(DTYPES[pool])
+    check_attention(c, q, lens, weights=True)
+
+
+@pytest.mark.parametrize("window", [1, 17, 128, 4000])
+@pytest.mark.parametrize("pool,group", [("f32", 1), ("f16", 5)])
+def test_attention_reference_and_window(cuda, window, pool, group):
+    """The R-SWA rule: hidden entries hold NaN and infinities."""
+    lens = [1, 40, 200, 300, 300, 300, 0, 513]
+    refs = [0, 40, 64, 300, 1000, -3, 5, 100]
+    c = Cache(lens, 2, 16, 64, DTYPES[pool], seed=window)
+    for r, n in enumerate(lens):
+        seen = set(visible(n, max(0, min(refs[r], n)), window))
+        for j in range(n):
+            if j not in seen:
+                at = int(c.table[r, j // 16])
+                c.k[at, :, j % 16] = math.inf if j % 2 else math.nan
+                c.v[at, :, j % 16] = -math.inf
+    q = torch.randn((len(lens), 2 * group, 64), generator=torch.Generator().manual_seed(5)).to(DTYPES[pool])
+    clamped = [max(0, min(a, n)) for a, n in zip(refs, lens)]
+    kp = c.cuda()
+    out = check_attention(c, q, lens, refs=clamped, window=window, weights=True, dev=kp)
+    from franken_ocr_b200 import paged
+    raw = paged.paged_attention(q.cuda(), *kp, torch.tensor(lens, dtype=torch.int32, device="cuda"), window=window,
+                                ref_lens=torch.tensor(refs, dtype=torch.int32, device="cuda"))
+    assert same_bits(raw, out)
+
+
+@pytest.mark.parametrize("rows,high", [(1, 20000), (3, 9000), (37, 700), (700, 9)])
+@pytest.mark.parametrize("pool,group,dim", [("f32", 1, 128), ("bf16", 8, 128), ("bf16", 2, 64)])
+def test_attention_split_and_joined(cuda, rows, high, pool, group, dim):
+    """Rows that many blocks share, and blocks that many rows share."""
+    lens = [(high * (7 * r % 11 + 1)) // 11 if r % 5 != 3 else 0 for r in range(rows)]
+    lens[0] = high
+    c = Cache(lens, 1, 16, dim, DTYPES[pool], seed=rows)
+    q = torch.randn((rows, group, dim), generator=torch.Generator().manual_seed(rows)).to(DTYPES[pool]) * 2
+    check_attention(c, q, lens, weights=rows == 3)
+
+
+def test_attention_over_a_thousand_rows(cuda):
+    lens = [(5 * r) % 23 for r in range(1500)]
+    c = Cache(lens, 1, 8, 64, torch.bfloat16, seed=1)
+    q = torch.randn((1500, 2, 64), generator=torch.Generator().manual_seed(1))
+    check_attention(c, q, lens, weights=True)
+
+
+def test_attention_peaks_and_scales(cuda):
+    """Scores far apart, a maximum at either end, another scale."""
+    n = 700
+    c = Cache([n, n, n], 1, 16, 128, torch.float32, seed=2)
+    q = torch.randn((3, 1, 128), generator=torch.Generator().manual_seed(3))
+    for r, j in enumerate((0, n - 1, n // 2)):
+        c.k[int(c.table[r, j // 16]), 0, j % 16] = q[r, 0] * 1.0
+    check_attention(c, q, [n] * 3, scale=0.7)
+    check_attention(c, q, [n] * 3, scale=1e-6)
+
+
+def test_attention_unseen_nan_and_bad_pages(cuda):
+    from franken_ocr_b200 import paged
+
+    lens = [40, 40, 40, 200, -4]
+    c = Cache([40, 40, 40, 40, 40], 2, 16, 64, torch.float32, seed=6)
+    kp, vp, table = c.cuda()
+    table[1, 1] = kp.shape[0]
+    table[2, 2] = -1
+    q = torch.randn((5, 4, 64), generator=torch.Generator().manual_seed(7)).cuda()
+    w = torch.ones((5, 2, 48), device="cuda")
+    out = paged.paged_attention(q, kp, vp, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), weights=w)
+    good = attention(c, q.cpu()[:1], [40], 1 / 8)[0]
+    assert torch.allclose(out[0].cpu().double(), good[0], atol=1e-4)
+    assert bool(out[1:4].isnan().all())
+    assert bool((out[4] == 0).all())
+    assert bool((w[1:] == 1).all())          # rows that give NaN, and empty ones, leave their weights
+    assert abs(float((w[0] - 1).sum()) - 4) < 1e-4  # two kv heads, two query heads each
+    q[0] = math.nan
+    out = paged.paged_attention(q, kp, vp, table, torch.tensor([40, 0, 0, 0, 0], dtype=torch.int32, device="cuda"))
+    assert bool(out[0].isnan().all()) and bool((out[1:] == 0).all())
+
+
+def test_attention_strided_queries_and_out(cuda):
+    from franken_ocr_b200 import paged
+
+    c = Cache([50, 60], 2, 16, 64, torch.bfloat16, seed=9)
+    kp, vp, table = c.cuda()
+    qkv = torch.randn((2, 3 * 4 * 64), generator=torch.Generator().manual_seed(1)).cuda()
+    q = qkv[:, 256:512].view(2, 4, 64)
+    lens = torch.tensor([50, 60], dtype=torch.int32, device="cuda")
+    want = paged.paged_attention(q.contiguous(), kp, vp, table, lens)
+    out = torch.empty((2, 4, 64), device="cuda")
+    assert paged.paged_attention(q, kp, vp, table, lens, out=out) is out
+    assert same_bits(out, want)
+
+
+def test_attention_is_the_same_every_time_and_in_a_graph(cuda):
+    """Repeated calls give the same bits; a captured call follows its inputs, also
+    beside another captured call."""
+    from franken_ocr_b200 import paged
+
+    c = Cache([4000, 17], 2, 16, 128, torch.bfloat16, seed=10)
+    kp, vp, table = c.cuda()
+    g = torch.Generator().manual_seed(1)
+    qs = [torch.randn((2, 8, 128), generator=g).to(torch.bfloat16).cuda() for _ in range(2)]
+    lens = torch.tensor([4000, 17], dtype=torch.int32, device="cuda")
+    want = [paged.paged_attention(q, kp, vp, table, lens) for q in qs]
+    for _ in range(3):
+        assert same_bits(paged.paged_attention(qs[0], kp, vp, table, lens), want[0])
+    held, graphs, outs = [q.clone() for q in qs], [], []
+    for q in held:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(paged.paged_attention(q, kp, vp, table, lens))
+        graphs.append(graph)
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        torch.cuda.synchronize()
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        assert same_bits(outs[0], want[0]) and same_bits(outs[1], want[1])
+    held[0].copy_(qs[1])
+    lens.copy_(torch.tensor([17, 4], dtype=torch.int32))
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert same_bits(outs[0], paged.paged_attention(qs[1], kp, vp, table, lens))
+
+
+def test_attention_offsets_past_32_bits(cuda):
+    """A pool of over 4 GB whose last pages hold the row."""
+    from franken_ocr_b200 import paged
+
+    pages, page, dim = 140000, 64, 256
+    kp = torch.empty((pages, 1, page, dim), dtype=torch.float16, device="cuda")
+    vp = torch.empty_like(kp)
+    c = Cache([150], 1, page, dim, torch.float16, seed=11)
+    table = c.table.clone()
+    for j in range(3):
+        kp[pages - 1 - j] = c.k[int(c.table[0, j])].cuda()
+        vp[pages - 1 - j] = c.v[int(c.table[0, j])].cuda()
+        table[0, j] = pages - 1 - j
+    q = torch.randn((1, 2, dim), generator=torch.Generator().manual_seed(1))
+    check_attention(c, q, [150], dev=(kp, vp, table.cuda()))
+    # and the write: the last slot of the last page
+    x = torch.ones((1, 1, dim), device="cuda")
+    paged.paged_write(x, x, kp, vp, table.cuda(), torch.tensor([page - 1], dtype=torch.int32, device="cuda"))
+    assert bool((kp[pages - 1, 0, page - 1] == 1).all()) and bool((vp[pages - 1, 0, page - 1] == 1).all())
+
+
+# ---- eviction --------------------------------------------------------------------
+
+def check_evict(c, w, lens, budget, sink, recent, strided=False):
+    from franken_ocr_b200 import paged
+
+    rows, heads, width = w.shape
+    small = -(-budget // c.page)
+    into = torch.tensor(c.spare[:rows * small], dtype=torch.int32).view(rows, small)
+    kp, vp, table = c.cuda()
+    dl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    dw = w.cuda()
+    if strided:
+        dw = torch.cat([dw, dw], 2)[:, :, :width]
+    kept, new, wo = paged.paged_evict(kp, vp, table, dl, dw, into.cuda(), budget, sink=sink, recent=recent)
+    k, v = c.k.clone(), c.v.clone()
+    want = torch.full((rows, heads, budget), -1, dtype=torch.int32)
+    want_w = torch.zeros_like(w)
+    for r, n in enumerate(lens):
+        for h in range(heads):
+            keep = evict_kept(w[r, h], n, budget, sink, recent)
+            want[r, h, :len(keep)] = torch.tensor(keep, dtype=torch.int32)
+            for j, p in enumerate(keep):
+                src, dst = int(c.table[r, p // c.page]), int(into[r, j // c.page])
+                k[dst, h, j % c.page] = c.k[src, h, p % c.page]
+                v[dst, h, j % c.page] = c.v[src, h, p % c.page]
+                want_w[r, h, j] = w[r, h, p]
+    assert torch.equal(kept.cpu(), want)
+    assert new.tolist() == [min(n, budget) for n in lens]
+    assert same_bits(wo, want_w)
+    assert same_bits(kp, k) and same_bits(vp, v)
+
+
+@pytest.mark.parametrize("pool", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("page,dim,budget,sink,recent", [(16, 64, 20, 4, 8), (7, 80, 1, 0, 0), (16, 128, 33, 0, 33),
+                                                         (1, 64, 10, 10, 0), (24, 64, 64, 1, 30)])
+def test_evict_matches_the_definition(cuda, pool, page, dim, budget, sink, recent):
+    lens = [1, 0, budget, budget + 1, 150, 149]
+    rows = len(lens)
+    c = Cache(lens, 3, page, dim, DTYPES[pool], seed=budget, spare=rows * -(-budget // page), strided=page == 7)
+    w = torch.rand((rows, 3, 160), generator=torch.Generator().manual_seed(budget))
+    check_evict(c, w, lens, budget, sink, recent, strided=page == 24)
+
+
+def test_evict_ties_infinities_and_nan(cuda):
+    lens = [90] * 6
+    c = Cache(lens, 2, 16, 64, torch.float32, seed=1, spare=6 * 2)
+    g = torch.Generator().manual_seed(2)
+    w = torch.zeros((6, 2, 90))
+    w[1] = torch.randint(0, 3, (2, 90), generator=g).float()
+    w[2] = torch.randint(0, 2, (2, 90), generator=g).float() * -0.0          # -0 and 0 are equal
+    w[3] = torch.where(torch.rand((2, 90), generator=g) < 0.8, torch.tensor(math.nan), torch.rand((2, 90), generator=g))
+    w[4] = torch.where(torch.rand((2, 90), generator=g) < 0.5, torch.tensor(-math.inf), torch.tensor(math.inf))
+    w[5] = -torch.rand((2, 90), generator=g) * 1e-42                          # negative subnormals
+    check_evict(c, w, lens, 32, 3, 5)
+
+
+@pytest.mark.parametrize("n,budget", [(5000, 700), (70000, 3), (40000, 39999), (140000, 9000)])
+def test_evict_long_rows(cuda, n, budget):
+    from franken_ocr_b200 import paged
+
+    heads, page = 2, 64
+    g = torch.Generator(device="cuda").manual_seed(n)
+    pages, small = -(-n // page), -(-budget // page)
+    kp = torch.randn((pages + small, heads, page, 64), generator=g, device="cuda", dtype=torch.float16)
+    vp = torch.randn((pages + small, heads, page, 64), generator=g, device="cuda", dtype=torch.float16)
+    order = torch.randperm(pages + small, generator=g, device="cuda").int()
+    table, into = order[None, :pages], order[None, pages:]
+    w = torch.rand((1, heads, n + 3), generator=g, device="cuda")
+    w[0, 1] = (w[0, 1] * 4).floor()   # many ties
+    sink, recent = min(2, budget), (budget - min(2, budget)) // 2
+    kept, lens, wo = paged.paged_evict(kp, vp, table, torch.tensor([n], dtype=torch.int32, device="cuda"), w, into,
+                                       budget, sink=sink, recent=recent)
+    for h in range(heads):
+        keep = torch.tensor(evict_kept(w[0, h].cpu(), n, budget, sink, recent))
+        assert torch.equal(kept[0, h].cpu().long(), keep)
+        keep = keep.cuda()
+        at = torch.arange(budget, device="cuda")
+        for pool in (kp, vp):
+            assert same_bits(pool[into[0].long()[at // page], h, at % page], pool[table[0].long()[keep // page], h, keep % page])
+        assert same_bits(wo[0, h, :budget], w[0, h, keep]) and bool((wo[0, h, budget:] == 0).all())
+    assert lens.tolist() == [budget]
+
+
+def test_evict_lengths_out_of_range_and_bad_pages(cuda):
+    from franken_ocr_b200 import paged
+
+    c = Cache([64] * 4, 1, 16, 64, torch.float32, seed=3, spare=8)
+    kp, vp, table = c.cuda()
+    table[3, 1] = -1
+    before = kp.clone()
+    into = torch.tensor(c.spare, dtype=torch.int32, device="cuda").view(4, 2)
+    w = torch.rand((4, 1, 64), generator=torch.Generator().manual_seed(1)).cuda()
+    kept, lens, wo = paged.paged_evict(kp, vp, table, torch.tensor([-1, 65, 1000, 64], dtype=torch.int32, device="cuda"),
+                                       w, into, 20, recent=20)
+    assert lens.tolist() == [0, 0, 0, 20]
+    assert bool((kept[:3] == -1).all()) and bool((wo[:3] == 0).all())
+    assert kept[3, 0].tolist() == list(range(44, 64))
+    assert same_bits(kp[into[:3].reshape(-1).long()], before[into[:3].reshape(-1).long()])
