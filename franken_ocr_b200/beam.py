@@ -8,12 +8,10 @@ CUDA tensors on one device, torch's current stream; both can be captured.
 """
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 
-from ._lib import check, lib
-from .paged import _On, _cache, _dtype, _need
+from ._lib import lib
+from .paged import _cache, _call, _dtype, _need, _workspace
 
 
 def beam_select(logits, scores, n: int | None = None, *, done=None, end_token: int = 1):
@@ -49,15 +47,12 @@ def beam_select(logits, scores, n: int | None = None, *, done=None, end_token: i
     out = torch.empty((batch, n), dtype=torch.float32, device=device)
     parent = torch.empty((batch, n), dtype=torch.int32, device=device)
     token = torch.empty((batch, n), dtype=torch.int32, device=device)
-    need = C.c_size_t()
-    check(lib.focr_beam_select_workspace(batch, beams, vocab, n, C.byref(need)))
-    with _On(device) as stream:
-        ws = torch.empty(need.value, dtype=torch.uint8, device=device)
-        check(lib.focr_beam_select(
-            logits.data_ptr(), code, batch, beams, vocab,
-            logits.stride(1) if beams > 1 else max(logits.stride(0), vocab), scores.data_ptr(),
-            None if done is None else done.data_ptr(), end_token, n, out.data_ptr(), parent.data_ptr(),
-            token.data_ptr(), ws.data_ptr(), need.value, stream))
+    need = _workspace("focr_beam_select_workspace", batch, beams, vocab, n)
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    _call(lib.focr_beam_select, device, logits.data_ptr(), code, batch, beams, vocab,
+          logits.stride(1) if beams > 1 else max(logits.stride(0), vocab), scores.data_ptr(),
+          None if done is None else done.data_ptr(), end_token, n, out.data_ptr(), parent.data_ptr(),
+          token.data_ptr(), ws.data_ptr(), need)
     return out, parent, token
 
 
@@ -75,12 +70,11 @@ def beam_reorder(k_pages, v_pages, table, lens, parent, fresh, *, weights=None):
     another and from every page the table uses."""
     ctx = "beam_reorder"
     layered = k_pages.dim() == 5
-    cache, device = _cache(ctx, k_pages, v_pages, table, 5 if layered else 4)
+    cache, device, heads, _, rows, width = _cache(ctx, k_pages, v_pages, table, 5 if layered else 4)
     layers = k_pages.shape[0] if layered else 1
     if parent.dim() != 2:
         raise ValueError(f"{ctx}: parent must be [batch, beams], not {tuple(parent.shape)}")
     batch, beams = parent.shape
-    rows, width = table.shape
     if batch * beams != rows:
         raise ValueError(f"{ctx}: table has {rows} rows for {batch} x {beams} beams")
     _need(ctx, "parent", parent, torch.int32, (batch, beams), device)
@@ -88,7 +82,7 @@ def beam_reorder(k_pages, v_pages, table, lens, parent, fresh, *, weights=None):
     _need(ctx, "fresh", fresh, torch.int32, (rows,), device)
     w_out, span, w_layer, w_row, w_head = None, 0, 0, 0, 0
     if weights is not None:
-        lead = (layers, rows, cache.kv_heads) if layered else (rows, cache.kv_heads)
+        lead = (layers, rows, heads) if layered else (rows, heads)
         if weights.dtype != torch.float32:
             raise TypeError(f"{ctx}: weights must be torch.float32, not {weights.dtype}")
         if weights.shape[:-1] != lead or weights.device != device:
@@ -101,10 +95,8 @@ def beam_reorder(k_pages, v_pages, table, lens, parent, fresh, *, weights=None):
         w_out = torch.empty(weights.shape, dtype=torch.float32, device=device)
     new_table = torch.empty((rows, width), dtype=torch.int32, device=device)
     new_lens = torch.empty((rows,), dtype=torch.int32, device=device)
-    with _On(device) as stream:
-        check(lib.focr_beam_reorder(
-            C.byref(cache), layers, k_pages.stride(0) if layered else 0, batch, beams, lens.data_ptr(),
-            parent.data_ptr(), fresh.data_ptr(), new_table.data_ptr(), new_lens.data_ptr(),
-            None if weights is None else weights.data_ptr(), span, w_layer, w_row, w_head,
-            None if w_out is None else w_out.data_ptr(), stream))
+    _call(lib.focr_beam_reorder, device, cache, layers, k_pages.stride(0) if layered else 0, batch, beams,
+          lens.data_ptr(), parent.data_ptr(), fresh.data_ptr(), new_table.data_ptr(), new_lens.data_ptr(),
+          None if weights is None else weights.data_ptr(), span, w_layer, w_row, w_head,
+          None if w_out is None else w_out.data_ptr())
     return new_table, new_lens, w_out

@@ -1,0 +1,238 @@
+// Attention of one new token per row over a paged K/V cache.
+//
+//   s_j = scale * q . k_j          over the row's visible positions j
+//   p   = softmax(s),  out = sum_j p_j v_j,  weights[j] += sum over the
+//   query heads of j's kv head of p_j
+//
+// A position j of a row of length n is visible when j < n and (no window, or
+// j < ref, or j >= n - window).  The visible positions are numbered 0..vis-1
+// without the gap, so hidden ones cost nothing.
+//
+// One pass over K and V with a running maximum and sum (base-2 exponentials
+// of c * s, c = scale * log2 e); partial results join by
+//   M = max m_i,  L = sum l_i 2^(c (m_i - M)),  out = sum a_i 2^(c (m_i - M)) / L.
+// Everything is held in f32; only K/V themselves have the cache's type, and
+// the output is rounded once to q's type.
+//
+// Work split: the lengths are on the device, so the host cannot lay out the
+// split.  The unit is a block tile (4 warp tiles of KEYS positions); all units
+// of all (row, head)s are numbered in order and every block of a fixed grid
+// takes an equal run of them, wherever rows begin and end.  A block that covers
+// a (row, head) whole writes the output; pieces go to the workspace (a block
+// has at most two) and paged_join_kernel joins them.  So no row length, however
+// ragged the batch, leaves SMs idle.
+#pragma once
+
+#include <type_traits>
+
+#include "paged.cuh"
+
+namespace focr {
+
+constexpr int ATTN_WARPS = 4, ATTN_ROWS = 1024;  // rows of one launch
+constexpr int ATTN_HEADS = 16;                   // most query heads a block takes together
+
+struct AttnArgs {
+    PagedView c;
+    const void *q;
+    const int32_t *lens, *refs;
+    void *out;
+    float *scores;   // raw s of every (row, q head, visible index), only when weights are asked for
+    float2 *stat;    // (M, 1 / L) of every (row, q head), likewise
+    float *part;     // [block][2][gp][dim] partial sums
+    float2 *ml;      // [block][2][gp] partial (m, l)
+    long long q_stride, out_stride;
+    int rows, group, q_heads, dim, q_type, window, cap, width;
+    int gp, head_chunks;  // query heads that a block takes together; blocks of them a kv head
+    int tile_shift;       // log2 of a block tile's positions
+    float c2;             // scale * log2(e)
+};
+
+// The visible positions of row r: index i is position i below `ref` and
+// i + gap from there on.  bad: the row's length passes its table or weights.
+struct RowView {
+    int vis, ref, gap;
+    bool bad;
+};
+__device__ __forceinline__ RowView row_view(const AttnArgs &a, int r) {
+    RowView v{0, 0, 0, false};
+    const int n = a.lens[r];
+    if (n <= 0) return v;
+    if (n > a.cap) {
+        v.bad = true;
+        return v;
+    }
+    v.ref = v.vis = n;
+    if (a.window > 0) {
+        int ref = a.refs ? a.refs[r] : 0;
+        ref = ref < 0 ? 0 : ref > n ? n : ref;
+        const int start = max(ref, n - min(a.window, n));
+        v.ref = ref;
+        v.gap = start - ref;
+        v.vis = n - v.gap;
+    }
+    return v;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 2^(c (s - m)) with m's product rounded once, the same for every s of a row.
+__device__ __forceinline__ float prob(float s, float c, float mc) { return ex2(__fmaf_rn(s, c, -mc)); }
+__device__ __forceinline__ float scaled_max(float m, float c) {
+    return m == -INFINITY ? 0.0f : __fmul_rn(m, c);
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+                 "r"(bytes));
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Prefix of the rows' tile counts into `pre` (ATTN_ROWS + 1 ints), by a block of
+// NT threads.
+template <int NT> __device__ void tile_prefix(const AttnArgs &a, int *pre) {
+    constexpr int PER = ATTN_ROWS / NT;
+    __shared__ int wsum[NT / 32];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int round = (1 << a.tile_shift) - 1;
+    if (a.rows <= 32) {  // one warp's scan; the usual small batch
+        if (warp == 0) {
+            int inc = lane < a.rows ? (row_view(a, lane).vis + round) >> a.tile_shift : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += x;
+            }
+            if (lane < a.rows) pre[lane + 1] = inc;
+            if (lane == 0) pre[0] = 0;
+        }
+        __syncthreads();
+        return;
+    }
+    int n[PER], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int r = t * PER + i;
+        n[i] = r < a.rows ? (row_view(a, r).vis + round) >> a.tile_shift : 0;
+        sum += n[i];
+    }
+    int inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+    }
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    int before = inc - sum;
+    for (int w = 0; w < warp; w++) before += wsum[w];
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int r = t * PER + i;
+        if (r <= a.rows) pre[r] = before;
+        before += n[i];
+    }
+    if (t == NT - 1 && a.rows == ATTN_ROWS) pre[ATTN_ROWS] = before;
+    __syncthreads();
+}
+
+// Blocks that get units: every one of them gets at least one.
+__device__ __forceinline__ unsigned long long run_count(unsigned long long total, int blocks) {
+    return min(total, (unsigned long long)blocks);
+}
+
+// The run of units of one block, and the piece of a (row, kv head, chunk of its
+// query heads) it stands at.
+struct Segment {
+    int r, kvh, heads, qh0, t0, t1, slot;
+    bool whole;
+    RowView rv;
+};
+struct Run {
+    unsigned long long u, begin, end;
+    int hc_count;
+
+    __device__ Run(const AttnArgs &a, const int *pre) {
+        hc_count = a.c.kv_heads * a.head_chunks;
+        const unsigned long long total = (unsigned long long)pre[a.rows] * hc_count;
+        const unsigned long long runs = run_count(total, gridDim.x);
+        begin = end = u = 0;
+        if (blockIdx.x >= runs) return;
+        u = begin = blockIdx.x * total / runs;
+        end = (blockIdx.x + 1ull) * total / runs;
+    }
+    __device__ bool next(const AttnArgs &a, const int *pre, Segment *s) {
+        if (u >= end) return false;
+        // the last row whose units begin at or before u
+        int lo = 0, hi = a.rows;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if ((unsigned long long)pre[mid] * hc_count <= u) lo = mid;
+            else hi = mid;
+        }
+        const int tiles = pre[lo + 1] - pre[lo];
+        const unsigned long long off = u - (unsigned long long)pre[lo] * hc_count;
+        const int hc = (int)(off / tiles);
+        s->r = lo;
+        s->t0 = (int)(off - (unsigned long long)hc * tiles);
+        s->t1 = (int)min((unsigned long long)tiles, s->t0 + (end - u));
+        s->whole = s->t0 == 0 && s->t1 == tiles;
+        s->slot = blockIdx.x * 2 + (u == begin ? 0 : 1);
+        s->kvh = hc / a.head_chunks;
+        const int g0 = (hc - s->kvh * a.head_chunks) * a.gp;
+        s->heads = min(a.gp, a.group - g0);
+        s->qh0 = s->kvh * a.group + g0;
+        s->rv = row_view(a, lo);
+        u += s->t1 - s->t0;
+        return true;
+    }
+};
+
+// Joins the block's warps, whose sums lie in shared memory `apart` floats from
+// one another ([GP][D], m[GP], l[GP]), and writes the segment's output or piece.
+template <int GP, int D>
+__device__ __forceinline__ void finish_segment(const AttnArgs &a, const Segment &s, const float *all, int apart) {
+    for (int x = threadIdx.x; x < GP * D; x += ATTN_WARPS * 32) {
+        const int g = x / D, d = x % D;
+        if (g >= s.heads || d >= a.dim) continue;
+        float M = -INFINITY, L = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int w = 0; w < ATTN_WARPS; w++) M = fmaxf(M, all[w * apart + GP * D + g]);
+        const float mc = scaled_max(M, a.c2);
+#pragma unroll
+        for (int w = 0; w < ATTN_WARPS; w++) {
+            const float f = prob(all[w * apart + GP * D + g], a.c2, mc);
+            L = __fmaf_rn(all[w * apart + GP * D + GP + g], f, L);
+            o = __fmaf_rn(all[w * apart + x], f, o);
+        }
+        if (s.whole) {
+            store_f32_as(a.out, a.q_type, s.r * a.out_stride + (long long)(s.qh0 + g) * a.dim + d,
+                         L == 0.0f ? 0.0f : o / L);
+            if (a.stat && d == 0) a.stat[(int64_t)s.r * a.q_heads + s.qh0 + g] = make_float2(M, 1.0f / L);
+        } else {
+            a.part[((int64_t)s.slot * GP + g) * a.dim + d] = o;
+            if (d == 0) a.ml[s.slot * GP + g] = make_float2(M, L);
+        }
+    }
+}
+
+inline int ilog2(int x) {
+    int n = 0;
+    while ((1 << n) < x) n++;
+    return n;
+}
+inline int attn_blocks() { return num_sms() * 2; }
+
+// The attention kernel for one type of cache, without the join; sets gp,
+// head_chunks and tile_shift of `a` as that kernel has them.
+int launch_attention_f32(AttnArgs &a, cudaStream_t st);
+int launch_attention_f16(AttnArgs &a, cudaStream_t st);
+int launch_attention_bf16(AttnArgs &a, cudaStream_t st);
+
+}  // namespace focr

@@ -1,0 +1,250 @@
+// Attention over a paged cache on the tensor cores: query and cache of one
+// 16-bit type, up to 16 query heads of a kv head as the rows of a matrix tile.
+//
+// A warp takes KEYS positions at a time: S = Q K^T and O += P V as 16x8x16 warp
+// products straight from the staged rows, whose 16-byte chunks are swizzled by
+// the row so that the transposing loads meet no bank twice.  One token's work is
+// bound by the cache's bytes, not by the products (48 of them, ~100 cycles of
+// an SM, for 8 KB that take ~350 cycles to arrive), so the warp products, which
+// leave every warp on its own without a block barrier, cost nothing against
+// larger tiles.  P stays exact to 16 bits more than its type: it is split
+// into a high and a low part and multiplied twice.
+#pragma once
+
+#include "paged_attention.cuh"
+
+namespace focr {
+namespace {
+
+template <int D> struct MmaTile {
+    static constexpr int DB = D * 2;
+    static constexpr int CH = DB / 16;
+    static constexpr int KEYS = D == 64 ? 32 : 16;
+    static constexpr int HALF = KEYS * DB;
+    static constexpr int STAGES = HALF > 4096 ? 2 : 3;
+    static constexpr int BLOCK = ATTN_WARPS * KEYS;
+};
+template <int D> constexpr int mma_smem() {
+    return ATTN_WARPS * MmaTile<D>::STAGES * 2 * MmaTile<D>::HALF + (ATTN_ROWS + 1) * 4;
+}
+
+template <typename T> __device__ __forceinline__ void mma16816(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool TRANS> __device__ __forceinline__ void ldmatrix4(uint32_t *r, uint32_t addr) {
+    if constexpr (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// The high parts of two values as a pair, and what they leave.
+template <typename T> __device__ __forceinline__ uint32_t split_pair(float x, float y, uint32_t *low) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(x, y);
+        const float2 f = __half22float2(h);
+        const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+        *low = *reinterpret_cast<const uint32_t *>(&l);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        const float2 f = __bfloat1622float2(h);
+        const __nv_bfloat162 l = __floats2bfloat162_rn(x - f.x, y - f.y);
+        *low = *reinterpret_cast<const uint32_t *>(&l);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_attention_mma_kernel(const AttnArgs a) {
+    using S = MmaTile<D>;
+    constexpr int GP = 16, KEYS = S::KEYS, NT = KEYS / 8, ITS = S::HALF / 512;
+    // f16 holds nothing below 2^-24: probabilities, at most 1, are scaled up
+    constexpr float PS = std::is_same<T, __half>::value ? 2048.0f : 1.0f;
+    extern __shared__ __align__(128) char smem[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    char *ring = smem + warp * S::STAGES * 2 * S::HALF;
+    int *pre = reinterpret_cast<int *>(smem + ATTN_WARPS * S::STAGES * 2 * S::HALF);
+    const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
+
+    pdl_wait();
+    pdl_trigger();
+    tile_prefix<ATTN_WARPS * 32>(a, pre);
+
+    const int qr = lane >> 2, qc = (lane & 3) * 2;   // this lane's row and columns of a tile
+    const int mi = lane >> 3, rr = lane & 7;         // its matrix and row when loading one
+    Run run(a, pre);
+    Segment sg;
+    while (run.next(a, pre, &sg)) {
+        const int r = sg.r, heads = sg.heads, t0 = sg.t0, t1 = sg.t1;
+        const RowView rv = sg.rv;
+        const int32_t *pages = a.c.table + r * a.c.table_stride;
+        const char *kb = a.c.k + sg.kvh * a.c.head_stride, *vb = a.c.v + sg.kvh * a.c.head_stride;
+
+        uint32_t qa[D / 16][4];
+        const uint16_t *qp = static_cast<const uint16_t *>(a.q) + r * a.q_stride + (long long)sg.qh0 * a.dim;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ks++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int g = qr + (x & 1) * 8, d = ks * 16 + (x >> 1) * 8 + qc;
+                qa[ks][x] = g < heads && d < a.dim ? qp[g * a.dim + d] | (uint32_t)qp[g * a.dim + d + 1] << 16 : 0;
+            }
+        float acc[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < D / 8; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+        bool bad = false;
+
+        auto key_offset = [&](int tile) -> int64_t {  // of index `lane` of the warp's tile
+            const int i = (tile * ATTN_WARPS + warp) * KEYS + lane;
+            if (lane >= KEYS || i >= rv.vis || tile >= t1) return -1;
+            const int64_t o = a.c.offset(pages, (uint32_t)(i < rv.ref ? i : i + rv.gap));
+            bad |= o < 0;
+            return o;
+        };
+        auto issue = [&](int stage, int64_t mine) {
+            const uint32_t dst = ring_s + stage * 2 * S::HALF;
+#pragma unroll
+            for (int it = 0; it < ITS; it++) {
+                const int x = it * 32 + lane, key = x / S::CH, c = x % S::CH;
+                const int64_t o = __shfl_sync(0xffffffffu, mine, key);
+                const bool have = o >= 0 && c * 16 < a.c.row_bytes;
+                const int64_t src = have ? o + c * 16 : 0;
+                const uint32_t to = dst + key * S::DB + ((c ^ (key & 7)) << 4);
+                cp_async16(to, kb + src, have ? 16 : 0);
+                cp_async16(to + S::HALF, vb + src, have ? 16 : 0);
+            }
+        };
+#pragma unroll
+        for (int s = 0; s < S::STAGES; s++) {
+            issue(s, key_offset(t0 + s));
+            cp_async_commit();
+        }
+        int stage = 0;
+        for (int tile = t0; tile < t1; tile++) {
+            const int64_t next = key_offset(tile + S::STAGES);
+            cp_async_wait<S::STAGES - 1>();
+            __syncwarp();
+            const uint32_t ks_s = ring_s + stage * 2 * S::HALF, vs_s = ks_s + S::HALF;
+            float s[NT][4];
+#pragma unroll
+            for (int t = 0; t < NT; t++) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ks++)
+#pragma unroll
+                for (int p = 0; p < KEYS / 16; p++) {
+                    uint32_t b[4];
+                    ldmatrix4<false>(b, ks_s + (p * 16 + (mi >> 1) * 8 + rr) * S::DB + (((ks * 2 + (mi & 1)) ^ rr) << 4));
+                    mma16816<T>(s[2 * p], qa[ks], b[0], b[1]);
+                    mma16816<T>(s[2 * p + 1], qa[ks], b[2], b[3]);
+                }
+            const int i0 = (tile * ATTN_WARPS + warp) * KEYS + qc;
+            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int i = i0 + t * 8 + (x & 1);
+                    if (i >= rv.vis) s[t][x] = -INFINITY;
+                    else if (a.scores) {
+                        const int g = qr + (x >> 1) * 8;
+                        if (g < heads) a.scores[((int64_t)r * a.q_heads + sg.qh0 + g) * a.width + i] = s[t][x];
+                    }
+                    top[x >> 1] = fmaxf(top[x >> 1], s[t][x]);
+                }
+            if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+                    float n = fmaxf(m[y], top[y]);
+                    n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 1));
+                    n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 2));
+                    const float f = prob(m[y], a.c2, scaled_max(n, a.c2));
+                    m[y] = n;
+                    l[y] *= f;
+#pragma unroll
+                    for (int j = 0; j < D / 8; j++) {
+                        acc[j][2 * y] *= f;
+                        acc[j][2 * y + 1] *= f;
+                    }
+                }
+            }
+            const float mc[2] = {scaled_max(m[0], a.c2), scaled_max(m[1], a.c2)};
+#pragma unroll
+            for (int kk = 0; kk < KEYS / 16; kk++) {
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int x = 0; x < 4; x++) {  // registers: (row, low keys), (row + 8, low), (row, high), (row + 8, high)
+                    const int t = 2 * kk + (x >> 1), y = x & 1;
+                    const float p0 = prob(s[t][2 * y], a.c2, mc[y]) * PS, p1 = prob(s[t][2 * y + 1], a.c2, mc[y]) * PS;
+                    l[y] += p0 + p1;
+                    hi[x] = split_pair<T>(p0, p1, &lo[x]);
+                }
+#pragma unroll
+                for (int jp = 0; jp < D / 16; jp++) {
+                    uint32_t b[4];
+                    ldmatrix4<true>(b, vs_s + (kk * 16 + (mi & 1) * 8 + rr) * S::DB + (((jp * 2 + (mi >> 1)) ^ rr) << 4));
+                    mma16816<T>(acc[2 * jp], hi, b[0], b[1]);
+                    mma16816<T>(acc[2 * jp + 1], hi, b[2], b[3]);
+                    mma16816<T>(acc[2 * jp], lo, b[0], b[1]);
+                    mma16816<T>(acc[2 * jp + 1], lo, b[2], b[3]);
+                }
+            }
+            __syncwarp();
+            issue(stage, next);
+            cp_async_commit();
+            stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+        }
+        cp_async_wait<0>();
+
+        const bool any_bad = __any_sync(0xffffffffu, bad);
+        __syncwarp();
+        float *mine = reinterpret_cast<float *>(ring);  // [GP][D], m[GP], l[GP]
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+            const int g = qr + y * 8;
+#pragma unroll
+            for (int j = 0; j < D / 8; j++) {
+                mine[g * D + j * 8 + qc] = acc[j][2 * y] * (1.0f / PS);
+                mine[g * D + j * 8 + qc + 1] = acc[j][2 * y + 1] * (1.0f / PS);
+            }
+            l[y] += __shfl_xor_sync(0xffffffffu, l[y], 1);
+            l[y] += __shfl_xor_sync(0xffffffffu, l[y], 2);
+            if ((lane & 3) == 0) {
+                mine[GP * D + g] = m[y];
+                mine[GP * D + GP + g] = any_bad ? NAN : l[y] * (1.0f / PS);
+            }
+        }
+        __syncthreads();
+        finish_segment<GP, D>(a, sg, reinterpret_cast<const float *>(smem), S::STAGES * 2 * S::HALF / 4);
+        __syncthreads();
+    }
+}
+
+template <typename T, int D> int launch_mma(AttnArgs &a, cudaStream_t st) {
+    constexpr int smem = mma_smem<D>();
+    FOCR_CUDA_TRY(set_max_dynamic_smem((const void *)paged_attention_mma_kernel<T, D>, smem));
+    a.gp = 16;
+    a.head_chunks = (a.group + 15) / 16;
+    a.tile_shift = ilog2(MmaTile<D>::BLOCK);
+    FOCR_CUDA_TRY(launch_pdl(paged_attention_mma_kernel<T, D>, attn_blocks(), ATTN_WARPS * 32, smem, st, a));
+    return FOCR_OK;
+}
+template <typename T> int launch_mma_dim(AttnArgs &a, cudaStream_t st) {
+    if (a.dim <= 64) return launch_mma<T, 64>(a, st);
+    if (a.dim <= 128) return launch_mma<T, 128>(a, st);
+    return launch_mma<T, 256>(a, st);
+}
+
+// Query heads of a kv head from which the tensor cores take them.
+constexpr int MMA_HEADS = 3;
+
+}  // namespace
+}  // namespace focr

@@ -1,0 +1,234 @@
+// Attention over a paged cache on the f32 units: any type of query over any type
+// of cache.
+#pragma once
+
+#include "paged_attention.cuh"
+
+namespace focr {
+namespace {
+
+// Shapes of a warp tile.  A row of D elements is DB bytes; LPK lanes share a
+// key (NC 16-byte chunks each), KPI keys go by per step, ITS steps a tile.
+template <typename T, int D> struct Tile {
+    static constexpr int DB = D * (int)sizeof(T);
+    static constexpr int LPK = DB / 16 < 32 ? DB / 16 : 32;
+    static constexpr int NC = DB / 16 / LPK;
+    static constexpr int KPI = 32 / LPK;
+    static constexpr int ITS = 8;
+    static constexpr int KEYS = ITS * KPI;
+    static constexpr int HALF = KEYS * DB;      // bytes of K, and of V, in a stage
+    static constexpr int STAGES = HALF > 4096 ? 2 : 3;
+    static constexpr int BLOCK = ATTN_WARPS * KEYS;  // positions of a block tile
+    static constexpr int EPL = NC * 16 / (int)sizeof(T);  // dimensions of a lane
+};
+
+template <typename T, int D, int GP> constexpr int simt_smem() {
+    using S = Tile<T, D>;
+    return ATTN_WARPS * S::STAGES * 2 * S::HALF + ATTN_WARPS * GP * S::KEYS * 4 + (ATTN_ROWS + 1) * 4;
+}
+
+// The arithmetic runs on the f32 units: with few query heads a kv head the
+// loads bound it (a key of 128 16-bit values costs a warp ~25 instructions a
+// head against 512 bytes).
+template <typename T, int D, int GP>
+__global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(const AttnArgs a) {
+    using S = Tile<T, D>;
+    constexpr int LPK = S::LPK, KPI = S::KPI, ITS = S::ITS, KEYS = S::KEYS, NC = S::NC, EPL = S::EPL;
+    constexpr int EPC = 16 / (int)sizeof(T);  // elements of a chunk
+    extern __shared__ __align__(128) char smem[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    char *ring = smem + warp * S::STAGES * 2 * S::HALF;
+    float *probs = reinterpret_cast<float *>(smem + ATTN_WARPS * S::STAGES * 2 * S::HALF) + warp * GP * KEYS;
+    int *pre = reinterpret_cast<int *>(smem + ATTN_WARPS * S::STAGES * 2 * S::HALF + ATTN_WARPS * GP * KEYS * 4);
+    const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
+
+    pdl_wait();
+    pdl_trigger();
+    tile_prefix<ATTN_WARPS * 32>(a, pre);
+
+    const int sub = lane / LPK, chunk = lane % LPK;
+    // the step whose score this lane holds after the transposing reduction
+    const int my_it = (lane & (LPK / 2) ? 4 : 0) + (lane & (LPK / 4) ? 2 : 0) + (lane & (LPK / 8) ? 1 : 0);
+    const int my_key = my_it * KPI + sub;
+
+    Run run(a, pre);
+    Segment sg;
+    while (run.next(a, pre, &sg)) {
+        const int r = sg.r, heads = sg.heads, qh0 = sg.qh0, t0 = sg.t0, t1 = sg.t1;
+        const RowView rv = sg.rv;
+        const int32_t *pages = a.c.table + r * a.c.table_stride;
+        const char *kb = a.c.k + sg.kvh * a.c.head_stride, *vb = a.c.v + sg.kvh * a.c.head_stride;
+
+        float q[GP][EPL], acc[GP][EPL], m[GP], l[GP];
+#pragma unroll
+        for (int g = 0; g < GP; g++) {
+            m[g] = -INFINITY;
+            l[g] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < EPL; e++) {
+                const int d = (e / EPC * LPK + chunk) * EPC + e % EPC;
+                q[g][e] = g < heads && d < a.dim
+                              ? load_as_f32(a.q, a.q_type, r * a.q_stride + (long long)(qh0 + g) * a.dim + d)
+                              : 0.0f;
+                acc[g][e] = 0.0f;
+            }
+        }
+        bool bad = false;
+
+        auto key_offset = [&](int tile) -> int64_t {  // of index `lane` of the warp's tile
+            const int i = (tile * ATTN_WARPS + warp) * KEYS + lane;
+            if (lane >= KEYS || i >= rv.vis || tile >= t1) return -1;
+            const int64_t o = a.c.offset(pages, (uint32_t)(i < rv.ref ? i : i + rv.gap));
+            bad |= o < 0;
+            return o;
+        };
+        auto issue = [&](int stage, int64_t mine) {
+            const uint32_t dst = ring_s + stage * 2 * S::HALF + lane * 16;
+#pragma unroll
+            for (int it = 0; it < ITS; it++) {
+                const int64_t o = __shfl_sync(0xffffffffu, mine, it * KPI + sub);
+#pragma unroll
+                for (int n = 0; n < NC; n++) {
+                    const int b = (n * LPK + chunk) * 16;
+                    const bool have = o >= 0 && b < a.c.row_bytes;
+                    const int64_t src = have ? o + b : 0;
+                    cp_async16(dst + (it * NC + n) * 512, kb + src, have ? 16 : 0);
+                    cp_async16(dst + S::HALF + (it * NC + n) * 512, vb + src, have ? 16 : 0);
+                }
+            }
+        };
+#pragma unroll
+        for (int s = 0; s < S::STAGES; s++) {
+            issue(s, key_offset(t0 + s));
+            cp_async_commit();
+        }
+        int stage = 0;
+        for (int tile = t0; tile < t1; tile++) {
+            const int64_t next = key_offset(tile + S::STAGES);
+            cp_async_wait<S::STAGES - 1>();
+            __syncwarp();
+            const char *ks = ring + stage * 2 * S::HALF + lane * 16, *vs = ks + S::HALF;
+            // scores: partial dots of every step, then each lane's own key
+            float s[GP][ITS];
+#pragma unroll
+            for (int it = 0; it < ITS; it++) {
+                float kf[EPL];
+#pragma unroll
+                for (int n = 0; n < NC; n++)
+                    unpack16<T>(*reinterpret_cast<const uint4 *>(ks + (it * NC + n) * 512), kf + n * EPC);
+#pragma unroll
+                for (int g = 0; g < GP; g++) {
+                    float d = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < EPL; e++) d = __fmaf_rn(q[g][e], kf[e], d);
+                    s[g][it] = d;
+                }
+            }
+            const int i = (tile * ATTN_WARPS + warp) * KEYS + my_key;
+            const bool live = i < rv.vis;
+#pragma unroll
+            for (int g = 0; g < GP; g++) {
+                // transposing reduction: 8 values over LPK lanes leave one a lane
+#pragma unroll
+                for (int half = 4; half > 0; half >>= 1) {
+                    const int o = LPK * half / 8;
+                    const bool up = lane & o;
+#pragma unroll
+                    for (int x = 0; x < half; x++) {
+                        const float give = up ? s[g][x] : s[g][x + half];
+                        const float keep = up ? s[g][x + half] : s[g][x];
+                        s[g][x] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+                    }
+                }
+#pragma unroll
+                for (int o = LPK / 16; o > 0; o >>= 1) s[g][0] += __shfl_xor_sync(0xffffffffu, s[g][0], o);
+                const float sc = live ? s[g][0] : -INFINITY;
+                if (__any_sync(0xffffffffu, sc > m[g])) {
+                    const float top = fmaxf(m[g], warp_max_f32(sc));
+                    const float f = prob(m[g], a.c2, scaled_max(top, a.c2));
+                    m[g] = top;
+                    l[g] *= f;
+#pragma unroll
+                    for (int e = 0; e < EPL; e++) acc[g][e] *= f;
+                }
+                const float p = prob(sc, a.c2, scaled_max(m[g], a.c2));
+                l[g] += p;
+                probs[g * KEYS + sub * ITS + my_it] = p;
+                if (a.scores && live && g < heads)
+                    a.scores[((int64_t)r * a.q_heads + qh0 + g) * a.width + i] = sc;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int it = 0; it < ITS; it++) {
+                float vf[EPL];
+#pragma unroll
+                for (int n = 0; n < NC; n++)
+                    unpack16<T>(*reinterpret_cast<const uint4 *>(vs + (it * NC + n) * 512), vf + n * EPC);
+#pragma unroll
+                for (int g = 0; g < GP; g++) {
+                    const float p = probs[g * KEYS + sub * ITS + it];
+#pragma unroll
+                    for (int e = 0; e < EPL; e++) acc[g][e] = __fmaf_rn(p, vf[e], acc[g][e]);
+                }
+            }
+            __syncwarp();
+            issue(stage, next);
+            cp_async_commit();
+            stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+        }
+        cp_async_wait<0>();
+
+        // the warp's sums over its lanes, then the block's over its warps,
+        // through the rings (no copy is in flight)
+        const bool any_bad = __any_sync(0xffffffffu, bad);
+        __syncwarp();
+        float *mine = reinterpret_cast<float *>(ring);  // [GP][D], then m[GP], l[GP]
+#pragma unroll
+        for (int g = 0; g < GP; g++) {
+            float lsum = l[g];
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, o);
+            lsum *= 8.0f / LPK;  // LPK / 8 lanes hold the same key
+#pragma unroll
+            for (int e = 0; e < EPL; e++) {
+                float x = acc[g][e];
+#pragma unroll
+                for (int o = LPK; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+                if (sub == 0) mine[g * D + (e / EPC * LPK + chunk) * EPC + e % EPC] = x;
+            }
+            if (lane == 0) {
+                mine[GP * D + g] = m[g];
+                mine[GP * D + GP + g] = any_bad ? NAN : lsum;
+            }
+        }
+        __syncthreads();
+        finish_segment<GP, D>(a, sg, reinterpret_cast<const float *>(smem), S::STAGES * 2 * S::HALF / 4);
+        __syncthreads();
+    }
+}
+
+template <typename T, int D, int GP> int launch_simt(AttnArgs &a, cudaStream_t st) {
+    constexpr int smem = simt_smem<T, D, GP>();
+    FOCR_CUDA_TRY(set_max_dynamic_smem((const void *)paged_attention_kernel<T, D, GP>, smem));
+    a.gp = GP;
+    a.head_chunks = (a.group + GP - 1) / GP;
+    a.tile_shift = ilog2(Tile<T, D>::BLOCK);
+    FOCR_CUDA_TRY(launch_pdl(paged_attention_kernel<T, D, GP>, attn_blocks(), ATTN_WARPS * 32, smem, st, a));
+    return FOCR_OK;
+}
+
+// 1, 2, 4 or 8 query heads a block.
+template <typename T, int D> int launch_simt_group(AttnArgs &a, cudaStream_t st) {
+    if (a.group <= 1) return launch_simt<T, D, 1>(a, st);
+    if (a.group <= 2) return launch_simt<T, D, 2>(a, st);
+    if (a.group <= 4) return launch_simt<T, D, 4>(a, st);
+    return launch_simt<T, D, 8>(a, st);
+}
+template <typename T> int launch_simt_dim(AttnArgs &a, cudaStream_t st) {
+    if (a.dim <= 64) return launch_simt_group<T, 64>(a, st);
+    if (a.dim <= 128) return launch_simt_group<T, 128>(a, st);
+    return launch_simt_group<T, 256>(a, st);
+}
+
+}  // namespace
+}  // namespace focr

@@ -18,13 +18,18 @@ and can be captured into a CUDA graph.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
+import struct
 
 import torch
 
-from ._lib import F32, F16, BF16, PagedCache, check, lib
+from ._lib import F32, F16, BF16, FOCR_OK, PagedCache, check, lib
 
 _TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+# a PagedCache's bytes: packing them costs a third of filling the ctypes structure
+_PACK = struct.Struct("6N5Ii")
+assert _PACK.size == C.sizeof(PagedCache)
 
 
 def _dtype(ctx: str, name: str, t) -> int:
@@ -47,7 +52,7 @@ def _need(ctx: str, name: str, t, dtype, shape, device) -> None:
 
 
 def _cache(ctx: str, k_pages, v_pages, table, dims: int = 4):
-    """The checked cache as the C ABI's struct, and the device it is on."""
+    """The checked cache as the C ABI's struct; its device, kv heads, head_dim and table's shape."""
     device = k_pages.device
     if device.type != "cuda":
         raise ValueError(f"{ctx}: the pages must be CUDA tensors, not on {device}")
@@ -66,25 +71,32 @@ def _cache(ctx: str, k_pages, v_pages, table, dims: int = 4):
     if table.dim() != 2 or table.stride(1) != 1 or table.device != device:
         raise ValueError(f"{ctx}: table must be [rows, pages] on {device} with contiguous rows")
     rows, width = table.shape
-    return PagedCache(k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), stride[-4], stride[-3],
-                      max(table.stride(0), width), pages, heads, page, dim, width, code), device
+    try:
+        packed = _PACK.pack(k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), stride[-4], stride[-3],
+                            max(table.stride(0), width), pages, heads, page, dim, width, code)
+    except struct.error as e:
+        raise ValueError(f"{ctx}: a dimension exceeds 32 bits") from e
+    return packed, device, heads, dim, rows, width
 
 
-class _On:
-    """Makes `device` the current one for a call; a call on the current device
-    pays one comparison."""
+def _call(fn, device, *args) -> None:
+    """One call of the C ABI on the device's current stream, its last argument."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != FOCR_OK:
+        check(rc)
 
-    def __init__(self, device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+@functools.lru_cache(maxsize=256)
+def _workspace(fn: str, *sizes) -> int:
+    """Bytes of a call's workspace, which go by its sizes alone."""
+    need = C.c_size_t()
+    check(getattr(lib, fn)(*sizes, C.byref(need)))
+    return need.value
 
 
 def _weights(ctx: str, w, rows: int, heads: int, device):
@@ -103,22 +115,20 @@ def paged_write(k, v, k_pages, v_pages, table, pos, row=None) -> None:
     Tokens with ``row[t] < 0`` are padding; rows, positions and pages out of
     range are skipped.  ``pos`` and ``row`` are int32 on the device."""
     ctx = "paged_write"
-    cache, device = _cache(ctx, k_pages, v_pages, table)
+    cache, device, heads, dim, rows, _ = _cache(ctx, k_pages, v_pages, table)
     src = _dtype(ctx, "k", k)
     tokens = k.shape[0]
-    heads, dim = cache.kv_heads, cache.head_dim
-    for name, t in (("k", k), ("v", v)):
-        if t.shape != (tokens, heads, dim) or t.dtype != k.dtype or t.device != device:
-            raise ValueError(f"{ctx}: {name} must be [{tokens}, {heads}, {dim}] of {k.dtype} on {device}")
-        if t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim):
-            raise ValueError(f"{ctx}: a token of {name} must be contiguous")
+    shape, ks, vs = (tokens, heads, dim), k.stride(), v.stride()
+    if k.shape != shape or v.shape != shape or v.dtype != k.dtype or k.device != device or v.device != device:
+        raise ValueError(f"{ctx}: k and v must be [tokens, {heads}, {dim}] of one type on {device}, not "
+                         f"{tuple(k.shape)} of {k.dtype} on {k.device} and {tuple(v.shape)} of {v.dtype} on {v.device}")
+    if ks[2] != 1 or vs[2] != 1 or (heads > 1 and (ks[1] != dim or vs[1] != dim)):
+        raise ValueError(f"{ctx}: a token of k and of v must be contiguous")
     _need(ctx, "pos", pos, torch.int32, (tokens,), device)
     if row is not None:
         _need(ctx, "row", row, torch.int32, (tokens,), device)
-    with _On(device) as stream:
-        check(lib.focr_paged_write(C.byref(cache), table.shape[0], k.data_ptr(), v.data_ptr(), src, tokens,
-                                   k.stride(0), v.stride(0), None if row is None else row.data_ptr(),
-                                   pos.data_ptr(), stream))
+    _call(lib.focr_paged_write, device, cache, rows, k.data_ptr(), v.data_ptr(), src, tokens, ks[0], vs[0],
+          None if row is None else row.data_ptr(), pos.data_ptr())
 
 
 def paged_attention(q, k_pages, v_pages, table, lens, *, scale: float | None = None, ref_lens=None,
@@ -134,14 +144,14 @@ def paged_attention(q, k_pages, v_pages, table, lens, *, scale: float | None = N
     A row that sees nothing gives zeros.  A length past the table (or the
     weights), or a page id outside the pool, gives NaN for that row."""
     ctx = "paged_attention"
-    cache, device = _cache(ctx, k_pages, v_pages, table)
+    cache, device, kv_heads, dim, rows, _ = _cache(ctx, k_pages, v_pages, table)
     code = _dtype(ctx, "q", q)
-    rows, dim = table.shape[0], cache.head_dim
-    if q.dim() != 3 or q.shape[0] != rows or q.shape[2] != dim or q.device != device:
+    shape, stride = q.shape, q.stride()
+    if len(shape) != 3 or shape[0] != rows or shape[2] != dim or q.device != device:
         raise ValueError(f"{ctx}: q must be [{rows}, q_heads, {dim}] on {device}, "
-                         f"not {tuple(q.shape)} on {q.device}")
-    heads = q.shape[1]
-    if q.stride(2) != 1 or (heads > 1 and q.stride(1) != dim):
+                         f"not {tuple(shape)} on {q.device}")
+    heads = shape[1]
+    if stride[2] != 1 or (heads > 1 and stride[1] != dim):
         raise ValueError(f"{ctx}: a row of q must be contiguous")
     if window < 0:
         raise ValueError(f"{ctx}: window must not be negative")
@@ -150,22 +160,18 @@ def paged_attention(q, k_pages, v_pages, table, lens, *, scale: float | None = N
         _need(ctx, "ref_lens", ref_lens, torch.int32, (rows,), device)
     width = w_row = w_head = 0
     if weights is not None:
-        _weights(ctx, weights, rows, cache.kv_heads, device)
+        _weights(ctx, weights, rows, kv_heads, device)
         width, w_row, w_head = weights.shape[2], weights.stride(0), weights.stride(1)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        out = torch.empty(shape, dtype=q.dtype, device=device)
     else:
-        _need(ctx, "out", out, q.dtype, q.shape, device)
-    need = C.c_size_t()
-    check(lib.focr_paged_attention_workspace(rows, heads, dim, width, C.byref(need)))
-    with _On(device) as stream:
-        ws = torch.empty(need.value, dtype=torch.uint8, device=device)
-        check(lib.focr_paged_attention(
-            C.byref(cache), q.data_ptr(), code, rows, heads, q.stride(0), lens.data_ptr(),
-            None if ref_lens is None else ref_lens.data_ptr(), window,
-            1.0 / math.sqrt(dim) if scale is None else scale, out.data_ptr(), heads * dim,
-            None if weights is None else weights.data_ptr(), width, w_row, w_head, ws.data_ptr(),
-            need.value, stream))
+        _need(ctx, "out", out, q.dtype, shape, device)
+    need = _workspace("focr_paged_attention_workspace", rows, heads, dim, width)
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    _call(lib.focr_paged_attention, device, cache, q.data_ptr(), code, rows, heads, stride[0], lens.data_ptr(),
+          None if ref_lens is None else ref_lens.data_ptr(), window,
+          1.0 / math.sqrt(dim) if scale is None else scale, out.data_ptr(), heads * dim,
+          None if weights is None else weights.data_ptr(), width, w_row, w_head, ws.data_ptr(), need)
     return out
 
 
@@ -182,8 +188,7 @@ def paged_evict(k_pages, v_pages, table, lens, weights, new_table, budget: int, 
     budget]`` (-1 behind the last), the new lengths, and the kept entries'
     weights in a tensor of ``weights``' shape, 0 behind them."""
     ctx = "paged_evict"
-    cache, device = _cache(ctx, k_pages, v_pages, table)
-    rows, heads = table.shape[0], cache.kv_heads
+    cache, device, heads, _, rows, _ = _cache(ctx, k_pages, v_pages, table)
     _need(ctx, "lens", lens, torch.int32, (rows,), device)
     _weights(ctx, weights, rows, heads, device)
     if new_table.dtype != torch.int32:
@@ -197,10 +202,7 @@ def paged_evict(k_pages, v_pages, table, lens, weights, new_table, budget: int, 
     kept = torch.empty((rows, heads, budget), dtype=torch.int32, device=device)
     new_lens = torch.empty((rows,), dtype=torch.int32, device=device)
     new_weights = torch.empty((rows, heads, width), dtype=torch.float32, device=device)
-    with _On(device) as stream:
-        check(lib.focr_paged_evict(
-            C.byref(cache), rows, lens.data_ptr(), weights.data_ptr(), width, weights.stride(0),
-            weights.stride(1), new_table.data_ptr(), max(new_table.stride(0), new_table.shape[1]),
-            new_table.shape[1], budget, sink, recent, kept.data_ptr(), new_lens.data_ptr(),
-            new_weights.data_ptr(), stream))
+    _call(lib.focr_paged_evict, device, cache, rows, lens.data_ptr(), weights.data_ptr(), width, weights.stride(0),
+          weights.stride(1), new_table.data_ptr(), max(new_table.stride(0), new_table.shape[1]),
+          new_table.shape[1], budget, sink, recent, kept.data_ptr(), new_lens.data_ptr(), new_weights.data_ptr())
     return kept, new_lens, new_weights
