@@ -17,10 +17,9 @@
 namespace focr {
 namespace {
 
-constexpr int ST = 256;              // threads of both kernels
-constexpr int PER = 32;              // logits a thread of a strip
-constexpr int STRIP = ST * PER;
+constexpr int ST = 256;    // threads of both kernels
 constexpr int MAX_N = 64;
+constexpr int LIST = 1024; // candidates ranked together
 
 struct SelectArgs {
     const void *x;
@@ -37,87 +36,203 @@ struct SelectArgs {
     double *ps;
 };
 
-// Order-preserving bits of a logit; NaN and -inf are no candidates (0), +inf
-// counts as the largest finite value.
-__device__ __forceinline__ uint32_t logit_key(float x) {
-    if (!(x > -INFINITY)) return 0;
-    const uint32_t b = __float_as_uint(fminf(x, 3.402823466e38f) + 0.0f);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float key_logit(uint32_t k) {
-    return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
-}
+// Threads of a group: 4 groups for each of n choices, 32 at least and 256 at most.
+__device__ __forceinline__ int group_lanes(int n) { return n <= 8 ? 8 : n <= 16 ? 4 : n <= 32 ? 2 : 1; }
 
-__device__ __forceinline__ uint64_t warp_max_u64(uint64_t v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const uint64_t w = __shfl_xor_sync(0xffffffffu, v, o);
-        v = w > v ? w : v;
-    }
-    return v;
-}
-
-// The strip's largest key below `below`, over the block.
-__device__ uint64_t block_max_u64(uint64_t v, uint64_t *sh) {
-    v = warp_max_u64(v);
-    __syncthreads();
+__device__ __forceinline__ float block_max_f32(float v, float *sh) {
+    v = warp_max_f32(v);
     if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
     __syncthreads();
-    uint64_t m = sh[0];
+    float m = sh[0];
 #pragma unroll
-    for (int w = 1; w < ST / 32; w++) m = sh[w] > m ? sh[w] : m;
+    for (int w = 1; w < ST / 32; w++) m = fmaxf(m, sh[w]);
     return m;
 }
 
-template <typename T>
+// A logit as a candidate: NaN becomes -inf (none), +inf the largest finite f32.
+__device__ __forceinline__ float clean(float x) { return x > -INFINITY ? fminf(x, 3.402823466e38f) : -INFINITY; }
+
+// 2^(x log2 e - base) to a rounding, for x that is at most some units above
+// base / log2 e.  Cody and Waite's reduction with log2 e in two parts, then the
+// Taylor polynomial of 2^r, |r| <= 1/2, to the 7th power (2^-27).
+__device__ __forceinline__ float exp_below(float x, float base) {
+    const float n = rintf(__fmul_rn(x, 1.44269502f));
+    float r = __fmaf_rn(x, 1.44269502f, -n);
+    r = __fmaf_rn(x, 1.92596299e-8f, r);
+    float p = 1.52527338e-5f;
+    p = __fmaf_rn(p, r, 1.54035304e-4f);
+    p = __fmaf_rn(p, r, 1.33335581e-3f);
+    p = __fmaf_rn(p, r, 9.61812911e-3f);
+    p = __fmaf_rn(p, r, 5.55041087e-2f);
+    p = __fmaf_rn(p, r, 2.40226507e-1f);
+    p = __fmaf_rn(p, r, 6.93147181e-1f);
+    p = __fmaf_rn(p, r, 1.0f);
+    const float e = n - base;
+    return e < -100.0f ? 0.0f : __int_as_float(__float_as_int(p) + ((int)e << 23));
+}
+
+// One strip of one row's logits, held in registers (PER a thread, read once, 16
+// bytes at a time but for the strip's ragged ends): its largest logit, its sum
+// of exponentials and its n largest candidates.
+//
+// The sum: terms above e^-4 of the largest are few and go through the 64-bit
+// exponential; the others' rounding to f32 then moves the sum by less than
+// 2^-24 e^-4 each, and not in one direction.  All of them in 64 bits cost 3 times
+// the strip's load.
+//
+// The n largest: at least n logits reach the n-th largest of the maxima of 2n or
+// more groups of threads, and hardly more do; these are collected and ranked by
+// counting.
+// Where too many reach it (a constant row), the n are taken one by one.
+template <typename T, int PER>
 __global__ void __launch_bounds__(ST) select_part_kernel(const SelectArgs a) {
-    __shared__ uint64_t sh[ST / 32];
+    constexpr int V = 16 / (int)sizeof(T), STRIP = ST * PER;
+    __shared__ __align__(16) float tops[ST];
+    __shared__ float sh[ST / 32], lx[LIST];
+    __shared__ int lt[LIST], count;
+    __shared__ float bound;
     __shared__ double shd[ST / 32];
+    const int strip = blockIdx.x, row = blockIdx.y, t = threadIdx.x;
     pdl_wait();
     pdl_trigger();
-    const int strip = blockIdx.x, row = blockIdx.y, t = threadIdx.x;
     const T *x = static_cast<const T *>(a.x) + row * a.row_stride;
-    const int first = strip * STRIP;
-    uint32_t key[PER];
-    uint32_t top = 0;
+    // elements before the row's first 16-byte boundary shift the strips down
+    const int skew = (int)((uintptr_t)x % 16 / sizeof(T));
+    const int first = strip * STRIP - skew;
+    float v[PER];
+    float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const int c = first + i * ST + t;
-        key[i] = c < a.vocab ? logit_key(to_f32<T>(x[c])) : 0;
-        top = max(top, key[i]);
+    for (int i = 0; i < PER / V; i++) {
+        const int c = first + (i * ST + t) * V;
+        if (c >= 0 && c + V <= a.vocab) {
+            unpack16<T>(*reinterpret_cast<const uint4 *>(x + c), v + i * V);
+#pragma unroll
+            for (int e = 0; e < V; e++) v[i * V + e] = clean(v[i * V + e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; e++)
+                v[i * V + e] = c + e >= 0 && c + e < a.vocab ? clean(to_f32<T>(x[c + e])) : -INFINITY;
+        }
     }
-    const uint32_t m = (uint32_t)block_max_u64(top, sh);
-    const double mx = key_logit(m);
-    double sum = 0.0;
-    if (m)
-#pragma unroll 1
-        for (int i = 0; i < PER; i++)
-            if (key[i]) sum += exp((double)key_logit(key[i]) - mx);
+    auto token = [&](int i) { return first + (i / V * ST + t) * V + i % V; };
+#pragma unroll
+    for (int i = 0; i < PER; i++) top = fmaxf(top, v[i]);
+    const int lanes = group_lanes(a.n), groups = ST / lanes;
+    for (int o = 1; o < lanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (t % lanes == 0) tops[t / lanes] = top;
+    if (t == 0) {
+        count = 0;
+        bound = -INFINITY;
+    }
+    const float m = block_max_f32(top, sh);
+    const long long at = (long long)row * a.strips + strip;
+    if (m == -INFINITY) {
+        for (int k = t; k < a.n; k += ST) a.ct[at * a.n + k] = -1;
+        if (t == 0) {
+            a.pm[at] = m;
+            a.ps[at] = 0.0;
+        }
+        return;
+    }
+    if (t < groups) {  // the group whose maximum ranks n-th names the bound
+        const float mine = tops[t];
+        int rank = 0;
+        for (int j = 0; j < groups; j += 4) {
+            const float4 o = *reinterpret_cast<const float4 *>(tops + j);
+            rank += (o.x > mine || (o.x == mine && j < t)) + (o.y > mine || (o.y == mine && j + 1 < t)) +
+                    (o.z > mine || (o.z == mine && j + 2 < t)) + (o.w > mine || (o.w == mine && j + 3 < t));
+        }
+        if (rank == a.n - 1) bound = mine;
+    }
+    // far from 0 the differences to the maximum are exact and stay small
+    const float zero = fabsf(m) >= 1024.0f ? m : 0.0f;
+    const float base = rintf(__fmul_rn(m - zero, 1.44269502f)), near = m - 4.0f;
+    // base counts powers of two below the maximum: undone in 64 bits
+    double sum = 0.0, large = 0.0;
+#pragma unroll
+    for (int i = 0; i < PER; i += 4) {
+        float s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float y = v[i + e];
+            if (y >= near) large += exp((double)y - (double)m);
+            else if (y > -INFINITY) s += exp_below(y - zero, base);
+        }
+        sum += s;
+    }
+    // the small terms were taken relative to 2^base
+    sum = sum * exp(base * 0.693147180559945309 - ((double)m - (double)zero)) + large;
+    __syncthreads();
+    const float low = bound;
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+        if (v[i] >= low && v[i] > -INFINITY) {
+            const int k = atomicAdd(&count, 1);
+            if (k < LIST) {
+                lx[k] = v[i];
+                lt[k] = token(i);
+            }
+        }
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if ((t & 31) == 0) shd[t >> 5] = sum;
     __syncthreads();
-    const long long at = (long long)row * a.strips + strip;
     if (t == 0) {
         for (int w = 1; w < ST / 32; w++) sum += shd[w];
-        a.pm[at] = m ? key_logit(m) : -INFINITY;
+        a.pm[at] = m;
         a.ps[at] = sum;
     }
-    // the n largest, one after the other: (key, ~token) as one number
-    uint64_t below = ~0ull;
-    for (int k = 0; k < a.n; k++) {
-        uint64_t best = 0;
+    const int got = count;
+    if (got <= LIST) {
+        for (int i = t; i < got; i += ST) {
+            const float y = lx[i];
+            const int c = lt[i];
+            int rank = 0;
+            for (int j = 0; j < got; j++) rank += lx[j] > y || (lx[j] == y && lt[j] < c);
+            if (rank < a.n) {
+                a.cx[at * a.n + rank] = y;
+                a.ct[at * a.n + rank] = c;
+            }
+        }
+        for (int k = got + t; k < a.n; k += ST) a.ct[at * a.n + k] = -1;
+        return;
+    }
+    float last = INFINITY;
+    int last_token = -1;
+    for (int k = 0; k < a.n; k++) {  // LIST > n: there are that many
+        float y = -INFINITY;
+        int c = INT_MAX;
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const uint64_t v = (uint64_t)key[i] << 32 | (uint32_t)~(first + i * ST + t);
-            if (key[i] && v < below && v > best) best = v;
+        for (int i = 0; i < PER; i++)
+            if (v[i] < last || (v[i] == last && token(i) > last_token))
+                if (v[i] > y || (v[i] == y && token(i) < c)) {
+                    y = v[i];
+                    c = token(i);
+                }
+        for (int o = 16; o > 0; o >>= 1) {
+            const float oy = __shfl_xor_sync(0xffffffffu, y, o);
+            const int oc = __shfl_xor_sync(0xffffffffu, c, o);
+            if (oy > y || (oy == y && oc < c)) {
+                y = oy;
+                c = oc;
+            }
         }
-        best = block_max_u64(best, sh);
+        __syncthreads();
+        if ((t & 31) == 0) {
+            lx[t >> 5] = y;
+            lt[t >> 5] = c;
+        }
+        __syncthreads();
+        last = lx[0];
+        last_token = lt[0];
+        for (int w = 1; w < ST / 32; w++)
+            if (lx[w] > last || (lx[w] == last && lt[w] < last_token)) {
+                last = lx[w];
+                last_token = lt[w];
+            }
         if (t == 0) {
-            a.cx[at * a.n + k] = best ? key_logit((uint32_t)(best >> 32)) : -INFINITY;
-            a.ct[at * a.n + k] = best ? (int32_t)~(uint32_t)best : -1;
+            a.cx[at * a.n + k] = last;
+            a.ct[at * a.n + k] = last_token;
         }
-        below = best;
-        if (!best) below = 0;
     }
 }
 
@@ -132,80 +247,147 @@ __device__ __forceinline__ bool before(const Cand &p, const Cand &q) {  // p ran
     if (p.x != q.x) return p.x > q.x;
     return p.token < q.token;
 }
+__device__ __forceinline__ Cand no_cand() { return Cand{-INFINITY, -INFINITY, INT_MAX, INT_MAX}; }
 
+// A block per entry: the rows' sums, then the n best of all strips' candidates, in
+// the same way as the strips' own.
 __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
-    __shared__ double lse_m[MAX_N], lse_s[MAX_N];
-    __shared__ Cand best[ST / 32];
+    __shared__ double row_m[MAX_N], row_s[MAX_N];
+    __shared__ float row_cum[MAX_N];
+    __shared__ uint8_t row_done[MAX_N];
+    __shared__ __align__(16) char list_mem[LIST * sizeof(Cand)];
+    __shared__ Cand bound;
+    __shared__ int count;
+    Cand *list = reinterpret_cast<Cand *>(list_mem);
     pdl_wait();
     pdl_trigger();
-    const int b = blockIdx.x, t = threadIdx.x;
-    for (int i = t; i < a.beams; i += ST) {
+    const int b = blockIdx.x, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    for (int i = warp; i < a.beams; i += ST / 32) {
         const long long row = (long long)b * a.beams + i;
         float m = -INFINITY;
-        for (int s = 0; s < a.strips; s++) m = fmaxf(m, a.pm[row * a.strips + s]);
+        for (int s = lane; s < a.strips; s += 32) m = fmaxf(m, a.pm[row * a.strips + s]);
+        m = warp_max_f32(m);
         double sum = 0.0;
-        for (int s = 0; s < a.strips; s++) {
+        for (int s = lane; s < a.strips; s += 32) {
             const float p = a.pm[row * a.strips + s];
             if (p > -INFINITY) sum += a.ps[row * a.strips + s] * exp((double)p - (double)m);
         }
-        lse_m[i] = m;
-        lse_s[i] = log(sum);
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) {
+            row_m[i] = m;
+            row_s[i] = log(sum);
+            row_cum[i] = a.cum[row];
+            row_done[i] = a.done ? a.done[row] : 0;
+        }
+    }
+    if (t == 0) {
+        count = 0;
+        bound = no_cand();
     }
     __syncthreads();
     const int per = a.strips * a.n, total = a.beams * per;
+    const long long at = (long long)b * total;
+    auto cand = [&](int j) {
+        const int beam = j / per, rest = j - beam * per;
+        const float cum = row_cum[beam];
+        Cand c = no_cand();
+        if (!isfinite(cum)) return c;
+        if (row_done[beam]) {
+            if (rest == 0) c = Cand{cum, 0.0f, beam, a.end_token};
+            return c;
+        }
+        const int token = a.ct[at + j];
+        if (token < 0) return c;
+        const float x = a.cx[at + j];
+        return Cand{(double)cum + (((double)x - row_m[beam]) - row_s[beam]), x, beam, token};
+    };
+    Cand mine = no_cand();
+    for (int j = t; j < total; j += ST) {
+        const Cand c = cand(j);
+        if (before(c, mine)) mine = c;
+    }
+    auto other = [](const Cand &c, int o) {
+        Cand d;
+        d.score = __shfl_xor_sync(0xffffffffu, c.score, o);
+        d.x = __shfl_xor_sync(0xffffffffu, c.x, o);
+        d.beam = __shfl_xor_sync(0xffffffffu, c.beam, o);
+        d.token = __shfl_xor_sync(0xffffffffu, c.token, o);
+        return d;
+    };
+    const int lanes = group_lanes(a.n), groups = ST / lanes;
+    for (int off = 1; off < lanes; off <<= 1) {
+        const Cand c = other(mine, off);
+        if (before(c, mine)) mine = c;
+    }
+    if (t % lanes == 0) list[t / lanes] = mine;
+    __syncthreads();
+    if (t < groups) {
+        const Cand c = list[t];
+        int rank = 0;
+        for (int j = 0; j < groups; j++) rank += before(list[j], c) || (j < t && !before(c, list[j]));
+        if (rank == a.n - 1) bound = c;
+    }
+    __syncthreads();
+    const Cand low = bound;
+    for (int j = t; j < total; j += ST) {
+        const Cand c = cand(j);
+        if (c.beam != INT_MAX && !before(low, c)) {
+            const int k = atomicAdd(&count, 1);
+            if (k < LIST) list[k] = c;
+        }
+    }
+    __syncthreads();
+    const int got = count;
+    const long long o = (long long)b * a.n;
+    auto put = [&](int k, const Cand &c) {
+        a.score_out[o + k] = c.beam == INT_MAX ? -INFINITY : (float)c.score;
+        a.parent_out[o + k] = c.beam == INT_MAX ? -1 : c.beam;
+        a.token_out[o + k] = c.beam == INT_MAX ? -1 : c.token;
+    };
+    if (got <= LIST) {
+        for (int i = t; i < got; i += ST) {
+            const Cand c = list[i];
+            int rank = 0;
+            for (int j = 0; j < got; j++) rank += before(list[j], c);
+            if (rank < a.n) put(rank, c);
+        }
+        for (int k = got + t; k < a.n; k += ST) put(k, no_cand());
+        return;
+    }
     Cand last{INFINITY, INFINITY, -1, -1};
     for (int k = 0; k < a.n; k++) {
-        Cand mine{-INFINITY, -INFINITY, INT_MAX, INT_MAX};
+        mine = no_cand();
         for (int j = t; j < total; j += ST) {
-            const int beam = j / per, rest = j - beam * per;
-            const long long row = (long long)b * a.beams + beam;
-            const float cum = a.cum[row];
-            if (!isfinite(cum)) continue;
-            Cand c;
-            c.beam = beam;
-            if (a.done && a.done[row]) {
-                if (rest) continue;
-                c.score = cum;
-                c.x = 0.0f;
-                c.token = a.end_token;
-            } else {
-                c.x = a.cx[row * per + rest];
-                c.token = a.ct[row * per + rest];
-                if (c.token < 0) continue;
-                c.score = (double)cum + (((double)c.x - lse_m[beam]) - lse_s[beam]);
-            }
-            if ((k == 0 || before(last, c)) && before(c, mine)) mine = c;
+            const Cand c = cand(j);
+            if (before(last, c) && before(c, mine)) mine = c;
         }
-        for (int o = 16; o > 0; o >>= 1) {
-            Cand c;
-            c.score = __shfl_xor_sync(0xffffffffu, mine.score, o);
-            c.x = __shfl_xor_sync(0xffffffffu, mine.x, o);
-            c.beam = __shfl_xor_sync(0xffffffffu, mine.beam, o);
-            c.token = __shfl_xor_sync(0xffffffffu, mine.token, o);
+        for (int off = 16; off > 0; off >>= 1) {
+            const Cand c = other(mine, off);
             if (before(c, mine)) mine = c;
         }
         __syncthreads();
-        if ((t & 31) == 0) best[t >> 5] = mine;
+        if (lane == 0) list[warp] = mine;
         __syncthreads();
-        last = best[0];
+        last = list[0];
         for (int w = 1; w < ST / 32; w++)
-            if (before(best[w], last)) last = best[w];
-        if (t == 0) {
-            const bool have = last.beam != INT_MAX;
-            const long long o = (long long)b * a.n + k;
-            a.score_out[o] = have ? (float)last.score : -INFINITY;
-            a.parent_out[o] = have ? last.beam : -1;
-            a.token_out[o] = have ? last.token : -1;
-        }
+            if (before(list[w], last)) last = list[w];
+        if (t == 0) put(k, last);
     }
 }
+
+// Logits a thread holds: with few rows, short strips spread them over the SMs.
+int strip_of(size_t rows, size_t vocab) {
+    return rows * ((vocab + ST * 32) / (ST * 32)) < (size_t)num_sms() * 2 ? ST * 8 : ST * 32;
+}
+// Strips of a row of any alignment (up to 7 elements of skew).
+size_t strip_count(size_t vocab, int strip) { return (vocab + 7 + strip - 1) / strip; }
 
 struct SelectSizes {
     size_t cx, ct, pm, ps, total;
 };
 SelectSizes select_sizes(size_t rows, size_t vocab, size_t n) {
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
-    const size_t parts = rows * ((vocab + STRIP - 1) / STRIP);
+    const size_t parts = rows * strip_count(vocab, strip_of(rows, vocab));
     SelectSizes s;
     s.cx = up(parts * n * 4);
     s.ct = up(parts * n * 4);
@@ -239,35 +421,57 @@ __device__ __forceinline__ int reorder_len(const ReorderArgs &a, int src) {
 
 // A block per (row, layer and kv head): the partly filled page's slots, and the
 // weights; the blocks of the first layer and head also write the row's table.
+// Loads are issued in groups ahead of their stores: the copies are short, so
+// their latency is what they cost.
 __global__ void __launch_bounds__(256) beam_reorder_kernel(const ReorderArgs a) {
     pdl_wait();
     pdl_trigger();
     const int i = blockIdx.y, lh = blockIdx.x, t = threadIdx.x;
     const int layer = lh / a.c.kv_heads, h = lh - layer * a.c.kv_heads;
     const int src = reorder_source(a, i), n = reorder_len(a, src);
-    const int full = n / a.c.page_size, rest = n - full * a.c.page_size;
+    const int full = a.c.page_div.div(n), rest = n - full * a.c.page_size;
     const int32_t *pages = a.c.table + (int64_t)(src < 0 ? 0 : src) * a.c.table_stride;
     const int here = a.fresh[i];
+    const int from = rest > 0 ? pages[full] : -1;
     if (lh == 0) {
         for (int j = t; j < a.c.max_pages; j += 256)
             a.table_out[(int64_t)i * a.c.max_pages + j] = j < full ? pages[j] : j == full ? here : -1;
         if (t == 0) a.lens_out[i] = n;
     }
-    if (rest > 0) {
-        const int from = pages[full];
-        if ((uint32_t)from < (uint32_t)a.c.n_pages && (uint32_t)here < (uint32_t)a.c.n_pages) {
-            const int64_t at = layer * a.layer_stride + h * a.c.head_stride;
-            const int64_t s = at + from * a.c.page_stride, d = at + here * a.c.page_stride;
-            for (int x = t; x < rest * (a.c.row_bytes / 16); x += 256) {
-                ((uint4 *)(a.c.k + d))[x] = ((const uint4 *)(a.c.k + s))[x];
-                ((uint4 *)(a.c.v + d))[x] = ((const uint4 *)(a.c.v + s))[x];
-            }
+    if ((uint32_t)from < (uint32_t)a.c.n_pages && (uint32_t)here < (uint32_t)a.c.n_pages) {
+        const int64_t at = layer * a.layer_stride + h * a.c.head_stride;
+        const int64_t s = at + from * a.c.page_stride, d = at + here * a.c.page_stride;
+        const int chunks = rest * (a.c.row_bytes / 16);
+        const uint4 *ks = (const uint4 *)(a.c.k + s), *vs = (const uint4 *)(a.c.v + s);
+        uint4 *kd = (uint4 *)(a.c.k + d), *vd = (uint4 *)(a.c.v + d);
+        for (int x0 = t; x0 < chunks; x0 += 1024) {
+            uint4 k[4], v[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (x0 + u * 256 < chunks) {
+                    k[u] = ks[x0 + u * 256];
+                    v[u] = vs[x0 + u * 256];
+                }
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (x0 + u * 256 < chunks) {
+                    kd[x0 + u * 256] = k[u];
+                    vd[x0 + u * 256] = v[u];
+                }
         }
     }
     if (a.w) {
         const float *w = a.w + layer * a.w_layer + (src < 0 ? 0 : src) * a.w_row + h * a.w_head;
+        const int live = min(n, a.width);
         float *o = a.w_out + layer * a.wo_layer + ((int64_t)i * a.c.kv_heads + h) * a.width;
-        for (int x = t; x < a.width; x += 256) o[x] = x < n ? w[x] : 0.0f;
+        for (int x0 = t; x0 < a.width; x0 += 2048) {
+            float y[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) y[u] = x0 + u * 256 < live ? w[x0 + u * 256] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < 8; u++)
+                if (x0 + u * 256 < a.width) o[x0 + u * 256] = y[u];
+        }
     }
 }
 
@@ -282,7 +486,7 @@ int focr_beam_select_workspace(size_t batch, size_t beams, size_t vocab, size_t 
     return guarded("beam_select_workspace", [&]() -> int {
         if (!bytes) return fail(FOCR_E_ARG, "beam_select_workspace: null pointer");
         size_t rows, x;
-        if (!checked_mul(batch, beams, &rows) || !checked_mul(rows, vocab / STRIP + 1, &x) || n > MAX_N ||
+        if (!checked_mul(batch, beams, &rows) || !checked_mul(rows, vocab / ST + 8, &x) || n > MAX_N ||
             x > SIZE_MAX / 1024)
             return fail(FOCR_E_SHAPE, "beam_select_workspace: size out of range");
         *bytes = select_sizes(rows, vocab, n).total;
@@ -301,7 +505,7 @@ int focr_beam_select(const void *logits, int dtype, size_t batch, size_t beams, 
             return fail(FOCR_E_SHAPE, "beam_select: beams, vocab and n must not be 0");
         if (beams > MAX_N || n > MAX_N)
             return fail(FOCR_E_UNSUPPORTED, "beam_select: beams and n are at most " + std::to_string(MAX_N));
-        if (vocab > (size_t)INT32_MAX - STRIP || batch > (size_t)65535 / beams)
+        if (vocab > (size_t)INT32_MAX - (1 << 20) || batch > (size_t)65535 / beams)
             return fail(FOCR_E_UNSUPPORTED, "beam_select: over 65535 rows, or vocab exceeds int32 range");
         if (batch == 0) return FOCR_OK;
         if (batch * beams > 1 && row_stride < vocab)
@@ -326,7 +530,8 @@ int focr_beam_select(const void *logits, int dtype, size_t batch, size_t beams, 
         a.beams = (int)beams;
         a.vocab = (int)vocab;
         a.n = (int)n;
-        a.strips = (int)((vocab + STRIP - 1) / STRIP);
+        const int strip = strip_of(batch * beams, vocab);
+        a.strips = (int)strip_count(vocab, strip);
         a.end_token = end_token;
         char *ws = (char *)workspace;
         a.ps = (double *)ws;
@@ -335,9 +540,10 @@ int focr_beam_select(const void *logits, int dtype, size_t batch, size_t beams, 
         a.pm = (float *)(ws + sz.ps + sz.cx + sz.ct);
         cudaStream_t st = (cudaStream_t)stream;
         const dim3 grid(a.strips, (unsigned)(batch * beams));
-        auto *part = dtype == FOCR_F32 ? select_part_kernel<float>
-                   : dtype == FOCR_F16 ? select_part_kernel<__half>
-                                       : select_part_kernel<__nv_bfloat16>;
+        const bool few = strip == ST * 8;
+        auto *part = dtype == FOCR_F32 ? (few ? select_part_kernel<float, 8> : select_part_kernel<float, 32>)
+                   : dtype == FOCR_F16 ? (few ? select_part_kernel<__half, 8> : select_part_kernel<__half, 32>)
+                                       : (few ? select_part_kernel<__nv_bfloat16, 8> : select_part_kernel<__nv_bfloat16, 32>);
         FOCR_CUDA_TRY(launch_pdl(part, grid, ST, 0, st, a));
         FOCR_CUDA_TRY(launch_pdl(select_join_kernel, (unsigned)batch, ST, 0, st, a));
         return FOCR_OK;
@@ -361,7 +567,7 @@ int focr_beam_reorder(const focr_paged_cache *cache, size_t layers, size_t layer
         if (!lens || !parent || !fresh || !table_out || !lens_out)
             return fail(FOCR_E_ARG, "beam_reorder: null pointer");
         size_t lh;
-        if (rows > 65535 || !checked_mul(layers, cache->kv_heads, &lh) || lh > INT32_MAX || width > INT32_MAX)
+        if (rows > 65535 || !checked_mul(layers, cache->kv_heads, &lh) || lh > INT32_MAX || width > (1u << 30))
             return fail(FOCR_E_UNSUPPORTED, "beam_reorder: dimension out of range");
         const size_t size = dtype_bytes(cache->dtype);
         if (layers > 1 && (layer_stride < (size_t)cache->page_size * cache->head_dim ||
