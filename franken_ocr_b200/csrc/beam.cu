@@ -29,6 +29,7 @@ struct SelectArgs {
     int32_t *parent_out, *token_out;
     long long row_stride;            // elements between the logits of two beams
     int beams, vocab, n, strips, end_token;
+    FastDiv by_n, by_strips;
     // workspace, per (row, strip): n (logit, token) pairs, (max, sum)
     float *cx;
     int32_t *ct;
@@ -50,68 +51,63 @@ __device__ __forceinline__ float block_max_f32(float v, float *sh) {
 }
 
 // A logit as a candidate: NaN becomes -inf (none), +inf the largest finite f32.
-__device__ __forceinline__ float clean(float x) { return x > -INFINITY ? fminf(x, 3.402823466e38f) : -INFINITY; }
+__device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, -INFINITY), 3.402823466e38f); }
 
-// 2^(x log2 e - base) to a rounding, for x that is at most some units above
-// base / log2 e.  Cody and Waite's reduction with log2 e in two parts, then the
-// Taylor polynomial of 2^r, |r| <= 1/2, to the 7th power (2^-27).
-__device__ __forceinline__ float exp_below(float x, float base) {
-    const float n = rintf(__fmul_rn(x, 1.44269502f));
+// 2^(x log2 e - base) to about one rounding, for x / log2 e between base - 100 and
+// base + 1: Cody and Waite's reduction with log2 e in two parts, and the hardware's
+// 2^r for the rest, |r| <= 1/2.  `base` comes as the bits of SHIFT + base.
+constexpr float SHIFT = 12582912.0f;   // 1.5 * 2^23: adding it rounds to an integer in the low bits
+__device__ __forceinline__ float exp_below(float x, int base) {
+    const float t = __fmaf_rn(x, 1.44269502f, SHIFT), n = t - SHIFT;
     float r = __fmaf_rn(x, 1.44269502f, -n);
     r = __fmaf_rn(x, 1.92596299e-8f, r);
-    float p = 1.52527338e-5f;
-    p = __fmaf_rn(p, r, 1.54035304e-4f);
-    p = __fmaf_rn(p, r, 1.33335581e-3f);
-    p = __fmaf_rn(p, r, 9.61812911e-3f);
-    p = __fmaf_rn(p, r, 5.55041087e-2f);
-    p = __fmaf_rn(p, r, 2.40226507e-1f);
-    p = __fmaf_rn(p, r, 6.93147181e-1f);
-    p = __fmaf_rn(p, r, 1.0f);
-    const float e = n - base;
-    return e < -100.0f ? 0.0f : __int_as_float(__float_as_int(p) + ((int)e << 23));
+    float p;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(r));
+    return __int_as_float(__float_as_int(p) + ((__float_as_int(t) - base) << 23));
 }
 
 // One strip of one row's logits, held in registers (PER a thread, read once, 16
-// bytes at a time but for the strip's ragged ends): its largest logit, its sum
-// of exponentials and its n largest candidates.
+// bytes at a time where the row begins on such a boundary): its largest logit,
+// its sum of exponentials and its n largest candidates.  A thread's logits do
+// not depend on the row's alignment, so equal rows give equal sums.
 //
-// The sum: terms above e^-4 of the largest are few and go through the 64-bit
+// The sum: terms above e^-2.5 of the largest are few and go through the 64-bit
 // exponential; the others' rounding to f32 then moves the sum by less than
-// 2^-24 e^-4 each, and not in one direction.  All of them in 64 bits cost 3 times
-// the strip's load.
+// 2^-22 e^-2.5 each, and not in one direction.  All of them in 64 bits cost several
+// times the strip's load.
 //
 // The n largest: at least n logits reach the n-th largest of the maxima of 2n or
 // more groups of threads, and hardly more do; these are collected and ranked by
 // counting.
 // Where too many reach it (a constant row), the n are taken one by one.
 template <typename T, int PER>
-__global__ void __launch_bounds__(ST) select_part_kernel(const SelectArgs a) {
+__global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) {
     constexpr int V = 16 / (int)sizeof(T), STRIP = ST * PER;
     __shared__ __align__(16) float tops[ST];
-    __shared__ float sh[ST / 32], lx[LIST];
-    __shared__ int lt[LIST], count;
+    __shared__ float sh[ST / 32], lx[LIST], nx[LIST];
+    __shared__ int lt[LIST], count, near_count;
     __shared__ float bound;
     __shared__ double shd[ST / 32];
+    __shared__ long long shl[ST / 32];
     const int strip = blockIdx.x, row = blockIdx.y, t = threadIdx.x;
     pdl_wait();
     pdl_trigger();
     const T *x = static_cast<const T *>(a.x) + row * a.row_stride;
-    // elements before the row's first 16-byte boundary shift the strips down
-    const int skew = (int)((uintptr_t)x % 16 / sizeof(T));
-    const int first = strip * STRIP - skew;
+    const bool vec = (uintptr_t)x % 16 == 0;
+    const int first = strip * STRIP;
     float v[PER];
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < PER / V; i++) {
         const int c = first + (i * ST + t) * V;
-        if (c >= 0 && c + V <= a.vocab) {
+        if (vec && c + V <= a.vocab) {
             unpack16<T>(*reinterpret_cast<const uint4 *>(x + c), v + i * V);
 #pragma unroll
             for (int e = 0; e < V; e++) v[i * V + e] = clean(v[i * V + e]);
         } else {
 #pragma unroll
             for (int e = 0; e < V; e++)
-                v[i * V + e] = c + e >= 0 && c + e < a.vocab ? clean(to_f32<T>(x[c + e])) : -INFINITY;
+                v[i * V + e] = c + e < a.vocab ? clean(to_f32<T>(x[c + e])) : -INFINITY;
         }
     }
     auto token = [&](int i) { return first + (i / V * ST + t) * V + i % V; };
@@ -121,7 +117,7 @@ __global__ void __launch_bounds__(ST) select_part_kernel(const SelectArgs a) {
     for (int o = 1; o < lanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (t % lanes == 0) tops[t / lanes] = top;
     if (t == 0) {
-        count = 0;
+        count = near_count = 0;
         bound = -INFINITY;
     }
     const float m = block_max_f32(top, sh);
@@ -145,55 +141,84 @@ __global__ void __launch_bounds__(ST) select_part_kernel(const SelectArgs a) {
         if (rank == a.n - 1) bound = mine;
     }
     // far from 0 the differences to the maximum are exact and stay small
-    const float zero = fabsf(m) >= 1024.0f ? m : 0.0f;
-    const float base = rintf(__fmul_rn(m - zero, 1.44269502f)), near = m - 4.0f;
-    // base counts powers of two below the maximum: undone in 64 bits
-    double sum = 0.0, large = 0.0;
+    const float zero = fabsf(m) >= 1024.0f ? m : 0.0f, high = m - zero;
+    const float base = rintf(__fmul_rn(high, 1.44269502f)), near = m - 2.5f;
+    const float near0 = near - zero, none = high - 65.0f;   // e^-65 of the largest adds nothing
+    const int base_bits = __float_as_int(SHIFT + base);
+    double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < PER; i += 4) {
         float s = 0.0f;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const float y = v[i + e];
-            if (y >= near) large += exp((double)y - (double)m);
-            else if (y > -INFINITY) s += exp_below(y - zero, base);
+            const float y = fmaxf(v[i + e] - zero, none), x = exp_below(y, base_bits);
+            if (y < near0) s += x;
         }
         sum += s;
     }
     // the small terms were taken relative to 2^base
-    sum = sum * exp(base * 0.693147180559945309 - ((double)m - (double)zero)) + large;
+    sum *= exp((double)base * 0.693147180559945309 - (double)high);
     __syncthreads();
-    const float low = bound;
+    // the few that are large or candidates
+    const float low = bound, few = fminf(low, near);
 #pragma unroll
-    for (int i = 0; i < PER; i++)
-        if (v[i] >= low && v[i] > -INFINITY) {
-            const int k = atomicAdd(&count, 1);
-            if (k < LIST) {
-                lx[k] = v[i];
-                lt[k] = token(i);
+    for (int g = 0; g < PER; g += 4) {
+        if (fmaxf(fmaxf(v[g], v[g + 1]), fmaxf(v[g + 2], v[g + 3])) < few) continue;
+#pragma unroll
+        for (int i = g; i < g + 4; i++) {
+            if (v[i] >= near) {
+                const int k = atomicAdd(&near_count, 1);
+                if (k < LIST) nx[k] = v[i];
+            }
+            if (v[i] >= low && v[i] > -INFINITY) {
+                const int k = atomicAdd(&count, 1);
+                if (k < LIST) {
+                    lx[k] = v[i];
+                    lt[k] = token(i);
+                }
             }
         }
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if ((t & 31) == 0) shd[t >> 5] = sum;
+    }
+    __syncthreads();
+    const int got = count, nears = near_count;
+    // the list's order is chance: a sum of whole multiples of 2^-48 has none
+    long long large = 0;
+    for (int i = t; i < (nears <= LIST ? nears : STRIP); i += ST) {
+        float y = -INFINITY;
+        if (nears <= LIST) y = nx[i];
+        else if (first + i < a.vocab) y = clean(to_f32<T>(x[first + i]));
+        if (y >= near) large += __double2ll_rn(exp((double)y - (double)m) * 0x1p48);
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        large += __shfl_xor_sync(0xffffffffu, large, o);
+    }
+    if ((t & 31) == 0) {
+        shd[t >> 5] = sum;
+        shl[t >> 5] = large;
+    }
     __syncthreads();
     if (t == 0) {
-        for (int w = 1; w < ST / 32; w++) sum += shd[w];
+        for (int w = 1; w < ST / 32; w++) {
+            sum += shd[w];
+            large += shl[w];
+        }
         a.pm[at] = m;
-        a.ps[at] = sum;
+        a.ps[at] = sum + (double)large * 0x1p-48;
     }
-    const int got = count;
     if (got <= LIST) {
         for (int i = t; i < got; i += ST) {
             const float y = lx[i];
             const int c = lt[i];
             int rank = 0;
-            for (int j = 0; j < got; j++) rank += lx[j] > y || (lx[j] == y && lt[j] < c);
+#pragma unroll 4
+            for (int j = 0; j < got; j++) rank += (lx[j] > y) | ((lx[j] == y) & (lt[j] < c));
             if (rank < a.n) {
                 a.cx[at * a.n + rank] = y;
                 a.ct[at * a.n + rank] = c;
             }
         }
-        for (int k = got + t; k < a.n; k += ST) a.ct[at * a.n + k] = -1;
+        for (int k = got + t; k < a.n; k += ST) a.ct[at * a.n + k] = -1;   // fewer than n: all are in the list
         return;
     }
     float last = INFINITY;
@@ -249,26 +274,41 @@ __device__ __forceinline__ bool before(const Cand &p, const Cand &q) {  // p ran
 }
 __device__ __forceinline__ Cand no_cand() { return Cand{-INFINITY, -INFINITY, INT_MAX, INT_MAX}; }
 
-// A block per entry: the rows' sums, then the n best of all strips' candidates, in
-// the same way as the strips' own.
+// A block per entry: the rows' sums, then the n best of all strips' candidates.
+// The n-th best score among the strips' first candidates (a thread takes the best
+// of those it sees) bounds the others; what reaches it is ranked by counting.
 __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
     __shared__ double row_m[MAX_N], row_s[MAX_N];
     __shared__ float row_cum[MAX_N];
     __shared__ uint8_t row_done[MAX_N];
     __shared__ __align__(16) char list_mem[LIST * sizeof(Cand)];
-    __shared__ Cand bound;
+    __shared__ double heads[ST], bound;  // per thread the best of the lists' first; the bound
     __shared__ int count;
     Cand *list = reinterpret_cast<Cand *>(list_mem);
     pdl_wait();
     pdl_trigger();
     const int b = blockIdx.x, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int lists = a.beams * a.strips;
+    const long long at = (long long)b * lists * a.n;
     for (int i = warp; i < a.beams; i += ST / 32) {
         const long long row = (long long)b * a.beams + i;
-        float m = -INFINITY;
-        for (int s = lane; s < a.strips; s += 32) m = fmaxf(m, a.pm[row * a.strips + s]);
+        const float cum = a.cum[row];
+        const uint8_t done = a.done ? a.done[row] : 0;
+        float m = -INFINITY, m2[2];
+        double s2[2], sum = 0.0;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {   // a row's strips are rarely more than 64
+            const int s = u * 32 + lane;
+            m2[u] = s < a.strips ? a.pm[row * a.strips + s] : -INFINITY;
+            s2[u] = s < a.strips ? a.ps[row * a.strips + s] : 0.0;
+            m = fmaxf(m, m2[u]);
+        }
+        for (int s = 64 + lane; s < a.strips; s += 32) m = fmaxf(m, a.pm[row * a.strips + s]);
         m = warp_max_f32(m);
-        double sum = 0.0;
-        for (int s = lane; s < a.strips; s += 32) {
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+            if (m2[u] > -INFINITY) sum += s2[u] * exp((double)m2[u] - (double)m);
+        for (int s = 64 + lane; s < a.strips; s += 32) {
             const float p = a.pm[row * a.strips + s];
             if (p > -INFINITY) sum += a.ps[row * a.strips + s] * exp((double)p - (double)m);
         }
@@ -276,36 +316,25 @@ __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
         if (lane == 0) {
             row_m[i] = m;
             row_s[i] = log(sum);
-            row_cum[i] = a.cum[row];
-            row_done[i] = a.done ? a.done[row] : 0;
+            row_cum[i] = cum;
+            row_done[i] = done;
         }
     }
     if (t == 0) {
         count = 0;
-        bound = no_cand();
+        bound = -INFINITY;
     }
-    __syncthreads();
-    const int per = a.strips * a.n, total = a.beams * per;
-    const long long at = (long long)b * total;
-    auto cand = [&](int j) {
-        const int beam = j / per, rest = j - beam * per;
-        const float cum = row_cum[beam];
-        Cand c = no_cand();
-        if (!isfinite(cum)) return c;
-        if (row_done[beam]) {
-            if (rest == 0) c = Cand{cum, 0.0f, beam, a.end_token};
-            return c;
-        }
-        const int token = a.ct[at + j];
-        if (token < 0) return c;
-        const float x = a.cx[at + j];
+    // the k-th candidate of a list; the first list of an ended beam is its end token
+    auto cand = [&](int l, int beam, int k) {
+        const long long j = at + (long long)l * a.n + k;
+        const int token = a.ct[j];
+        const float x = a.cx[j], cum = row_cum[beam];
+        if (!isfinite(cum)) return no_cand();
+        if (row_done[beam])
+            return k || l != beam * a.strips ? no_cand() : Cand{cum, 0.0f, beam, a.end_token};
+        if (token < 0) return no_cand();
         return Cand{(double)cum + (((double)x - row_m[beam]) - row_s[beam]), x, beam, token};
     };
-    Cand mine = no_cand();
-    for (int j = t; j < total; j += ST) {
-        const Cand c = cand(j);
-        if (before(c, mine)) mine = c;
-    }
     auto other = [](const Cand &c, int o) {
         Cand d;
         d.score = __shfl_xor_sync(0xffffffffu, c.score, o);
@@ -314,26 +343,30 @@ __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
         d.token = __shfl_xor_sync(0xffffffffu, c.token, o);
         return d;
     };
-    const int lanes = group_lanes(a.n), groups = ST / lanes;
-    for (int off = 1; off < lanes; off <<= 1) {
-        const Cand c = other(mine, off);
+    __syncthreads();
+    Cand mine = no_cand();
+    for (int l = t; l < lists; l += ST) {
+        const Cand c = cand(l, (int)a.by_strips.div(l), 0);
         if (before(c, mine)) mine = c;
     }
-    if (t % lanes == 0) list[t / lanes] = mine;
+    heads[t] = mine.score;
     __syncthreads();
-    if (t < groups) {
-        const Cand c = list[t];
+    if (mine.beam != INT_MAX) {
+        const int most = min(lists, ST);
         int rank = 0;
-        for (int j = 0; j < groups; j++) rank += before(list[j], c) || (j < t && !before(c, list[j]));
-        if (rank == a.n - 1) bound = c;
+#pragma unroll 8
+        for (int j = 0; j < most; j++) rank += heads[j] > mine.score || (heads[j] == mine.score && j < t);
+        if (rank == a.n - 1) bound = mine.score;
     }
     __syncthreads();
-    const Cand low = bound;
-    for (int j = t; j < total; j += ST) {
-        const Cand c = cand(j);
-        if (c.beam != INT_MAX && !before(low, c)) {
-            const int k = atomicAdd(&count, 1);
-            if (k < LIST) list[k] = c;
+    const double low = bound;
+#pragma unroll 4
+    for (int j = t; j < lists * a.n; j += ST) {
+        const int l = (int)a.by_n.div(j);
+        const Cand c = cand(l, (int)a.by_strips.div(l), j - l * a.n);
+        if (c.beam != INT_MAX && c.score >= low) {
+            const int i = atomicAdd(&count, 1);
+            if (i < LIST) list[i] = c;
         }
     }
     __syncthreads();
@@ -348,17 +381,19 @@ __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
         for (int i = t; i < got; i += ST) {
             const Cand c = list[i];
             int rank = 0;
+#pragma unroll 4
             for (int j = 0; j < got; j++) rank += before(list[j], c);
             if (rank < a.n) put(rank, c);
         }
         for (int k = got + t; k < a.n; k += ST) put(k, no_cand());
         return;
     }
-    Cand last{INFINITY, INFINITY, -1, -1};
+    Cand last{INFINITY, INFINITY, -1, -1};   // too many ties for the list: one by one
     for (int k = 0; k < a.n; k++) {
         mine = no_cand();
-        for (int j = t; j < total; j += ST) {
-            const Cand c = cand(j);
+        for (int j = t; j < lists * a.n; j += ST) {
+            const int l = (int)a.by_n.div(j);
+            const Cand c = cand(l, (int)a.by_strips.div(l), j - l * a.n);
             if (before(last, c) && before(c, mine)) mine = c;
         }
         for (int off = 16; off > 0; off >>= 1) {
@@ -379,8 +414,7 @@ __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
 int strip_of(size_t rows, size_t vocab) {
     return rows * ((vocab + ST * 32) / (ST * 32)) < (size_t)num_sms() * 2 ? ST * 8 : ST * 32;
 }
-// Strips of a row of any alignment (up to 7 elements of skew).
-size_t strip_count(size_t vocab, int strip) { return (vocab + 7 + strip - 1) / strip; }
+size_t strip_count(size_t vocab, int strip) { return (vocab + strip - 1) / strip; }
 
 struct SelectSizes {
     size_t cx, ct, pm, ps, total;
@@ -533,6 +567,8 @@ int focr_beam_select(const void *logits, int dtype, size_t batch, size_t beams, 
         const int strip = strip_of(batch * beams, vocab);
         a.strips = (int)strip_count(vocab, strip);
         a.end_token = end_token;
+        a.by_n = FastDiv((uint32_t)n);
+        a.by_strips = FastDiv((uint32_t)a.strips);
         char *ws = (char *)workspace;
         a.ps = (double *)ws;
         a.cx = (float *)(ws + sz.ps);

@@ -11,8 +11,6 @@
 // evict_gather_kernel copies their K, V and weights.
 #include <cooperative_groups.h>
 
-#include <algorithm>
-
 #include "paged.cuh"
 
 namespace cg = cooperative_groups;
@@ -20,9 +18,11 @@ namespace cg = cooperative_groups;
 namespace focr {
 namespace {
 
-constexpr int SEL = 1024;              // threads of a select block
+constexpr int SEL = 512;      // threads of a select block
+constexpr int HELD = 40;      // most keys of a thread that shared memory holds
 constexpr int BINS = 2048;
-constexpr int HELD = 40960;            // weights a block keeps in shared memory
+constexpr int MOST = 8;       // blocks of a cluster
+constexpr uint32_t ZERO = 0x80000000u;   // the key of weight 0
 
 // Unsigned integers that order like the weights: -0 equals 0, NaN lies below
 // every number.
@@ -49,15 +49,21 @@ __device__ __forceinline__ int evict_len(const EvictArgs &a, int r) {
     return n < 0 || n > a.width || n > a.c.max_pages * a.c.page_size ? 0 : n;
 }
 
-// One cluster a (row, head): every block takes an equal run of the positions
-// between sink and recent, reads its weights once and keeps their keys.  Three
-// passes of 11, 11 and 10 bits narrow the threshold; the blocks' histograms meet
-// in block 0's shared memory.  It ends early when a whole bin stays.  Then the
-// kept positions of each run are counted, and written behind those of the runs
-// before.
-__global__ void __launch_bounds__(SEL) evict_select_kernel(const EvictArgs a, int held) {
-    extern __shared__ uint32_t keys[];   // held
-    __shared__ int hist[BINS], counts[2], before[2], wsum[2][32], chosen[2];
+// One cluster a (row, head): every warp takes an equal run of the positions
+// between sink and recent, reads its weights once and keeps their keys in shared
+// memory.  Three passes of 11, 11 and 10 bits narrow the threshold, fewer where
+// a whole bin stays; after each the blocks add up a share of the bins each and
+// hand the sums to all.  Then the kept positions of each run are counted, and
+// written behind those of the runs before.
+//
+// The weights are a hundredth of the bytes that the gather moves: instructions and
+// the barriers bound it, so zeros (all that was never looked at) are counted by
+// vote and not one by one, and equal weights are told apart only where the
+// threshold falls among them.
+__global__ void __launch_bounds__(SEL, 2) evict_select_kernel(const EvictArgs a, int held) {
+    extern __shared__ uint32_t keys[];   // [held steps][SEL], a warp's run together
+    __shared__ int hist[BINS], totals[2][BINS];
+    __shared__ int counts[2], before[2], wsum[2][SEL / 32], chosen[2];
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = (int)cluster.block_rank(), size = (int)cluster.num_blocks();
     pdl_wait();
@@ -75,39 +81,75 @@ __global__ void __launch_bounds__(SEL) evict_select_kernel(const EvictArgs a, in
     for (int i = rank * SEL + t; i < a.sink; i += size * SEL) kept[i] = i;
     for (int i = rank * SEL + t; i < a.recent; i += size * SEL) kept[a.sink + want + i] = hi + i;
     if (want == 0) return;   // the same for the whole cluster
-    const int per = (hi - lo + size - 1) / size;
-    const int begin = min(hi, lo + rank * per), end = min(hi, begin + per), m = end - begin;
-    for (int i = t; i < min(m, held); i += SEL) keys[i] = weight_key(w[begin + i]);
-    auto key = [&](int i) { return i < held ? keys[i] : weight_key(w[begin + i]); };
+    // this warp's run: [run, run + 32 steps), of which `mine` are this lane's
+    const int steps = (hi - lo + size * SEL - 1) / (size * SEL);
+    const int run = lo + (rank * (SEL / 32) + warp) * 32 * steps;
+    const int mine = run + lane < hi ? min(steps, (hi - run - lane + 31) >> 5) : 0;
+    w += run + lane;
+    const int near = min(steps, held);
+    uint32_t *own = keys + warp * 32 * near + lane;
+    // f(step, key, whether there is one) for every step, the warp together
+    auto every = [&](auto f) {
+#pragma unroll 4
+        for (int k = 0; k < near; k++) f(k, own[32 * k], k < mine);
+#pragma unroll 1
+        for (int k = near; k < steps; k++) f(k, k < mine ? weight_key(w[32ll * k]) : 0, k < mine);
+    };
 
     uint32_t prefix = 0;
     int left = want, shift = 32;   // `left` of the keys that match `prefix` above `shift` stay
     bool all = false;              // all of them do
-    int *hist0 = cluster.map_shared_rank(hist, 0);
 #pragma unroll 1
     for (int pass = 0; pass < 3 && !all; pass++) {
         const int bits = pass < 2 ? 11 : 10, next = shift - bits;
         for (int i = t; i < BINS; i += SEL) hist[i] = 0;
         __syncthreads();
-        for (int i0 = 0; i0 < m; i0 += SEL) {
-            const int i = i0 + t;
-            const uint32_t k = i < m ? key(i) : 0;
-            const bool in = i < m && (pass == 0 || k >> shift == prefix >> shift);
-            const int bin = in ? (int)(k >> next & ((1u << bits) - 1)) : -1;
-            // many equal weights (all that was never looked at) would queue up
-            int same;
-            __match_all_sync(0xffffffffu, bin, &same);
-            if (same) {
-                if (in && lane == 0) atomicAdd(&hist[bin], 32);
-            } else if (in) {
-                atomicAdd(&hist[bin], 1);
+        int zeros = 0;
+        if (pass == 0) {
+            constexpr int U = 8;
+            for (int k0 = 0; k0 < steps; k0 += U) {
+                float x[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) x[u] = k0 + u < mine ? w[32ll * (k0 + u)] : 0.0f;
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const bool have = k0 + u < mine;
+                    const uint32_t k = weight_key(x[u]);
+                    if (k0 + u < near) own[32 * (k0 + u)] = k;
+                    zeros += __popc(__ballot_sync(0xffffffffu, have && k == ZERO));
+                    if (have && k != ZERO) atomicAdd(&hist[k >> 21], 1);
+                }
             }
+        } else {
+            const uint32_t match = prefix >> shift;
+            const bool with_zero = match == ZERO >> shift;
+            if (with_zero)
+                every([&](int, uint32_t x, bool have) {
+                    zeros += __popc(__ballot_sync(0xffffffffu, have && x == ZERO));
+                    if (have && x >> shift == match && x != ZERO) atomicAdd(&hist[x >> next & ((1u << bits) - 1)], 1);
+                });
+            else
+                every([&](int, uint32_t x, bool have) {
+                    if (have && x >> shift == match) atomicAdd(&hist[x >> next & ((1u << bits) - 1)], 1);
+                });
         }
+        if (lane == 0 && zeros) atomicAdd(&hist[ZERO >> next & ((1u << bits) - 1)], zeros);
+        int *total = hist;
         if (size > 1) {
+            total = totals[pass & 1];   // the other one may still be read
             cluster.sync();
-            if (rank)
-                for (int i = t; i < BINS; i += SEL)
-                    if (hist[i]) atomicAdd(&hist0[i], hist[i]);
+            const int share = BINS / size;
+            for (int i = t; i < share; i += SEL) {
+                const int bin = rank * share + i;
+                int x[MOST], sum = 0;
+#pragma unroll
+                for (int q = 0; q < MOST; q++) x[q] = q < size ? cluster.map_shared_rank(hist, q)[bin] : 0;
+#pragma unroll
+                for (int q = 0; q < MOST; q++) sum += x[q];
+#pragma unroll
+                for (int q = 0; q < MOST; q++)
+                    if (q < size) cluster.map_shared_rank(total, q)[bin] = sum;
+            }
             cluster.sync();
         } else {
             __syncthreads();
@@ -118,7 +160,7 @@ __global__ void __launch_bounds__(SEL) evict_select_kernel(const EvictArgs a, in
         int c[PER], sum = 0;
 #pragma unroll
         for (int i = 0; i < PER; i++) {
-            c[i] = top - i >= 0 ? hist0[top - i] : 0;
+            c[i] = top - i >= 0 ? total[top - i] : 0;
             sum += c[i];
         }
         int inc = sum;
@@ -130,7 +172,8 @@ __global__ void __launch_bounds__(SEL) evict_select_kernel(const EvictArgs a, in
         if (lane == 31) wsum[0][warp] = inc;
         __syncthreads();
         int above = inc - sum;
-        for (int x = 0; x < warp; x++) above += wsum[0][x];
+#pragma unroll
+        for (int x = 0; x < SEL / 32; x++) above += x < warp ? wsum[0][x] : 0;
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             if (above < left && above + c[i] >= left) {
@@ -139,24 +182,21 @@ __global__ void __launch_bounds__(SEL) evict_select_kernel(const EvictArgs a, in
             }
             above += c[i];
         }
-        if (size > 1) cluster.sync();   // block 0's bins have been read
-        else __syncthreads();
+        __syncthreads();
         prefix |= (uint32_t)chosen[0] << next;
         left = chosen[1] & ~(1 << 30);
         all = chosen[1] >> 30;
         shift = next;
         __syncthreads();
     }
-    // larger keys stay, and of the equal ones all or the first `left`.  Each warp
-    // has a run of its own, so the order is the positions'.
-    const uint32_t limit = prefix >> shift;
-    const int each = ((m + SEL - 1) / SEL) * 32, w0 = min(m, warp * each), w1 = min(m, w0 + each);
+    // larger keys stay, and of the equal ones all or the first `left`
+    const uint32_t limit = prefix >> shift, over = all ? limit : limit + 1;
     int larger = 0, equal = 0;
-    for (int i = w0 + lane; i < w1; i += 32) {
-        const uint32_t k = key(i) >> shift;
-        larger += k > limit;
-        equal += k == limit;
-    }
+    every([&](int, uint32_t k, bool have) {
+        const uint32_t x = k >> shift;
+        larger += have && x >= over;
+        equal += have && x == limit;
+    });
     larger = __reduce_add_sync(0xffffffffu, larger);
     equal = __reduce_add_sync(0xffffffffu, equal);
     if (lane == 0) {
@@ -165,23 +205,23 @@ __global__ void __launch_bounds__(SEL) evict_select_kernel(const EvictArgs a, in
     }
     __syncthreads();
     if (warp < 2) {   // prefix over the warps, and the block's total
-        const int x = wsum[warp][lane];
+        const int x = lane < SEL / 32 ? wsum[warp][lane] : 0;
         int inc = x;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int y = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += y;
         }
-        wsum[warp][lane] = inc - x;
+        if (lane < SEL / 32) wsum[warp][lane] = inc - x;
         if (lane == 31) counts[warp] = inc;
     }
     __syncthreads();
     if (size > 1) {
         cluster.sync();
-        if (t < 2) {
-            int x = 0;
-            for (int b = 0; b < rank; b++) x += cluster.map_shared_rank(counts, b)[t];
-            before[t] = x;
+        if (warp < 2) {
+            int x = lane < rank ? cluster.map_shared_rank(counts, lane)[warp] : 0;
+            x = __reduce_add_sync(0xffffffffu, x);
+            if (lane == 0) before[warp] = x;
         }
         cluster.sync();   // and nobody leaves while its counts are read
     } else {
@@ -190,18 +230,25 @@ __global__ void __launch_bounds__(SEL) evict_select_kernel(const EvictArgs a, in
     }
     int L = before[0] + wsum[0][warp], E = before[1] + wsum[1][warp];
     kept += a.sink;
-    for (int i0 = w0; i0 < w1; i0 += 32) {
-        const int i = i0 + lane;
-        const uint32_t k = i < w1 ? key(i) >> shift : 0;
-        const bool gt = i < w1 && k > limit, eq = i < w1 && k == limit;
+    const unsigned below = (1u << lane) - 1;
+    if (all) {
+        every([&](int step, uint32_t k, bool have) {
+            const bool in = have && k >> shift >= limit;
+            const unsigned ins = __ballot_sync(0xffffffffu, in);
+            if (in) kept[L + __popc(ins & below)] = run + 32 * step + lane;
+            L += __popc(ins);
+        });
+        return;
+    }
+    every([&](int step, uint32_t k, bool have) {
+        const uint32_t x = k >> shift;
+        const bool gt = have && x > limit, eq = have && x == limit;
         const unsigned gts = __ballot_sync(0xffffffffu, gt), eqs = __ballot_sync(0xffffffffu, eq);
-        const unsigned below = (1u << lane) - 1;
         const int e = E + __popc(eqs & below);
-        if (gt || (eq && (all || e < left)))
-            kept[L + __popc(gts & below) + (all ? e : min(e, left))] = begin + i;
+        if (gt || (eq && e < left)) kept[L + __popc(gts & below) + min(e, left)] = run + 32 * step + lane;
         L += __popc(gts);
         E += __popc(eqs);
-    }
+    });
 }
 
 // A thread per 16-byte chunk of U kept entries at a time (position, page and chunk
@@ -266,22 +313,17 @@ __global__ void __launch_bounds__(256) evict_gather_kernel(const EvictArgs a) {
     }
 }
 
-// Blocks of a cluster: enough that each has at most 4096 of the weights a row may
-// have, 8 at most.
-int select_blocks(size_t width) {
-    int n = 1;
-    while (n < 8 && (size_t)n * 4096 < width) n <<= 1;
-    return n;
-}
-
+// Blocks of a cluster: enough that a thread has at most 16 of the weights a row may
+// have, 8 at most (clusters of 16 take fewer rows and heads side by side).
 int launch_select(const EvictArgs &a, cudaStream_t st) {
-    const int size = select_blocks((size_t)a.width);
-    const int held = (int)std::min<size_t>(HELD, ((size_t)a.width + size - 1) / size);
-    FOCR_CUDA_TRY(set_max_dynamic_smem((const void *)evict_select_kernel, HELD * 4));
+    int size = 1;
+    while (size < MOST && size * SEL * 16 < a.width) size <<= 1;
+    const int most = (a.width + size * SEL - 1) / (size * SEL), held = most < HELD ? most : HELD;
+    FOCR_CUDA_TRY(set_max_dynamic_smem((const void *)evict_select_kernel, HELD * SEL * 4));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(size, a.c.kv_heads, a.rows);
     cfg.blockDim = SEL;
-    cfg.dynamicSmemBytes = (size_t)held * 4;
+    cfg.dynamicSmemBytes = (size_t)held * SEL * 4;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

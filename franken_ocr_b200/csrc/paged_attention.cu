@@ -109,22 +109,45 @@ __global__ void __launch_bounds__(JT) paged_join_kernel(const AttnArgs a, int bl
 // kept scores.  A row whose output is NaN leaves its weights as they were.
 __global__ void __launch_bounds__(256) paged_weights_kernel(const AttnArgs a, float *weights,
                                                             long long w_row, long long w_head) {
+    constexpr int U = 4;   // positions of a thread, loaded together
+    __shared__ float2 st[256];
     pdl_wait();
     pdl_trigger();
-    const int r = blockIdx.z, kvh = blockIdx.y;
+    const int r = blockIdx.z, kvh = blockIdx.y, t = threadIdx.x;
     const RowView rv = row_view(a, r);
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= rv.vis) return;
-    const float *s = a.scores + ((int64_t)r * a.q_heads + kvh * a.group) * a.width + i;
-    const float2 *st = a.stat + (int64_t)r * a.q_heads + kvh * a.group;
-    float sum = 0.0f;
-    for (int g = 0; g < a.group; g++) {
-        const float2 t = st[g];
-        sum = __fmaf_rn(prob(s[(int64_t)g * a.width], a.c2, scaled_max(t.x, a.c2)), t.y, sum);
+    const int i0 = blockIdx.x * (256 * U) + t;
+    if (i0 - t >= rv.vis) return;
+    float *w = weights + r * w_row + kvh * w_head;
+    float sum[U], old[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int i = i0 + u * 256;
+        old[u] = i < rv.vis ? w[i < rv.ref ? i : i + rv.gap] : 0.0f;
+        sum[u] = 0.0f;
     }
-    if (isfinite(sum)) {
-        float *w = weights + r * w_row + kvh * w_head + (i < rv.ref ? i : i + rv.gap);
-        *w += sum;
+    for (int g0 = 0; g0 < a.group; g0 += 256) {
+        const int heads = min(256, a.group - g0);
+        __syncthreads();
+        if (t < heads) {   // (c M, 1 / L)
+            const float2 x = a.stat[(int64_t)r * a.q_heads + kvh * a.group + g0 + t];
+            st[t] = make_float2(scaled_max(x.x, a.c2), x.y);
+        }
+        __syncthreads();
+        const float *s = a.scores + ((int64_t)r * a.q_heads + kvh * a.group + g0) * a.width;
+#pragma unroll 2
+        for (int g = 0; g < heads; g++) {
+            float x[U];
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                x[u] = i0 + u * 256 < rv.vis ? s[(int64_t)g * a.width + i0 + u * 256] : -INFINITY;
+#pragma unroll
+            for (int u = 0; u < U; u++) sum[u] = __fmaf_rn(prob(x[u], a.c2, st[g].x), st[g].y, sum[u]);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int i = i0 + u * 256;
+        if (i < rv.vis && isfinite(sum[u])) w[i < rv.ref ? i : i + rv.gap] = old[u] + sum[u];
     }
 }
 
@@ -152,7 +175,7 @@ int launch_attention(AttnArgs a, int dtype, float *weights, size_t w_row, size_t
     if (smem > 24 * 1024) FOCR_CUDA_TRY(set_max_dynamic_smem((const void *)paged_join_kernel, 96 * 1024));
     FOCR_CUDA_TRY(launch_pdl(paged_join_kernel, dim3(a.c.kv_heads * a.head_chunks, a.rows), JT, smem, st, a, blocks));
     if (weights)
-        FOCR_CUDA_TRY(launch_pdl(paged_weights_kernel, dim3((a.width + 255) / 256, a.c.kv_heads, a.rows), 256, 0, st,
+        FOCR_CUDA_TRY(launch_pdl(paged_weights_kernel, dim3((a.width + 1023) / 1024, a.c.kv_heads, a.rows), 256, 0, st,
                                  a, weights, (long long)w_row, (long long)w_head));
     return FOCR_OK;
 }
