@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from ._lib import lib
-from .paged import _cache, _call, _dtype, _need, _workspace
+from .paged import _F32, _I32, _U8, _cache, _call, _dtype, _empty, _need, _workspace
 
 
 def beam_select(logits, scores, n: int | None = None, *, done=None, end_token: int = 1):
@@ -26,31 +26,32 @@ def beam_select(logits, scores, n: int | None = None, *, done=None, end_token: i
     alone with its score unchanged; -inf and NaN logits and beams with a score
     that is not finite offer nothing.  Missing candidates: -inf, -1, -1."""
     ctx = "beam_select"
-    if logits.dim() != 3:
-        raise ValueError(f"{ctx}: logits must be [batch, beams, vocab], not {tuple(logits.shape)}")
-    device = logits.device
-    if device.type != "cuda":
-        raise ValueError(f"{ctx}: logits must be a CUDA tensor, not on {device}")
+    shape, stride = logits.shape, logits.stride()
+    if len(shape) != 3:
+        raise ValueError(f"{ctx}: logits must be [batch, beams, vocab], not {tuple(shape)}")
+    index = logits.get_device()
+    if index < 0:
+        raise ValueError(f"{ctx}: logits must be a CUDA tensor, not on {logits.device}")
     code = _dtype(ctx, "logits", logits)
-    batch, beams, vocab = logits.shape
-    if logits.stride(2) != 1 or (batch > 1 and beams > 1 and logits.stride(0) != beams * logits.stride(1)):
+    batch, beams, vocab = shape
+    if (stride[2] != 1 and vocab > 1) or (batch > 1 and beams > 1 and stride[0] != beams * stride[1]):
         raise ValueError(f"{ctx}: the rows of logits must be contiguous and evenly spaced")
-    _need(ctx, "scores", scores, torch.float32, (batch, beams), device)
+    _need(ctx, "scores", scores, _F32, (batch, beams), index)
     if done is not None:
-        if done.dtype == torch.bool:
-            done = done.view(torch.uint8)
-        _need(ctx, "done", done, torch.uint8, (batch, beams), device)
+        if done.dtype is torch.bool:
+            done = done.view(_U8)
+        _need(ctx, "done", done, _U8, (batch, beams), index)
     if n is None:
         n = beams
     if n < 1:
         raise ValueError(f"{ctx}: n must be positive")
-    out = torch.empty((batch, n), dtype=torch.float32, device=device)
-    parent = torch.empty((batch, n), dtype=torch.int32, device=device)
-    token = torch.empty((batch, n), dtype=torch.int32, device=device)
+    out = _empty((batch, n), _F32, index)
+    parent = _empty((batch, n), _I32, index)
+    token = _empty((batch, n), _I32, index)
     need = _workspace("focr_beam_select_workspace", batch, beams, vocab, n)
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
-    _call(lib.focr_beam_select, device, logits.data_ptr(), code, batch, beams, vocab,
-          logits.stride(1) if beams > 1 else max(logits.stride(0), vocab), scores.data_ptr(),
+    ws = _empty((need,), _U8, index)  # lives until the kernels are enqueued
+    row = stride[1] if beams > 1 else stride[0] if batch > 1 else vocab
+    _call(lib.focr_beam_select, index, logits.data_ptr(), code, batch, beams, vocab, row, scores.data_ptr(),
           None if done is None else done.data_ptr(), end_token, n, out.data_ptr(), parent.data_ptr(),
           token.data_ptr(), ws.data_ptr(), need)
     return out, parent, token
@@ -70,32 +71,33 @@ def beam_reorder(k_pages, v_pages, table, lens, parent, fresh, *, weights=None):
     another and from every page the table uses."""
     ctx = "beam_reorder"
     layered = k_pages.dim() == 5
-    cache, device, heads, _, rows, width = _cache(ctx, k_pages, v_pages, table, 5 if layered else 4)
+    cache, index, heads, _, rows, width = _cache(ctx, k_pages, v_pages, table, 5 if layered else 4)
     layers = k_pages.shape[0] if layered else 1
     if parent.dim() != 2:
         raise ValueError(f"{ctx}: parent must be [batch, beams], not {tuple(parent.shape)}")
     batch, beams = parent.shape
     if batch * beams != rows:
         raise ValueError(f"{ctx}: table has {rows} rows for {batch} x {beams} beams")
-    _need(ctx, "parent", parent, torch.int32, (batch, beams), device)
-    _need(ctx, "lens", lens, torch.int32, (rows,), device)
-    _need(ctx, "fresh", fresh, torch.int32, (rows,), device)
+    _need(ctx, "parent", parent, _I32, (batch, beams), index)
+    _need(ctx, "lens", lens, _I32, (rows,), index)
+    _need(ctx, "fresh", fresh, _I32, (rows,), index)
     w_out, span, w_layer, w_row, w_head = None, 0, 0, 0, 0
     if weights is not None:
         lead = (layers, rows, heads) if layered else (rows, heads)
-        if weights.dtype != torch.float32:
+        shape, stride = weights.shape, weights.stride()
+        if weights.dtype is not _F32:
             raise TypeError(f"{ctx}: weights must be torch.float32, not {weights.dtype}")
-        if weights.shape[:-1] != lead or weights.device != device:
-            raise ValueError(f"{ctx}: weights must be {list(lead)} + [width] on {device}, "
-                             f"not {tuple(weights.shape)} on {weights.device}")
-        if weights.stride(-1) != 1:
+        if shape[:-1] != lead or weights.get_device() != index:
+            raise ValueError(f"{ctx}: weights must be {list(lead)} + [width] on cuda:{index}, "
+                             f"not {tuple(shape)} on {weights.device}")
+        span, w_row, w_head = shape[-1], stride[-3], stride[-2]
+        if stride[-1] != 1 and span > 1:
             raise ValueError(f"{ctx}: the last dimension of weights must be contiguous")
-        span, w_row, w_head = weights.shape[-1], weights.stride(-3), weights.stride(-2)
-        w_layer = weights.stride(0) if layered else 0
-        w_out = torch.empty(weights.shape, dtype=torch.float32, device=device)
-    new_table = torch.empty((rows, width), dtype=torch.int32, device=device)
-    new_lens = torch.empty((rows,), dtype=torch.int32, device=device)
-    _call(lib.focr_beam_reorder, device, cache, layers, k_pages.stride(0) if layered else 0, batch, beams,
+        w_layer = stride[0] if layered else 0
+        w_out = _empty(shape, _F32, index)
+    new_table = _empty((rows, width), _I32, index)
+    new_lens = _empty((rows,), _I32, index)
+    _call(lib.focr_beam_reorder, index, cache, layers, k_pages.stride(0) if layered else 0, batch, beams,
           lens.data_ptr(), parent.data_ptr(), fresh.data_ptr(), new_table.data_ptr(), new_lens.data_ptr(),
           None if weights is None else weights.data_ptr(), span, w_layer, w_row, w_head,
           None if w_out is None else w_out.data_ptr())

@@ -14,6 +14,9 @@ K and one for V with the same strides; a row's position ``p`` lies in page
 ``table[row, p // page_size]``, slot ``p % page_size``.  The calls take CUDA
 tensors on one device, enqueue work on torch's current stream of that device
 and can be captured into a CUDA graph.
+
+The checks are written for speed: a decode step makes these calls for every
+layer, and the smallest run 2 us on the device.
 """
 from __future__ import annotations
 
@@ -27,9 +30,28 @@ import torch
 from ._lib import F32, F16, BF16, FOCR_OK, PagedCache, check, lib
 
 _TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+_F32, _I32, _U8 = torch.float32, torch.int32, torch.uint8
 # a PagedCache's bytes: packing them costs a third of filling the ctypes structure
 _PACK = struct.Struct("6N5Ii")
 assert _PACK.size == C.sizeof(PagedCache)
+_device = torch._C._cuda_getDevice
+_stream = torch._C._cuda_getCurrentRawStream
+
+try:  # an allocation on the current device without the dispatcher: half the time
+    from torch._C._dynamo.guards import _empty_strided_cuda as _raw_empty
+except ImportError:  # pragma: no cover
+    _raw_empty = None
+
+
+def _empty(shape, dtype, index: int):
+    """An uninitialised contiguous tensor on CUDA device `index`."""
+    if _raw_empty is None or index != _device():
+        return torch.empty(shape, dtype=dtype, device=torch.device("cuda", index))
+    stride, n = [], 1
+    for d in reversed(shape):
+        stride.append(n)
+        n *= d if d > 1 else 1
+    return _raw_empty(tuple(shape), tuple(stride[::-1]), dtype)
 
 
 def _dtype(ctx: str, name: str, t) -> int:
@@ -39,54 +61,63 @@ def _dtype(ctx: str, name: str, t) -> int:
     return code
 
 
-def _need(ctx: str, name: str, t, dtype, shape, device) -> None:
+def _need(ctx: str, name: str, t, dtype, shape, index: int) -> None:
     """A contiguous tensor of that type and shape on that device."""
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{ctx}: {name} must be {dtype}, not {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{ctx}: {name} has shape {tuple(t.shape)}, not {tuple(shape)}")
-    if t.device != device:
-        raise ValueError(f"{ctx}: {name} is on {t.device}, not {device}")
+    if t.get_device() != index:
+        raise ValueError(f"{ctx}: {name} is on {t.device}, not cuda:{index}")
     if not t.is_contiguous():
         raise ValueError(f"{ctx}: {name} must be contiguous")
 
 
+def _table(ctx: str, name: str, t, index: int):
+    """(rows, columns, row stride) of an int32 page table."""
+    if t.dtype is not _I32:
+        raise TypeError(f"{ctx}: {name} must be torch.int32, not {t.dtype}")
+    if t.dim() != 2 or t.get_device() != index:
+        raise ValueError(f"{ctx}: {name} must be [rows, pages] on cuda:{index}")
+    rows, width = t.shape
+    step, unit = t.stride()
+    if unit != 1 and width > 1:
+        raise ValueError(f"{ctx}: the rows of {name} must be contiguous")
+    return rows, width, step if rows > 1 else width
+
+
 def _cache(ctx: str, k_pages, v_pages, table, dims: int = 4):
-    """The checked cache as the C ABI's struct; its device, kv heads, head_dim and table's shape."""
-    device = k_pages.device
-    if device.type != "cuda":
-        raise ValueError(f"{ctx}: the pages must be CUDA tensors, not on {device}")
+    """The checked cache as the C ABI's struct; its device's index, kv heads,
+    head_dim and table's shape."""
+    index = k_pages.get_device()
+    if index < 0:
+        raise ValueError(f"{ctx}: the pages must be CUDA tensors, not on {k_pages.device}")
     code = _dtype(ctx, "k_pages", k_pages)
     shape, stride = k_pages.shape, k_pages.stride()
     if len(shape) != dims:
         raise ValueError(f"{ctx}: k_pages must have {dims} dimensions, not {len(shape)}")
-    if v_pages.shape != shape or v_pages.stride() != stride or v_pages.dtype != k_pages.dtype \
-            or v_pages.device != device:
+    if v_pages.shape != shape or v_pages.stride() != stride or v_pages.dtype is not k_pages.dtype \
+            or v_pages.get_device() != index:
         raise ValueError(f"{ctx}: v_pages must match k_pages in shape, strides, type and device")
     pages, heads, page, dim = shape[-4:]
-    if stride[-1] != 1 or stride[-2] != dim:
+    if stride[-1] != 1 or (stride[-2] != dim and page > 1):
         raise ValueError(f"{ctx}: the entries of a head's page must be contiguous")
-    if table.dtype != torch.int32:
-        raise TypeError(f"{ctx}: table must be torch.int32, not {table.dtype}")
-    if table.dim() != 2 or table.stride(1) != 1 or table.device != device:
-        raise ValueError(f"{ctx}: table must be [rows, pages] on {device} with contiguous rows")
-    rows, width = table.shape
+    rows, width, step = _table(ctx, "table", table, index)
     try:
         packed = _PACK.pack(k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), stride[-4], stride[-3],
-                            max(table.stride(0), width), pages, heads, page, dim, width, code)
+                            step, pages, heads, page, dim, width, code)
     except struct.error as e:
         raise ValueError(f"{ctx}: a dimension exceeds 32 bits") from e
-    return packed, device, heads, dim, rows, width
+    return packed, index, heads, dim, rows, width
 
 
-def _call(fn, device, *args) -> None:
+def _call(fn, index: int, *args) -> None:
     """One call of the C ABI on the device's current stream, its last argument."""
-    index = device.index
-    if index == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if index == _device():
+        rc = fn(*args, _stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream(index))
     if rc != FOCR_OK:
         check(rc)
 
@@ -99,35 +130,41 @@ def _workspace(fn: str, *sizes) -> int:
     return need.value
 
 
-def _weights(ctx: str, w, rows: int, heads: int, device):
-    if w.dtype != torch.float32:
+def _weights(ctx: str, w, rows: int, heads: int, index: int):
+    """(width, row stride, head stride) of accumulated weights."""
+    if w.dtype is not _F32:
         raise TypeError(f"{ctx}: weights must be torch.float32, not {w.dtype}")
-    if w.dim() != 3 or w.shape[0] != rows or w.shape[1] != heads or w.device != device:
-        raise ValueError(f"{ctx}: weights must be [{rows}, {heads}, width] on {device}, "
-                         f"not {tuple(w.shape)} on {w.device}")
-    if w.stride(2) != 1:
+    shape = w.shape
+    if len(shape) != 3 or shape[0] != rows or shape[1] != heads or w.get_device() != index:
+        raise ValueError(f"{ctx}: weights must be [{rows}, {heads}, width] on cuda:{index}, "
+                         f"not {tuple(shape)} on {w.device}")
+    row, head, unit = w.stride()
+    if unit != 1 and shape[2] > 1:
         raise ValueError(f"{ctx}: the last dimension of weights must be contiguous")
+    return shape[2], row, head
 
 
 def paged_write(k, v, k_pages, v_pages, table, pos, row=None) -> None:
     """Write ``k``, ``v`` ``[tokens, kv_heads, head_dim]`` into pages: token ``t``
     to position ``pos[t]`` of table row ``row[t]`` (``row`` None: row ``t``).
     Tokens with ``row[t] < 0`` are padding; rows, positions and pages out of
-    range are skipped.  ``pos`` and ``row`` are int32 on the device."""
+    range are skipped.  No two tokens of a call may name the same place.
+    ``pos`` and ``row`` are int32 on the device."""
     ctx = "paged_write"
-    cache, device, heads, dim, rows, _ = _cache(ctx, k_pages, v_pages, table)
+    cache, index, heads, dim, rows, _ = _cache(ctx, k_pages, v_pages, table)
     src = _dtype(ctx, "k", k)
-    tokens = k.shape[0]
-    shape, ks, vs = (tokens, heads, dim), k.stride(), v.stride()
-    if k.shape != shape or v.shape != shape or v.dtype != k.dtype or k.device != device or v.device != device:
-        raise ValueError(f"{ctx}: k and v must be [tokens, {heads}, {dim}] of one type on {device}, not "
-                         f"{tuple(k.shape)} of {k.dtype} on {k.device} and {tuple(v.shape)} of {v.dtype} on {v.device}")
+    shape = k.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim or v.shape != shape or v.dtype is not k.dtype \
+            or k.get_device() != index or v.get_device() != index:
+        raise ValueError(f"{ctx}: k and v must be [tokens, {heads}, {dim}] of one type on cuda:{index}, not "
+                         f"{tuple(shape)} of {k.dtype} on {k.device} and {tuple(v.shape)} of {v.dtype} on {v.device}")
+    tokens, ks, vs = shape[0], k.stride(), v.stride()
     if ks[2] != 1 or vs[2] != 1 or (heads > 1 and (ks[1] != dim or vs[1] != dim)):
         raise ValueError(f"{ctx}: a token of k and of v must be contiguous")
-    _need(ctx, "pos", pos, torch.int32, (tokens,), device)
+    _need(ctx, "pos", pos, _I32, (tokens,), index)
     if row is not None:
-        _need(ctx, "row", row, torch.int32, (tokens,), device)
-    _call(lib.focr_paged_write, device, cache, rows, k.data_ptr(), v.data_ptr(), src, tokens, ks[0], vs[0],
+        _need(ctx, "row", row, _I32, (tokens,), index)
+    _call(lib.focr_paged_write, index, cache, rows, k.data_ptr(), v.data_ptr(), src, tokens, ks[0], vs[0],
           None if row is None else row.data_ptr(), pos.data_ptr())
 
 
@@ -144,34 +181,34 @@ def paged_attention(q, k_pages, v_pages, table, lens, *, scale: float | None = N
     A row that sees nothing gives zeros.  A length past the table (or the
     weights), or a page id outside the pool, gives NaN for that row."""
     ctx = "paged_attention"
-    cache, device, kv_heads, dim, rows, _ = _cache(ctx, k_pages, v_pages, table)
+    cache, index, kv_heads, dim, rows, _ = _cache(ctx, k_pages, v_pages, table)
     code = _dtype(ctx, "q", q)
     shape, stride = q.shape, q.stride()
-    if len(shape) != 3 or shape[0] != rows or shape[2] != dim or q.device != device:
-        raise ValueError(f"{ctx}: q must be [{rows}, q_heads, {dim}] on {device}, "
+    if len(shape) != 3 or shape[0] != rows or shape[2] != dim or q.get_device() != index:
+        raise ValueError(f"{ctx}: q must be [{rows}, q_heads, {dim}] on cuda:{index}, "
                          f"not {tuple(shape)} on {q.device}")
     heads = shape[1]
     if stride[2] != 1 or (heads > 1 and stride[1] != dim):
         raise ValueError(f"{ctx}: a row of q must be contiguous")
     if window < 0:
         raise ValueError(f"{ctx}: window must not be negative")
-    _need(ctx, "lens", lens, torch.int32, (rows,), device)
+    _need(ctx, "lens", lens, _I32, (rows,), index)
     if ref_lens is not None:
-        _need(ctx, "ref_lens", ref_lens, torch.int32, (rows,), device)
+        _need(ctx, "ref_lens", ref_lens, _I32, (rows,), index)
     width = w_row = w_head = 0
     if weights is not None:
-        _weights(ctx, weights, rows, kv_heads, device)
-        width, w_row, w_head = weights.shape[2], weights.stride(0), weights.stride(1)
+        width, w_row, w_head = _weights(ctx, weights, rows, kv_heads, index)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=device)
+        out = _empty(shape, q.dtype, index)
     else:
-        _need(ctx, "out", out, q.dtype, shape, device)
+        _need(ctx, "out", out, q.dtype, shape, index)
     need = _workspace("focr_paged_attention_workspace", rows, heads, dim, width)
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
-    _call(lib.focr_paged_attention, device, cache, q.data_ptr(), code, rows, heads, stride[0], lens.data_ptr(),
+    ws = _empty((need,), _U8, index)  # lives until the kernels are enqueued
+    _call(lib.focr_paged_attention, index, cache, q.data_ptr(), code, rows, heads, stride[0], lens.data_ptr(),
           None if ref_lens is None else ref_lens.data_ptr(), window,
           1.0 / math.sqrt(dim) if scale is None else scale, out.data_ptr(), heads * dim,
-          None if weights is None else weights.data_ptr(), width, w_row, w_head, ws.data_ptr(), need)
+          None if weights is None else weights.data_ptr(), width, w_row, w_head,
+          ws.data_ptr(), need)
     return out
 
 
@@ -188,21 +225,18 @@ def paged_evict(k_pages, v_pages, table, lens, weights, new_table, budget: int, 
     budget]`` (-1 behind the last), the new lengths, and the kept entries'
     weights in a tensor of ``weights``' shape, 0 behind them."""
     ctx = "paged_evict"
-    cache, device, heads, _, rows, _ = _cache(ctx, k_pages, v_pages, table)
-    _need(ctx, "lens", lens, torch.int32, (rows,), device)
-    _weights(ctx, weights, rows, heads, device)
-    if new_table.dtype != torch.int32:
-        raise TypeError(f"{ctx}: new_table must be torch.int32, not {new_table.dtype}")
-    if new_table.dim() != 2 or new_table.shape[0] != rows or new_table.stride(1) != 1 \
-            or new_table.device != device:
-        raise ValueError(f"{ctx}: new_table must be [{rows}, pages] on {device} with contiguous rows")
+    cache, index, heads, _, rows, _ = _cache(ctx, k_pages, v_pages, table)
+    _need(ctx, "lens", lens, _I32, (rows,), index)
+    width, w_row, w_head = _weights(ctx, weights, rows, heads, index)
+    new_rows, new_pages, new_step = _table(ctx, "new_table", new_table, index)
+    if new_rows != rows:
+        raise ValueError(f"{ctx}: new_table has {new_rows} rows, table {rows}")
     if budget < 1 or sink < 0 or recent < 0:
         raise ValueError(f"{ctx}: budget must be positive, sink and recent not negative")
-    width = weights.shape[2]
-    kept = torch.empty((rows, heads, budget), dtype=torch.int32, device=device)
-    new_lens = torch.empty((rows,), dtype=torch.int32, device=device)
-    new_weights = torch.empty((rows, heads, width), dtype=torch.float32, device=device)
-    _call(lib.focr_paged_evict, device, cache, rows, lens.data_ptr(), weights.data_ptr(), width, weights.stride(0),
-          weights.stride(1), new_table.data_ptr(), max(new_table.stride(0), new_table.shape[1]),
-          new_table.shape[1], budget, sink, recent, kept.data_ptr(), new_lens.data_ptr(), new_weights.data_ptr())
+    kept = _empty((rows, heads, budget), _I32, index)
+    new_lens = _empty((rows,), _I32, index)
+    new_weights = _empty((rows, heads, width), _F32, index)
+    _call(lib.focr_paged_evict, index, cache, rows, lens.data_ptr(), weights.data_ptr(), width, w_row, w_head,
+          new_table.data_ptr(), new_step, new_pages, budget, sink, recent, kept.data_ptr(), new_lens.data_ptr(),
+          new_weights.data_ptr())
     return kept, new_lens, new_weights

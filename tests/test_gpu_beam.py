@@ -114,6 +114,29 @@ def test_select_strided_and_unaligned_rows(cuda):
         check_select(apart[:, 1:2], torch.zeros((4, 1)), 2, dev=apart.cuda()[:, 1:2])
 
 
+def test_broadcast_inputs_are_refused(cuda):
+    """An expanded tensor has no rows of its own to read."""
+    from franken_ocr_b200 import beam, paged
+    from franken_ocr_b200._lib import FocrError
+
+    x = torch.randn((1, 1, 50), device="cuda")
+    with pytest.raises(FocrError, match="row_stride 0"):
+        beam.beam_select(x.expand(1, 4, 50), torch.zeros((1, 4), device="cuda"))
+    with pytest.raises(FocrError, match="row_stride 0"):
+        beam.beam_select(x.expand(4, 1, 50), torch.zeros((4, 1), device="cuda"))
+    kp = torch.zeros((4, 1, 16, 64), device="cuda")
+    table = torch.zeros((1, 2), dtype=torch.int32, device="cuda").expand(3, 2)
+    lens = torch.ones((3,), dtype=torch.int32, device="cuda")
+    with pytest.raises(FocrError, match="table_stride 0"):
+        paged.paged_attention(torch.zeros((3, 1, 64), device="cuda"), kp, kp, table, lens)
+    with pytest.raises(FocrError, match="shorter"):
+        paged.paged_attention(torch.zeros((3, 2, 64), device="cuda"), kp.expand(4, 2, 16, 64), kp.expand(4, 2, 16, 64),
+                              table.contiguous(), lens)
+    with pytest.raises(FocrError, match="weights stride"):
+        paged.paged_attention(torch.zeros((3, 1, 64), device="cuda"), kp, kp, table.contiguous(), lens,
+                              weights=torch.zeros((1, 1, 32), device="cuda").expand(3, 1, 32))
+
+
 def test_select_in_a_graph_and_twice_the_same(cuda):
     from franken_ocr_b200 import beam
 
