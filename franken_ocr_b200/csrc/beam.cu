@@ -50,20 +50,39 @@ __device__ __forceinline__ float block_max_f32(float v, float *sh) {
     return m;
 }
 
-// A logit as a candidate: NaN becomes -inf (none), +inf the largest finite f32.
-__device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, -INFINITY), 3.402823466e38f); }
+constexpr float LARGEST = 3.402823466e38f;
+constexpr float SHIFT = 12582912.0f;   // 1.5 * 2^23: adding it rounds to an integer in the low bits
+
+// Two f32 operations at a time.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{.reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+        " fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{.reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 d, a, b;\n"
+        " mov.b64 {%0, %1}, d;}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 
 // 2^(x log2 e - base) to about one rounding, for x / log2 e between base - 100 and
 // base + 1: Cody and Waite's reduction with log2 e in two parts, and the hardware's
-// 2^r for the rest, |r| <= 1/2.  `base` comes as the bits of SHIFT + base.
-constexpr float SHIFT = 12582912.0f;   // 1.5 * 2^23: adding it rounds to an integer in the low bits
-__device__ __forceinline__ float exp_below(float x, int base) {
-    const float t = __fmaf_rn(x, 1.44269502f, SHIFT), n = t - SHIFT;
-    float r = __fmaf_rn(x, 1.44269502f, -n);
-    r = __fmaf_rn(x, 1.92596299e-8f, r);
-    float p;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(r));
-    return __int_as_float(__float_as_int(p) + ((__float_as_int(t) - base) << 23));
+// 2^r for the rest, |r| <= 1/2.
+__device__ __forceinline__ float2 exp_below(float2 x, float base) {
+    const float2 high = make_float2(1.44269502f, 1.44269502f), low = make_float2(1.92596299e-8f, 1.92596299e-8f);
+    const float up = SHIFT - base;                     // base is an integer: exact
+    const float2 t = fma2(x, high, make_float2(up, up));
+    const float2 n = add2(t, make_float2(-up, -up));   // the nearest integer
+    const float2 r = fma2(x, low, fma2(x, high, make_float2(-n.x, -n.y)));
+    float2 p;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p.x) : "f"(r.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p.y) : "f"(r.y));
+    // t's low bits are n - base
+    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
 // One strip of one row's logits, held in registers (PER a thread, read once, 16
@@ -71,10 +90,10 @@ __device__ __forceinline__ float exp_below(float x, int base) {
 // its sum of exponentials and its n largest candidates.  A thread's logits do
 // not depend on the row's alignment, so equal rows give equal sums.
 //
-// The sum: terms above e^-2.5 of the largest are few and go through the 64-bit
-// exponential; the others' rounding to f32 then moves the sum by less than
-// 2^-22 e^-2.5 each, and not in one direction.  All of them in 64 bits cost several
-// times the strip's load.
+// The sum: terms above 1/e of the largest are few and go through the 64-bit
+// exponential; the others are rounded to f32, each by 2^-22 of itself at most and
+// not in one direction, which leaves some 1e-8 of the sum at worst and 1e-9 as a
+// rule.  All of them in 64 bits cost several times the strip's load.
 //
 // The n largest: at least n logits reach the n-th largest of the maxima of 2n or
 // more groups of threads, and hardly more do; these are collected and ranked by
@@ -84,8 +103,8 @@ template <typename T, int PER>
 __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) {
     constexpr int V = 16 / (int)sizeof(T), STRIP = ST * PER;
     __shared__ __align__(16) float tops[ST];
-    __shared__ float sh[ST / 32], lx[LIST], nx[LIST];
-    __shared__ int lt[LIST], count, near_count;
+    __shared__ float sh[ST / 32], lx[LIST];
+    __shared__ int lt[LIST], count;
     __shared__ float bound;
     __shared__ double shd[ST / 32];
     __shared__ long long shl[ST / 32];
@@ -102,22 +121,26 @@ __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) 
         const int c = first + (i * ST + t) * V;
         if (vec && c + V <= a.vocab) {
             unpack16<T>(*reinterpret_cast<const uint4 *>(x + c), v + i * V);
-#pragma unroll
-            for (int e = 0; e < V; e++) v[i * V + e] = clean(v[i * V + e]);
         } else {
 #pragma unroll
             for (int e = 0; e < V; e++)
-                v[i * V + e] = c + e < a.vocab ? clean(to_f32<T>(x[c + e])) : -INFINITY;
+                v[i * V + e] = c + e < a.vocab ? to_f32<T>(x[c + e]) : -INFINITY;
         }
     }
     auto token = [&](int i) { return first + (i / V * ST + t) * V + i % V; };
+    // NaN loses every maximum and comparison; +inf counts as the largest number
 #pragma unroll
     for (int i = 0; i < PER; i++) top = fmaxf(top, v[i]);
+    if (top == INFINITY) {
+#pragma unroll
+        for (int i = 0; i < PER; i++) v[i] = v[i] == INFINITY ? LARGEST : v[i];
+        top = LARGEST;
+    }
     const int lanes = group_lanes(a.n), groups = ST / lanes;
     for (int o = 1; o < lanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (t % lanes == 0) tops[t / lanes] = top;
     if (t == 0) {
-        count = near_count = 0;
+        count = 0;
         bound = -INFINITY;
     }
     const float m = block_max_f32(top, sh);
@@ -142,51 +165,53 @@ __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) 
     }
     // far from 0 the differences to the maximum are exact and stay small
     const float zero = fabsf(m) >= 1024.0f ? m : 0.0f, high = m - zero;
-    const float base = rintf(__fmul_rn(high, 1.44269502f)), near = m - 2.5f;
+    const float base = rintf(__fmul_rn(high, 1.44269502f)), near = m - 1.0f;
     const float near0 = near - zero, none = high - 65.0f;   // e^-65 of the largest adds nothing
-    const int base_bits = __float_as_int(SHIFT + base);
+    const float2 minus = make_float2(-zero, -zero);
     double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < PER; i += 4) {
         float s = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const float y = fmaxf(v[i + e] - zero, none), x = exp_below(y, base_bits);
-            if (y < near0) s += x;
+        for (int e = 0; e < 4; e += 2) {
+            float2 y = add2(make_float2(v[i + e], v[i + e + 1]), minus);
+            y = make_float2(fmaxf(y.x, none), fmaxf(y.y, none));
+            const float2 x = exp_below(y, base);
+            if (y.x < near0) s += x.x;
+            if (y.y < near0) s += x.y;
         }
         sum += s;
     }
-    // the small terms were taken relative to 2^base
-    sum *= exp((double)base * 0.693147180559945309 - (double)high);
     __syncthreads();
     // the few that are large or candidates
     const float low = bound, few = fminf(low, near);
+    int c = 0;
 #pragma unroll
-    for (int g = 0; g < PER; g += 4) {
-        if (fmaxf(fmaxf(v[g], v[g + 1]), fmaxf(v[g + 2], v[g + 3])) < few) continue;
+    for (int g = 0; g < PER; g += 4)
+        if (fmaxf(fmaxf(v[g], v[g + 1]), fmaxf(v[g + 2], v[g + 3])) >= few)
 #pragma unroll
-        for (int i = g; i < g + 4; i++) {
-            if (v[i] >= near) {
-                const int k = atomicAdd(&near_count, 1);
-                if (k < LIST) nx[k] = v[i];
-            }
-            if (v[i] >= low && v[i] > -INFINITY) {
-                const int k = atomicAdd(&count, 1);
-                if (k < LIST) {
-                    lx[k] = v[i];
-                    lt[k] = token(i);
-                }
-            }
-        }
+            for (int i = g; i < g + 4; i++) c += v[i] >= few && v[i] > -INFINITY;
+    if (c) {
+        int k = atomicAdd(&count, c);
+        if (k + c <= LIST)
+#pragma unroll
+            for (int g = 0; g < PER; g += 4)
+                if (fmaxf(fmaxf(v[g], v[g + 1]), fmaxf(v[g + 2], v[g + 3])) >= few)
+#pragma unroll
+                    for (int i = g; i < g + 4; i++)
+                        if (v[i] >= few && v[i] > -INFINITY) {
+                            lx[k] = v[i];
+                            lt[k++] = token(i);
+                        }
     }
     __syncthreads();
-    const int got = count, nears = near_count;
+    const int got = count;
     // the list's order is chance: a sum of whole multiples of 2^-48 has none
     long long large = 0;
-    for (int i = t; i < (nears <= LIST ? nears : STRIP); i += ST) {
+    for (int i = t; i < (got <= LIST ? got : STRIP); i += ST) {
         float y = -INFINITY;
-        if (nears <= LIST) y = nx[i];
-        else if (first + i < a.vocab) y = clean(to_f32<T>(x[first + i]));
+        if (got <= LIST) y = lx[i];
+        else if (first + i < a.vocab) y = fminf(to_f32<T>(x[first + i]), LARGEST);
         if (y >= near) large += __double2ll_rn(exp((double)y - (double)m) * 0x1p48);
     }
     for (int o = 16; o > 0; o >>= 1) {
@@ -204,14 +229,16 @@ __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) 
             large += shl[w];
         }
         a.pm[at] = m;
-        a.ps[at] = sum + (double)large * 0x1p-48;
+        // the small terms were taken relative to 2^base
+        a.ps[at] = sum * exp((double)base * 0.693147180559945309 - (double)high) + (double)large * 0x1p-48;
     }
     if (got <= LIST) {
         for (int i = t; i < got; i += ST) {
             const float y = lx[i];
             const int c = lt[i];
+            if (y < low) continue;
             int rank = 0;
-#pragma unroll 4
+#pragma unroll 8
             for (int j = 0; j < got; j++) rank += (lx[j] > y) | ((lx[j] == y) & (lt[j] < c));
             if (rank < a.n) {
                 a.cx[at * a.n + rank] = y;
