@@ -7,102 +7,73 @@ namespace {
 
 constexpr int JT = 256;
 
-// Joins the pieces of one (row, kv head, chunk of its query heads) and writes
-// the rows that no unit reached: zeros where nothing is visible, NaN for a
-// length that passes the table.  A long row of a small batch has pieces of
-// nearly every block, so the pieces' factors are found side by side first and
-// the threads split the pieces as well as the columns.
+// Joins the pieces of the (row, kv head, chunk of query heads)s that block
+// boundaries cut: a block per boundary and query head of the chunk, of which the
+// one at a cut's first boundary does the work.  A long row of a small batch has
+// pieces of nearly every block, so the pieces' factors are found side by side
+// first, and the threads split the pieces as well as the columns.
 __global__ void __launch_bounds__(JT) paged_join_kernel(const AttnArgs a, int blocks) {
-    extern __shared__ __align__(16) float jsm[];
+    extern __shared__ float factor[];   // [pieces]
     __shared__ int pre[ATTN_ROWS + 1];
     __shared__ float4 red[JT];
-    __shared__ float top[ATTN_HEADS], sum[ATTN_HEADS];
-    float *fm = jsm, *fl = jsm + blocks * a.gp;  // [piece][gp]
+    __shared__ float warp_m[JT / 32], warp_l[JT / 32];
     // the kernel before has waited for all that came before it: lengths may be
     // read while it still runs
     tile_prefix<JT>(a, pre);
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = blockIdx.y, HC = a.c.kv_heads * a.head_chunks;
+    const unsigned long long total = (unsigned long long)pre[a.rows] * HC, n = run_count(total, blocks);
+    const unsigned long long b = blockIdx.x + 1;
     pdl_wait();
     pdl_trigger();
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int r = blockIdx.y, hc = blockIdx.x, HC = a.c.kv_heads * a.head_chunks;
-    const int kvh = hc / a.head_chunks, g0 = (hc - kvh * a.head_chunks) * a.gp;
-    const int heads = min(a.gp, a.group - g0), qh0 = kvh * a.group + g0;
-    const int tiles = pre[r + 1] - pre[r];
-    const long long out = r * a.out_stride + (long long)qh0 * a.dim;
-    if (tiles == 0) {
-        const float x = row_view(a, r).bad ? NAN : 0.0f;
-        for (int i = t; i < heads * a.dim; i += JT) store_f32_as(a.out, a.q_type, out + i, x);
-        if (a.stat && t < heads) a.stat[(int64_t)r * a.q_heads + qh0 + t] = make_float2(-INFINITY, NAN);
-        return;
-    }
-    const unsigned long long total = (unsigned long long)pre[a.rows] * HC, n = run_count(total, blocks);
+    if (b >= n) return;
+    const unsigned long long u = b * total / n;
+    const int r = row_of_unit(pre, a.rows, HC, u), tiles = pre[r + 1] - pre[r];
+    const int hc = (int)((u - (unsigned long long)pre[r] * HC) / tiles);
     const unsigned long long u0 = (unsigned long long)pre[r] * HC + (unsigned long long)hc * tiles;
-    // the block whose run holds unit u: the last b with b * total / n <= u
-    const int b0 = (int)(((u0 + 1) * n - 1) / total), b1 = (int)(((u0 + tiles) * n - 1) / total);
-    if (b0 == b1) return;
-    const int pieces = b1 - b0 + 1, slot0 = 2 * b0 + (b0 * total / n == u0 ? 0 : 1);
+    if (u == u0 || (b - 1) * total / n > u0) return;   // nothing is cut, or it was cut before
+    const int kvh = hc / a.head_chunks, g0 = (hc - kvh * a.head_chunks) * a.gp;
+    if (g >= min(a.gp, a.group - g0)) return;
+    const int qh = kvh * a.group + g0 + g;
+    // the last block whose run begins before the cut ends
+    const int b0 = (int)b - 1, b1 = (int)(((u0 + tiles) * n - 1) / total);
+    const int pieces = b1 - b0 + 1, slot0 = 2 * b0 + ((b - 1) * total / n == u0 ? 0 : 1);
     auto slot = [&](int p) { return p ? 2 * (b0 + p) : slot0; };
-    for (int x = t; x < pieces * heads; x += JT) {
-        const int p = x / heads, g = x - p * heads;
+    float M = -INFINITY, L = 0.0f;
+    for (int p = t; p < pieces; p += JT) M = fmaxf(M, a.ml[slot(p) * a.gp + g].x);
+    M = warp_max_f32(M);
+    if (lane == 0) warp_m[warp] = M;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < JT / 32; w++) M = fmaxf(M, warp_m[w]);
+    const float mc = scaled_max(M, a.c2);
+    for (int p = t; p < pieces; p += JT) {
         const float2 ml = a.ml[slot(p) * a.gp + g];
-        fm[p * a.gp + g] = ml.x;
-        fl[p * a.gp + g] = ml.y;
+        const float f = prob(ml.x, a.c2, mc);
+        factor[p] = f;
+        L = __fmaf_rn(ml.y, f, L);
     }
-    __syncthreads();
-    for (int g = warp; g < heads; g += JT / 32) {
-        float M = -INFINITY, L = 0.0f;
-        for (int p = lane; p < pieces; p += 32) M = fmaxf(M, fm[p * a.gp + g]);
-        M = warp_max_f32(M);
-        const float mc = scaled_max(M, a.c2);
-        for (int p = lane; p < pieces; p += 32) {
-            const float f = prob(fm[p * a.gp + g], a.c2, mc);
-            fm[p * a.gp + g] = f;
-            L = __fmaf_rn(fl[p * a.gp + g], f, L);
-        }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-        if (lane == 0) {
-            top[g] = M;
-            sum[g] = L;
-        }
-    }
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if (lane == 0) warp_l[warp] = L;
     __syncthreads();
-    if (a.stat && t < heads) a.stat[(int64_t)r * a.q_heads + qh0 + t] = make_float2(top[t], 1.0f / sum[t]);
-    const int columns = heads * a.dim / 4;  // dim is a multiple of 4
-    int ct = 32;
-    while (ct < columns && ct < JT) ct <<= 1;
-    const int splits = JT / ct, part = t / ct;
-    for (int c0 = 0; c0 < columns; c0 += ct) {
-        const int c = c0 + t % ct, g = c < columns ? 4 * c / a.dim : 0;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (c < columns) {
-#pragma unroll 8
-            for (int p = part; p < pieces; p += splits) {
-                const float4 x = reinterpret_cast<const float4 *>(a.part + (int64_t)slot(p) * a.gp * a.dim)[c];
-                const float f = fm[p * a.gp + g];
-                o.x = __fmaf_rn(x.x, f, o.x);
-                o.y = __fmaf_rn(x.y, f, o.y);
-                o.z = __fmaf_rn(x.z, f, o.z);
-                o.w = __fmaf_rn(x.w, f, o.w);
-            }
-        }
-        red[t] = o;
-        __syncthreads();
-        if (part == 0 && c < columns) {
-            for (int s = 1; s < splits; s++) {
-                const float4 x = red[t + s * ct];
-                o.x += x.x;
-                o.y += x.y;
-                o.z += x.z;
-                o.w += x.w;
-            }
-            const float L = sum[g], y[4] = {o.x, o.y, o.z, o.w};
+    L = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                store_f32_as(a.out, a.q_type, out + 4 * c + e, L == 0.0f ? 0.0f : y[e] / L);
-        }
-        __syncthreads();
-    }
+    for (int w = 0; w < JT / 32; w++) L += warp_l[w];
+    if (a.stat && t == 0) a.stat[(int64_t)r * a.q_heads + qh] = make_float2(M, 1.0f / L);
+    const int columns = a.dim / 4;   // at most 64
+    int ct = 8;
+    while (ct < columns) ct <<= 1;
+    const int splits = JT / ct, part = t / ct, c = t % ct;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (c < columns)
+#pragma unroll 4
+        for (int p = part; p < pieces; p += splits)
+            o = fma4(reinterpret_cast<const float4 *>(a.part + ((int64_t)slot(p) * a.gp + g) * a.dim)[c], factor[p], o);
+    red[t] = o;
+    __syncthreads();
+    if (part || c >= columns) return;
+    for (int s = 1; s < splits; s++) o = fma4(red[t + s * ct], 1.0f, o);
+    store4_as(a.out, a.q_type, r * a.out_stride + (long long)qh * a.dim + 4 * c, over4(o, L));
 }
 
 // weights[r][kv head][j] += sum over the kv head's query heads of p_j, from the
@@ -133,13 +104,13 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(const AttnArgs a, fl
             st[t] = make_float2(scaled_max(x.x, a.c2), x.y);
         }
         __syncthreads();
-        const float *s = a.scores + ((int64_t)r * a.q_heads + kvh * a.group + g0) * a.width;
+        const float *s = a.scores + ((int64_t)r * a.q_heads + kvh * a.group + g0) * a.score_stride;
 #pragma unroll 2
         for (int g = 0; g < heads; g++) {
             float x[U];
 #pragma unroll
             for (int u = 0; u < U; u++)
-                x[u] = i0 + u * 256 < rv.vis ? s[(int64_t)g * a.width + i0 + u * 256] : -INFINITY;
+                x[u] = i0 + u * 256 < rv.vis ? s[(int64_t)g * a.score_stride + i0 + u * 256] : -INFINITY;
 #pragma unroll
             for (int u = 0; u < U; u++) sum[u] = __fmaf_rn(prob(x[u], a.c2, st[g].x), st[g].y, sum[u]);
         }
@@ -161,7 +132,7 @@ Sizes attn_sizes(size_t rows, size_t q_heads, size_t dim, size_t width) {
     s.part = up(slots * dim * 4);
     s.ml = up(slots * 8);
     s.stat = width ? up(rows * q_heads * 8) : 0;
-    s.scores = width ? up(rows * q_heads * width * 4) : 0;
+    s.scores = width ? up(rows * q_heads * ((width + 1) & ~(size_t)1) * 4) : 0;
     s.total = s.part + s.ml + s.stat + s.scores;
     return s;
 }
@@ -171,9 +142,9 @@ int launch_attention(AttnArgs a, int dtype, float *weights, size_t w_row, size_t
                    : dtype == FOCR_F16 ? launch_attention_f16(a, st)
                                        : launch_attention_bf16(a, st);
     if (rc) return rc;
-    const int blocks = attn_blocks(), smem = blocks * a.gp * 8;
-    if (smem > 24 * 1024) FOCR_CUDA_TRY(set_max_dynamic_smem((const void *)paged_join_kernel, 96 * 1024));
-    FOCR_CUDA_TRY(launch_pdl(paged_join_kernel, dim3(a.c.kv_heads * a.head_chunks, a.rows), JT, smem, st, a, blocks));
+    const int blocks = attn_blocks();
+    if (blocks > 1)
+        FOCR_CUDA_TRY(launch_pdl(paged_join_kernel, dim3(blocks - 1, a.gp < a.group ? a.gp : a.group), JT, blocks * 4, st, a, blocks));
     if (weights)
         FOCR_CUDA_TRY(launch_pdl(paged_weights_kernel, dim3((a.width + 1023) / 1024, a.c.kv_heads, a.rows), 256, 0, st,
                                  a, weights, (long long)w_row, (long long)w_head));
@@ -255,6 +226,7 @@ int focr_paged_attention(const focr_paged_cache *cache, const void *q, int q_dty
         a.q_type = q_dtype;
         a.window = window > INT32_MAX ? 0 : (int)window;
         a.width = (int)width;
+        a.score_stride = (int)((width + 1) & ~(size_t)1);
         a.cap = weights ? (int)width : (int)cap;
         a.c2 = (float)(scale * 1.4426950408889634);
         const size_t q_size = dtype_bytes(q_dtype);

@@ -43,6 +43,7 @@ struct AttnArgs {
     float2 *ml;      // [block][2][gp] partial (m, l)
     long long q_stride, out_stride;
     int rows, group, q_heads, dim, q_type, window, cap, width;
+    int score_stride;     // floats between the scores of two query heads, even
     int gp, head_chunks;  // query heads that a block takes together; blocks of them a kv head
     int tile_shift;       // log2 of a block tile's positions
     float c2;             // scale * log2(e)
@@ -147,6 +148,17 @@ __device__ __forceinline__ unsigned long long run_count(unsigned long long total
     return min(total, (unsigned long long)blocks);
 }
 
+// The last row whose units begin at or before u.
+__device__ __forceinline__ int row_of_unit(const int *pre, int rows, int hc_count, unsigned long long u) {
+    int lo = 0, hi = rows;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if ((unsigned long long)pre[mid] * hc_count <= u) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
 // The run of units of one block, and the piece of a (row, kv head, chunk of its
 // query heads) it stands at.
 struct Segment {
@@ -169,13 +181,7 @@ struct Run {
     }
     __device__ bool next(const AttnArgs &a, const int *pre, Segment *s) {
         if (u >= end) return false;
-        // the last row whose units begin at or before u
-        int lo = 0, hi = a.rows;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if ((unsigned long long)pre[mid] * hc_count <= u) lo = mid;
-            else hi = mid;
-        }
+        const int lo = row_of_unit(pre, a.rows, hc_count, u);
         const int tiles = pre[lo + 1] - pre[lo];
         const unsigned long long off = u - (unsigned long long)pre[lo] * hc_count;
         const int hc = (int)(off / tiles);
@@ -194,14 +200,48 @@ struct Run {
     }
 };
 
+// Four neighbouring elements, as one store where they lie on its boundary.
+__device__ __forceinline__ void store4_as(void *p, int dtype, int64_t i, float4 x) {
+    if (dtype == FOCR_F32) {
+        float *q = static_cast<float *>(p) + i;
+        if ((uintptr_t)q % 16 == 0) {
+            *reinterpret_cast<float4 *>(q) = x;
+            return;
+        }
+    } else {
+        uint16_t *q = static_cast<uint16_t *>(p) + i;
+        if ((uintptr_t)q % 8 == 0) {
+            alignas(8) uint16_t y[4];
+            store_f32_as(y, dtype, 0, x.x);
+            store_f32_as(y, dtype, 1, x.y);
+            store_f32_as(y, dtype, 2, x.z);
+            store_f32_as(y, dtype, 3, x.w);
+            *reinterpret_cast<uint2 *>(q) = *reinterpret_cast<const uint2 *>(y);
+            return;
+        }
+    }
+    store_f32_as(p, dtype, i, x.x);
+    store_f32_as(p, dtype, i + 1, x.y);
+    store_f32_as(p, dtype, i + 2, x.z);
+    store_f32_as(p, dtype, i + 3, x.w);
+}
+__device__ __forceinline__ float4 fma4(float4 x, float f, float4 o) {
+    return make_float4(__fmaf_rn(x.x, f, o.x), __fmaf_rn(x.y, f, o.y), __fmaf_rn(x.z, f, o.z),
+                       __fmaf_rn(x.w, f, o.w));
+}
+__device__ __forceinline__ float4 over4(float4 x, float L) {
+    return L == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(x.x / L, x.y / L, x.z / L, x.w / L);
+}
+
 // Joins the block's warps, whose sums lie in shared memory `apart` floats from
 // one another ([GP][D], m[GP], l[GP]), and writes the segment's output or piece.
 template <int GP, int D>
 __device__ __forceinline__ void finish_segment(const AttnArgs &a, const Segment &s, const float *all, int apart) {
-    for (int x = threadIdx.x; x < GP * D; x += ATTN_WARPS * 32) {
-        const int g = x / D, d = x % D;
-        if (g >= s.heads || d >= a.dim) continue;
-        float M = -INFINITY, L = 0.0f, o = 0.0f;
+    for (int x = threadIdx.x; x < s.heads * (D / 4); x += ATTN_WARPS * 32) {
+        const int g = x / (D / 4), d = x % (D / 4) * 4;
+        if (d >= a.dim) continue;   // a multiple of 4
+        float M = -INFINITY, L = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int w = 0; w < ATTN_WARPS; w++) M = fmaxf(M, all[w * apart + GP * D + g]);
         const float mc = scaled_max(M, a.c2);
@@ -209,16 +249,26 @@ __device__ __forceinline__ void finish_segment(const AttnArgs &a, const Segment 
         for (int w = 0; w < ATTN_WARPS; w++) {
             const float f = prob(all[w * apart + GP * D + g], a.c2, mc);
             L = __fmaf_rn(all[w * apart + GP * D + GP + g], f, L);
-            o = __fmaf_rn(all[w * apart + x], f, o);
+            o = fma4(*reinterpret_cast<const float4 *>(all + w * apart + g * D + d), f, o);
         }
         if (s.whole) {
-            store_f32_as(a.out, a.q_type, s.r * a.out_stride + (long long)(s.qh0 + g) * a.dim + d,
-                         L == 0.0f ? 0.0f : o / L);
+            store4_as(a.out, a.q_type, s.r * a.out_stride + (long long)(s.qh0 + g) * a.dim + d, over4(o, L));
             if (a.stat && d == 0) a.stat[(int64_t)s.r * a.q_heads + s.qh0 + g] = make_float2(M, 1.0f / L);
         } else {
-            a.part[((int64_t)s.slot * GP + g) * a.dim + d] = o;
+            *reinterpret_cast<float4 *>(a.part + ((int64_t)s.slot * GP + g) * a.dim + d) = o;
             if (d == 0) a.ml[s.slot * GP + g] = make_float2(M, L);
         }
+    }
+}
+
+// The rows that have no units, shared out over the blocks: zeros where nothing is
+// visible, NaN for a length that passes the table.
+__device__ __forceinline__ void finish_empty_rows(const AttnArgs &a, const int *pre) {
+    for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        if (pre[r + 1] != pre[r]) continue;
+        const float x = row_view(a, r).bad ? NAN : 0.0f;
+        for (int i = threadIdx.x; i < a.q_heads * a.dim; i += ATTN_WARPS * 32)
+            store_f32_as(a.out, a.q_type, r * a.out_stride + i, x);
     }
 }
 

@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
 
     const int qr = lane >> 2, qc = (lane & 3) * 2;   // this lane's row and columns of a tile
     const int mi = lane >> 3, rr = lane & 7;         // its matrix and row when loading one
+    finish_empty_rows(a, pre);
     Run run(a, pre);
     Segment sg;
     while (run.next(a, pre, &sg)) {
@@ -91,12 +92,16 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
 
         uint32_t qa[D / 16][4];
         const uint16_t *qp = static_cast<const uint16_t *>(a.q) + r * a.q_stride + (long long)sg.qh0 * a.dim;
+        const bool pairs = (uintptr_t)qp % 4 == 0;   // dim is even
 #pragma unroll
         for (int ks = 0; ks < D / 16; ks++)
 #pragma unroll
             for (int x = 0; x < 4; x++) {
                 const int g = qr + (x & 1) * 8, d = ks * 16 + (x >> 1) * 8 + qc;
-                qa[ks][x] = g < heads && d < a.dim ? qp[g * a.dim + d] | (uint32_t)qp[g * a.dim + d + 1] << 16 : 0;
+                const uint16_t *p = qp + g * a.dim + d;
+                qa[ks][x] = 0;
+                if (g < heads && d < a.dim)
+                    qa[ks][x] = pairs ? *reinterpret_cast<const uint32_t *>(p) : p[0] | (uint32_t)p[1] << 16;
             }
         float acc[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -147,19 +152,27 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
                     mma16816<T>(s[2 * p + 1], qa[ks], b[2], b[3]);
                 }
             const int i0 = (tile * ATTN_WARPS + warp) * KEYS + qc;
+            if (a.scores) {   // pairs: the stride is even, what lies behind vis is never read
+                float *sp = a.scores + ((int64_t)r * a.q_heads + sg.qh0 + qr) * a.score_stride + i0;
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    if (i0 + t * 8 >= rv.vis) break;
+                    if (qr < heads) *reinterpret_cast<float2 *>(sp + t * 8) = make_float2(s[t][0], s[t][1]);
+                    if (qr + 8 < heads)
+                        *reinterpret_cast<float2 *>(sp + 8ll * a.score_stride + t * 8) = make_float2(s[t][2], s[t][3]);
+                }
+            }
             float top[2] = {-INFINITY, -INFINITY};
+            if (i0 - qc + KEYS > rv.vis)   // the row's last tile
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+                        if (i0 + t * 8 + (x & 1) >= rv.vis) s[t][x] = -INFINITY;
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    const int i = i0 + t * 8 + (x & 1);
-                    if (i >= rv.vis) s[t][x] = -INFINITY;
-                    else if (a.scores) {
-                        const int g = qr + (x >> 1) * 8;
-                        if (g < heads) a.scores[((int64_t)r * a.q_heads + sg.qh0 + g) * a.width + i] = s[t][x];
-                    }
-                    top[x >> 1] = fmaxf(top[x >> 1], s[t][x]);
-                }
+                for (int x = 0; x < 4; x++) top[x >> 1] = fmaxf(top[x >> 1], s[t][x]);
             if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
 #pragma unroll
                 for (int y = 0; y < 2; y++) {

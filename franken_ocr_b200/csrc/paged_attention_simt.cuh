@@ -51,6 +51,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
     const int my_it = (lane & (LPK / 2) ? 4 : 0) + (lane & (LPK / 4) ? 2 : 0) + (lane & (LPK / 8) ? 1 : 0);
     const int my_key = my_it * KPI + sub;
 
+    finish_empty_rows(a, pre);
     Run run(a, pre);
     Segment sg;
     while (run.next(a, pre, &sg)) {
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
                 l[g] += p;
                 probs[g * KEYS + sub * ITS + my_it] = p;
                 if (a.scores && live && g < heads)
-                    a.scores[((int64_t)r * a.q_heads + qh0 + g) * a.width + i] = sc;
+                    a.scores[((int64_t)r * a.q_heads + qh0 + g) * a.score_stride + i] = sc;
             }
             __syncwarp();
 #pragma unroll
