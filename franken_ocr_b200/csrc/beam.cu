@@ -75,8 +75,8 @@ __device__ __forceinline__ float2 exp_below(float2 x, float base) {
     const float2 high = make_float2(1.44269502f, 1.44269502f), low = make_float2(1.92596299e-8f, 1.92596299e-8f);
     const float up = SHIFT - base;                     // base is an integer: exact
     const float2 t = fma2(x, high, make_float2(up, up));
-    const float2 n = add2(t, make_float2(-up, -up));   // the nearest integer
-    const float2 r = fma2(x, low, fma2(x, high, make_float2(-n.x, -n.y)));
+    const float2 n = fma2(t, make_float2(-1.0f, -1.0f), make_float2(up, up));   // minus the nearest integer
+    const float2 r = fma2(x, low, fma2(x, high, n));
     float2 p;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p.x) : "f"(r.x));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p.y) : "f"(r.y));
@@ -186,17 +186,20 @@ __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) 
     // the few that are large or candidates
     const float low = bound, few = fminf(low, near);
     int c = 0;
+    uint32_t hits = 0;   // groups of 4 with one of them
 #pragma unroll
     for (int g = 0; g < PER; g += 4)
-        if (fmaxf(fmaxf(v[g], v[g + 1]), fmaxf(v[g + 2], v[g + 3])) >= few)
+        if (fmaxf(fmaxf(v[g], v[g + 1]), fmaxf(v[g + 2], v[g + 3])) >= few) {
+            hits |= 1u << g / 4;
 #pragma unroll
             for (int i = g; i < g + 4; i++) c += v[i] >= few && v[i] > -INFINITY;
+        }
     if (c) {
         int k = atomicAdd(&count, c);
         if (k + c <= LIST)
 #pragma unroll
             for (int g = 0; g < PER; g += 4)
-                if (fmaxf(fmaxf(v[g], v[g + 1]), fmaxf(v[g + 2], v[g + 3])) >= few)
+                if (hits >> g / 4 & 1)
 #pragma unroll
                     for (int i = g; i < g + 4; i++)
                         if (v[i] >= few && v[i] > -INFINITY) {
@@ -213,6 +216,21 @@ __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) 
         if (got <= LIST) y = lx[i];
         else if (first + i < a.vocab) y = fminf(to_f32<T>(x[first + i]), LARGEST);
         if (y >= near) large += __double2ll_rn(exp((double)y - (double)m) * 0x1p48);
+    }
+    if (got <= LIST) {   // ranked by other warps than the first, which has the terms above
+        for (int i = (t + ST - 32) % ST; i < got; i += ST) {
+            const float y = lx[i];
+            const int c = lt[i];
+            if (y < low) continue;
+            int rank = 0;
+#pragma unroll 8
+            for (int j = 0; j < got; j++) rank += (lx[j] > y) | ((lx[j] == y) & (lt[j] < c));
+            if (rank < a.n) {
+                a.cx[at * a.n + rank] = y;
+                a.ct[at * a.n + rank] = c;
+            }
+        }
+        for (int k = got + t; k < a.n; k += ST) a.ct[at * a.n + k] = -1;   // fewer than n: all are in the list
     }
     for (int o = 16; o > 0; o >>= 1) {
         sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -232,22 +250,7 @@ __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) 
         // the small terms were taken relative to 2^base
         a.ps[at] = sum * exp((double)base * 0.693147180559945309 - (double)high) + (double)large * 0x1p-48;
     }
-    if (got <= LIST) {
-        for (int i = t; i < got; i += ST) {
-            const float y = lx[i];
-            const int c = lt[i];
-            if (y < low) continue;
-            int rank = 0;
-#pragma unroll 8
-            for (int j = 0; j < got; j++) rank += (lx[j] > y) | ((lx[j] == y) & (lt[j] < c));
-            if (rank < a.n) {
-                a.cx[at * a.n + rank] = y;
-                a.ct[at * a.n + rank] = c;
-            }
-        }
-        for (int k = got + t; k < a.n; k += ST) a.ct[at * a.n + k] = -1;   // fewer than n: all are in the list
-        return;
-    }
+    if (got <= LIST) return;
     float last = INFINITY;
     int last_token = -1;
     for (int k = 0; k < a.n; k++) {  // LIST > n: there are that many
@@ -439,7 +442,7 @@ __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
 
 // Logits a thread holds: with few rows, short strips spread them over the SMs.
 int strip_of(size_t rows, size_t vocab) {
-    return rows * ((vocab + ST * 32) / (ST * 32)) < (size_t)num_sms() * 2 ? ST * 8 : ST * 32;
+    return rows * ((vocab + ST * 32) / (ST * 32)) < (size_t)num_sms() * 2 ? ST * 16 : ST * 32;
 }
 size_t strip_count(size_t vocab, int strip) { return (vocab + strip - 1) / strip; }
 
@@ -603,10 +606,10 @@ int focr_beam_select(const void *logits, int dtype, size_t batch, size_t beams, 
         a.pm = (float *)(ws + sz.ps + sz.cx + sz.ct);
         cudaStream_t st = (cudaStream_t)stream;
         const dim3 grid(a.strips, (unsigned)(batch * beams));
-        const bool few = strip == ST * 8;
-        auto *part = dtype == FOCR_F32 ? (few ? select_part_kernel<float, 8> : select_part_kernel<float, 32>)
-                   : dtype == FOCR_F16 ? (few ? select_part_kernel<__half, 8> : select_part_kernel<__half, 32>)
-                                       : (few ? select_part_kernel<__nv_bfloat16, 8> : select_part_kernel<__nv_bfloat16, 32>);
+        const bool few = strip == ST * 16;
+        auto *part = dtype == FOCR_F32 ? (few ? select_part_kernel<float, 16> : select_part_kernel<float, 32>)
+                   : dtype == FOCR_F16 ? (few ? select_part_kernel<__half, 16> : select_part_kernel<__half, 32>)
+                                       : (few ? select_part_kernel<__nv_bfloat16, 16> : select_part_kernel<__nv_bfloat16, 32>);
         FOCR_CUDA_TRY(launch_pdl(part, grid, ST, 0, st, a));
         FOCR_CUDA_TRY(launch_pdl(select_join_kernel, (unsigned)batch, ST, 0, st, a));
         return FOCR_OK;
