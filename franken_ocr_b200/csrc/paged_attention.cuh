@@ -200,6 +200,38 @@ struct Run {
     }
 };
 
+// The tiles of a block's run in order, across its segments, for the copies that run
+// ahead of the arithmetic.  A warp's lane `i` finds the place of the tile's i-th
+// position.
+template <int KEYS> struct Feed {
+    Run run;
+    const int32_t *pages;
+    int64_t head;          // the kv head's offset in a page
+    RowView rv;
+    int tile, end;
+
+    __device__ Feed(const AttnArgs &a, const int *pre) : run(a, pre), tile(0), end(0) {}
+    // The byte offset of this lane's position of the next tile, -1 where there is
+    // none; *bad if its page is not in the pool.
+    __device__ int64_t next(const AttnArgs &a, const int *pre, int warp, int lane, bool *bad) {
+        *bad = false;
+        if (tile == end) {
+            Segment s;
+            if (!run.next(a, pre, &s)) return -1;
+            pages = a.c.table + s.r * a.c.table_stride;
+            head = s.kvh * a.c.head_stride;
+            rv = s.rv;
+            tile = s.t0;
+            end = s.t1;
+        }
+        const int i = (tile++ * ATTN_WARPS + warp) * KEYS + lane;
+        if (lane >= KEYS || i >= rv.vis) return -1;
+        const int64_t o = a.c.offset(pages, (uint32_t)(i < rv.ref ? i : i + rv.gap));
+        *bad = o < 0;
+        return o < 0 ? o : o + head;
+    }
+};
+
 // Four neighbouring elements, as one store where they lie on its boundary.
 __device__ __forceinline__ void store4_as(void *p, int dtype, int64_t i, float4 x) {
     if (dtype == FOCR_F32) {
@@ -233,23 +265,29 @@ __device__ __forceinline__ float4 over4(float4 x, float L) {
     return L == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(x.x / L, x.y / L, x.z / L, x.w / L);
 }
 
-// Joins the block's warps, whose sums lie in shared memory `apart` floats from
-// one another ([GP][D], m[GP], l[GP]), and writes the segment's output or piece.
-template <int GP, int D>
-__device__ __forceinline__ void finish_segment(const AttnArgs &a, const Segment &s, const float *all, int apart) {
-    for (int x = threadIdx.x; x < s.heads * (D / 4); x += ATTN_WARPS * 32) {
-        const int g = x / (D / 4), d = x % (D / 4) * 4;
+// What the warps of a block hand over at the end of a segment: HR heads at a time,
+// beside the rings, into which the next segment's rows are already flowing.
+template <int HR, int D> struct Handover {
+    float o[ATTN_WARPS][HR][D], m[ATTN_WARPS][HR], l[ATTN_WARPS][HR];
+};
+
+// Joins the block's warps for the heads g0 .. g0 + HR - 1 of the segment, and
+// writes their output or piece.
+template <int GP, int HR, int D>
+__device__ __forceinline__ void finish_heads(const AttnArgs &a, const Segment &s, const Handover<HR, D> &h, int g0) {
+    for (int x = threadIdx.x; x < min(HR, s.heads - g0) * (D / 4); x += ATTN_WARPS * 32) {
+        const int i = x / (D / 4), g = g0 + i, d = x % (D / 4) * 4;
         if (d >= a.dim) continue;   // a multiple of 4
         float M = -INFINITY, L = 0.0f;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int w = 0; w < ATTN_WARPS; w++) M = fmaxf(M, all[w * apart + GP * D + g]);
+        for (int w = 0; w < ATTN_WARPS; w++) M = fmaxf(M, h.m[w][i]);
         const float mc = scaled_max(M, a.c2);
 #pragma unroll
         for (int w = 0; w < ATTN_WARPS; w++) {
-            const float f = prob(all[w * apart + GP * D + g], a.c2, mc);
-            L = __fmaf_rn(all[w * apart + GP * D + GP + g], f, L);
-            o = fma4(*reinterpret_cast<const float4 *>(all + w * apart + g * D + d), f, o);
+            const float f = prob(h.m[w][i], a.c2, mc);
+            L = __fmaf_rn(h.l[w][i], f, L);
+            o = fma4(*reinterpret_cast<const float4 *>(&h.o[w][i][d]), f, o);
         }
         if (s.whole) {
             store4_as(a.out, a.q_type, s.r * a.out_stride + (long long)(s.qh0 + g) * a.dim + d, over4(o, L));

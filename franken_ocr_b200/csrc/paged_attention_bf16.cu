@@ -5,8 +5,7 @@
 namespace focr {
 
 int launch_attention_bf16(AttnArgs &a, cudaStream_t st) {
-    if (a.q_type == FOCR_BF16 && a.group >= MMA_HEADS) return launch_mma_dim<__nv_bfloat16>(a, st);
-    return launch_simt_dim<__nv_bfloat16>(a, st);
+    return mma_takes<__nv_bfloat16>(a) ? launch_mma_dim<__nv_bfloat16>(a, st) : launch_simt_dim<__nv_bfloat16>(a, st);
 }
 
 }  // namespace focr

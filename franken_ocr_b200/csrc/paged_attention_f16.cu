@@ -5,8 +5,7 @@
 namespace focr {
 
 int launch_attention_f16(AttnArgs &a, cudaStream_t st) {
-    if (a.q_type == FOCR_F16 && a.group >= MMA_HEADS) return launch_mma_dim<__half>(a, st);
-    return launch_simt_dim<__half>(a, st);
+    return mma_takes<__half>(a) ? launch_mma_dim<__half>(a, st) : launch_simt_dim<__half>(a, st);
 }
 
 }  // namespace focr

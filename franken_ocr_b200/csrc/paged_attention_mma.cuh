@@ -1,5 +1,5 @@
-// Attention over a paged cache on the tensor cores: query and cache of one
-// 16-bit type, up to 16 query heads of a kv head as the rows of a matrix tile.
+// Attention over a paged 16-bit cache on the tensor cores: up to 16 query heads of a
+// kv head, of the cache's type or f32, as the rows of a matrix tile.
 //
 // A warp takes KEYS positions at a time: S = Q K^T and O += P V as 16x8x16 warp
 // products straight from the staged rows, whose 16-byte chunks are swizzled by
@@ -7,8 +7,9 @@
 // bound by the cache's bytes, not by the products (48 of them, ~100 cycles of
 // an SM, for 8 KB that take ~350 cycles to arrive), so the warp products, which
 // leave every warp on its own without a block barrier, cost nothing against
-// larger tiles.  P stays exact to 16 bits more than its type: it is split
-// into a high and a low part and multiplied twice.
+// larger tiles.  P, and a query in f32, are split into parts of the cache's type that
+// are multiplied one after the other, so nothing is rounded to fewer bits than the
+// output has.
 #pragma once
 
 #include "paged_attention.cuh"
@@ -24,8 +25,12 @@ template <int D> struct MmaTile {
     static constexpr int STAGES = HALF > 4096 ? 2 : 3;
     static constexpr int BLOCK = ATTN_WARPS * KEYS;
 };
+// Heads that the warps hand over at a time: 2 KB a warp, or all where one block
+// fills an SM.
+template <int D> constexpr int mma_round() { return D == 256 ? 16 : 512 / D; }
 template <int D> constexpr int mma_smem() {
-    return ATTN_WARPS * MmaTile<D>::STAGES * 2 * MmaTile<D>::HALF + (ATTN_ROWS + 1) * 4;
+    return ATTN_WARPS * MmaTile<D>::STAGES * 2 * MmaTile<D>::HALF + (int)sizeof(Handover<mma_round<D>(), D>) +
+           (ATTN_ROWS + 1) * 4;
 }
 
 template <typename T> __device__ __forceinline__ void mma16816(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
@@ -46,33 +51,41 @@ template <bool TRANS> __device__ __forceinline__ void ldmatrix4(uint32_t *r, uin
         asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-// The high parts of two values as a pair, and what they leave.
-template <typename T> __device__ __forceinline__ uint32_t split_pair(float x, float y, uint32_t *low) {
+// The pair (x, y) in T, and in *x, *y what it leaves of them.
+template <typename T> __device__ __forceinline__ uint32_t take_pair(float *x, float *y) {
     if constexpr (std::is_same<T, __half>::value) {
-        const __half2 h = __floats2half2_rn(x, y);
+        const __half2 h = __floats2half2_rn(*x, *y);
         const float2 f = __half22float2(h);
-        const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-        *low = *reinterpret_cast<const uint32_t *>(&l);
+        *x -= f.x;
+        *y -= f.y;
         return *reinterpret_cast<const uint32_t *>(&h);
     } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        const __nv_bfloat162 h = __floats2bfloat162_rn(*x, *y);
         const float2 f = __bfloat1622float2(h);
-        const __nv_bfloat162 l = __floats2bfloat162_rn(x - f.x, y - f.y);
-        *low = *reinterpret_cast<const uint32_t *>(&l);
+        *x -= f.x;
+        *y -= f.y;
         return *reinterpret_cast<const uint32_t *>(&h);
     }
 }
 
-template <typename T, int D>
+// PARTS: how many values of T a query element and a probability are split into.
+// A query of type T is one, and its probabilities two; an f32 query takes three
+// of both (24 bits of bf16, 33 of f16).
+template <typename T, int D, bool F32Q>
 __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_attention_mma_kernel(const AttnArgs a) {
     using S = MmaTile<D>;
-    constexpr int GP = 16, KEYS = S::KEYS, NT = KEYS / 8, ITS = S::HALF / 512;
-    // f16 holds nothing below 2^-24: probabilities, at most 1, are scaled up
-    constexpr float PS = std::is_same<T, __half>::value ? 2048.0f : 1.0f;
+    constexpr int GP = 16, KEYS = S::KEYS, NT = KEYS / 8, ITS = S::HALF / 512, HR = mma_round<D>();
+    constexpr int QP = F32Q ? 3 : 1, PP = F32Q ? 3 : 2;
+    constexpr bool HALF = std::is_same<T, __half>::value;
+    // f16 holds nothing below 2^-24: probabilities, at most 1, are scaled up, and a
+    // head's f32 query by the power of two that brings its largest value near 2^14
+    constexpr float PS = HALF ? 2048.0f : 1.0f;
+    constexpr int RINGS = ATTN_WARPS * S::STAGES * 2 * S::HALF;
     extern __shared__ __align__(128) char smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     char *ring = smem + warp * S::STAGES * 2 * S::HALF;
-    int *pre = reinterpret_cast<int *>(smem + ATTN_WARPS * S::STAGES * 2 * S::HALF);
+    auto &hand = *reinterpret_cast<Handover<HR, D> *>(smem + RINGS);
+    int *pre = reinterpret_cast<int *>(smem + RINGS + sizeof(hand));
     const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
 
     pdl_wait();
@@ -81,94 +94,134 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
 
     const int qr = lane >> 2, qc = (lane & 3) * 2;   // this lane's row and columns of a tile
     const int mi = lane >> 3, rr = lane & 7;         // its matrix and row when loading one
+    Feed<KEYS> feed(a, pre);
+    uint32_t bad_stages = 0;   // of the stages in flight, those with a page outside the pool
+    auto issue = [&](int stage, int64_t mine) {
+        const uint32_t dst = ring_s + stage * 2 * S::HALF;
+#pragma unroll
+        for (int it = 0; it < ITS; it++) {
+            const int x = it * 32 + lane, key = x / S::CH, c = x % S::CH;
+            const int64_t o = __shfl_sync(0xffffffffu, mine, key);
+            const bool have = o >= 0 && c * 16 < a.c.row_bytes;
+            const int64_t src = have ? o + c * 16 : 0;
+            const uint32_t to = dst + key * S::DB + ((c ^ (key & 7)) << 4);
+            cp_async16(to, a.c.k + src, have ? 16 : 0);
+            cp_async16(to + S::HALF, a.c.v + src, have ? 16 : 0);
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < S::STAGES; s++) {
+        bool bad;
+        issue(s, feed.next(a, pre, warp, lane, &bad));
+        bad_stages |= (uint32_t)bad << s;
+        cp_async_commit();
+    }
     finish_empty_rows(a, pre);
+
+    int stage = 0;
     Run run(a, pre);
     Segment sg;
     while (run.next(a, pre, &sg)) {
-        const int r = sg.r, heads = sg.heads, t0 = sg.t0, t1 = sg.t1;
-        const RowView rv = sg.rv;
-        const int32_t *pages = a.c.table + r * a.c.table_stride;
-        const char *kb = a.c.k + sg.kvh * a.c.head_stride, *vb = a.c.v + sg.kvh * a.c.head_stride;
-
-        uint32_t qa[D / 16][4];
-        const uint16_t *qp = static_cast<const uint16_t *>(a.q) + r * a.q_stride + (long long)sg.qh0 * a.dim;
-        const bool pairs = (uintptr_t)qp % 4 == 0;   // dim is even
+        const int r = sg.r, heads = sg.heads, vis = sg.rv.vis;
+        uint32_t qa[QP][D / 16][4];
+        float unscale[2] = {1.0f, 1.0f};
+        if constexpr (F32Q) {
+            const float *qp = static_cast<const float *>(a.q) + r * a.q_stride + (long long)sg.qh0 * a.dim;
+            float scale[2] = {1.0f, 1.0f};
+            if constexpr (HALF) {
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ks++)
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const int g = qr + (x & 1) * 8, d = ks * 16 + (x >> 1) * 8 + qc;
-                const uint16_t *p = qp + g * a.dim + d;
-                qa[ks][x] = 0;
-                if (g < heads && d < a.dim)
-                    qa[ks][x] = pairs ? *reinterpret_cast<const uint32_t *>(p) : p[0] | (uint32_t)p[1] << 16;
+                for (int y = 0; y < 2; y++) {
+                    float top = 0.0f;
+                    if (qr + y * 8 < heads)
+                        for (int d = lane & 3; d < a.dim; d += 4) top = fmaxf(top, fabsf(qp[(qr + y * 8) * a.dim + d]));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    // 2^(13 - exponent), between 2^-100 and 2^100; 0, inf and NaN as they are
+                    const int e = (int)(__float_as_uint(top) >> 23) - 127;
+                    if (top > 0.0f && e < 128) {
+                        const int up = max(-100, min(100, 13 - e));
+                        scale[y] = __int_as_float((127 + up) << 23);
+                        unscale[y] = __int_as_float((127 - up) << 23);
+                    }
+                }
             }
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ks++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int g = qr + (x & 1) * 8, d = ks * 16 + (x >> 1) * 8 + qc;
+                    const bool have = g < heads && d < a.dim;   // dim is even
+                    float q0 = have ? qp[g * a.dim + d] * scale[x & 1] : 0.0f;
+                    float q1 = have ? qp[g * a.dim + d + 1] * scale[x & 1] : 0.0f;
+#pragma unroll
+                    for (int p = 0; p < QP; p++) qa[p][ks][x] = take_pair<T>(&q0, &q1);
+                }
+        } else {
+            const uint16_t *qp = static_cast<const uint16_t *>(a.q) + r * a.q_stride + (long long)sg.qh0 * a.dim;
+            const bool pairs = (uintptr_t)qp % 4 == 0;   // dim is even
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ks++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int g = qr + (x & 1) * 8, d = ks * 16 + (x >> 1) * 8 + qc;
+                    const uint16_t *p = qp + g * a.dim + d;
+                    qa[0][ks][x] = 0;
+                    if (g < heads && d < a.dim)
+                        qa[0][ks][x] = pairs ? *reinterpret_cast<const uint32_t *>(p) : p[0] | (uint32_t)p[1] << 16;
+                }
+        }
         float acc[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < D / 8; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
         bool bad = false;
 
-        auto key_offset = [&](int tile) -> int64_t {  // of index `lane` of the warp's tile
-            const int i = (tile * ATTN_WARPS + warp) * KEYS + lane;
-            if (lane >= KEYS || i >= rv.vis || tile >= t1) return -1;
-            const int64_t o = a.c.offset(pages, (uint32_t)(i < rv.ref ? i : i + rv.gap));
-            bad |= o < 0;
-            return o;
-        };
-        auto issue = [&](int stage, int64_t mine) {
-            const uint32_t dst = ring_s + stage * 2 * S::HALF;
-#pragma unroll
-            for (int it = 0; it < ITS; it++) {
-                const int x = it * 32 + lane, key = x / S::CH, c = x % S::CH;
-                const int64_t o = __shfl_sync(0xffffffffu, mine, key);
-                const bool have = o >= 0 && c * 16 < a.c.row_bytes;
-                const int64_t src = have ? o + c * 16 : 0;
-                const uint32_t to = dst + key * S::DB + ((c ^ (key & 7)) << 4);
-                cp_async16(to, kb + src, have ? 16 : 0);
-                cp_async16(to + S::HALF, vb + src, have ? 16 : 0);
-            }
-        };
-#pragma unroll
-        for (int s = 0; s < S::STAGES; s++) {
-            issue(s, key_offset(t0 + s));
-            cp_async_commit();
-        }
-        int stage = 0;
-        for (int tile = t0; tile < t1; tile++) {
-            const int64_t next = key_offset(tile + S::STAGES);
+        for (int tile = sg.t0; tile < sg.t1; tile++) {
+            bad |= bad_stages >> stage & 1;
+            bool next_bad;
+            const int64_t next = feed.next(a, pre, warp, lane, &next_bad);
+            bad_stages = (bad_stages & ~(1u << stage)) | (uint32_t)next_bad << stage;
             cp_async_wait<S::STAGES - 1>();
             __syncwarp();
             const uint32_t ks_s = ring_s + stage * 2 * S::HALF, vs_s = ks_s + S::HALF;
             float s[NT][4];
 #pragma unroll
             for (int t = 0; t < NT; t++) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
+            // the smallest parts first: the sum's last steps are the ones that count
 #pragma unroll
             for (int ks = 0; ks < D / 16; ks++)
 #pragma unroll
                 for (int p = 0; p < KEYS / 16; p++) {
                     uint32_t b[4];
                     ldmatrix4<false>(b, ks_s + (p * 16 + (mi >> 1) * 8 + rr) * S::DB + (((ks * 2 + (mi & 1)) ^ rr) << 4));
-                    mma16816<T>(s[2 * p], qa[ks], b[0], b[1]);
-                    mma16816<T>(s[2 * p + 1], qa[ks], b[2], b[3]);
+#pragma unroll
+                    for (int part = QP - 1; part >= 0; part--) {
+                        mma16816<T>(s[2 * p], qa[part][ks], b[0], b[1]);
+                        mma16816<T>(s[2 * p + 1], qa[part][ks], b[2], b[3]);
+                    }
                 }
+            if constexpr (F32Q && HALF)
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) s[t][x] *= unscale[x >> 1];
             const int i0 = (tile * ATTN_WARPS + warp) * KEYS + qc;
             if (a.scores) {   // pairs: the stride is even, what lies behind vis is never read
                 float *sp = a.scores + ((int64_t)r * a.q_heads + sg.qh0 + qr) * a.score_stride + i0;
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    if (i0 + t * 8 >= rv.vis) break;
+                    if (i0 + t * 8 >= vis) break;
                     if (qr < heads) *reinterpret_cast<float2 *>(sp + t * 8) = make_float2(s[t][0], s[t][1]);
                     if (qr + 8 < heads)
                         *reinterpret_cast<float2 *>(sp + 8ll * a.score_stride + t * 8) = make_float2(s[t][2], s[t][3]);
                 }
             }
             float top[2] = {-INFINITY, -INFINITY};
-            if (i0 - qc + KEYS > rv.vis)   // the row's last tile
+            if (i0 - qc + KEYS > vis)   // the row's last tile
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
                     for (int x = 0; x < 4; x++)
-                        if (i0 + t * 8 + (x & 1) >= rv.vis) s[t][x] = -INFINITY;
+                        if (i0 + t * 8 + (x & 1) >= vis) s[t][x] = -INFINITY;
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -192,22 +245,24 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
             const float mc[2] = {scaled_max(m[0], a.c2), scaled_max(m[1], a.c2)};
 #pragma unroll
             for (int kk = 0; kk < KEYS / 16; kk++) {
-                uint32_t hi[4], lo[4];
+                uint32_t pa[PP][4];
 #pragma unroll
                 for (int x = 0; x < 4; x++) {  // registers: (row, low keys), (row + 8, low), (row, high), (row + 8, high)
                     const int t = 2 * kk + (x >> 1), y = x & 1;
-                    const float p0 = prob(s[t][2 * y], a.c2, mc[y]) * PS, p1 = prob(s[t][2 * y + 1], a.c2, mc[y]) * PS;
+                    float p0 = prob(s[t][2 * y], a.c2, mc[y]) * PS, p1 = prob(s[t][2 * y + 1], a.c2, mc[y]) * PS;
                     l[y] += p0 + p1;
-                    hi[x] = split_pair<T>(p0, p1, &lo[x]);
+#pragma unroll
+                    for (int p = 0; p < PP; p++) pa[p][x] = take_pair<T>(&p0, &p1);
                 }
 #pragma unroll
                 for (int jp = 0; jp < D / 16; jp++) {
                     uint32_t b[4];
                     ldmatrix4<true>(b, vs_s + (kk * 16 + (mi & 1) * 8 + rr) * S::DB + (((jp * 2 + (mi >> 1)) ^ rr) << 4));
-                    mma16816<T>(acc[2 * jp], hi, b[0], b[1]);
-                    mma16816<T>(acc[2 * jp + 1], hi, b[2], b[3]);
-                    mma16816<T>(acc[2 * jp], lo, b[0], b[1]);
-                    mma16816<T>(acc[2 * jp + 1], lo, b[2], b[3]);
+#pragma unroll
+                    for (int p = PP - 1; p >= 0; p--) {
+                        mma16816<T>(acc[2 * jp], pa[p], b[0], b[1]);
+                        mma16816<T>(acc[2 * jp + 1], pa[p], b[2], b[3]);
+                    }
                 }
             }
             __syncwarp();
@@ -215,49 +270,61 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
             cp_async_commit();
             stage = stage + 1 == S::STAGES ? 0 : stage + 1;
         }
-        cp_async_wait<0>();
 
         const bool any_bad = __any_sync(0xffffffffu, bad);
-        __syncwarp();
-        float *mine = reinterpret_cast<float *>(ring);  // [GP][D], m[GP], l[GP]
 #pragma unroll
         for (int y = 0; y < 2; y++) {
-            const int g = qr + y * 8;
-#pragma unroll
-            for (int j = 0; j < D / 8; j++) {
-                mine[g * D + j * 8 + qc] = acc[j][2 * y] * (1.0f / PS);
-                mine[g * D + j * 8 + qc + 1] = acc[j][2 * y + 1] * (1.0f / PS);
-            }
             l[y] += __shfl_xor_sync(0xffffffffu, l[y], 1);
             l[y] += __shfl_xor_sync(0xffffffffu, l[y], 2);
-            if ((lane & 3) == 0) {
-                mine[GP * D + g] = m[y];
-                mine[GP * D + GP + g] = any_bad ? NAN : l[y] * (1.0f / PS);
-            }
         }
-        __syncthreads();
-        finish_segment<GP, D>(a, sg, reinterpret_cast<const float *>(smem), S::STAGES * 2 * S::HALF / 4);
-        __syncthreads();
+#pragma unroll
+        for (int g0 = 0; g0 < GP; g0 += HR) {
+            if (g0 >= heads) break;
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                const int i = qr + y * 8 - g0;
+                if (i < 0 || i >= HR) continue;
+#pragma unroll
+                for (int j = 0; j < D / 8; j++)
+                    *reinterpret_cast<float2 *>(&hand.o[warp][i][j * 8 + qc]) =
+                        make_float2(acc[j][2 * y] * (1.0f / PS), acc[j][2 * y + 1] * (1.0f / PS));
+                if ((lane & 3) == 0) {
+                    hand.m[warp][i] = m[y];
+                    hand.l[warp][i] = any_bad ? NAN : l[y] * (1.0f / PS);
+                }
+            }
+            __syncthreads();
+            finish_heads<GP, HR, D>(a, sg, hand, g0);
+            __syncthreads();
+        }
     }
+    cp_async_wait<0>();
 }
 
-template <typename T, int D> int launch_mma(AttnArgs &a, cudaStream_t st) {
+template <typename T, int D, bool F32Q> int launch_mma(AttnArgs &a, cudaStream_t st) {
     constexpr int smem = mma_smem<D>();
-    FOCR_CUDA_TRY(set_max_dynamic_smem((const void *)paged_attention_mma_kernel<T, D>, smem));
+    FOCR_CUDA_TRY(set_max_dynamic_smem((const void *)paged_attention_mma_kernel<T, D, F32Q>, smem));
     a.gp = 16;
     a.head_chunks = (a.group + 15) / 16;
     a.tile_shift = ilog2(MmaTile<D>::BLOCK);
-    FOCR_CUDA_TRY(launch_pdl(paged_attention_mma_kernel<T, D>, attn_blocks(), ATTN_WARPS * 32, smem, st, a));
+    FOCR_CUDA_TRY(launch_pdl(paged_attention_mma_kernel<T, D, F32Q>, attn_blocks(), ATTN_WARPS * 32, smem, st, a));
     return FOCR_OK;
 }
-template <typename T> int launch_mma_dim(AttnArgs &a, cudaStream_t st) {
-    if (a.dim <= 64) return launch_mma<T, 64>(a, st);
-    if (a.dim <= 128) return launch_mma<T, 128>(a, st);
-    return launch_mma<T, 256>(a, st);
+// Whether this kernel takes the call: from 3 query heads a kv head (with 2 the f32
+// units are as fast), an f32 query from 4, and only up to head_dim 128, where its
+// parts fit the registers.
+template <typename T> bool mma_takes(const AttnArgs &a) {
+    constexpr int own = std::is_same<T, __half>::value ? FOCR_F16 : FOCR_BF16;
+    if (a.q_type == own) return a.group >= 3;
+    return a.q_type == FOCR_F32 && a.group >= 4 && a.dim <= 128;
 }
-
-// Query heads of a kv head from which the tensor cores take them.
-constexpr int MMA_HEADS = 3;
+template <typename T> int launch_mma_dim(AttnArgs &a, cudaStream_t st) {
+    if (a.q_type == FOCR_F32)
+        return a.dim <= 64 ? launch_mma<T, 64, true>(a, st) : launch_mma<T, 128, true>(a, st);
+    if (a.dim <= 64) return launch_mma<T, 64, false>(a, st);
+    if (a.dim <= 128) return launch_mma<T, 128, false>(a, st);
+    return launch_mma<T, 256, false>(a, st);
+}
 
 }  // namespace
 }  // namespace focr

@@ -22,9 +22,12 @@ template <typename T, int D> struct Tile {
     static constexpr int EPL = NC * 16 / (int)sizeof(T);  // dimensions of a lane
 };
 
+// Heads that the warps hand over at a time: 2 KB a warp.
+template <int D, int GP> constexpr int simt_round() { return GP * D <= 512 ? GP : 512 / D; }
 template <typename T, int D, int GP> constexpr int simt_smem() {
     using S = Tile<T, D>;
-    return ATTN_WARPS * S::STAGES * 2 * S::HALF + ATTN_WARPS * GP * S::KEYS * 4 + (ATTN_ROWS + 1) * 4;
+    return ATTN_WARPS * S::STAGES * 2 * S::HALF + (int)sizeof(Handover<simt_round<D, GP>(), D>) +
+           ATTN_WARPS * GP * S::KEYS * 4 + (ATTN_ROWS + 1) * 4;
 }
 
 // The arithmetic runs on the f32 units: with few query heads a kv head the
@@ -35,11 +38,13 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
     using S = Tile<T, D>;
     constexpr int LPK = S::LPK, KPI = S::KPI, ITS = S::ITS, KEYS = S::KEYS, NC = S::NC, EPL = S::EPL;
     constexpr int EPC = 16 / (int)sizeof(T);  // elements of a chunk
+    constexpr int RINGS = ATTN_WARPS * S::STAGES * 2 * S::HALF, HR = simt_round<D, GP>();
     extern __shared__ __align__(128) char smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     char *ring = smem + warp * S::STAGES * 2 * S::HALF;
-    float *probs = reinterpret_cast<float *>(smem + ATTN_WARPS * S::STAGES * 2 * S::HALF) + warp * GP * KEYS;
-    int *pre = reinterpret_cast<int *>(smem + ATTN_WARPS * S::STAGES * 2 * S::HALF + ATTN_WARPS * GP * KEYS * 4);
+    auto &hand = *reinterpret_cast<Handover<HR, D> *>(smem + RINGS);
+    float *probs = reinterpret_cast<float *>(smem + RINGS + sizeof(hand)) + warp * GP * KEYS;
+    int *pre = reinterpret_cast<int *>(smem + RINGS + sizeof(hand) + ATTN_WARPS * GP * KEYS * 4);
     const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
 
     pdl_wait();
@@ -51,15 +56,37 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
     const int my_it = (lane & (LPK / 2) ? 4 : 0) + (lane & (LPK / 4) ? 2 : 0) + (lane & (LPK / 8) ? 1 : 0);
     const int my_key = my_it * KPI + sub;
 
+    Feed<KEYS> feed(a, pre);
+    uint32_t bad_stages = 0;   // of the stages in flight, those with a page outside the pool
+    auto issue = [&](int stage, int64_t mine) {
+        const uint32_t dst = ring_s + stage * 2 * S::HALF + lane * 16;
+#pragma unroll
+        for (int it = 0; it < ITS; it++) {
+            const int64_t o = __shfl_sync(0xffffffffu, mine, it * KPI + sub);
+#pragma unroll
+            for (int n = 0; n < NC; n++) {
+                const int b = (n * LPK + chunk) * 16;
+                const bool have = o >= 0 && b < a.c.row_bytes;
+                const int64_t src = have ? o + b : 0;
+                cp_async16(dst + (it * NC + n) * 512, a.c.k + src, have ? 16 : 0);
+                cp_async16(dst + S::HALF + (it * NC + n) * 512, a.c.v + src, have ? 16 : 0);
+            }
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < S::STAGES; s++) {
+        bool bad;
+        issue(s, feed.next(a, pre, warp, lane, &bad));
+        bad_stages |= (uint32_t)bad << s;
+        cp_async_commit();
+    }
     finish_empty_rows(a, pre);
+
+    int stage = 0;
     Run run(a, pre);
     Segment sg;
     while (run.next(a, pre, &sg)) {
-        const int r = sg.r, heads = sg.heads, qh0 = sg.qh0, t0 = sg.t0, t1 = sg.t1;
-        const RowView rv = sg.rv;
-        const int32_t *pages = a.c.table + r * a.c.table_stride;
-        const char *kb = a.c.k + sg.kvh * a.c.head_stride, *vb = a.c.v + sg.kvh * a.c.head_stride;
-
+        const int r = sg.r, heads = sg.heads, qh0 = sg.qh0, vis = sg.rv.vis;
         float q[GP][EPL], acc[GP][EPL], m[GP], l[GP];
 #pragma unroll
         for (int g = 0; g < GP; g++) {
@@ -76,36 +103,11 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
         }
         bool bad = false;
 
-        auto key_offset = [&](int tile) -> int64_t {  // of index `lane` of the warp's tile
-            const int i = (tile * ATTN_WARPS + warp) * KEYS + lane;
-            if (lane >= KEYS || i >= rv.vis || tile >= t1) return -1;
-            const int64_t o = a.c.offset(pages, (uint32_t)(i < rv.ref ? i : i + rv.gap));
-            bad |= o < 0;
-            return o;
-        };
-        auto issue = [&](int stage, int64_t mine) {
-            const uint32_t dst = ring_s + stage * 2 * S::HALF + lane * 16;
-#pragma unroll
-            for (int it = 0; it < ITS; it++) {
-                const int64_t o = __shfl_sync(0xffffffffu, mine, it * KPI + sub);
-#pragma unroll
-                for (int n = 0; n < NC; n++) {
-                    const int b = (n * LPK + chunk) * 16;
-                    const bool have = o >= 0 && b < a.c.row_bytes;
-                    const int64_t src = have ? o + b : 0;
-                    cp_async16(dst + (it * NC + n) * 512, kb + src, have ? 16 : 0);
-                    cp_async16(dst + S::HALF + (it * NC + n) * 512, vb + src, have ? 16 : 0);
-                }
-            }
-        };
-#pragma unroll
-        for (int s = 0; s < S::STAGES; s++) {
-            issue(s, key_offset(t0 + s));
-            cp_async_commit();
-        }
-        int stage = 0;
-        for (int tile = t0; tile < t1; tile++) {
-            const int64_t next = key_offset(tile + S::STAGES);
+        for (int tile = sg.t0; tile < sg.t1; tile++) {
+            bad |= bad_stages >> stage & 1;
+            bool next_bad;
+            const int64_t next = feed.next(a, pre, warp, lane, &next_bad);
+            bad_stages = (bad_stages & ~(1u << stage)) | (uint32_t)next_bad << stage;
             cp_async_wait<S::STAGES - 1>();
             __syncwarp();
             const char *ks = ring + stage * 2 * S::HALF + lane * 16, *vs = ks + S::HALF;
@@ -126,7 +128,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
                 }
             }
             const int i = (tile * ATTN_WARPS + warp) * KEYS + my_key;
-            const bool live = i < rv.vis;
+            const bool live = i < vis;
 #pragma unroll
             for (int g = 0; g < GP; g++) {
                 // transposing reduction: 8 values over LPK lanes leave one a lane
@@ -177,35 +179,37 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
             cp_async_commit();
             stage = stage + 1 == S::STAGES ? 0 : stage + 1;
         }
-        cp_async_wait<0>();
 
-        // the warp's sums over its lanes, then the block's over its warps,
-        // through the rings (no copy is in flight)
+        // the warp's sums over its lanes, then the block's over its warps
         const bool any_bad = __any_sync(0xffffffffu, bad);
-        __syncwarp();
-        float *mine = reinterpret_cast<float *>(ring);  // [GP][D], then m[GP], l[GP]
 #pragma unroll
-        for (int g = 0; g < GP; g++) {
-            float lsum = l[g];
+        for (int g0 = 0; g0 < GP; g0 += HR) {
+            if (g0 >= heads) break;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, o);
-            lsum *= 8.0f / LPK;  // LPK / 8 lanes hold the same key
+            for (int i = 0; i < HR; i++) {
+                const int g = g0 + i;
+                float lsum = l[g];
 #pragma unroll
-            for (int e = 0; e < EPL; e++) {
-                float x = acc[g][e];
+                for (int o = 16; o > 0; o >>= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, o);
+                lsum *= 8.0f / LPK;  // LPK / 8 lanes hold the same key
 #pragma unroll
-                for (int o = LPK; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-                if (sub == 0) mine[g * D + (e / EPC * LPK + chunk) * EPC + e % EPC] = x;
+                for (int e = 0; e < EPL; e++) {
+                    float x = acc[g][e];
+#pragma unroll
+                    for (int o = LPK; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+                    if (sub == 0) hand.o[warp][i][(e / EPC * LPK + chunk) * EPC + e % EPC] = x;
+                }
+                if (lane == 0) {
+                    hand.m[warp][i] = m[g];
+                    hand.l[warp][i] = any_bad ? NAN : lsum;
+                }
             }
-            if (lane == 0) {
-                mine[GP * D + g] = m[g];
-                mine[GP * D + GP + g] = any_bad ? NAN : lsum;
-            }
+            __syncthreads();
+            finish_heads<GP, HR, D>(a, sg, hand, g0);
+            __syncthreads();
         }
-        __syncthreads();
-        finish_segment<GP, D>(a, sg, reinterpret_cast<const float *>(smem), S::STAGES * 2 * S::HALF / 4);
-        __syncthreads();
     }
+    cp_async_wait<0>();
 }
 
 template <typename T, int D, int GP> int launch_simt(AttnArgs &a, cudaStream_t st) {
