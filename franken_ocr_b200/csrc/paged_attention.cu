@@ -26,17 +26,17 @@ __global__ void __launch_bounds__(JT) paged_join_kernel(const AttnArgs a, int bl
     pdl_wait();
     pdl_trigger();
     if (b >= n) return;
-    const unsigned long long u = b * total / n;
+    const unsigned long long u = quotient(b * total, n), before = quotient((b - 1) * total, n);
     const int r = row_of_unit(pre, a.rows, HC, u), tiles = pre[r + 1] - pre[r];
-    const int hc = (int)((u - (unsigned long long)pre[r] * HC) / tiles);
+    const int hc = (int)quotient(u - (unsigned long long)pre[r] * HC, tiles);
     const unsigned long long u0 = (unsigned long long)pre[r] * HC + (unsigned long long)hc * tiles;
-    if (u == u0 || (b - 1) * total / n > u0) return;   // nothing is cut, or it was cut before
+    if (u == u0 || before > u0) return;   // nothing is cut, or it was cut before
     const int kvh = hc / a.head_chunks, g0 = (hc - kvh * a.head_chunks) * a.gp;
     if (g >= min(a.gp, a.group - g0)) return;
     const int qh = kvh * a.group + g0 + g;
     // the last block whose run begins before the cut ends
-    const int b0 = (int)b - 1, b1 = (int)(((u0 + tiles) * n - 1) / total);
-    const int pieces = b1 - b0 + 1, slot0 = 2 * b0 + ((b - 1) * total / n == u0 ? 0 : 1);
+    const int b0 = (int)b - 1, b1 = (int)quotient((u0 + tiles) * n - 1, total);
+    const int pieces = b1 - b0 + 1, slot0 = 2 * b0 + (before == u0 ? 0 : 1);
     auto slot = [&](int p) { return p ? 2 * (b0 + p) : slot0; };
     float M = -INFINITY, L = 0.0f;
     for (int p = t; p < pieces; p += JT) M = fmaxf(M, a.ml[slot(p) * a.gp + g].x);
@@ -143,7 +143,7 @@ int launch_attention(AttnArgs a, int dtype, float *weights, size_t w_row, size_t
                                        : launch_attention_bf16(a, st);
     if (rc) return rc;
     const int blocks = attn_blocks();
-    if (blocks > 1)
+    if (!a.cluster && blocks > 1)
         FOCR_CUDA_TRY(launch_pdl(paged_join_kernel, dim3(blocks - 1, a.gp < a.group ? a.gp : a.group), JT, blocks * 4, st, a, blocks));
     if (weights)
         FOCR_CUDA_TRY(launch_pdl(paged_weights_kernel, dim3((a.width + 1023) / 1024, a.c.kv_heads, a.rows), 256, 0, st,

@@ -21,13 +21,21 @@
 // a (row, head) whole writes the output; pieces go to the workspace (a block
 // has at most two) and paged_join_kernel joins them.  So no row length, however
 // ragged the batch, leaves SMs idle.
+//
+// A few short rows wait on latency, not on bytes.  There a cluster of blocks shares
+// each (row, head) and joins its pieces through distributed shared memory, which
+// saves the second kernel.
 #pragma once
+
+#include <cooperative_groups.h>
 
 #include <type_traits>
 
 #include "paged.cuh"
 
 namespace focr {
+
+namespace cg = cooperative_groups;
 
 constexpr int ATTN_WARPS = 4, ATTN_ROWS = 1024;  // rows of one launch
 constexpr int ATTN_HEADS = 16;                   // most query heads a block takes together
@@ -46,6 +54,7 @@ struct AttnArgs {
     int score_stride;     // floats between the scores of two query heads, even
     int gp, head_chunks;  // query heads that a block takes together; blocks of them a kv head
     int tile_shift;       // log2 of a block tile's positions
+    int cluster;          // blocks of a cluster that shares one (row, head), or 0: runs
     float c2;             // scale * log2(e)
 };
 
@@ -166,36 +175,77 @@ struct Segment {
     bool whole;
     RowView rv;
 };
-struct Run {
-    unsigned long long u, begin, end;
-    int hc_count;
+// n / d; most calls fit 32 bits, whose division is several times shorter.
+__device__ __forceinline__ unsigned long long quotient(unsigned long long n, unsigned long long d) {
+    return (n | d) >> 32 ? n / d : (uint32_t)n / (uint32_t)d;
+}
 
+struct Run {
+    unsigned long long left;     // units to come
+    int r, kvh, chunk, t, tiles; // where the next one lies: tile t of `tiles`
+    bool first;
+
+    // The run of this block; in a cluster its share of the cluster's (row, head),
+    // which may be empty.
     __device__ Run(const AttnArgs &a, const int *pre) {
-        hc_count = a.c.kv_heads * a.head_chunks;
+        if (a.cluster) {
+            const int unit = blockIdx.x / a.cluster, rank = blockIdx.x - unit * a.cluster;
+            const int row_units = a.c.kv_heads * a.head_chunks;
+            r = unit / row_units;
+            kvh = (unit - r * row_units) / a.head_chunks;
+            chunk = unit - r * row_units - kvh * a.head_chunks;
+            const int n = (row_view(a, r).vis + (1 << a.tile_shift) - 1) >> a.tile_shift;
+            const int per = n / a.cluster, rest = n - per * a.cluster;   // the first `rest` blocks have one more
+            t = rank * per + min(rank, rest);
+            tiles = t + per + (rank < rest);
+            left = tiles - t;
+            first = true;
+            return;
+        }
+        const int hc_count = a.c.kv_heads * a.head_chunks;
         const unsigned long long total = (unsigned long long)pre[a.rows] * hc_count;
         const unsigned long long runs = run_count(total, gridDim.x);
-        begin = end = u = 0;
+        left = 0;
         if (blockIdx.x >= runs) return;
-        u = begin = blockIdx.x * total / runs;
-        end = (blockIdx.x + 1ull) * total / runs;
+        const unsigned long long u = quotient(blockIdx.x * total, runs);
+        left = quotient((blockIdx.x + 1ull) * total, runs) - u;
+        r = row_of_unit(pre, a.rows, hc_count, u);
+        tiles = pre[r + 1] - pre[r];
+        const unsigned long long off = u - (unsigned long long)pre[r] * hc_count;
+        const int hc = (int)quotient(off, tiles);
+        t = (int)(off - (unsigned long long)hc * tiles);
+        kvh = hc / a.head_chunks;
+        chunk = hc - kvh * a.head_chunks;
+        first = true;
     }
     __device__ bool next(const AttnArgs &a, const int *pre, Segment *s) {
-        if (u >= end) return false;
-        const int lo = row_of_unit(pre, a.rows, hc_count, u);
-        const int tiles = pre[lo + 1] - pre[lo];
-        const unsigned long long off = u - (unsigned long long)pre[lo] * hc_count;
-        const int hc = (int)(off / tiles);
-        s->r = lo;
-        s->t0 = (int)(off - (unsigned long long)hc * tiles);
-        s->t1 = (int)min((unsigned long long)tiles, s->t0 + (end - u));
-        s->whole = s->t0 == 0 && s->t1 == tiles;
-        s->slot = blockIdx.x * 2 + (u == begin ? 0 : 1);
-        s->kvh = hc / a.head_chunks;
-        const int g0 = (hc - s->kvh * a.head_chunks) * a.gp;
-        s->heads = min(a.gp, a.group - g0);
-        s->qh0 = s->kvh * a.group + g0;
-        s->rv = row_view(a, lo);
-        u += s->t1 - s->t0;
+        // a cluster's blocks all take part in its join
+        if (a.cluster ? !first : !left) return false;
+        if (t == tiles && !a.cluster) {   // the next (row, kv head, chunk)
+            t = 0;
+            if (++chunk == a.head_chunks) {
+                chunk = 0;
+                if (++kvh == a.c.kv_heads) {
+                    kvh = 0;
+                    do {
+                        r++;
+                        tiles = pre[r + 1] - pre[r];
+                    } while (tiles == 0);   // units are left: a row with some follows
+                }
+            }
+        }
+        s->r = r;
+        s->t0 = t;
+        s->t1 = (int)min((unsigned long long)tiles, t + left);
+        s->whole = t == 0 && s->t1 == tiles;
+        s->slot = blockIdx.x * 2 + (first ? 0 : 1);
+        s->kvh = kvh;
+        s->heads = min(a.gp, a.group - chunk * a.gp);
+        s->qh0 = kvh * a.group + chunk * a.gp;
+        s->rv = row_view(a, r);
+        left -= s->t1 - t;
+        t = s->t1;
+        first = false;
         return true;
     }
 };
@@ -210,14 +260,14 @@ template <int KEYS> struct Feed {
     RowView rv;
     int tile, end;
 
-    __device__ Feed(const AttnArgs &a, const int *pre) : run(a, pre), tile(0), end(0) {}
+    __device__ explicit Feed(const Run &r) : run(r), tile(0), end(0) {}
     // The byte offset of this lane's position of the next tile, -1 where there is
     // none; *bad if its page is not in the pool.
     __device__ int64_t next(const AttnArgs &a, const int *pre, int warp, int lane, bool *bad) {
         *bad = false;
         if (tile == end) {
             Segment s;
-            if (!run.next(a, pre, &s)) return -1;
+            if (!run.left || !run.next(a, pre, &s)) return -1;
             pages = a.c.table + s.r * a.c.table_stride;
             head = s.kvh * a.c.head_stride;
             rv = s.rv;
@@ -266,16 +316,19 @@ __device__ __forceinline__ float4 over4(float4 x, float L) {
 }
 
 // What the warps of a block hand over at the end of a segment: HR heads at a time,
-// beside the rings, into which the next segment's rows are already flowing.
+// beside the rings, into which the next segment's rows are already flowing.  A
+// cluster's blocks then hand their joined part to one another in the first warp's
+// place.
 template <int HR, int D> struct Handover {
     float o[ATTN_WARPS][HR][D], m[ATTN_WARPS][HR], l[ATTN_WARPS][HR];
 };
 
 // Joins the block's warps for the heads g0 .. g0 + HR - 1 of the segment, and
-// writes their output or piece.
+// writes their output or piece.  The block waits for it at the end.
 template <int GP, int HR, int D>
-__device__ __forceinline__ void finish_heads(const AttnArgs &a, const Segment &s, const Handover<HR, D> &h, int g0) {
-    for (int x = threadIdx.x; x < min(HR, s.heads - g0) * (D / 4); x += ATTN_WARPS * 32) {
+__device__ __forceinline__ void finish_heads(const AttnArgs &a, const Segment &s, Handover<HR, D> &h, int g0) {
+    const int n = min(HR, s.heads - g0) * (D / 4);
+    for (int x = threadIdx.x; x < n; x += ATTN_WARPS * 32) {
         const int i = x / (D / 4), g = g0 + i, d = x % (D / 4) * 4;
         if (d >= a.dim) continue;   // a multiple of 4
         float M = -INFINITY, L = 0.0f;
@@ -289,7 +342,14 @@ __device__ __forceinline__ void finish_heads(const AttnArgs &a, const Segment &s
             L = __fmaf_rn(h.l[w][i], f, L);
             o = fma4(*reinterpret_cast<const float4 *>(&h.o[w][i][d]), f, o);
         }
-        if (s.whole) {
+        if (a.cluster) {
+            // only this thread reads these four; the other threads still read m and l
+            *reinterpret_cast<float4 *>(&h.o[0][i][d]) = o;
+            if (d == 0) {
+                h.o[1][i][0] = M;
+                h.o[1][i][1] = L;
+            }
+        } else if (s.whole) {
             store4_as(a.out, a.q_type, s.r * a.out_stride + (long long)(s.qh0 + g) * a.dim + d, over4(o, L));
             if (a.stat && d == 0) a.stat[(int64_t)s.r * a.q_heads + s.qh0 + g] = make_float2(M, 1.0f / L);
         } else {
@@ -297,11 +357,37 @@ __device__ __forceinline__ void finish_heads(const AttnArgs &a, const Segment &s
             if (d == 0) a.ml[s.slot * GP + g] = make_float2(M, L);
         }
     }
+    if (!a.cluster) {
+        __syncthreads();
+        return;
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    for (int x = cluster.block_rank() * (ATTN_WARPS * 32) + threadIdx.x; x < n; x += a.cluster * (ATTN_WARPS * 32)) {
+        const int i = x / (D / 4), g = g0 + i, d = x % (D / 4) * 4;
+        if (d >= a.dim) continue;
+        float M = -INFINITY, L = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int q = 0; q < a.cluster; q++) M = fmaxf(M, cluster.map_shared_rank(&h, q)->o[1][i][0]);
+        const float mc = scaled_max(M, a.c2);
+#pragma unroll 8
+        for (int q = 0; q < a.cluster; q++) {
+            const Handover<HR, D> *y = cluster.map_shared_rank(&h, q);
+            const float2 ml = *reinterpret_cast<const float2 *>(&y->o[1][i][0]);
+            const float f = prob(ml.x, a.c2, mc);
+            L = __fmaf_rn(ml.y, f, L);
+            o = fma4(*reinterpret_cast<const float4 *>(&y->o[0][i][d]), f, o);
+        }
+        store4_as(a.out, a.q_type, s.r * a.out_stride + (long long)(s.qh0 + g) * a.dim + d, over4(o, L));
+        if (a.stat && d == 0) a.stat[(int64_t)s.r * a.q_heads + s.qh0 + g] = make_float2(M, 1.0f / L);
+    }
+    cluster.sync();   // nobody overwrites or leaves what another still reads
 }
 
 // The rows that have no units, shared out over the blocks: zeros where nothing is
 // visible, NaN for a length that passes the table.
 __device__ __forceinline__ void finish_empty_rows(const AttnArgs &a, const int *pre) {
+    if (a.cluster) return;   // a row of a cluster has a segment, if an empty one
     for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
         if (pre[r + 1] != pre[r]) continue;
         const float x = row_view(a, r).bad ? NAN : 0.0f;
@@ -316,6 +402,38 @@ inline int ilog2(int x) {
     return n;
 }
 inline int attn_blocks() { return num_sms() * 2; }
+
+// Launches an attention kernel in runs, or in clusters where a.cluster says so.
+template <typename K> int launch_attn(K kernel, int smem, const AttnArgs &a, cudaStream_t st) {
+    FOCR_CUDA_TRY(set_max_dynamic_smem((const void *)kernel, smem));
+    if (!a.cluster) {
+        FOCR_CUDA_TRY(launch_pdl(kernel, attn_blocks(), ATTN_WARPS * 32, smem, st, a));
+        return FOCR_OK;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = a.rows * a.c.kv_heads * a.head_chunks * a.cluster;
+    cfg.blockDim = ATTN_WARPS * 32;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = a.cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    FOCR_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
+    return FOCR_OK;
+}
+
+// The blocks of a cluster for each (row, head), or 0 for runs: the visible positions
+// of a row are not known here, only its table's capacity, so clusters are for tables
+// of at most 2 MB a (row, head) and as many of them as fit the SMs at once.
+inline int cluster_of(const AttnArgs &a) {
+    const size_t units = (size_t)a.rows * a.c.kv_heads * a.head_chunks;
+    return units * 8 <= (size_t)attn_blocks() && (size_t)a.cap * a.c.row_bytes <= (1u << 20) ? 8 : 0;
+}
 
 // The attention kernel for one type of cache, without the join; sets gp,
 // head_chunks and tile_shift of `a` as that kernel has them.

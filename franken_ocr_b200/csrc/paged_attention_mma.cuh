@@ -28,9 +28,12 @@ template <int D> struct MmaTile {
 // Heads that the warps hand over at a time: 2 KB a warp, or all where one block
 // fills an SM.
 template <int D> constexpr int mma_round() { return D == 256 ? 16 : 512 / D; }
+// At head_dim 256 the query's registers are needed elsewhere: it lies in shared
+// memory, swizzled like the rows.
+template <int D> constexpr int mma_q_bytes() { return D == 256 ? 16 * D * 2 : 0; }
 template <int D> constexpr int mma_smem() {
     return ATTN_WARPS * MmaTile<D>::STAGES * 2 * MmaTile<D>::HALF + (int)sizeof(Handover<mma_round<D>(), D>) +
-           (ATTN_ROWS + 1) * 4;
+           mma_q_bytes<D>() + (ATTN_ROWS + 1) * 4;
 }
 
 template <typename T> __device__ __forceinline__ void mma16816(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
@@ -76,6 +79,8 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
     using S = MmaTile<D>;
     constexpr int GP = 16, KEYS = S::KEYS, NT = KEYS / 8, ITS = S::HALF / 512, HR = mma_round<D>();
     constexpr int QP = F32Q ? 3 : 1, PP = F32Q ? 3 : 2;
+    constexpr bool QS = mma_q_bytes<D>() > 0;
+    static_assert(!(QS && F32Q), "an f32 query's parts are kept in registers");
     constexpr bool HALF = std::is_same<T, __half>::value;
     // f16 holds nothing below 2^-24: probabilities, at most 1, are scaled up, and a
     // head's f32 query by the power of two that brings its largest value near 2^14
@@ -85,16 +90,19 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     char *ring = smem + warp * S::STAGES * 2 * S::HALF;
     auto &hand = *reinterpret_cast<Handover<HR, D> *>(smem + RINGS);
-    int *pre = reinterpret_cast<int *>(smem + RINGS + sizeof(hand));
+    char *qs = smem + RINGS + sizeof(hand);
+    int *pre = reinterpret_cast<int *>(qs + mma_q_bytes<D>());
+    const uint32_t qs_s = (uint32_t)__cvta_generic_to_shared(qs);
     const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
 
     pdl_wait();
     pdl_trigger();
-    tile_prefix<ATTN_WARPS * 32>(a, pre);
+    if (!a.cluster) tile_prefix<ATTN_WARPS * 32>(a, pre);
 
     const int qr = lane >> 2, qc = (lane & 3) * 2;   // this lane's row and columns of a tile
     const int mi = lane >> 3, rr = lane & 7;         // its matrix and row when loading one
-    Feed<KEYS> feed(a, pre);
+    Run run(a, pre);
+    Feed<KEYS> feed(run);
     uint32_t bad_stages = 0;   // of the stages in flight, those with a page outside the pool
     auto issue = [&](int stage, int64_t mine) {
         const uint32_t dst = ring_s + stage * 2 * S::HALF;
@@ -119,11 +127,10 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
     finish_empty_rows(a, pre);
 
     int stage = 0;
-    Run run(a, pre);
     Segment sg;
     while (run.next(a, pre, &sg)) {
         const int r = sg.r, heads = sg.heads, vis = sg.rv.vis;
-        uint32_t qa[QP][D / 16][4];
+        uint32_t qa[QP][QS ? 1 : D / 16][4];
         float unscale[2] = {1.0f, 1.0f};
         if constexpr (F32Q) {
             const float *qp = static_cast<const float *>(a.q) + r * a.q_stride + (long long)sg.qh0 * a.dim;
@@ -156,6 +163,14 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
 #pragma unroll
                     for (int p = 0; p < QP; p++) qa[p][ks][x] = take_pair<T>(&q0, &q1);
                 }
+        } else if constexpr (QS) {
+            const uint16_t *qp = static_cast<const uint16_t *>(a.q) + r * a.q_stride + (long long)sg.qh0 * a.dim;
+            for (int x = threadIdx.x; x < GP * D; x += ATTN_WARPS * 32) {   // the block is past its last use
+                const int g = x / D, d = x % D;
+                *reinterpret_cast<uint16_t *>(qs + g * S::DB + ((d / 8 ^ (g & 7)) << 4) + d % 8 * 2) =
+                    g < heads && d < a.dim ? qp[g * a.dim + d] : (uint16_t)0;
+            }
+            __syncthreads();
         } else {
             const uint16_t *qp = static_cast<const uint16_t *>(a.q) + r * a.q_stride + (long long)sg.qh0 * a.dim;
             const bool pairs = (uintptr_t)qp % 4 == 0;   // dim is even
@@ -173,7 +188,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
         float acc[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < D / 8; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
-        bool bad = false;
+        bool bad = sg.rv.bad;
 
         for (int tile = sg.t0; tile < sg.t1; tile++) {
             bad |= bad_stages >> stage & 1;
@@ -188,17 +203,19 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
             for (int t = 0; t < NT; t++) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
             // the smallest parts first: the sum's last steps are the ones that count
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ks++)
+            for (int ks = 0; ks < D / 16; ks++) {
+                if constexpr (QS) ldmatrix4<false>(qa[0][0], qs_s + ((mi & 1) * 8 + rr) * S::DB + (((ks * 2 + (mi >> 1)) ^ rr) << 4));
 #pragma unroll
                 for (int p = 0; p < KEYS / 16; p++) {
                     uint32_t b[4];
                     ldmatrix4<false>(b, ks_s + (p * 16 + (mi >> 1) * 8 + rr) * S::DB + (((ks * 2 + (mi & 1)) ^ rr) << 4));
 #pragma unroll
                     for (int part = QP - 1; part >= 0; part--) {
-                        mma16816<T>(s[2 * p], qa[part][ks], b[0], b[1]);
-                        mma16816<T>(s[2 * p + 1], qa[part][ks], b[2], b[3]);
+                        mma16816<T>(s[2 * p], qa[part][QS ? 0 : ks], b[0], b[1]);
+                        mma16816<T>(s[2 * p + 1], qa[part][QS ? 0 : ks], b[2], b[3]);
                     }
                 }
+            }
             if constexpr (F32Q && HALF)
 #pragma unroll
                 for (int t = 0; t < NT; t++)
@@ -295,20 +312,17 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
             }
             __syncthreads();
             finish_heads<GP, HR, D>(a, sg, hand, g0);
-            __syncthreads();
         }
     }
     cp_async_wait<0>();
 }
 
 template <typename T, int D, bool F32Q> int launch_mma(AttnArgs &a, cudaStream_t st) {
-    constexpr int smem = mma_smem<D>();
-    FOCR_CUDA_TRY(set_max_dynamic_smem((const void *)paged_attention_mma_kernel<T, D, F32Q>, smem));
     a.gp = 16;
     a.head_chunks = (a.group + 15) / 16;
     a.tile_shift = ilog2(MmaTile<D>::BLOCK);
-    FOCR_CUDA_TRY(launch_pdl(paged_attention_mma_kernel<T, D, F32Q>, attn_blocks(), ATTN_WARPS * 32, smem, st, a));
-    return FOCR_OK;
+    a.cluster = cluster_of(a);
+    return launch_attn(paged_attention_mma_kernel<T, D, F32Q>, mma_smem<D>(), a, st);
 }
 // Whether this kernel takes the call: from 3 query heads a kv head (with 2 the f32
 // units are as fast), an f32 query from 4, and only up to head_dim 128, where its

@@ -49,14 +49,15 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
 
     pdl_wait();
     pdl_trigger();
-    tile_prefix<ATTN_WARPS * 32>(a, pre);
+    if (!a.cluster) tile_prefix<ATTN_WARPS * 32>(a, pre);
 
     const int sub = lane / LPK, chunk = lane % LPK;
     // the step whose score this lane holds after the transposing reduction
     const int my_it = (lane & (LPK / 2) ? 4 : 0) + (lane & (LPK / 4) ? 2 : 0) + (lane & (LPK / 8) ? 1 : 0);
     const int my_key = my_it * KPI + sub;
 
-    Feed<KEYS> feed(a, pre);
+    Run run(a, pre);
+    Feed<KEYS> feed(run);
     uint32_t bad_stages = 0;   // of the stages in flight, those with a page outside the pool
     auto issue = [&](int stage, int64_t mine) {
         const uint32_t dst = ring_s + stage * 2 * S::HALF + lane * 16;
@@ -83,7 +84,6 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
     finish_empty_rows(a, pre);
 
     int stage = 0;
-    Run run(a, pre);
     Segment sg;
     while (run.next(a, pre, &sg)) {
         const int r = sg.r, heads = sg.heads, qh0 = sg.qh0, vis = sg.rv.vis;
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
                 acc[g][e] = 0.0f;
             }
         }
-        bool bad = false;
+        bool bad = sg.rv.bad;
 
         for (int tile = sg.t0; tile < sg.t1; tile++) {
             bad |= bad_stages >> stage & 1;
@@ -206,20 +206,17 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
             }
             __syncthreads();
             finish_heads<GP, HR, D>(a, sg, hand, g0);
-            __syncthreads();
         }
     }
     cp_async_wait<0>();
 }
 
 template <typename T, int D, int GP> int launch_simt(AttnArgs &a, cudaStream_t st) {
-    constexpr int smem = simt_smem<T, D, GP>();
-    FOCR_CUDA_TRY(set_max_dynamic_smem((const void *)paged_attention_kernel<T, D, GP>, smem));
     a.gp = GP;
     a.head_chunks = (a.group + GP - 1) / GP;
     a.tile_shift = ilog2(Tile<T, D>::BLOCK);
-    FOCR_CUDA_TRY(launch_pdl(paged_attention_kernel<T, D, GP>, attn_blocks(), ATTN_WARPS * 32, smem, st, a));
-    return FOCR_OK;
+    a.cluster = cluster_of(a);
+    return launch_attn(paged_attention_kernel<T, D, GP>, simt_smem<T, D, GP>(), a, st);
 }
 
 // 1, 2, 4 or 8 query heads a block.
