@@ -10,8 +10,8 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import lib
-from .paged import _F32, _I32, _U8, _cache, _call, _dtype, _empty, _need, _workspace
+from ._lib import FOCR_OK, check, lib
+from .paged import _F32, _I32, _U8, _cache, _device, _dtype, _elsewhere, _empty, _need, _stream, _workspace
 
 
 def beam_select(logits, scores, n: int | None = None, *, done=None, end_token: int = 1):
@@ -32,6 +32,8 @@ def beam_select(logits, scores, n: int | None = None, *, done=None, end_token: i
     index = logits.get_device()
     if index < 0:
         raise ValueError(f"{ctx}: logits must be a CUDA tensor, not on {logits.device}")
+    if index != _device():
+        return _elsewhere(beam_select, index, logits, scores, n, done=done, end_token=end_token)
     code = _dtype(ctx, "logits", logits)
     batch, beams, vocab = shape
     if (stride[2] != 1 and vocab > 1) or (batch > 1 and beams > 1 and stride[0] != beams * stride[1]):
@@ -45,15 +47,16 @@ def beam_select(logits, scores, n: int | None = None, *, done=None, end_token: i
         n = beams
     if n < 1:
         raise ValueError(f"{ctx}: n must be positive")
-    out = _empty((batch, n), _F32, index)
-    parent = _empty((batch, n), _I32, index)
-    token = _empty((batch, n), _I32, index)
+    shape = (batch, n)
+    out, parent, token = _empty(shape, (n, 1), _F32), _empty(shape, (n, 1), _I32), _empty(shape, (n, 1), _I32)
     need = _workspace("focr_beam_select_workspace", batch, beams, vocab, n)
-    ws = _empty((need,), _U8, index)  # lives until the kernels are enqueued
-    row = stride[1] if beams > 1 else stride[0] if batch > 1 else vocab
-    _call(lib.focr_beam_select, index, logits.data_ptr(), code, batch, beams, vocab, row, scores.data_ptr(),
-          None if done is None else done.data_ptr(), end_token, n, out.data_ptr(), parent.data_ptr(),
-          token.data_ptr(), ws.data_ptr(), need)
+    ws = _empty((need,), (1,), _U8)  # lives until the kernels are enqueued
+    rc = lib.focr_beam_select(
+        logits.data_ptr(), code, batch, beams, vocab, stride[1] if beams > 1 else stride[0] if batch > 1 else vocab,
+        scores.data_ptr(), None if done is None else done.data_ptr(), end_token, n, out.data_ptr(), parent.data_ptr(),
+        token.data_ptr(), ws.data_ptr(), need, _stream(index))
+    if rc != FOCR_OK:
+        check(rc)
     return out, parent, token
 
 
@@ -72,6 +75,8 @@ def beam_reorder(k_pages, v_pages, table, lens, parent, fresh, *, weights=None):
     ctx = "beam_reorder"
     layered = k_pages.dim() == 5
     cache, index, heads, _, rows, width = _cache(ctx, k_pages, v_pages, table, 5 if layered else 4)
+    if index != _device():
+        return _elsewhere(beam_reorder, index, k_pages, v_pages, table, lens, parent, fresh, weights=weights)
     layers = k_pages.shape[0] if layered else 1
     if parent.dim() != 2:
         raise ValueError(f"{ctx}: parent must be [batch, beams], not {tuple(parent.shape)}")
@@ -94,11 +99,13 @@ def beam_reorder(k_pages, v_pages, table, lens, parent, fresh, *, weights=None):
         if stride[-1] != 1 and span > 1:
             raise ValueError(f"{ctx}: the last dimension of weights must be contiguous")
         w_layer = stride[0] if layered else 0
-        w_out = _empty(shape, _F32, index)
-    new_table = _empty((rows, width), _I32, index)
-    new_lens = _empty((rows,), _I32, index)
-    _call(lib.focr_beam_reorder, index, cache, layers, k_pages.stride(0) if layered else 0, batch, beams,
-          lens.data_ptr(), parent.data_ptr(), fresh.data_ptr(), new_table.data_ptr(), new_lens.data_ptr(),
-          None if weights is None else weights.data_ptr(), span, w_layer, w_row, w_head,
-          None if w_out is None else w_out.data_ptr())
+        w_out = torch.empty(shape, dtype=_F32, device="cuda")
+    new_table = _empty((rows, width), (width, 1), _I32)
+    new_lens = _empty((rows,), (1,), _I32)
+    rc = lib.focr_beam_reorder(
+        cache, layers, k_pages.stride(0) if layered else 0, batch, beams, lens.data_ptr(), parent.data_ptr(),
+        fresh.data_ptr(), new_table.data_ptr(), new_lens.data_ptr(), None if weights is None else weights.data_ptr(),
+        span, w_layer, w_row, w_head, None if w_out is None else w_out.data_ptr(), _stream(index))
+    if rc != FOCR_OK:
+        check(rc)
     return new_table, new_lens, w_out

@@ -38,20 +38,10 @@ _device = torch._C._cuda_getDevice
 _stream = torch._C._cuda_getCurrentRawStream
 
 try:  # an allocation on the current device without the dispatcher: half the time
-    from torch._C._dynamo.guards import _empty_strided_cuda as _raw_empty
+    from torch._C._dynamo.guards import _empty_strided_cuda as _empty
 except ImportError:  # pragma: no cover
-    _raw_empty = None
-
-
-def _empty(shape, dtype, index: int):
-    """An uninitialised contiguous tensor on CUDA device `index`."""
-    if _raw_empty is None or index != _device():
-        return torch.empty(shape, dtype=dtype, device=torch.device("cuda", index))
-    stride, n = [], 1
-    for d in reversed(shape):
-        stride.append(n)
-        n *= d if d > 1 else 1
-    return _raw_empty(tuple(shape), tuple(stride[::-1]), dtype)
+    def _empty(shape, stride, dtype):
+        return torch.empty_strided(shape, stride, dtype=dtype, device="cuda")
 
 
 def _dtype(ctx: str, name: str, t) -> int:
@@ -63,14 +53,15 @@ def _dtype(ctx: str, name: str, t) -> int:
 
 def _need(ctx: str, name: str, t, dtype, shape, index: int) -> None:
     """A contiguous tensor of that type and shape on that device."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == index and t.is_contiguous():
+        return
     if t.dtype is not dtype:
         raise TypeError(f"{ctx}: {name} must be {dtype}, not {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{ctx}: {name} has shape {tuple(t.shape)}, not {tuple(shape)}")
     if t.get_device() != index:
         raise ValueError(f"{ctx}: {name} is on {t.device}, not cuda:{index}")
-    if not t.is_contiguous():
-        raise ValueError(f"{ctx}: {name} must be contiguous")
+    raise ValueError(f"{ctx}: {name} must be contiguous")
 
 
 def _table(ctx: str, name: str, t, index: int):
@@ -111,15 +102,10 @@ def _cache(ctx: str, k_pages, v_pages, table, dims: int = 4):
     return packed, index, heads, dim, rows, width
 
 
-def _call(fn, index: int, *args) -> None:
-    """One call of the C ABI on the device's current stream, its last argument."""
-    if index == _device():
-        rc = fn(*args, _stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, _stream(index))
-    if rc != FOCR_OK:
-        check(rc)
+def _elsewhere(fn, index: int, *args, **kw):
+    """The same call with its tensors' device as the current one."""
+    with torch.cuda.device(index):
+        return fn(*args, **kw)
 
 
 @functools.lru_cache(maxsize=256)
@@ -152,6 +138,8 @@ def paged_write(k, v, k_pages, v_pages, table, pos, row=None) -> None:
     ``pos`` and ``row`` are int32 on the device."""
     ctx = "paged_write"
     cache, index, heads, dim, rows, _ = _cache(ctx, k_pages, v_pages, table)
+    if index != _device():
+        return _elsewhere(paged_write, index, k, v, k_pages, v_pages, table, pos, row)
     src = _dtype(ctx, "k", k)
     shape = k.shape
     if len(shape) != 3 or shape[1] != heads or shape[2] != dim or v.shape != shape or v.dtype is not k.dtype \
@@ -164,8 +152,10 @@ def paged_write(k, v, k_pages, v_pages, table, pos, row=None) -> None:
     _need(ctx, "pos", pos, _I32, (tokens,), index)
     if row is not None:
         _need(ctx, "row", row, _I32, (tokens,), index)
-    _call(lib.focr_paged_write, index, cache, rows, k.data_ptr(), v.data_ptr(), src, tokens, ks[0], vs[0],
-          None if row is None else row.data_ptr(), pos.data_ptr())
+    rc = lib.focr_paged_write(cache, rows, k.data_ptr(), v.data_ptr(), src, tokens, ks[0], vs[0],
+                              None if row is None else row.data_ptr(), pos.data_ptr(), _stream(index))
+    if rc != FOCR_OK:
+        check(rc)
 
 
 def paged_attention(q, k_pages, v_pages, table, lens, *, scale: float | None = None, ref_lens=None,
@@ -182,6 +172,9 @@ def paged_attention(q, k_pages, v_pages, table, lens, *, scale: float | None = N
     weights), or a page id outside the pool, gives NaN for that row."""
     ctx = "paged_attention"
     cache, index, kv_heads, dim, rows, _ = _cache(ctx, k_pages, v_pages, table)
+    if index != _device():
+        return _elsewhere(paged_attention, index, q, k_pages, v_pages, table, lens, scale=scale, ref_lens=ref_lens,
+                          window=window, weights=weights, out=out)
     code = _dtype(ctx, "q", q)
     shape, stride = q.shape, q.stride()
     if len(shape) != 3 or shape[0] != rows or shape[2] != dim or q.get_device() != index:
@@ -198,17 +191,20 @@ def paged_attention(q, k_pages, v_pages, table, lens, *, scale: float | None = N
     width = w_row = w_head = 0
     if weights is not None:
         width, w_row, w_head = _weights(ctx, weights, rows, kv_heads, index)
+    wide = heads * dim
     if out is None:
-        out = _empty(shape, q.dtype, index)
+        out = _empty((rows, heads, dim), (wide, dim, 1), q.dtype)
     else:
         _need(ctx, "out", out, q.dtype, shape, index)
     need = _workspace("focr_paged_attention_workspace", rows, heads, dim, width)
-    ws = _empty((need,), _U8, index)  # lives until the kernels are enqueued
-    _call(lib.focr_paged_attention, index, cache, q.data_ptr(), code, rows, heads, stride[0], lens.data_ptr(),
-          None if ref_lens is None else ref_lens.data_ptr(), window,
-          1.0 / math.sqrt(dim) if scale is None else scale, out.data_ptr(), heads * dim,
-          None if weights is None else weights.data_ptr(), width, w_row, w_head,
-          ws.data_ptr(), need)
+    ws = _empty((need,), (1,), _U8)  # lives until the kernels are enqueued
+    rc = lib.focr_paged_attention(
+        cache, q.data_ptr(), code, rows, heads, stride[0], lens.data_ptr(),
+        None if ref_lens is None else ref_lens.data_ptr(), window, 1.0 / math.sqrt(dim) if scale is None else scale,
+        out.data_ptr(), wide, None if weights is None else weights.data_ptr(), width, w_row, w_head, ws.data_ptr(),
+        need, _stream(index))
+    if rc != FOCR_OK:
+        check(rc)
     return out
 
 
@@ -226,6 +222,9 @@ def paged_evict(k_pages, v_pages, table, lens, weights, new_table, budget: int, 
     weights in a tensor of ``weights``' shape, 0 behind them."""
     ctx = "paged_evict"
     cache, index, heads, _, rows, _ = _cache(ctx, k_pages, v_pages, table)
+    if index != _device():
+        return _elsewhere(paged_evict, index, k_pages, v_pages, table, lens, weights, new_table, budget, sink=sink,
+                          recent=recent)
     _need(ctx, "lens", lens, _I32, (rows,), index)
     width, w_row, w_head = _weights(ctx, weights, rows, heads, index)
     new_rows, new_pages, new_step = _table(ctx, "new_table", new_table, index)
@@ -233,10 +232,12 @@ def paged_evict(k_pages, v_pages, table, lens, weights, new_table, budget: int, 
         raise ValueError(f"{ctx}: new_table has {new_rows} rows, table {rows}")
     if budget < 1 or sink < 0 or recent < 0:
         raise ValueError(f"{ctx}: budget must be positive, sink and recent not negative")
-    kept = _empty((rows, heads, budget), _I32, index)
-    new_lens = _empty((rows,), _I32, index)
-    new_weights = _empty((rows, heads, width), _F32, index)
-    _call(lib.focr_paged_evict, index, cache, rows, lens.data_ptr(), weights.data_ptr(), width, w_row, w_head,
-          new_table.data_ptr(), new_step, new_pages, budget, sink, recent, kept.data_ptr(), new_lens.data_ptr(),
-          new_weights.data_ptr())
+    kept = _empty((rows, heads, budget), (heads * budget, budget, 1), _I32)
+    new_lens = _empty((rows,), (1,), _I32)
+    new_weights = _empty((rows, heads, width), (heads * width, width, 1), _F32)
+    rc = lib.focr_paged_evict(cache, rows, lens.data_ptr(), weights.data_ptr(), width, w_row, w_head,
+                              new_table.data_ptr(), new_step, new_pages, budget, sink, recent, kept.data_ptr(),
+                              new_lens.data_ptr(), new_weights.data_ptr(), _stream(index))
+    if rc != FOCR_OK:
+        check(rc)
     return kept, new_lens, new_weights
