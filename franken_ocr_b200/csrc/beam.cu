@@ -207,18 +207,13 @@ __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) 
                             lt[k++] = token(i);
                         }
     }
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((t & 31) == 0) shd[t >> 5] = sum;
     __syncthreads();
     const int got = count;
-    // the list's order is chance: a sum of whole multiples of 2^-48 has none
-    long long large = 0;
-    for (int i = t; i < (got <= LIST ? got : STRIP); i += ST) {
-        float y = -INFINITY;
-        if (got <= LIST) y = lx[i];
-        else if (first + i < a.vocab) y = fminf(to_f32<T>(x[first + i]), LARGEST);
-        if (y >= near) large += __double2ll_rn(exp((double)y - (double)m) * 0x1p48);
-    }
-    if (got <= LIST) {   // ranked by other warps than the first, which has the terms above
-        for (int i = (t + ST - 32) % ST; i < got; i += ST) {
+    const bool listed = got <= LIST;
+    if (listed && t >= 32) {   // ranked by the other warps, while the first one sums up
+        for (int i = t - 32; i < got; i += ST - 32) {
             const float y = lx[i];
             const int c = lt[i];
             if (y < low) continue;
@@ -230,27 +225,30 @@ __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) 
                 a.ct[at * a.n + rank] = c;
             }
         }
-        for (int k = got + t; k < a.n; k += ST) a.ct[at * a.n + k] = -1;   // fewer than n: all are in the list
+        for (int k = got + t - 32; k < a.n; k += ST - 32) a.ct[at * a.n + k] = -1;   // fewer than n: all are listed
+        return;
     }
-    for (int o = 16; o > 0; o >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        large += __shfl_xor_sync(0xffffffffu, large, o);
+    // the list's order is chance: a sum of whole multiples of 2^-48 has none
+    long long large = 0;
+    for (int i = t; i < (listed ? got : STRIP); i += listed ? 32 : ST) {
+        float y = -INFINITY;
+        if (listed) y = lx[i];
+        else if (first + i < a.vocab) y = fminf(to_f32<T>(x[first + i]), LARGEST);
+        if (y >= near) large += __double2ll_rn(exp((double)y - (double)m) * 0x1p48);
     }
-    if ((t & 31) == 0) {
-        shd[t >> 5] = sum;
-        shl[t >> 5] = large;
+    for (int o = 16; o > 0; o >>= 1) large += __shfl_xor_sync(0xffffffffu, large, o);
+    if (!listed) {
+        if ((t & 31) == 0) shl[t >> 5] = large;
+        __syncthreads();
+        for (int w = 1; t == 0 && w < ST / 32; w++) large += shl[w];
     }
-    __syncthreads();
     if (t == 0) {
-        for (int w = 1; w < ST / 32; w++) {
-            sum += shd[w];
-            large += shl[w];
-        }
+        for (int w = 1; w < ST / 32; w++) sum += shd[w];
         a.pm[at] = m;
         // the small terms were taken relative to 2^base
         a.ps[at] = sum * exp((double)base * 0.693147180559945309 - (double)high) + (double)large * 0x1p-48;
     }
-    if (got <= LIST) return;
+    if (listed) return;
     float last = INFINITY;
     int last_token = -1;
     for (int k = 0; k < a.n; k++) {  // LIST > n: there are that many
