@@ -182,7 +182,7 @@ int focr_paged_attention(const focr_paged_cache *cache, const void *q, int q_dty
         if (rc) return rc;
         if (q_dtype != FOCR_F32 && q_dtype != FOCR_F16 && q_dtype != FOCR_BF16)
             return fail(FOCR_E_ARG, "paged_attention: unknown query type " + std::to_string(q_dtype));
-        if (q_heads == 0 || q_heads % cache->kv_heads || q_heads > INT32_MAX)
+        if (q_heads == 0 || q_heads % cache->kv_heads || q_heads > (1u << 20))
             return fail(FOCR_E_SHAPE, "paged_attention: " + std::to_string(q_heads) +
                                           " query heads over " + std::to_string(cache->kv_heads) +
                                           " kv heads");

@@ -90,12 +90,16 @@ def attention(cache, q, lens, scale, refs=None, window=0):
             probs[r, h] = (at, p.sum(0))
             # A score is a dot of dim products and one product with the scale:
             # (dim + 2) roundings of sums no larger than scale * |q| . |k|. A
-            # probability is exp of that (2 units of 2^-23 for the exponential and
-            # 2 for its argument of at most 2^7 in base 2, relative to the row's
-            # own maximum), and is divided by a sum of n of them; numerator and
-            # denominator add n terms each.
+            # probability is exp of a difference of two scores (2^-22 for the
+            # exponential, and 2^-24 of its argument, which is no larger than the
+            # scores' span); numerator and denominator add n terms each. With a
+            # 16-bit query a probability enters the product as two parts of 8
+            # bits or more, which leaves 2^-18 of it.
             ds = (dim + 2) * eps * (scale * qs.abs() @ k[h].abs().T).amax(-1, keepdim=True)
-            rel = 2 * ds + 2 * (len(at) + 16) * eps + 2.0 ** -21 + 2.0 ** -15 * (s.amax(-1, keepdim=True) - s).clamp(max=127).amax(-1, keepdim=True) * 2.0 ** -8
+            span = s.amax(-1, keepdim=True) - s.amin(-1, keepdim=True)
+            rel = 2 * ds + 2 * (len(at) + 16) * eps + 2.0 ** -21 + 2 * eps * span
+            if q.dtype != torch.float32:
+                rel = rel + 2.0 ** -18
             bound[r, h * group:(h + 1) * group] = rel * (p @ v[h].abs()) + 1e-30
     bound = bound + out.abs() * HALF_STEP[q.dtype]
     if q.dtype == torch.float16:

@@ -89,6 +89,25 @@ def test_select_close_scores_of_different_beams(cuda):
         check_select(x, scores, 4)
 
 
+@pytest.mark.parametrize("at", [1.0, -900.0, 1023.5, 5000.0, -70000.0, 1e12, -3e38])
+def test_select_logits_far_from_zero(cuda, at):
+    """Log probabilities do not depend on where the logits lie."""
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn((2, 3, 5000), generator=g) * 3 + at
+    check_select(x, torch.randn((2, 3), generator=g), 6)
+
+
+def test_select_probabilities_add_up(cuda):
+    """Flat, steep and mixed rows: exp of the scores of a whole small vocabulary is 1."""
+    from franken_ocr_b200 import beam
+
+    g = torch.Generator().manual_seed(9)
+    for scale in (0.0, 1e-3, 1.0, 30.0):
+        x = (torch.randn((1, 1, 64), generator=g) * scale).cuda()
+        score, _, _ = beam.beam_select(x, torch.zeros((1, 1), device="cuda"), 64)
+        assert abs(float(score.double().exp().sum()) - 1) <= 64 * 2.0 ** -23   # each rounded to f32
+
+
 @pytest.mark.parametrize("kind", ["bool", "uint8"])
 def test_select_ended_beams(cuda, kind):
     g = torch.Generator().manual_seed(5)
@@ -220,6 +239,33 @@ def test_reorder_one_layer_without_its_dimension_and_parents_out_of_range(cuda):
     check_reorder(*case, flat=True)
     case[3][0] = torch.tensor([-1, 4, 100, 2])
     check_reorder(*case)
+
+
+def test_reorder_beyond_32_bits_and_in_a_replayed_graph(cuda):
+    from franken_ocr_b200 import beam
+
+    layers, pages, page, dim = 3, 50000, 64, 256
+    kp = torch.empty((layers, pages, 1, page, dim), dtype=torch.float16, device="cuda")
+    vp = torch.empty_like(kp)
+    table = torch.tensor([[0, pages - 1, -1], [1, pages - 2, -1]], dtype=torch.int32, device="cuda")
+    fresh = torch.tensor([pages - 3, pages - 4], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([90, 90], dtype=torch.int32, device="cuda")
+    parent = torch.tensor([[1, 1]], dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for p in (pages - 1, pages - 2):
+        kp[:, p] = torch.randn((layers, 1, page, dim), generator=g, device="cuda")
+        vp[:, p] = torch.randn((layers, 1, page, dim), generator=g, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        new, _, _ = beam.beam_reorder(kp, vp, table, lens, parent, fresh)
+    for want in ([1, 1], [1, 0]):
+        parent.copy_(torch.tensor([want]))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert new.tolist() == [[table[w, 0].item(), f, -1] for w, f in zip(want, (pages - 3, pages - 4))]
+        for i, w in enumerate(want):
+            for pool in (kp, vp):
+                assert same_bits(pool[:, pages - 3 - i, :, :26], pool[:, pages - 1 - w, :, :26])
 
 
 def test_reorder_skips_pages_outside_the_pool(cuda):

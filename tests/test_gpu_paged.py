@@ -138,7 +138,7 @@ def test_attention_types(cuda, q_type, pool, dim):
 
 
 @pytest.mark.parametrize("group", [1, 2, 3, 4, 5, 7, 8, 9, 16, 17, 33])
-@pytest.mark.parametrize("q_type,pool", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16"), ("f16", "f16")])
+@pytest.mark.parametrize("q_type,pool", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16"), ("f16", "f16"), ("f32", "f16")])
 def test_attention_head_groups_with_weights(cuda, group, q_type, pool):
     lens = [130, 1, 0, 77]
     c = Cache(lens, 3, 16, 128, DTYPES[pool], seed=group)
@@ -255,6 +255,105 @@ def test_attention_strided_queries_and_out(cuda):
     assert same_bits(out, want)
 
 
+@pytest.mark.parametrize("pool", ["f16", "bf16"])
+@pytest.mark.parametrize("size", [1e-30, 1e-5, 300.0, 1e6])
+def test_attention_f32_queries_of_any_size(cuda, pool, size):
+    """Split queries keep 24 bits whatever their size; heads of one group differ."""
+    c = Cache([90, 40], 2, 16, 128, DTYPES[pool], seed=12)
+    q = torch.randn((2, 12, 128), generator=torch.Generator().manual_seed(13))
+    q[:, ::2] *= size
+    q[0, 5] = 0.0
+    check_attention(c, q, [90, 40], scale=min(0.1, 0.5 / size))
+
+
+@pytest.mark.parametrize("pool,group,dim", [("f32", 1, 128), ("bf16", 1, 64), ("bf16", 6, 128), ("f16", 20, 256)])
+@pytest.mark.parametrize("heads", [1, 3])
+def test_attention_small_and_large_tables_agree(cuda, pool, group, dim, heads):
+    """The same rows behind a table of their own size (shared by a cluster of blocks) and
+    behind one for long contexts (runs of tiles and a join); lengths of 0 and out of
+    range among them."""
+    from franken_ocr_b200 import paged
+
+    lens = [300, 0, 1, 33]
+    c = Cache(lens, heads, 16, dim, DTYPES[pool], seed=dim)
+    q = torch.randn((4, heads * group, dim), generator=torch.Generator().manual_seed(1)).to(DTYPES[pool])
+    kp, vp, table = c.cuda()
+    wide = torch.full((4, 1 << 16), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    outs, sums = [], []
+    for t in (table, wide):
+        w = torch.zeros((4, heads, 320), device="cuda")
+        outs.append(check_attention(c, q, lens, dev=(kp, vp, t)))
+        outs.append(paged.paged_attention(q.cuda(), kp, vp, t, torch.tensor(lens, dtype=torch.int32, device="cuda"), weights=w))
+        sums.append(w)
+    want, _, bound = attention(c, q, lens, 1 / math.sqrt(dim))
+    for out in outs:
+        assert bool(((out.cpu().double() - want).abs() <= bound).all())
+    for w in sums:
+        # every query head's probabilities add up to 1: 300 f32 values below 1 each
+        assert torch.allclose(w.sum(-1).cpu(), torch.tensor([[group] * heads if n else [0] * heads for n in lens]).float(),
+                              rtol=0, atol=group * 320 * 2.0 ** -20)
+    bad = torch.tensor([300, 0, 1, 1 << 21], dtype=torch.int32, device="cuda")
+    for t in (table, wide):
+        out = paged.paged_attention(q.cuda(), kp, vp, t, bad)
+        assert bool(out[3].isnan().all()) and bool((out[1] == 0).all()) and bool(out[0].isfinite().all())
+
+
+def test_calls_on_other_streams(cuda):
+    """Work goes to the current stream, also two calls at once on two streams."""
+    from franken_ocr_b200 import paged
+
+    c = Cache([3000, 900], 2, 16, 128, torch.bfloat16, seed=14)
+    kp, vp, table = c.cuda()
+    lens = torch.tensor([3000, 900], dtype=torch.int32, device="cuda")
+    g = torch.Generator().manual_seed(15)
+    qs = [torch.randn((2, 8, 128), generator=g).to(torch.bfloat16).cuda() for _ in range(2)]
+    want = [paged.paged_attention(q, kp, vp, table, lens) for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                outs[i].append(paged.paged_attention(qs[i], kp, vp, table, lens))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(same_bits(o, want[i]) for o in outs[i])
+    # a value written on the side stream is seen by the call behind it there
+    with torch.cuda.stream(streams[0]):
+        q = torch.zeros_like(qs[0])
+        torch.cuda._sleep(2_000_000)
+        q.copy_(qs[1])
+        out = paged.paged_attention(q, kp, vp, table, lens)
+    torch.cuda.synchronize()
+    assert same_bits(out, want[1])
+
+
+def test_weights_in_a_replayed_graph(cuda):
+    """A captured step adds its weights once a replay, and sees changed lengths."""
+    from franken_ocr_b200 import paged
+
+    c = Cache([70, 50], 2, 16, 64, torch.float32, seed=16)
+    kp, vp, table = c.cuda()
+    q = torch.randn((2, 2, 64), generator=torch.Generator().manual_seed(1)).cuda()
+    lens = torch.tensor([70, 50], dtype=torch.int32, device="cuda")
+    once = torch.zeros((2, 2, 80), device="cuda")
+    paged.paged_attention(q, kp, vp, table, lens, weights=once)
+    w = torch.zeros_like(once)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        paged.paged_attention(q, kp, vp, table, lens, weights=w)
+    w.zero_()
+    for _ in range(4):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.allclose(w, 4 * once, rtol=2.0 ** -20, atol=0)
+    lens.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.allclose(w, 4 * once, rtol=2.0 ** -20, atol=0)
+
+
 def test_attention_is_the_same_every_time_and_in_a_graph(cuda):
     """Repeated calls give the same bits; a captured call follows its inputs, also
     beside another captured call."""
@@ -366,7 +465,7 @@ def test_evict_ties_infinities_and_nan(cuda):
     check_evict(c, w, lens, 32, 3, 5)
 
 
-@pytest.mark.parametrize("n,budget", [(5000, 700), (70000, 3), (40000, 39999), (140000, 9000)])
+@pytest.mark.parametrize("n,budget", [(5000, 700), (70000, 3), (40000, 39999), (140000, 9000), (300000, 2000)])
 def test_evict_long_rows(cuda, n, budget):
     from franken_ocr_b200 import paged
 
@@ -391,6 +490,34 @@ def test_evict_long_rows(cuda, n, budget):
             assert same_bits(pool[into[0].long()[at // page], h, at % page], pool[table[0].long()[keep // page], h, keep % page])
         assert same_bits(wo[0, h, :budget], w[0, h, keep]) and bool((wo[0, h, budget:] == 0).all())
     assert lens.tolist() == [budget]
+
+
+def test_evict_in_a_replayed_graph_and_beyond_32_bits(cuda):
+    """A captured eviction follows its weights; its pages lie past 4 GB."""
+    from franken_ocr_b200 import paged
+
+    pages, page, dim = 140000, 64, 256
+    kp = torch.empty((pages, 1, page, dim), dtype=torch.float16, device="cuda")
+    vp = torch.empty_like(kp)
+    table = torch.tensor([[pages - 1, pages - 2, 3]], dtype=torch.int32, device="cuda")
+    into = torch.tensor([[pages - 3]], dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for p in table[0].tolist():
+        kp[p], vp[p] = torch.randn((1, page, dim), generator=g, device="cuda"), torch.randn((1, page, dim), generator=g, device="cuda")
+    lens = torch.tensor([150], dtype=torch.int32, device="cuda")
+    w = torch.rand((1, 1, 160), generator=g, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept, new, wo = paged.paged_evict(kp, vp, table, lens, w, into, 50, sink=2, recent=7)
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        keep = evict_kept(w[0, 0].cpu(), 150, 50, 2, 7)
+        assert kept[0, 0].tolist() == keep and new.tolist() == [50]
+        keep = torch.tensor(keep, device="cuda")
+        for pool in (kp, vp):
+            assert same_bits(pool[pages - 3, 0, :50], pool[table[0].long()[keep // page], 0, keep % page])
+        w.copy_(torch.rand(w.shape, generator=g, device="cuda"))
 
 
 def test_evict_lengths_out_of_range_and_bad_pages(cuda):
