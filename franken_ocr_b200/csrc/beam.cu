@@ -129,11 +129,17 @@ __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) 
     }
     auto token = [&](int i) { return first + (i / V * ST + t) * V + i % V; };
     // NaN loses every maximum and comparison; +inf counts as the largest number
+    float most[PER / 4];   // of each four
 #pragma unroll
-    for (int i = 0; i < PER; i++) top = fmaxf(top, v[i]);
+    for (int g = 0; g < PER / 4; g++) {
+        most[g] = fmaxf(fmaxf(v[4 * g], v[4 * g + 1]), fmaxf(v[4 * g + 2], v[4 * g + 3]));
+        top = fmaxf(top, most[g]);
+    }
     if (top == INFINITY) {
 #pragma unroll
         for (int i = 0; i < PER; i++) v[i] = v[i] == INFINITY ? LARGEST : v[i];
+#pragma unroll
+        for (int g = 0; g < PER / 4; g++) most[g] = fminf(most[g], LARGEST);
         top = LARGEST;
     }
     const int lanes = group_lanes(a.n), groups = ST / lanes;
@@ -170,38 +176,37 @@ __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) 
     const float2 minus = make_float2(-zero, -zero);
     double sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < PER; i += 4) {
-        float s = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-            float2 y = add2(make_float2(v[i + e], v[i + e + 1]), minus);
-            y = make_float2(fmaxf(y.x, none), fmaxf(y.y, none));
-            const float2 x = exp_below(y, base);
-            if (y.x < near0) s += x.x;
-            if (y.y < near0) s += x.y;
+    for (int g = 0; g < PER / 4; g++) {
+        float2 y0 = add2(make_float2(v[4 * g], v[4 * g + 1]), minus), y1 = add2(make_float2(v[4 * g + 2], v[4 * g + 3]), minus);
+        y0 = make_float2(fmaxf(y0.x, none), fmaxf(y0.y, none));
+        y1 = make_float2(fmaxf(y1.x, none), fmaxf(y1.y, none));
+        float2 x0 = exp_below(y0, base), x1 = exp_below(y1, base);
+        if (most[g] >= near) {   // rarely: those are summed in 64 bits below
+            x0.x = y0.x < near0 ? x0.x : 0.0f;
+            x0.y = y0.y < near0 ? x0.y : 0.0f;
+            x1.x = y1.x < near0 ? x1.x : 0.0f;
+            x1.y = y1.y < near0 ? x1.y : 0.0f;
         }
-        sum += s;
+        x0 = add2(x0, x1);
+        sum += x0.x + x0.y;
     }
     __syncthreads();
     // the few that are large or candidates
     const float low = bound, few = fminf(low, near);
     int c = 0;
-    uint32_t hits = 0;   // groups of 4 with one of them
 #pragma unroll
-    for (int g = 0; g < PER; g += 4)
-        if (fmaxf(fmaxf(v[g], v[g + 1]), fmaxf(v[g + 2], v[g + 3])) >= few) {
-            hits |= 1u << g / 4;
+    for (int g = 0; g < PER / 4; g++)
+        if (most[g] >= few)
 #pragma unroll
-            for (int i = g; i < g + 4; i++) c += v[i] >= few && v[i] > -INFINITY;
-        }
+            for (int i = 4 * g; i < 4 * g + 4; i++) c += v[i] >= few && v[i] > -INFINITY;
     if (c) {
         int k = atomicAdd(&count, c);
         if (k + c <= LIST)
 #pragma unroll
-            for (int g = 0; g < PER; g += 4)
-                if (hits >> g / 4 & 1)
+            for (int g = 0; g < PER / 4; g++)
+                if (most[g] >= few)
 #pragma unroll
-                    for (int i = g; i < g + 4; i++)
+                    for (int i = 4 * g; i < 4 * g + 4; i++)
                         if (v[i] >= few && v[i] > -INFINITY) {
                             lx[k] = v[i];
                             lt[k++] = token(i);
