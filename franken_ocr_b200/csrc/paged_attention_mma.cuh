@@ -10,6 +10,9 @@
 // larger tiles.  P, and a query in f32, are split into parts of the cache's type that
 // are multiplied one after the other, so nothing is rounded to fewer bits than the
 // output has.
+//
+// Measured: 8 rows x 131072 positions, 64 / 8 heads of 128, bf16: 656 us, 6.5 TB/s;
+// 16 x 8192 x 8 heads: 93 us at 3 query heads each, 98 at 8, 109 at 16 (4.9 TB/s).
 #pragma once
 
 #include "paged_attention.cuh"
@@ -324,13 +327,16 @@ template <typename T, int D, bool F32Q> int launch_mma(AttnArgs &a, cudaStream_t
     a.cluster = cluster_of(a);
     return launch_attn(paged_attention_mma_kernel<T, D, F32Q>, mma_smem<D>(), a, st);
 }
-// Whether this kernel takes the call: from 3 query heads a kv head (with 2 the f32
-// units are as fast), an f32 query from 4, and only up to head_dim 128, where its
-// parts fit the registers.
+// Whether this kernel takes the call: from 3 query heads a kv head on, an f32 query
+// up to head_dim 128 only, where its parts fit the registers.  16 rows x 8192
+// positions x 8 kv heads, head_dim 128, this kernel against the f32 units:
+//   query of the cache's type: 2 heads 94 / 93 us, 3 heads 93 / 116, 5 heads 96 / 212;
+//   f32 query:                 2 heads 108 / 90,   3 heads 109 / 113, 5 heads 114 / 206;
+//   head_dim 64: 2 heads 52 / 54, 3 heads 53 / 67; 256: 2 heads 184 / 174, 3 heads 188 / 226.
 template <typename T> bool mma_takes(const AttnArgs &a) {
     constexpr int own = std::is_same<T, __half>::value ? FOCR_F16 : FOCR_BF16;
     if (a.q_type == own) return a.group >= 3;
-    return a.q_type == FOCR_F32 && a.group >= 4 && a.dim <= 128;
+    return a.q_type == FOCR_F32 && a.group >= 3 && a.dim <= 128;
 }
 template <typename T> int launch_mma_dim(AttnArgs &a, cudaStream_t st) {
     if (a.q_type == FOCR_F32)
