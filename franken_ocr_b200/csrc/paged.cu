@@ -17,7 +17,7 @@ int paged_view(const char *ctx, const focr_paged_cache *c, size_t rows, PagedVie
     if (c->head_dim > 256 || c->head_dim * size % 16)
         return fail(FOCR_E_UNSUPPORTED, at + "head_dim " + std::to_string(c->head_dim) +
                                             " is over 256 or not a multiple of 16 bytes");
-    if ((uint64_t)c->max_pages * c->page_size >= (uint64_t)INT32_MAX)
+    if ((uint64_t)c->max_pages * c->page_size > (uint64_t)INT32_MAX - 65535)   // room for whole tiles
         return fail(FOCR_E_UNSUPPORTED, at + "max_pages * page_size exceeds int32 range");
     const size_t rows_bytes = (size_t)c->page_size * c->head_dim;
     if (c->page_stride > (size_t)INT64_MAX / size / c->n_pages ||

@@ -191,10 +191,12 @@ int focr_paged_attention(const focr_paged_cache *cache, const void *q, int q_dty
             return fail(FOCR_E_SHAPE, "paged_attention: " + std::to_string(q_heads) +
                                           " query heads over " + std::to_string(cache->kv_heads) +
                                           " kv heads");
-        if (!(scale > 0.0f) || !std::isfinite(scale))
+        a.c2 = (float)(scale * 1.4426950408889634);
+        if (!(a.c2 > 0.0f) || !std::isfinite(a.c2))
             return fail(FOCR_E_ARG, "paged_attention: scale must be positive and finite");
         if (rows == 0) return FOCR_OK;
         if (!q || !lens || !out || !workspace) return fail(FOCR_E_ARG, "paged_attention: null pointer");
+        if (out == q) return fail(FOCR_E_ARG, "paged_attention: out must not be q");
         if (rows > INT32_MAX) return fail(FOCR_E_UNSUPPORTED, "paged_attention: dimension exceeds int32 range");
         const size_t wide = q_heads * cache->head_dim;
         if (rows > 1 && (q_stride < wide || out_stride < wide))
@@ -233,7 +235,6 @@ int focr_paged_attention(const focr_paged_cache *cache, const void *q, int q_dty
         a.width = (int)width;
         a.score_stride = (int)((width + 1) & ~(size_t)1);
         a.cap = weights ? (int)width : (int)cap;
-        a.c2 = (float)(scale * 1.4426950408889634);
         const size_t q_size = dtype_bytes(q_dtype);
         for (size_t r0 = 0; r0 < rows; r0 += ATTN_ROWS) {
             AttnArgs b = a;

@@ -513,7 +513,7 @@ int focr_decoder_generate(focr_decoder *d, const float *embeds, size_t seq, size
  * [0, n_pages) name no page: entries that no position below the row's length
  * uses are never read.  head_dim * element size and both strides are
  * multiples of 16 bytes, k and v 16-byte aligned, head_dim <= 256, and
- * max_pages * page_size < 2^31. */
+ * max_pages * page_size <= 2^31 - 2^16. */
 typedef struct focr_paged_cache {
     void *k, *v;
     const int32_t *table; /* [rows][table_stride], max_pages entries used */
@@ -536,7 +536,7 @@ int focr_paged_write(const focr_paged_cache *c, size_t rows, const void *k, cons
 /* Attention of one new token per row: q, out [rows][q_heads][head_dim] of
  * `q_dtype` (rows q_stride / out_stride elements apart); query head h reads
  * kv head h / (q_heads / kv_heads).  Row r sees the positions j < lens[r]
- * of its pages; with window > 0 only j < ref_lens[r] (NULL: 0) and
+ * of its pages; out must not overlap q; with window > 0 only j < ref_lens[r] (NULL: 0) and
  * j >= lens[r] - window, which is the R-SWA rule of decode_attention
  * (rswa.rs:855-944).  out = softmax(scale * q.k) . v, all sums in f32, rounded
  * once.  A row that sees nothing gives zeros; a row whose length passes
@@ -603,7 +603,8 @@ int focr_beam_select(const void *logits, int dtype, size_t batch, size_t beams, 
  * where nothing is copied, so every beam can go on writing.  lens_out [rows].
  * Entries behind that page become -1.  weights [layers][rows][kv_heads][width]
  * (may be NULL) follow into weights_out, contiguous, with 0 from the new
- * length on.  A parent outside [0, beams) leaves an empty row.  The fresh pages
+ * length on.  A parent outside [0, beams) leaves an empty row, and a length past
+ * the table counts as 0.  The fresh pages
  * must differ from one another and from every page the table uses.  The paged
  * form of compacting BatchedRingCache slots (rswa.rs:620-700). */
 int focr_beam_reorder(const focr_paged_cache *c, size_t layers, size_t layer_stride,

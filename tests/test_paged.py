@@ -20,7 +20,7 @@ def write(c, rows=4, k=PTR, v=PTR, src=F32, tokens=4, ks=128, vs=128, row=None, 
     check(lib.focr_paged_write(C.byref(c) if c else None, rows, k, v, src, tokens, ks, vs, row, pos, None))
 
 
-def attend(c, q=PTR, qt=F32, rows=4, heads=4, qs=256, lens=PTR, refs=None, window=0, scale=0.125, out=PTR, os=256,
+def attend(c, q=PTR, qt=F32, rows=4, heads=4, qs=256, lens=PTR, refs=None, window=0, scale=0.125, out=2 * PTR, os=256,
            w=None, ww=0, wr=0, wh=0, ws=PTR, wsb=1 << 40):
     check(lib.focr_paged_attention(C.byref(c), q, qt, rows, heads, qs, lens, refs, window, scale, out, os, w, ww, wr,
                                    wh, ws, wsb, None))
@@ -49,6 +49,7 @@ def reorder(c, layers=2, ls=10 * 2 * 16 * 64, batch=2, beams=2, lens=PTR, parent
     (dict(head_dim=260, head_stride=16 * 260, page_stride=32 * 260), -7, "head_dim 260"),
     (dict(head_dim=62), -7, "head_dim 62"), (dict(head_dim=68, dtype=BF16), -7, "head_dim 68"),
     (dict(max_pages=1 << 27, table_stride=1 << 27), -7, "max_pages * page_size"),
+    (dict(max_pages=(1 << 27) - 4095, table_stride=1 << 27), -7, "max_pages * page_size"),
     (dict(page_stride=2049), -7, "multiples of 16"), (dict(head_stride=1023 * 4, dtype=F16), -7, "multiples of 16"),
     (dict(head_stride=512), -1, "shorter than"), (dict(page_stride=512), -1, "shorter than"),
     (dict(page_stride=1 << 62), -1, "stride overflow"), (dict(table_stride=3), -1, "table_stride 3 < max_pages 4"),
@@ -85,7 +86,7 @@ def test_write_refusals(bad, code, text):
 @pytest.mark.parametrize("bad,code,text", [
     (dict(qt=-1), -2, "unknown query type"), (dict(heads=3), -1, "3 query heads over 2 kv heads"),
     (dict(heads=0), -1, "0 query heads"), (dict(scale=0.0), -2, "scale"), (dict(scale=-1.0), -2, "scale"),
-    (dict(scale=float("nan")), -2, "scale"), (dict(scale=float("inf")), -2, "scale"), (dict(q=None), -2, "null"),
+    (dict(scale=float("nan")), -2, "scale"), (dict(scale=3e38), -2, "scale"), (dict(out=PTR), -2, "out must not be q"), (dict(scale=float("inf")), -2, "scale"), (dict(q=None), -2, "null"),
     (dict(lens=None), -2, "null"), (dict(out=None), -2, "null"), (dict(ws=None), -2, "null"),
     (dict(qs=255), -1, "row stride"), (dict(os=255), -1, "row stride"), (dict(wsb=100), -2, "workspace needs"),
     (dict(ws=PTR + 8), -2, "workspace needs"), (dict(w=PTR, ww=0, wr=10, wh=10), -1, "weights_width"),
