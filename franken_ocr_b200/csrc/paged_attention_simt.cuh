@@ -147,21 +147,33 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
                 }
 #pragma unroll
                 for (int o = LPK / 16; o > 0; o >>= 1) s[g][0] += __shfl_xor_sync(0xffffffffu, s[g][0], o);
-                const float sc = live ? s[g][0] : -INFINITY;
-                if (__any_sync(0xffffffffu, sc > m[g])) {
-                    const float top = fmaxf(m[g], warp_max_f32(sc));
+                if (!live) s[g][0] = -INFINITY;
+            }
+            // one vote for all heads: their chains run side by side
+            bool rises = false;
+#pragma unroll
+            for (int g = 0; g < GP; g++) rises |= s[g][0] > m[g];
+            if (__any_sync(0xffffffffu, rises)) {
+#pragma unroll
+                for (int g = 0; g < GP; g++) {
+                    const float top = fmaxf(m[g], warp_max_f32(s[g][0]));
                     const float f = prob(m[g], a.c2, scaled_max(top, a.c2));
                     m[g] = top;
                     l[g] *= f;
 #pragma unroll
                     for (int e = 0; e < EPL; e++) acc[g][e] *= f;
                 }
-                const float p = prob(sc, a.c2, scaled_max(m[g], a.c2));
+            }
+#pragma unroll
+            for (int g = 0; g < GP; g++) {
+                const float p = prob(s[g][0], a.c2, scaled_max(m[g], a.c2));
                 l[g] += p;
                 probs[g * KEYS + sub * ITS + my_it] = p;
-                if (a.scores && live && g < heads)
-                    a.scores[((int64_t)r * a.q_heads + qh0 + g) * a.score_stride + i] = sc;
             }
+            if (a.scores && live)
+#pragma unroll
+                for (int g = 0; g < GP; g++)
+                    if (g < heads) a.scores[((int64_t)r * a.q_heads + qh0 + g) * a.score_stride + i] = s[g][0];
             __syncwarp();
 #pragma unroll
             for (int it = 0; it < ITS; it++) {
