@@ -327,16 +327,18 @@ template <typename T, int D, bool F32Q> int launch_mma(AttnArgs &a, cudaStream_t
     a.cluster = cluster_of(a);
     return launch_attn(paged_attention_mma_kernel<T, D, F32Q>, mma_smem<D>(), a, st);
 }
-// Whether this kernel takes the call: from 3 query heads a kv head on, an f32 query
-// up to head_dim 128 only, where its parts fit the registers.  16 rows x 8192
-// positions x 8 kv heads, head_dim 128, this kernel against the f32 units:
-//   query of the cache's type: 2 heads 94 / 93 us, 3 heads 93 / 116, 5 heads 96 / 212;
-//   f32 query:                 2 heads 108 / 90,   3 heads 109 / 113, 5 heads 114 / 206;
-//   head_dim 64: 2 heads 52 / 54, 3 heads 53 / 67; 256: 2 heads 184 / 174, 3 heads 188 / 226.
+// Whether this kernel takes the call.  16 rows x 8192 positions x 8 kv heads, bf16, this
+// kernel against the f32 units:
+//   query of the cache's type, from 3 query heads a kv head on: head_dim 64: 2 heads
+//   53.8 / 53.5 us, 3 heads 52.5 / 62.6; 128: 92.9 / 91.3, 92.8 / 104.9; 256: 184 / 177,
+//   187.8 / 188.7, 6 heads 195 / 308;
+//   f32 query, three times the products: head_dim 64 from 3 heads on, 57.0 / 59.8; 128
+//   from 5 on, 4 heads 110 / 104, 6 heads 114 / 176; not at 256, where its parts do
+//   not fit the registers.
 template <typename T> bool mma_takes(const AttnArgs &a) {
     constexpr int own = std::is_same<T, __half>::value ? FOCR_F16 : FOCR_BF16;
     if (a.q_type == own) return a.group >= 3;
-    return a.q_type == FOCR_F32 && a.group >= 3 && a.dim <= 128;
+    return a.q_type == FOCR_F32 && a.dim <= 128 && a.group >= (a.dim <= 64 ? 3 : 5);
 }
 template <typename T> int launch_mma_dim(AttnArgs &a, cudaStream_t st) {
     if (a.q_type == FOCR_F32)

@@ -33,8 +33,8 @@ template <typename T, int D, int GP> constexpr int simt_smem() {
 // The arithmetic runs on the f32 units: with few query heads a kv head the
 // loads bound it (a key of 128 16-bit values costs a warp ~25 instructions a
 // head against 512 bytes).  16 rows x 8192 positions x 8 kv heads of 128: bf16 90 us
-// with one query head (6.0 TB/s), 93 with two; f32 165 us (6.5 TB/s), 174 with four
-// query heads, 279 with eight, where the f32 units bound it.
+// with one query head (6.0 TB/s), 92 with two; f32 167 us (6.4 TB/s), 174 with four
+// query heads, 203 with eight, where 8 warps an SM leave the f32 units waiting.
 template <typename T, int D, int GP>
 __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(const AttnArgs a) {
     using S = Tile<T, D>;
