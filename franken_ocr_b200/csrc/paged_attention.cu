@@ -47,10 +47,9 @@ __global__ void __launch_bounds__(JT) paged_join_kernel(const AttnArgs a, int bl
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < JT / 32; w++) M = fmaxf(M, warp_m[w]);
-    const float mc = scaled_max(M, a.c2);
     for (int p = t; p < pieces; p += JT) {
         const float2 ml = a.ml[slot(p) * a.gp + g];
-        const float f = prob(ml.x, a.c2, mc);
+        const float f = rescale(ml.x, M, a.c2);
         factor[p] = f;
         L = __fmaf_rn(ml.y, f, L);
     }

@@ -10,7 +10,7 @@
 //
 // One pass over K and V with a running maximum and sum (base-2 exponentials
 // of c * s, c = scale * log2 e); partial results join by
-//   M = max m_i,  L = sum l_i 2^(c (m_i - M)),  out = sum a_i 2^(c (m_i - M)) / L.
+//   M = max m_i,  L = sum l_i 2^(c m_i - c M),  out = sum a_i 2^(c m_i - c M) / L.
 // Everything is held in f32; only K/V themselves have the cache's type, and
 // the output is rounded once to q's type.
 //
@@ -93,6 +93,12 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ float prob(float s, float c, float mc) { return ex2(__fmaf_rn(s, c, -mc)); }
 __device__ __forceinline__ float scaled_max(float m, float c) {
     return m == -INFINITY ? 0.0f : __fmul_rn(m, c);
+}
+// What takes sums relative to the maximum m over to the maximum top >= m: the
+// probabilities were formed with the rounded products, so the factor is too, and is
+// exactly 1 where the maximum stays.
+__device__ __forceinline__ float rescale(float m, float top, float c) {
+    return m == -INFINITY ? 0.0f : ex2(__fsub_rn(__fmul_rn(m, c), scaled_max(top, c)));
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {
@@ -335,10 +341,9 @@ __device__ __forceinline__ void finish_heads(const AttnArgs &a, const Segment &s
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int w = 0; w < ATTN_WARPS; w++) M = fmaxf(M, h.m[w][i]);
-        const float mc = scaled_max(M, a.c2);
 #pragma unroll
         for (int w = 0; w < ATTN_WARPS; w++) {
-            const float f = prob(h.m[w][i], a.c2, mc);
+            const float f = rescale(h.m[w][i], M, a.c2);
             L = __fmaf_rn(h.l[w][i], f, L);
             o = fma4(*reinterpret_cast<const float4 *>(&h.o[w][i][d]), f, o);
         }
@@ -369,12 +374,11 @@ __device__ __forceinline__ void finish_heads(const AttnArgs &a, const Segment &s
         float M = -INFINITY, L = 0.0f;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int q = 0; q < a.cluster; q++) M = fmaxf(M, cluster.map_shared_rank(&h, q)->o[1][i][0]);
-        const float mc = scaled_max(M, a.c2);
 #pragma unroll 8
         for (int q = 0; q < a.cluster; q++) {
             const Handover<HR, D> *y = cluster.map_shared_rank(&h, q);
             const float2 ml = *reinterpret_cast<const float2 *>(&y->o[1][i][0]);
-            const float f = prob(ml.x, a.c2, mc);
+            const float f = rescale(ml.x, M, a.c2);
             L = __fmaf_rn(ml.y, f, L);
             o = fma4(*reinterpret_cast<const float4 *>(&y->o[0][i][d]), f, o);
         }

@@ -201,10 +201,15 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
             cp_async_wait<S::STAGES - 1>();
             __syncwarp();
             const uint32_t ks_s = ring_s + stage * 2 * S::HALF, vs_s = ks_s + S::HALF;
-            float s[NT][4];
+            // The tensor cores cut their sums off where f32 would round, always
+            // towards zero.  That is far below a 16-bit output, but not below an f32
+            // one: there the chains are kept short and joined by f32 additions.
+            constexpr int CHAINS = F32Q ? 3 : 1;   // even steps, odd steps, the query's lower parts
+            float s[NT][4], sc[CHAINS][NT][4];
 #pragma unroll
-            for (int t = 0; t < NT; t++) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
-            // the smallest parts first: the sum's last steps are the ones that count
+            for (int c = 0; c < CHAINS; c++)
+#pragma unroll
+                for (int t = 0; t < NT; t++) sc[c][t][0] = sc[c][t][1] = sc[c][t][2] = sc[c][t][3] = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < D / 16; ks++) {
                 if constexpr (QS) ldmatrix4<false>(qa[0][0], qs_s + ((mi & 1) * 8 + rr) * S::DB + (((ks * 2 + (mi >> 1)) ^ rr) << 4));
@@ -214,11 +219,17 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
                     ldmatrix4<false>(b, ks_s + (p * 16 + (mi >> 1) * 8 + rr) * S::DB + (((ks * 2 + (mi & 1)) ^ rr) << 4));
 #pragma unroll
                     for (int part = QP - 1; part >= 0; part--) {
-                        mma16816<T>(s[2 * p], qa[part][QS ? 0 : ks], b[0], b[1]);
-                        mma16816<T>(s[2 * p + 1], qa[part][QS ? 0 : ks], b[2], b[3]);
+                        auto &to = sc[F32Q ? (part ? 2 : ks & 1) : 0];
+                        mma16816<T>(to[2 * p], qa[part][QS ? 0 : ks], b[0], b[1]);
+                        mma16816<T>(to[2 * p + 1], qa[part][QS ? 0 : ks], b[2], b[3]);
                     }
                 }
             }
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+                    s[t][x] = F32Q ? sc[0][t][x] + sc[CHAINS / 2][t][x] + sc[CHAINS - 1][t][x] : sc[0][t][x];
             if constexpr (F32Q && HALF)
 #pragma unroll
                 for (int t = 0; t < NT; t++)
@@ -252,7 +263,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
                     float n = fmaxf(m[y], top[y]);
                     n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 1));
                     n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 2));
-                    const float f = prob(m[y], a.c2, scaled_max(n, a.c2));
+                    const float f = rescale(m[y], n, a.c2);
                     m[y] = n;
                     l[y] *= f;
 #pragma unroll
@@ -263,27 +274,36 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
                 }
             }
             const float mc[2] = {scaled_max(m[0], a.c2), scaled_max(m[1], a.c2)};
+            uint32_t pa[KEYS / 16][PP][4];
 #pragma unroll
-            for (int kk = 0; kk < KEYS / 16; kk++) {
-                uint32_t pa[PP][4];
+            for (int kk = 0; kk < KEYS / 16; kk++)
 #pragma unroll
                 for (int x = 0; x < 4; x++) {  // registers: (row, low keys), (row + 8, low), (row, high), (row + 8, high)
                     const int t = 2 * kk + (x >> 1), y = x & 1;
                     float p0 = prob(s[t][2 * y], a.c2, mc[y]) * PS, p1 = prob(s[t][2 * y + 1], a.c2, mc[y]) * PS;
                     l[y] += p0 + p1;
 #pragma unroll
-                    for (int p = 0; p < PP; p++) pa[p][x] = take_pair<T>(&p0, &p1);
+                    for (int p = 0; p < PP; p++) pa[kk][p][x] = take_pair<T>(&p0, &p1);
                 }
 #pragma unroll
-                for (int jp = 0; jp < D / 16; jp++) {
+            for (int jp = 0; jp < D / 16; jp++) {
+                float short_sum[2][4] = {};
+#pragma unroll
+                for (int kk = 0; kk < KEYS / 16; kk++) {
                     uint32_t b[4];
                     ldmatrix4<true>(b, vs_s + (kk * 16 + (mi & 1) * 8 + rr) * S::DB + (((jp * 2 + (mi >> 1)) ^ rr) << 4));
 #pragma unroll
                     for (int p = PP - 1; p >= 0; p--) {
-                        mma16816<T>(acc[2 * jp], pa[p], b[0], b[1]);
-                        mma16816<T>(acc[2 * jp + 1], pa[p], b[2], b[3]);
+                        mma16816<T>(F32Q ? short_sum[0] : acc[2 * jp], pa[kk][p], b[0], b[1]);
+                        mma16816<T>(F32Q ? short_sum[1] : acc[2 * jp + 1], pa[kk][p], b[2], b[3]);
                     }
                 }
+                if constexpr (F32Q)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        acc[2 * jp][x] += short_sum[0][x];
+                        acc[2 * jp + 1][x] += short_sum[1][x];
+                    }
             }
             __syncwarp();
             issue(stage, next);
@@ -332,13 +352,13 @@ template <typename T, int D, bool F32Q> int launch_mma(AttnArgs &a, cudaStream_t
 //   query of the cache's type, from 3 query heads a kv head on: head_dim 64: 2 heads
 //   53.8 / 53.5 us, 3 heads 52.5 / 62.6; 128: 92.9 / 91.3, 92.8 / 104.9; 256: 184 / 177,
 //   187.8 / 188.7, 6 heads 195 / 308;
-//   f32 query, three times the products: head_dim 64 from 3 heads on, 57.0 / 59.8; 128
-//   from 5 on, 4 heads 110 / 104, 6 heads 114 / 176; not at 256, where its parts do
-//   not fit the registers.
+//   f32 query, three times the products and short chains, from 5 heads on: head_dim 64:
+//   4 heads 61.7 / 61.1, 6 heads 64 / 100; 128: 4 heads 110 / 104, 6 heads 119 / 176; not
+//   at 256, where its parts do not fit the registers.
 template <typename T> bool mma_takes(const AttnArgs &a) {
     constexpr int own = std::is_same<T, __half>::value ? FOCR_F16 : FOCR_BF16;
     if (a.q_type == own) return a.group >= 3;
-    return a.q_type == FOCR_F32 && a.dim <= 128 && a.group >= (a.dim <= 64 ? 3 : 5);
+    return a.q_type == FOCR_F32 && a.dim <= 128 && a.group >= 5;
 }
 template <typename T> int launch_mma_dim(AttnArgs &a, cudaStream_t st) {
     if (a.q_type == FOCR_F32)

@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
 #pragma unroll
                 for (int g = 0; g < GP; g++) {
                     const float top = fmaxf(m[g], warp_max_f32(s[g][0]));
-                    const float f = prob(m[g], a.c2, scaled_max(top, a.c2));
+                    const float f = rescale(m[g], top, a.c2);
                     m[g] = top;
                     l[g] *= f;
 #pragma unroll

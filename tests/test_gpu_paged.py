@@ -266,6 +266,31 @@ def test_attention_f32_queries_of_any_size(cuda, pool, size):
     check_attention(c, q, [90, 40], scale=min(0.1, 0.5 / size))
 
 
+@pytest.mark.parametrize("pool,group,dim", [("f32", 1, 128), ("f32", 7, 64), ("bf16", 2, 128), ("bf16", 6, 64), ("f16", 16, 128)])
+def test_attention_long_rows_stay_exact(cuda, pool, group, dim):
+    """An f32 output over 60000 positions: sums that take many steps, with maxima that
+    rise along the row and fall behind it, lose no more than their roundings."""
+    from franken_ocr_b200 import paged
+
+    n = 60000
+    c = Cache([n, n], 1, 64, dim, DTYPES[pool], seed=17)
+    # scores that climb over the first row, and peak early in the second
+    q = torch.randn((2, group, dim), generator=torch.Generator().manual_seed(18))
+    for r in range(2):
+        slope = torch.linspace(0, 0.4, n) if r == 0 else torch.linspace(0.4, 0, n)
+        at = torch.arange(n)
+        pages = c.table[r].long()[at // 64]
+        c.k[pages, 0, at % 64] = (c.k[pages, 0, at % 64].float() + slope[:, None] * q[r, 0]).to(c.dtype)
+    out = paged.paged_attention(q.cuda(), *c.cuda(), c.lens.cuda())
+    want, _, _ = attention(c, q, [n, n], 1 / math.sqrt(dim))
+    # A value's error is a sum of n roundings of either sign, 2^-24 of partial sums
+    # that are no larger than about |v| sqrt(n) weights: relative to the output's own
+    # size, which is that of |v| sqrt(n) weights too, some 2^-24 sqrt(steps); 512 steps
+    # and more a warp would be 2^-19.5.
+    rel = float((out.cpu().double() - want).norm() / want.norm())
+    assert rel < 2.0 ** -19.5, rel
+
+
 @pytest.mark.parametrize("pool,group,dim", [("f32", 1, 128), ("bf16", 1, 64), ("bf16", 6, 128), ("f16", 20, 256)])
 @pytest.mark.parametrize("heads", [1, 3])
 def test_attention_small_and_large_tables_agree(cuda, pool, group, dim, heads):
