@@ -110,6 +110,27 @@ class PagedCache(C.Structure):
                     "n_pages", "kv_heads", "page_size", "head_dim", "max_pages")] + [("dtype", i32)]
 
 
+def _args(name: str, pointers: str, sizes: str = "", **rest):
+    """A ctypes structure of pointers, then sizes, then what else there is."""
+    return type(name, (C.Structure,), {"_fields_": [(n, vp) for n in pointers.split()] + [
+        (n, sz) for n in sizes.split()] + list(rest.items())})
+
+
+PagedWriteArgs = _args("PagedWriteArgs", "k v row pos", "rows tokens k_stride v_stride", src_dtype=i32)
+PagedAttentionArgs = _args(
+    "PagedAttentionArgs", "q lens ref_lens out weights workspace", "rows q_heads q_stride out_stride window "
+    "weights_width weights_row_stride weights_head_stride workspace_bytes", q_dtype=i32, scale=C.c_float)
+PagedEvictArgs = _args(
+    "PagedEvictArgs", "lens weights new_table kept lens_out weights_out", "rows width weights_row_stride "
+    "weights_head_stride new_table_stride new_pages budget sink recent")
+BeamSelectArgs = _args(
+    "BeamSelectArgs", "logits scores done scores_out parent_out token_out workspace",
+    "batch beams vocab row_stride n workspace_bytes", dtype=i32, end_token=i32)
+BeamReorderArgs = _args(
+    "BeamReorderArgs", "lens parent fresh table_out lens_out weights weights_out", "layers layer_stride batch beams "
+    "width weights_layer_stride weights_row_stride weights_head_stride")
+
+
 lib.focr_last_error.restype = C.c_char_p
 lib.focr_tier_string.restype = C.c_char_p
 for _name in ("focr_igemm_s8s8", "focr_igemm_u8s8"):
@@ -172,15 +193,11 @@ lib.focr_rope_apply_at.argtypes = [vp, sz, sz, vp, vp, vp, vp]
 lib.focr_ring_write.argtypes = [vp, vp, sz, sz, vp, vp, sz, vp, vp]
 lib.focr_add_rms_norm.argtypes = [vp, vp, sz, sz, vp, C.c_float, vp, vp, vp]
 lib.focr_attention_decode_at.argtypes = [vp, vp, vp, sz, sz, vp, vp, sz, sz, sz, vp, vp, vp]
-lib.focr_paged_write.argtypes = [vp, sz, vp, vp, i32, sz, sz, sz, vp, vp, vp]
+for _name in ("paged_write", "paged_attention", "paged_evict", "beam_reorder"):
+    getattr(lib, "focr_" + _name).argtypes = [vp, vp, vp]
 lib.focr_paged_attention_workspace.argtypes = [sz, sz, sz, sz, vp]
-lib.focr_paged_attention.argtypes = [vp, vp, i32, sz, sz, sz, vp, vp, sz, C.c_float, vp, sz, vp, sz,
-                                     sz, sz, vp, sz, vp]
-lib.focr_paged_evict.argtypes = [vp, sz, vp, vp, sz, sz, sz, vp, sz, sz, sz, sz, sz, vp, vp, vp, vp]
 lib.focr_beam_select_workspace.argtypes = [sz, sz, sz, sz, vp]
-lib.focr_beam_select.argtypes = [vp, i32, sz, sz, sz, sz, vp, vp, C.c_int32, sz, vp, vp, vp, vp, sz,
-                                 vp]
-lib.focr_beam_reorder.argtypes = [vp, sz, sz, sz, sz, vp, vp, vp, vp, vp, vp, sz, sz, sz, sz, vp, vp]
+lib.focr_beam_select.argtypes = [vp, vp]
 STATE_POS, STATE_RING_LEN, STATE_RING_POS, STATE_SLOT, STATE_NEXT_POS, STATE_STEP = range(6)
 STATE_ERROR, STATE_WORDS = 6, 8
 

@@ -10,8 +10,11 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import FOCR_OK, check, lib
-from .paged import _F32, _I32, _U8, _cache, _device, _dtype, _elsewhere, _empty, _need, _stream, _workspace
+from ._lib import FOCR_OK, BeamReorderArgs, BeamSelectArgs, check, lib
+from .paged import _F32, _I32, _U8, _cache, _device, _dtype, _elsewhere, _empty, _need, _packer, _stream, _workspace
+
+_pack_select = _packer(BeamSelectArgs, "13Nii")
+_pack_reorder = _packer(BeamReorderArgs, "15N")
 
 
 def beam_select(logits, scores, n: int | None = None, *, done=None, end_token: int = 1):
@@ -51,10 +54,10 @@ def beam_select(logits, scores, n: int | None = None, *, done=None, end_token: i
     out, parent, token = _empty(shape, (n, 1), _F32), _empty(shape, (n, 1), _I32), _empty(shape, (n, 1), _I32)
     need = _workspace("focr_beam_select_workspace", batch, beams, vocab, n)
     ws = _empty((need,), (1,), _U8)  # lives until the kernels are enqueued
-    rc = lib.focr_beam_select(
-        logits.data_ptr(), code, batch, beams, vocab, stride[1] if beams > 1 else stride[0] if batch > 1 else vocab,
-        scores.data_ptr(), None if done is None else done.data_ptr(), end_token, n, out.data_ptr(), parent.data_ptr(),
-        token.data_ptr(), ws.data_ptr(), need, _stream(index))
+    row = stride[1] if beams > 1 else stride[0] if batch > 1 else vocab
+    rc = lib.focr_beam_select(_pack_select(
+        logits.data_ptr(), scores.data_ptr(), 0 if done is None else done.data_ptr(), out.data_ptr(), parent.data_ptr(),
+        token.data_ptr(), ws.data_ptr(), batch, beams, vocab, row, n, need, code, end_token), _stream(index))
     if rc != FOCR_OK:
         check(rc)
     return out, parent, token
@@ -99,13 +102,14 @@ def beam_reorder(k_pages, v_pages, table, lens, parent, fresh, *, weights=None):
         if stride[-1] != 1 and span > 1:
             raise ValueError(f"{ctx}: the last dimension of weights must be contiguous")
         w_layer = stride[0] if layered else 0
-        w_out = torch.empty(shape, dtype=_F32, device="cuda")
+        wide = rows * heads * span
+        w_out = _empty(tuple(shape), (wide, heads * span, span, 1)[0 if layered else 1:], _F32)
     new_table = _empty((rows, width), (width, 1), _I32)
     new_lens = _empty((rows,), (1,), _I32)
-    rc = lib.focr_beam_reorder(
-        cache, layers, k_pages.stride(0) if layered else 0, batch, beams, lens.data_ptr(), parent.data_ptr(),
-        fresh.data_ptr(), new_table.data_ptr(), new_lens.data_ptr(), None if weights is None else weights.data_ptr(),
-        span, w_layer, w_row, w_head, None if w_out is None else w_out.data_ptr(), _stream(index))
+    rc = lib.focr_beam_reorder(cache, _pack_reorder(
+        lens.data_ptr(), parent.data_ptr(), fresh.data_ptr(), new_table.data_ptr(), new_lens.data_ptr(),
+        0 if weights is None else weights.data_ptr(), 0 if w_out is None else w_out.data_ptr(), layers,
+        k_pages.stride(0) if layered else 0, batch, beams, span, w_layer, w_row, w_head), _stream(index))
     if rc != FOCR_OK:
         check(rc)
     return new_table, new_lens, w_out

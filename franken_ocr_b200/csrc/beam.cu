@@ -593,11 +593,24 @@ int focr_beam_select_workspace(size_t batch, size_t beams, size_t vocab, size_t 
     });
 }
 
-int focr_beam_select(const void *logits, int dtype, size_t batch, size_t beams, size_t vocab,
-                     size_t row_stride, const float *scores, const uint8_t *done, int32_t end_token,
-                     size_t n, float *scores_out, int32_t *parent_out, int32_t *token_out,
-                     void *workspace, size_t workspace_bytes, void *stream) {
+int focr_beam_select(const focr_beam_select_args *args, void *stream) {
     return guarded("beam_select", [&]() -> int {
+        if (!args) return fail(FOCR_E_ARG, "beam_select: null arguments");
+        const void *logits = args->logits;
+        const float *scores = args->scores;
+        const uint8_t *done = args->done;
+        float *scores_out = args->scores_out;
+        int32_t *parent_out = args->parent_out;
+        int32_t *token_out = args->token_out;
+        void *workspace = args->workspace;
+        const size_t batch = args->batch;
+        const size_t beams = args->beams;
+        const size_t vocab = args->vocab;
+        const size_t row_stride = args->row_stride;
+        const size_t n = args->n;
+        const size_t workspace_bytes = args->workspace_bytes;
+        const int dtype = args->dtype;
+        const int32_t end_token = args->end_token;
         if (dtype != FOCR_F32 && dtype != FOCR_F16 && dtype != FOCR_BF16)
             return fail(FOCR_E_ARG, "beam_select: unknown logits type " + std::to_string(dtype));
         if (beams == 0 || vocab == 0 || n == 0)
@@ -651,13 +664,24 @@ int focr_beam_select(const void *logits, int dtype, size_t batch, size_t beams, 
     });
 }
 
-int focr_beam_reorder(const focr_paged_cache *cache, size_t layers, size_t layer_stride,
-                      size_t batch, size_t beams, const int32_t *lens, const int32_t *parent,
-                      const int32_t *fresh, int32_t *table_out, int32_t *lens_out,
-                      const float *weights, size_t width, size_t weights_layer_stride,
-                      size_t weights_row_stride, size_t weights_head_stride, float *weights_out,
-                      void *stream) {
+int focr_beam_reorder(const focr_paged_cache *cache, const focr_beam_reorder_args *args, void *stream) {
     return guarded("beam_reorder", [&]() -> int {
+        if (!args) return fail(FOCR_E_ARG, "beam_reorder: null arguments");
+        const int32_t *lens = args->lens;
+        const int32_t *parent = args->parent;
+        const int32_t *fresh = args->fresh;
+        int32_t *table_out = args->table_out;
+        int32_t *lens_out = args->lens_out;
+        const float *weights = args->weights;
+        float *weights_out = args->weights_out;
+        const size_t layers = args->layers;
+        const size_t layer_stride = args->layer_stride;
+        const size_t batch = args->batch;
+        const size_t beams = args->beams;
+        const size_t width = args->width;
+        const size_t weights_layer_stride = args->weights_layer_stride;
+        const size_t weights_row_stride = args->weights_row_stride;
+        const size_t weights_head_stride = args->weights_head_stride;
         ReorderArgs a{};
         size_t rows;
         if (!checked_mul(batch, beams, &rows)) return fail(FOCR_E_SHAPE, "beam_reorder: batch*beams overflow");

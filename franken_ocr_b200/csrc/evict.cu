@@ -346,13 +346,24 @@ int launch_select(const EvictArgs &a, cudaStream_t st) {
 
 using namespace focr;
 
-extern "C" int focr_paged_evict(const focr_paged_cache *cache, size_t rows, const int32_t *lens,
-                                const float *weights, size_t width, size_t weights_row_stride,
-                                size_t weights_head_stride, const int32_t *new_table,
-                                size_t new_table_stride, size_t new_pages, size_t budget,
-                                size_t sink, size_t recent, int32_t *kept, int32_t *lens_out,
-                                float *weights_out, void *stream) {
+extern "C" int focr_paged_evict(const focr_paged_cache *cache, const focr_paged_evict_args *args, void *stream) {
     return guarded("paged_evict", [&]() -> int {
+        if (!args) return fail(FOCR_E_ARG, "paged_evict: null arguments");
+        const int32_t *lens = args->lens;
+        const float *weights = args->weights;
+        const int32_t *new_table = args->new_table;
+        int32_t *kept = args->kept;
+        int32_t *lens_out = args->lens_out;
+        float *weights_out = args->weights_out;
+        const size_t rows = args->rows;
+        const size_t width = args->width;
+        const size_t weights_row_stride = args->weights_row_stride;
+        const size_t weights_head_stride = args->weights_head_stride;
+        const size_t new_table_stride = args->new_table_stride;
+        const size_t new_pages = args->new_pages;
+        const size_t budget = args->budget;
+        const size_t sink = args->sink;
+        const size_t recent = args->recent;
         EvictArgs a{};
         int rc = paged_view("paged_evict", cache, rows, &a.c);
         if (rc) return rc;

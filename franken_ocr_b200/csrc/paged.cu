@@ -147,11 +147,18 @@ int write_from(int dtype, const PagedView &c, size_t rows, const void *k, const 
 
 using namespace focr;
 
-extern "C" int focr_paged_write(const focr_paged_cache *cache, size_t rows, const void *k,
-                                const void *v, int src_dtype, size_t tokens, size_t k_stride,
-                                size_t v_stride, const int32_t *row, const int32_t *pos,
-                                void *stream) {
+extern "C" int focr_paged_write(const focr_paged_cache *cache, const focr_paged_write_args *args, void *stream) {
     return guarded("paged_write", [&]() -> int {
+        if (!args) return fail(FOCR_E_ARG, "paged_write: null arguments");
+        const void *k = args->k;
+        const void *v = args->v;
+        const int32_t *row = args->row;
+        const int32_t *pos = args->pos;
+        const size_t rows = args->rows;
+        const size_t tokens = args->tokens;
+        const size_t k_stride = args->k_stride;
+        const size_t v_stride = args->v_stride;
+        const int src_dtype = args->src_dtype;
         PagedView c;
         int rc = paged_view("paged_write", cache, rows, &c);
         if (rc) return rc;

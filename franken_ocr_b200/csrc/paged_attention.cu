@@ -174,13 +174,26 @@ int focr_paged_attention_workspace(size_t rows, size_t q_heads, size_t head_dim,
     });
 }
 
-int focr_paged_attention(const focr_paged_cache *cache, const void *q, int q_dtype, size_t rows,
-                         size_t q_heads, size_t q_stride, const int32_t *lens,
-                         const int32_t *ref_lens, size_t window, float scale, void *out,
-                         size_t out_stride, float *weights, size_t weights_width,
-                         size_t weights_row_stride, size_t weights_head_stride, void *workspace,
-                         size_t workspace_bytes, void *stream) {
+int focr_paged_attention(const focr_paged_cache *cache, const focr_paged_attention_args *args, void *stream) {
     return guarded("paged_attention", [&]() -> int {
+        if (!args) return fail(FOCR_E_ARG, "paged_attention: null arguments");
+        const void *q = args->q;
+        const int32_t *lens = args->lens;
+        const int32_t *ref_lens = args->ref_lens;
+        void *out = args->out;
+        float *weights = args->weights;
+        void *workspace = args->workspace;
+        const size_t rows = args->rows;
+        const size_t q_heads = args->q_heads;
+        const size_t q_stride = args->q_stride;
+        const size_t out_stride = args->out_stride;
+        const size_t window = args->window;
+        const size_t weights_width = args->weights_width;
+        const size_t weights_row_stride = args->weights_row_stride;
+        const size_t weights_head_stride = args->weights_head_stride;
+        const size_t workspace_bytes = args->workspace_bytes;
+        const int q_dtype = args->q_dtype;
+        const float scale = args->scale;
         AttnArgs a{};
         int rc = paged_view("paged_attention", cache, rows, &a.c);
         if (rc) return rc;

@@ -27,13 +27,25 @@ import struct
 
 import torch
 
-from ._lib import F32, F16, BF16, FOCR_OK, PagedCache, check, lib
+from ._lib import (BF16, F16, F32, FOCR_OK, PagedAttentionArgs, PagedCache, PagedEvictArgs, PagedWriteArgs, check,
+                   lib)
 
 _TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 _F32, _I32, _U8 = torch.float32, torch.int32, torch.uint8
-# a PagedCache's bytes: packing them costs a third of filling the ctypes structure
-_PACK = struct.Struct("6N5Ii")
-assert _PACK.size == C.sizeof(PagedCache)
+
+
+def _packer(kind, form: str):
+    """The bytes of a ctypes structure: packing them costs a tenth of filling it, or
+    of passing its fields one by one."""
+    s = struct.Struct(form + "0N")
+    assert s.size == C.sizeof(kind), kind
+    return s.pack
+
+
+_pack_cache = _packer(PagedCache, "6N5Ii")
+_pack_write = _packer(PagedWriteArgs, "8Ni")
+_pack_attention = _packer(PagedAttentionArgs, "15Nif")
+_pack_evict = _packer(PagedEvictArgs, "15N")
 _device = torch._C._cuda_getDevice
 _stream = torch._C._cuda_getCurrentRawStream
 
@@ -95,7 +107,7 @@ def _cache(ctx: str, k_pages, v_pages, table, dims: int = 4):
         raise ValueError(f"{ctx}: the entries of a head's page must be contiguous")
     rows, width, step = _table(ctx, "table", table, index)
     try:
-        packed = _PACK.pack(k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), stride[-4], stride[-3],
+        packed = _pack_cache(k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), stride[-4], stride[-3],
                             step, pages, heads, page, dim, width, code)
     except struct.error as e:
         raise ValueError(f"{ctx}: a dimension exceeds 32 bits") from e
@@ -152,8 +164,9 @@ def paged_write(k, v, k_pages, v_pages, table, pos, row=None) -> None:
     _need(ctx, "pos", pos, _I32, (tokens,), index)
     if row is not None:
         _need(ctx, "row", row, _I32, (tokens,), index)
-    rc = lib.focr_paged_write(cache, rows, k.data_ptr(), v.data_ptr(), src, tokens, ks[0], vs[0],
-                              None if row is None else row.data_ptr(), pos.data_ptr(), _stream(index))
+    rc = lib.focr_paged_write(cache, _pack_write(
+        k.data_ptr(), v.data_ptr(), 0 if row is None else row.data_ptr(), pos.data_ptr(), rows, tokens, ks[0], vs[0],
+        src), _stream(index))
     if rc != FOCR_OK:
         check(rc)
 
@@ -198,11 +211,10 @@ def paged_attention(q, k_pages, v_pages, table, lens, *, scale: float | None = N
         _need(ctx, "out", out, q.dtype, shape, index)
     need = _workspace("focr_paged_attention_workspace", rows, heads, dim, width)
     ws = _empty((need,), (1,), _U8)  # lives until the kernels are enqueued
-    rc = lib.focr_paged_attention(
-        cache, q.data_ptr(), code, rows, heads, stride[0], lens.data_ptr(),
-        None if ref_lens is None else ref_lens.data_ptr(), window, 1.0 / math.sqrt(dim) if scale is None else scale,
-        out.data_ptr(), wide, None if weights is None else weights.data_ptr(), width, w_row, w_head, ws.data_ptr(),
-        need, _stream(index))
+    rc = lib.focr_paged_attention(cache, _pack_attention(
+        q.data_ptr(), lens.data_ptr(), 0 if ref_lens is None else ref_lens.data_ptr(), out.data_ptr(),
+        0 if weights is None else weights.data_ptr(), ws.data_ptr(), rows, heads, stride[0], wide, window, width, w_row,
+        w_head, need, code, 1.0 / math.sqrt(dim) if scale is None else scale), _stream(index))
     if rc != FOCR_OK:
         check(rc)
     return out
@@ -235,9 +247,9 @@ def paged_evict(k_pages, v_pages, table, lens, weights, new_table, budget: int, 
     kept = _empty((rows, heads, budget), (heads * budget, budget, 1), _I32)
     new_lens = _empty((rows,), (1,), _I32)
     new_weights = _empty((rows, heads, width), (heads * width, width, 1), _F32)
-    rc = lib.focr_paged_evict(cache, rows, lens.data_ptr(), weights.data_ptr(), width, w_row, w_head,
-                              new_table.data_ptr(), new_step, new_pages, budget, sink, recent, kept.data_ptr(),
-                              new_lens.data_ptr(), new_weights.data_ptr(), _stream(index))
+    rc = lib.focr_paged_evict(cache, _pack_evict(
+        lens.data_ptr(), weights.data_ptr(), new_table.data_ptr(), kept.data_ptr(), new_lens.data_ptr(),
+        new_weights.data_ptr(), rows, width, w_row, w_head, new_step, new_pages, budget, sink, recent), _stream(index))
     if rc != FOCR_OK:
         check(rc)
     return kept, new_lens, new_weights

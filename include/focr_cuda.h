@@ -529,9 +529,13 @@ typedef struct focr_paged_cache {
  * the table, and pages outside the pool are skipped; nothing else is touched.
  * Two tokens of a call must not name the same place.  The paged form of
  * RingCache::record_prefill / write_decode_step (rswa.rs:389, :451-500). */
-int focr_paged_write(const focr_paged_cache *c, size_t rows, const void *k, const void *v,
-                     int src_dtype, size_t tokens, size_t k_stride, size_t v_stride,
-                     const int32_t *row, const int32_t *pos, void *stream);
+typedef struct focr_paged_write_args {
+    const void *k, *v;
+    const int32_t *row, *pos;
+    size_t rows, tokens, k_stride, v_stride; /* rows of the table */
+    int32_t src_dtype;
+} focr_paged_write_args;
+int focr_paged_write(const focr_paged_cache *c, const focr_paged_write_args *a, void *stream);
 
 /* Attention of one new token per row: q, out [rows][q_heads][head_dim] of
  * `q_dtype` (rows q_stride / out_stride elements apart); query head h reads
@@ -550,12 +554,19 @@ int focr_paged_write(const focr_paged_cache *c, size_t rows, const void *k, cons
  * weights_width 0 for the workspace without weights. */
 int focr_paged_attention_workspace(size_t rows, size_t q_heads, size_t head_dim,
                                    size_t weights_width, size_t *bytes);
-int focr_paged_attention(const focr_paged_cache *c, const void *q, int q_dtype, size_t rows,
-                         size_t q_heads, size_t q_stride, const int32_t *lens,
-                         const int32_t *ref_lens, size_t window, float scale, void *out,
-                         size_t out_stride, float *weights, size_t weights_width,
-                         size_t weights_row_stride, size_t weights_head_stride, void *workspace,
-                         size_t workspace_bytes, void *stream);
+typedef struct focr_paged_attention_args {
+    const void *q;
+    const int32_t *lens, *ref_lens;
+    void *out;
+    float *weights;
+    void *workspace;
+    size_t rows, q_heads, q_stride, out_stride, window;
+    size_t weights_width, weights_row_stride, weights_head_stride, workspace_bytes;
+    int32_t q_dtype;
+    float scale;
+} focr_paged_attention_args;
+int focr_paged_attention(const focr_paged_cache *c, const focr_paged_attention_args *a,
+                         void *stream);
 
 /* Shrink rows to `budget` entries by accumulated attention weight.  A row of
  * n <= budget entries keeps all; a longer one keeps its first `sink`, its last
@@ -570,12 +581,16 @@ int focr_paged_attention(const focr_paged_cache *c, const void *q, int q_dtype, 
  * The new pages must not be among the pages that any row of the call reads;
  * the old pages are left as they were.  A length below 0, or past `width` or
  * the table, counts as 0; entries on pages outside the pool are not copied. */
-int focr_paged_evict(const focr_paged_cache *c, size_t rows, const int32_t *lens,
-                     const float *weights, size_t width, size_t weights_row_stride,
-                     size_t weights_head_stride, const int32_t *new_table,
-                     size_t new_table_stride, size_t new_pages, size_t budget, size_t sink,
-                     size_t recent, int32_t *kept, int32_t *lens_out, float *weights_out,
-                     void *stream);
+typedef struct focr_paged_evict_args {
+    const int32_t *lens;
+    const float *weights;
+    const int32_t *new_table;
+    int32_t *kept, *lens_out;
+    float *weights_out;
+    size_t rows, width, weights_row_stride, weights_head_stride, new_table_stride, new_pages;
+    size_t budget, sink, recent;
+} focr_paged_evict_args;
+int focr_paged_evict(const focr_paged_cache *c, const focr_paged_evict_args *a, void *stream);
 
 /* Beam search's choice: from logits [batch][beams][vocab] (rows row_stride
  * elements apart) and the beams' cumulated log probabilities scores
@@ -590,10 +605,17 @@ int focr_paged_evict(const focr_paged_cache *c, size_t rows, const int32_t *lens
  * candidates exist: score -inf, parent and token -1.  beams, n <= 64.
  * Beside argmax_row (sampler.rs:168-186), which it equals for one beam, n = 1. */
 int focr_beam_select_workspace(size_t batch, size_t beams, size_t vocab, size_t n, size_t *bytes);
-int focr_beam_select(const void *logits, int dtype, size_t batch, size_t beams, size_t vocab,
-                     size_t row_stride, const float *scores, const uint8_t *done, int32_t end_token,
-                     size_t n, float *scores_out, int32_t *parent_out, int32_t *token_out,
-                     void *workspace, size_t workspace_bytes, void *stream);
+typedef struct focr_beam_select_args {
+    const void *logits;
+    const float *scores;
+    const uint8_t *done;
+    float *scores_out;
+    int32_t *parent_out, *token_out;
+    void *workspace;
+    size_t batch, beams, vocab, row_stride, n, workspace_bytes;
+    int32_t dtype, end_token;
+} focr_beam_select_args;
+int focr_beam_select(const focr_beam_select_args *a, void *stream);
 
 /* Give every beam its parent's cache: row i of entry b = i / beams becomes row
  * b * beams + parent[i] of the table, in all `layers` (layer l's pages
@@ -607,12 +629,15 @@ int focr_beam_select(const void *logits, int dtype, size_t batch, size_t beams, 
  * the table counts as 0.  The fresh pages
  * must differ from one another and from every page the table uses.  The paged
  * form of compacting BatchedRingCache slots (rswa.rs:620-700). */
-int focr_beam_reorder(const focr_paged_cache *c, size_t layers, size_t layer_stride,
-                      size_t batch, size_t beams, const int32_t *lens, const int32_t *parent,
-                      const int32_t *fresh, int32_t *table_out, int32_t *lens_out,
-                      const float *weights, size_t width, size_t weights_layer_stride,
-                      size_t weights_row_stride, size_t weights_head_stride, float *weights_out,
-                      void *stream);
+typedef struct focr_beam_reorder_args {
+    const int32_t *lens, *parent, *fresh;
+    int32_t *table_out, *lens_out;
+    const float *weights;
+    float *weights_out;
+    size_t layers, layer_stride, batch, beams;
+    size_t width, weights_layer_stride, weights_row_stride, weights_head_stride;
+} focr_beam_reorder_args;
+int focr_beam_reorder(const focr_paged_cache *c, const focr_beam_reorder_args *a, void *stream);
 
 /* ---- device event trace (GPU counterpart of FOCR_PROFILE_DECODE,
  * native_engine/decoder.rs:986-1024) ------------------------------------

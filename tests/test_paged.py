@@ -4,7 +4,8 @@ import ctypes as C
 
 import pytest
 
-from franken_ocr_b200._lib import BF16, F16, F32, FocrError, PagedCache, check, lib
+from franken_ocr_b200._lib import (BF16, F16, F32, BeamReorderArgs, BeamSelectArgs, FocrError, PagedAttentionArgs,
+                                   PagedCache, PagedEvictArgs, PagedWriteArgs, check, lib)
 
 PTR = 1 << 20  # never read: the calls refuse first
 
@@ -17,29 +18,31 @@ def cache(**kw):
 
 
 def write(c, rows=4, k=PTR, v=PTR, src=F32, tokens=4, ks=128, vs=128, row=None, pos=PTR):
-    check(lib.focr_paged_write(C.byref(c) if c else None, rows, k, v, src, tokens, ks, vs, row, pos, None))
+    check(lib.focr_paged_write(C.byref(c) if c else None, C.byref(PagedWriteArgs(k, v, row, pos, rows, tokens, ks, vs,
+                                                                                 src)), None))
 
 
 def attend(c, q=PTR, qt=F32, rows=4, heads=4, qs=256, lens=PTR, refs=None, window=0, scale=0.125, out=2 * PTR, os=256,
            w=None, ww=0, wr=0, wh=0, ws=PTR, wsb=1 << 40):
-    check(lib.focr_paged_attention(C.byref(c), q, qt, rows, heads, qs, lens, refs, window, scale, out, os, w, ww, wr,
-                                   wh, ws, wsb, None))
+    check(lib.focr_paged_attention(C.byref(c), C.byref(PagedAttentionArgs(
+        q, lens, refs, out, w, ws, rows, heads, qs, os, window, ww, wr, wh, wsb, qt, scale)), None))
 
 
 def evict(c, rows=2, lens=PTR, w=PTR, width=64, wr=128, wh=64, into=2 * PTR, is_=4, ip=4, budget=32, sink=4, recent=8,
           kept=PTR, lo=3 * PTR, wo=2 * PTR):
-    check(lib.focr_paged_evict(C.byref(c), rows, lens, w, width, wr, wh, into, is_, ip, budget, sink, recent, kept, lo,
-                               wo, None))
+    check(lib.focr_paged_evict(C.byref(c), C.byref(PagedEvictArgs(lens, w, into, kept, lo, wo, rows, width, wr, wh, is_,
+                                                                  ip, budget, sink, recent)), None))
 
 
 def select(x=PTR, dt=F32, batch=2, beams=4, vocab=100, stride=100, scores=PTR, n=4, out=PTR, ws=PTR, wsb=1 << 30):
-    check(lib.focr_beam_select(x, dt, batch, beams, vocab, stride, scores, None, 1, n, out, out, out, ws, wsb, None))
+    check(lib.focr_beam_select(C.byref(BeamSelectArgs(x, scores, None, out, out, out, ws, batch, beams, vocab, stride, n,
+                                                      wsb, dt, 1)), None))
 
 
 def reorder(c, layers=2, ls=10 * 2 * 16 * 64, batch=2, beams=2, lens=PTR, parent=PTR, fresh=PTR, to=2 * PTR, lo=3 * PTR,
             w=None, width=0, wl=0, wr=0, wh=0, wo=None):
-    check(lib.focr_beam_reorder(C.byref(c), layers, ls, batch, beams, lens, parent, fresh, to, lo, w, width, wl, wr, wh,
-                                wo, None))
+    check(lib.focr_beam_reorder(C.byref(c), C.byref(BeamReorderArgs(lens, parent, fresh, to, lo, w, wo, layers, ls, batch,
+                                                                    beams, width, wl, wr, wh)), None))
 
 
 @pytest.mark.parametrize("bad,code,text", [
@@ -67,9 +70,15 @@ def test_every_call_checks_its_cache(bad, code, text):
         assert e.value.code == code and text in str(e.value) and str(e.value).startswith(name)
 
 
-def test_null_cache():
+def test_null_cache_and_arguments():
     with pytest.raises(FocrError, match="paged_write: null cache"):
         write(None)
+    c = cache()
+    for name in ("paged_write", "paged_attention", "paged_evict", "beam_reorder"):
+        with pytest.raises(FocrError, match=name + ": null arguments"):
+            check(getattr(lib, "focr_" + name)(C.byref(c), None, None))
+    with pytest.raises(FocrError, match="beam_select: null arguments"):
+        check(lib.focr_beam_select(None, None))
 
 
 @pytest.mark.parametrize("bad,code,text", [
