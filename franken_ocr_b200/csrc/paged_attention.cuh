@@ -22,9 +22,9 @@
 // has at most two) and paged_join_kernel joins them.  So no row length, however
 // ragged the batch, leaves SMs idle.
 //
-// A few short rows wait on latency, not on bytes.  There a cluster of blocks shares
-// each (row, head) and joins its pieces through distributed shared memory, which
-// saves the second kernel.
+// Short rows wait on latency, not on bytes.  There a block, or a cluster of blocks,
+// has each (row, head) to itself and joins its pieces through distributed shared
+// memory, which saves the second kernel.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -347,7 +347,7 @@ __device__ __forceinline__ void finish_heads(const AttnArgs &a, const Segment &s
             L = __fmaf_rn(h.l[w][i], f, L);
             o = fma4(*reinterpret_cast<const float4 *>(&h.o[w][i][d]), f, o);
         }
-        if (a.cluster) {
+        if (a.cluster > 1) {
             // only this thread reads these four; the other threads still read m and l
             *reinterpret_cast<float4 *>(&h.o[0][i][d]) = o;
             if (d == 0) {
@@ -362,7 +362,7 @@ __device__ __forceinline__ void finish_heads(const AttnArgs &a, const Segment &s
             if (d == 0) a.ml[s.slot * GP + g] = make_float2(M, L);
         }
     }
-    if (!a.cluster) {
+    if (a.cluster <= 1) {
         __syncthreads();
         return;
     }
@@ -431,15 +431,25 @@ template <typename K> int launch_attn(K kernel, int smem, const AttnArgs &a, cud
     return FOCR_OK;
 }
 
-// The blocks of a cluster for each (row, head), or 0 for runs: the visible positions
-// of a row are not known here, only its table's capacity, so clusters are for tables
-// of at most 2 MB a (row, head), K and V, and as many of them as fit the SMs at once.
-// Clusters against runs, 10 heads of f32: 1024 positions 7.6 / 10.2 us, 2048 10.1 /
-// 11.8, 4096 (4 MB) 15.3 / 13.5; 4 rows x 8 heads of bf16: 1024 7.8 / 12.0, 4096 (2 MB)
-// 13.8 / 17.3, 8192 26.4 / 30.5.
+// The blocks of a cluster for each (row, head), or 0 for runs.  The visible positions
+// of a row are not known here, only its table's capacity.  A cluster saves the prefix,
+// the cuts and the join, and the hardware hands out the rows; runs are even however
+// long one row is.  So: as many blocks as fit the SMs at once, 8 at most, where each
+// has at most 128 KB of K to read, 256 KB where most SMs are busy; and one block a
+// (row, head) for up to four times as many as fit.  Clusters against runs:
+//   1 row, 10 heads of f32: 1024 positions 7.6 / 10.2 us, 2048 10.1 / 11.8, 4096 (256 KB
+//   on a quarter of the SMs) 15.3 / 13.5;
+//   8 rows x 8 heads of bf16: 256 positions 7.1 / 9.8, 2048 14.3 / 17.2; 32 x 8: 64 5.4 /
+//   7.5, 512 12.6 / 17.4, 1024 (256 KB) 25.5 / 30.4; all but one row short: 15.9 / 11.9;
+//   64 x 10 of 1 to 512 positions 22.1 / 27.8, of 512 each 38.6 / 36.9; 4 query heads 26.5
+//   / 43.3 and 42.7 / 44.5; 256 x 16 of 128 each 79 / 64.
 inline int cluster_of(const AttnArgs &a) {
-    const size_t units = (size_t)a.rows * a.c.kv_heads * a.head_chunks;
-    return units * 8 <= (size_t)attn_blocks() && (size_t)a.cap * a.c.row_bytes <= (1u << 20) ? 8 : 0;
+    const size_t units = (size_t)a.rows * a.c.kv_heads * a.head_chunks, most = (size_t)attn_blocks();
+    size_t n = 8;
+    while (n > 1 && units * n > most) n >>= 1;
+    const size_t bytes = (size_t)a.cap * a.c.row_bytes;
+    if (units > most * 4 || bytes > n << (units * n * 4 >= most * 3 ? 18 : 17)) return 0;
+    return (int)n;
 }
 
 // The attention kernel for one type of cache, without the join; sets gp,
