@@ -324,6 +324,32 @@ def test_attention_small_and_large_tables_agree(cuda, pool, group, dim, heads):
         assert bool(out[3].isnan().all()) and bool((out[1] == 0).all()) and bool(out[0].isfinite().all())
 
 
+@pytest.mark.parametrize("prefill,ring,more", [(1024, 128, 0), (1000, 37, 500), (1, 1, 300), (300, 128, 7)])
+def test_window_over_pages_equals_the_dense_caches(cuda, prefill, ring, more):
+    """The R-SWA decode attention of the dense caches (reference block and ring) and the
+    paged form of it, where the window is the ring and `more` entries between the two
+    have left it."""
+    from franken_ocr_b200 import decoder_ops, paged
+
+    heads, dim, page = 10, 128, 16
+    n = prefill + more + ring
+    g = torch.Generator().manual_seed(prefill)
+    k, v = torch.randn((n, heads, dim), generator=g), torch.randn((n, heads, dim), generator=g)
+    q = torch.randn((1, heads, dim), generator=g)
+    c = Cache([n], heads, page, dim, torch.float32, seed=19)
+    kp, vp, table = c.cuda()
+    pos = torch.arange(n, dtype=torch.int32)
+    paged.paged_write(k.cuda(), v.cuda(), kp, vp, table, pos.cuda(), row=torch.zeros_like(pos).cuda())
+    at = pos.long()
+    c.k[c.table[0].long()[at // page], :, at % page], c.v[c.table[0].long()[at // page], :, at % page] = k, v
+    got = paged.paged_attention(q.cuda(), kp, vp, table, torch.tensor([n], dtype=torch.int32, device="cuda"),
+                                ref_lens=torch.tensor([prefill], dtype=torch.int32, device="cuda"), window=ring)[0]
+    dense = [t.transpose(0, 1).contiguous().cuda() for t in (k[:prefill], v[:prefill], k[n - ring:], v[n - ring:])]
+    want = decoder_ops.attention_decode(q[0].cuda(), dense[0], dense[1], prefill, dense[2], dense[3], ring)
+    _, _, bound = attention(c, q, [n], 1 / math.sqrt(dim), [prefill], ring)
+    assert bool(((got - want).abs().cpu() <= 2 * bound[0]).all())   # each is within one bound
+
+
 def test_calls_on_other_streams(cuda):
     """Work goes to the current stream, also two calls at once on two streams."""
     from franken_ocr_b200 import paged
