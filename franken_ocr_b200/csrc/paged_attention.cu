@@ -147,7 +147,7 @@ int launch_attention(AttnArgs a, int dtype, float *weights, size_t w_row, size_t
                                        : launch_attention_bf16(a, st);
     if (rc) return rc;
     const int blocks = attn_blocks();
-    if (!a.cluster && blocks > 1)
+    if (a.cluster == RUNS && blocks > 1)
         FOCR_CUDA_TRY(launch_pdl(paged_join_kernel, dim3(blocks - 1, a.gp < a.group ? a.gp : a.group), JT, blocks * 4, st, a, blocks));
     if (weights)
         FOCR_CUDA_TRY(launch_pdl(paged_weights_kernel, dim3((a.width + 1023) / 1024, a.c.kv_heads, a.rows), 256, 0, st,

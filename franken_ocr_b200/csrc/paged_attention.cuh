@@ -24,7 +24,8 @@
 //
 // Short rows wait on latency, not on bytes.  There a block, or a cluster of blocks,
 // has each (row, head) to itself and joins its pieces through distributed shared
-// memory, which saves the second kernel.
+// memory, which saves the second kernel; and where there are many of a few tiles, a
+// warp has each and joins nothing.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -40,6 +41,10 @@ namespace cg = cooperative_groups;
 constexpr int ATTN_WARPS = 4, ATTN_ROWS = 1024;  // rows of one launch
 constexpr int ATTN_HEADS = 16;                   // most query heads a block takes together
 
+// How the work is shared out, where not by clusters: runs of block tiles, or a (row,
+// head) for each warp.
+constexpr int RUNS = 0, SOLO = -1;
+
 struct AttnArgs {
     PagedView c;
     const void *q;
@@ -54,7 +59,7 @@ struct AttnArgs {
     int score_stride;     // floats between the scores of two query heads, even
     int gp, head_chunks;  // query heads that a block takes together; blocks of them a kv head
     int tile_shift;       // log2 of a block tile's positions
-    int cluster;          // blocks of a cluster that shares one (row, head), or 0: runs
+    int cluster;          // blocks that share one (row, head); RUNS or SOLO
     float c2;             // scale * log2(e)
 };
 
@@ -177,7 +182,8 @@ __device__ __forceinline__ int row_of_unit(const int *pre, int rows, int hc_coun
 // The run of units of one block, and the piece of a (row, kv head, chunk of its
 // query heads) it stands at.
 struct Segment {
-    int r, kvh, heads, qh0, t0, t1, slot;
+    int r, kvh, heads, qh0, t0, t1;
+    int slot;      // of a piece, in runs
     bool whole;
     RowView rv;
 };
@@ -189,11 +195,16 @@ __device__ __forceinline__ unsigned long long quotient(unsigned long long n, uns
 struct Run {
     unsigned long long left;     // units to come
     int r, kvh, chunk, t, tiles; // where the next one lies: tile t of `tiles`
+    int unit;                    // the next (row, head), counted, of a warp of its own
     bool first;
 
     // The run of this block; in a cluster its share of the cluster's (row, head),
     // which may be empty.
     __device__ Run(const AttnArgs &a, const int *pre) {
+        if (a.cluster == SOLO) {
+            unit = blockIdx.x * ATTN_WARPS + (threadIdx.x >> 5);
+            return;
+        }
         if (a.cluster) {
             const int unit = blockIdx.x / a.cluster, rank = blockIdx.x - unit * a.cluster;
             const int row_units = a.c.kv_heads * a.head_chunks;
@@ -225,6 +236,22 @@ struct Run {
         first = true;
     }
     __device__ bool next(const AttnArgs &a, const int *pre, Segment *s) {
+        if (a.cluster == SOLO) {
+            const int per_row = a.c.kv_heads * a.head_chunks;
+            r = unit / per_row;
+            if (r >= a.rows) return false;
+            kvh = (unit - r * per_row) / a.head_chunks;
+            chunk = unit - r * per_row - kvh * a.head_chunks;
+            unit += gridDim.x * ATTN_WARPS;
+            s->rv = row_view(a, r);
+            s->t0 = 0;
+            s->t1 = (s->rv.vis + (1 << a.tile_shift) - 1) >> a.tile_shift;
+            s->r = r;
+            s->kvh = kvh;
+            s->heads = min(a.gp, a.group - chunk * a.gp);
+            s->qh0 = kvh * a.group + chunk * a.gp;
+            return true;
+        }
         // a cluster's blocks all take part in its join
         if (a.cluster ? !first : !left) return false;
         if (t == tiles && !a.cluster) {   // the next (row, kv head, chunk)
@@ -256,6 +283,11 @@ struct Run {
     }
 };
 
+// The first position of a warp's part of a tile.
+template <int KEYS> __device__ __forceinline__ int first_key(const AttnArgs &a, int tile, int warp) {
+    return (a.cluster == SOLO ? tile : tile * ATTN_WARPS + warp) * KEYS;
+}
+
 // The tiles of a block's run in order, across its segments, for the copies that run
 // ahead of the arithmetic.  A warp's lane `i` finds the place of the tile's i-th
 // position.
@@ -271,16 +303,16 @@ template <int KEYS> struct Feed {
     // none; *bad if its page is not in the pool.
     __device__ int64_t next(const AttnArgs &a, const int *pre, int warp, int lane, bool *bad) {
         *bad = false;
-        if (tile == end) {
+        while (tile == end) {   // a row may have no tiles
             Segment s;
-            if (!run.left || !run.next(a, pre, &s)) return -1;
+            if (!run.next(a, pre, &s)) return -1;
             pages = a.c.table + s.r * a.c.table_stride;
             head = s.kvh * a.c.head_stride;
             rv = s.rv;
             tile = s.t0;
             end = s.t1;
         }
-        const int i = (tile++ * ATTN_WARPS + warp) * KEYS + lane;
+        const int i = first_key<KEYS>(a, tile++, warp) + lane;
         if (lane >= KEYS || i >= rv.vis) return -1;
         const int64_t o = a.c.offset(pages, (uint32_t)(i < rv.ref ? i : i + rv.gap));
         *bad = o < 0;
@@ -312,6 +344,27 @@ __device__ __forceinline__ void store4_as(void *p, int dtype, int64_t i, float4 
     store_f32_as(p, dtype, i + 1, x.y);
     store_f32_as(p, dtype, i + 2, x.z);
     store_f32_as(p, dtype, i + 3, x.w);
+}
+// Two of them.
+__device__ __forceinline__ void store2_as(void *p, int dtype, int64_t i, float x, float y) {
+    if (dtype == FOCR_F32) {
+        float *q = static_cast<float *>(p) + i;
+        if ((uintptr_t)q % 8 == 0) {
+            *reinterpret_cast<float2 *>(q) = make_float2(x, y);
+            return;
+        }
+    } else {
+        uint16_t *q = static_cast<uint16_t *>(p) + i;
+        if ((uintptr_t)q % 4 == 0) {
+            alignas(4) uint16_t z[2];
+            store_f32_as(z, dtype, 0, x);
+            store_f32_as(z, dtype, 1, y);
+            *reinterpret_cast<uint32_t *>(q) = *reinterpret_cast<const uint32_t *>(z);
+            return;
+        }
+    }
+    store_f32_as(p, dtype, i, x);
+    store_f32_as(p, dtype, i + 1, y);
 }
 __device__ __forceinline__ float4 fma4(float4 x, float f, float4 o) {
     return make_float4(__fmaf_rn(x.x, f, o.x), __fmaf_rn(x.y, f, o.y), __fmaf_rn(x.z, f, o.z),
@@ -391,7 +444,7 @@ __device__ __forceinline__ void finish_heads(const AttnArgs &a, const Segment &s
 // The rows that have no units, shared out over the blocks: zeros where nothing is
 // visible, NaN for a length that passes the table.
 __device__ __forceinline__ void finish_empty_rows(const AttnArgs &a, const int *pre) {
-    if (a.cluster) return;   // a row of a cluster has a segment, if an empty one
+    if (a.cluster != RUNS) return;   // elsewhere a row has a segment, if an empty one
     for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
         if (pre[r + 1] != pre[r]) continue;
         const float x = row_view(a, r).bad ? NAN : 0.0f;
@@ -407,11 +460,13 @@ inline int ilog2(int x) {
 }
 inline int attn_blocks() { return num_sms() * 2; }
 
-// Launches an attention kernel in runs, or in clusters where a.cluster says so.
+// Launches an attention kernel as a.cluster says.
 template <typename K> int launch_attn(K kernel, int smem, const AttnArgs &a, cudaStream_t st) {
     FOCR_CUDA_TRY(set_max_dynamic_smem((const void *)kernel, smem));
-    if (!a.cluster) {
-        FOCR_CUDA_TRY(launch_pdl(kernel, attn_blocks(), ATTN_WARPS * 32, smem, st, a));
+    if (a.cluster <= 0) {
+        const size_t units = (size_t)a.rows * a.c.kv_heads * a.head_chunks, warps = (size_t)attn_blocks() * ATTN_WARPS;
+        const int blocks = a.cluster == SOLO && units < warps ? (int)((units + ATTN_WARPS - 1) / ATTN_WARPS) : attn_blocks();
+        FOCR_CUDA_TRY(launch_pdl(kernel, blocks, ATTN_WARPS * 32, smem, st, a));
         return FOCR_OK;
     }
     cudaLaunchConfig_t cfg = {};
@@ -431,24 +486,35 @@ template <typename K> int launch_attn(K kernel, int smem, const AttnArgs &a, cud
     return FOCR_OK;
 }
 
-// The blocks of a cluster for each (row, head), or 0 for runs.  The visible positions
-// of a row are not known here, only its table's capacity.  A cluster saves the prefix,
-// the cuts and the join, and the hardware hands out the rows; runs are even however
-// long one row is.  So: as many blocks as fit the SMs at once, 8 at most, where each
-// has at most 128 KB of K to read, 256 KB where most SMs are busy; and one block a
-// (row, head) for up to four times as many as fit.  Clusters against runs:
+// How a call is shared out.  The visible positions of a row are not known here, only
+// its table's capacity.
+// A cluster saves the prefix, the cuts and the join, and the hardware hands out the
+// rows; runs are even however long one row is.  So: as many blocks as fit the SMs at
+// once, 8 at most, where each has at most 128 KB of K to read, 256 KB where most SMs are
+// busy; and one block a (row, head) for up to four times as many as fit.  Clusters
+// against runs:
 //   1 row, 10 heads of f32: 1024 positions 7.6 / 10.2 us, 2048 10.1 / 11.8, 4096 (256 KB
 //   on a quarter of the SMs) 15.3 / 13.5;
 //   8 rows x 8 heads of bf16: 256 positions 7.1 / 9.8, 2048 14.3 / 17.2; 32 x 8: 64 5.4 /
 //   7.5, 512 12.6 / 17.4, 1024 (256 KB) 25.5 / 30.4; all but one row short: 15.9 / 11.9;
 //   64 x 10 of 1 to 512 positions 22.1 / 27.8, of 512 each 38.6 / 36.9; 4 query heads 26.5
 //   / 43.3 and 42.7 / 44.5; 256 x 16 of 128 each 79 / 64.
-inline int cluster_of(const AttnArgs &a) {
+// Where there are more (row, head)s than blocks fit, a warp takes one: nothing is joined
+// or waited for, but its tiles, about 0.9 us each, follow one another.  Up to a
+// fortieth of the (row, head)s, 48 at most, the longest row ends about when the others
+// do.  bf16, full tables, warps against the better of the above: 40 x 8: 64 positions (4
+// tiles) 8.1 / 11.0 us, 128 11.0 / 12.8, 256 (16 tiles, not taken) 16.9 / 17.1, ragged
+// 16.7 / 13.4; 128 x 8: 16 6.6 / 20.2, 256 26.2 / 40.5; 224 x 16: 16 16.0 / 44.2, 128
+// 51.1 / 66.4, 512 (32 tiles) 156 / 152, ragged 93.5 / 122.5.  `keys`: of a warp's tile,
+// 0 where the kernel's warps cannot work alone.
+inline int cluster_of(const AttnArgs &a, int keys) {
     const size_t units = (size_t)a.rows * a.c.kv_heads * a.head_chunks, most = (size_t)attn_blocks();
+    const size_t tiles = keys ? ((size_t)a.cap + keys - 1) / keys : SIZE_MAX;
+    if (units > most && tiles <= 48 && tiles * 40 <= units) return SOLO;
     size_t n = 8;
     while (n > 1 && units * n > most) n >>= 1;
     const size_t bytes = (size_t)a.cap * a.c.row_bytes;
-    if (units > most * 4 || bytes > n << (units * n * 4 >= most * 3 ? 18 : 17)) return 0;
+    if (units > most * 4 || bytes > n << (units * n * 4 >= most * 3 ? 18 : 17)) return RUNS;
     return (int)n;
 }
 

@@ -89,6 +89,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
     // head's f32 query by the power of two that brings its largest value near 2^14
     constexpr float PS = HALF ? 2048.0f : 1.0f;
     constexpr int RINGS = ATTN_WARPS * S::STAGES * 2 * S::HALF;
+    static_assert(sizeof(Handover<GP, D>) <= RINGS, "all heads fit the rings");
     extern __shared__ __align__(128) char smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     char *ring = smem + warp * S::STAGES * 2 * S::HALF;
@@ -100,7 +101,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
 
     pdl_wait();
     pdl_trigger();
-    if (!a.cluster) tile_prefix<ATTN_WARPS * 32>(a, pre);
+    if (a.cluster == RUNS) tile_prefix<ATTN_WARPS * 32>(a, pre);
 
     const int qr = lane >> 2, qc = (lane & 3) * 2;   // this lane's row and columns of a tile
     const int mi = lane >> 3, rr = lane & 7;         // its matrix and row when loading one
@@ -235,7 +236,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
                 for (int t = 0; t < NT; t++)
 #pragma unroll
                     for (int x = 0; x < 4; x++) s[t][x] *= unscale[x >> 1];
-            const int i0 = (tile * ATTN_WARPS + warp) * KEYS + qc;
+            const int i0 = first_key<KEYS>(a, tile, warp) + qc;
             if (a.scores) {   // pairs: the stride is even, what lies behind vis is never read
                 float *sp = a.scores + ((int64_t)r * a.q_heads + sg.qh0 + qr) * a.score_stride + i0;
 #pragma unroll
@@ -316,6 +317,41 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
         for (int y = 0; y < 2; y++) {
             l[y] += __shfl_xor_sync(0xffffffffu, l[y], 1);
             l[y] += __shfl_xor_sync(0xffffffffu, l[y], 2);
+            l[y] = any_bad ? NAN : l[y] * (1.0f / PS);
+        }
+        if (a.cluster == SOLO) {
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                const int g = qr + y * 8;
+                if (g >= heads) break;
+                const float by = l[y] == 0.0f ? 0.0f : 1.0f / PS, L = l[y] == 0.0f ? 1.0f : l[y];
+                const int64_t to = r * a.out_stride + (long long)(sg.qh0 + g) * a.dim + qc;
+#pragma unroll
+                for (int j = 0; j < D / 8; j++)
+                    if (j * 8 < a.dim) store2_as(a.out, a.q_type, to + j * 8, acc[j][2 * y] * by / L, acc[j][2 * y + 1] * by / L);
+                if (a.stat && (lane & 3) == 0) a.stat[(int64_t)r * a.q_heads + sg.qh0 + g] = make_float2(m[y], 1.0f / l[y]);
+            }
+            continue;
+        }
+        auto give = [&](int y, float *o, float *to_m, float *to_l) {
+#pragma unroll
+            for (int j = 0; j < D / 8; j++)
+                *reinterpret_cast<float2 *>(o + j * 8 + qc) =
+                    make_float2(acc[j][2 * y] * (1.0f / PS), acc[j][2 * y + 1] * (1.0f / PS));
+            if ((lane & 3) == 0) {
+                *to_m = m[y];
+                *to_l = l[y];
+            }
+        };
+        if (a.cluster) {   // nothing is to come: all heads at once, where the rings were
+            auto &all = *reinterpret_cast<Handover<GP, D> *>(smem);
+            cp_async_wait<0>();
+            __syncthreads();
+#pragma unroll
+            for (int y = 0; y < 2; y++) give(y, all.o[warp][qr + y * 8], &all.m[warp][qr + y * 8], &all.l[warp][qr + y * 8]);
+            __syncthreads();
+            finish_heads<GP, GP, D>(a, sg, all, 0);
+            continue;
         }
 #pragma unroll
         for (int g0 = 0; g0 < GP; g0 += HR) {
@@ -323,15 +359,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
 #pragma unroll
             for (int y = 0; y < 2; y++) {
                 const int i = qr + y * 8 - g0;
-                if (i < 0 || i >= HR) continue;
-#pragma unroll
-                for (int j = 0; j < D / 8; j++)
-                    *reinterpret_cast<float2 *>(&hand.o[warp][i][j * 8 + qc]) =
-                        make_float2(acc[j][2 * y] * (1.0f / PS), acc[j][2 * y + 1] * (1.0f / PS));
-                if ((lane & 3) == 0) {
-                    hand.m[warp][i] = m[y];
-                    hand.l[warp][i] = any_bad ? NAN : l[y] * (1.0f / PS);
-                }
+                if (i >= 0 && i < HR) give(y, hand.o[warp][i], &hand.m[warp][i], &hand.l[warp][i]);
             }
             __syncthreads();
             finish_heads<GP, HR, D>(a, sg, hand, g0);
@@ -343,8 +371,8 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
 template <typename T, int D, bool F32Q> int launch_mma(AttnArgs &a, cudaStream_t st) {
     a.gp = 16;
     a.head_chunks = (a.group + 15) / 16;
-    a.tile_shift = ilog2(MmaTile<D>::BLOCK);
-    a.cluster = cluster_of(a);
+    a.cluster = mma_q_bytes<D>() ? cluster_of(a, 0) : cluster_of(a, MmaTile<D>::KEYS);   // a query in shared memory is the block's
+    a.tile_shift = ilog2(a.cluster == SOLO ? MmaTile<D>::KEYS : MmaTile<D>::BLOCK);
     return launch_attn(paged_attention_mma_kernel<T, D, F32Q>, mma_smem<D>(), a, st);
 }
 // Whether this kernel takes the call.  16 rows x 8192 positions x 8 kv heads, bf16, this

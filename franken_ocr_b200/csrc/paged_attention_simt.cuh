@@ -26,6 +26,7 @@ template <typename T, int D> struct Tile {
 template <int D, int GP> constexpr int simt_round() { return GP * D <= 512 ? GP : 512 / D; }
 template <typename T, int D, int GP> constexpr int simt_smem() {
     using S = Tile<T, D>;
+    static_assert(sizeof(Handover<GP, D>) <= ATTN_WARPS * S::STAGES * 2 * S::HALF, "all heads fit the rings");
     return ATTN_WARPS * S::STAGES * 2 * S::HALF + (int)sizeof(Handover<simt_round<D, GP>(), D>) +
            ATTN_WARPS * GP * S::KEYS * 4 + (ATTN_ROWS + 1) * 4;
 }
@@ -51,7 +52,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
 
     pdl_wait();
     pdl_trigger();
-    if (!a.cluster) tile_prefix<ATTN_WARPS * 32>(a, pre);
+    if (a.cluster == RUNS) tile_prefix<ATTN_WARPS * 32>(a, pre);
 
     const int sub = lane / LPK, chunk = lane % LPK;
     // the step whose score this lane holds after the transposing reduction
@@ -129,7 +130,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
                     s[g][it] = d;
                 }
             }
-            const int i = (tile * ATTN_WARPS + warp) * KEYS + my_key;
+            const int i = first_key<KEYS>(a, tile, warp) + my_key;
             const bool live = i < vis;
 #pragma unroll
             for (int g = 0; g < GP; g++) {
@@ -197,27 +198,55 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
         // the warp's sums over its lanes, then the block's over its warps
         const bool any_bad = __any_sync(0xffffffffu, bad);
 #pragma unroll
+        for (int g = 0; g < GP; g++) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) l[g] += __shfl_xor_sync(0xffffffffu, l[g], o);
+            l[g] = any_bad ? NAN : l[g] * (8.0f / LPK);  // LPK / 8 lanes hold the same key
+#pragma unroll
+            for (int e = 0; e < EPL; e++)
+#pragma unroll
+                for (int o = LPK; o < 32; o <<= 1) acc[g][e] += __shfl_xor_sync(0xffffffffu, acc[g][e], o);
+        }
+        if (a.cluster == SOLO) {
+#pragma unroll
+            for (int g = 0; g < GP; g++) {
+                if (g >= heads) break;
+                if (sub == 0)
+#pragma unroll
+                    for (int e = 0; e < EPL; e += 4) {
+                        const int d = (e / EPC * LPK + chunk) * EPC + e % EPC;
+                        if (d < a.dim)
+                            store4_as(a.out, a.q_type, r * a.out_stride + (long long)(qh0 + g) * a.dim + d,
+                                      over4(make_float4(acc[g][e], acc[g][e + 1], acc[g][e + 2], acc[g][e + 3]), l[g]));
+                    }
+                if (a.stat && lane == 0) a.stat[(int64_t)r * a.q_heads + qh0 + g] = make_float2(m[g], 1.0f / l[g]);
+            }
+            continue;
+        }
+        auto give = [&](int g, float *o, float *to_m, float *to_l) {
+            if (sub == 0)
+#pragma unroll
+                for (int e = 0; e < EPL; e++) o[(e / EPC * LPK + chunk) * EPC + e % EPC] = acc[g][e];
+            if (lane == 0) {
+                *to_m = m[g];
+                *to_l = l[g];
+            }
+        };
+        if (a.cluster) {   // nothing is to come: all heads at once, where the rings were
+            auto &all = *reinterpret_cast<Handover<GP, D> *>(smem);
+            cp_async_wait<0>();
+            __syncthreads();
+#pragma unroll
+            for (int g = 0; g < GP; g++) give(g, all.o[warp][g], &all.m[warp][g], &all.l[warp][g]);
+            __syncthreads();
+            finish_heads<GP, GP, D>(a, sg, all, 0);
+            continue;
+        }
+#pragma unroll
         for (int g0 = 0; g0 < GP; g0 += HR) {
             if (g0 >= heads) break;
 #pragma unroll
-            for (int i = 0; i < HR; i++) {
-                const int g = g0 + i;
-                float lsum = l[g];
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, o);
-                lsum *= 8.0f / LPK;  // LPK / 8 lanes hold the same key
-#pragma unroll
-                for (int e = 0; e < EPL; e++) {
-                    float x = acc[g][e];
-#pragma unroll
-                    for (int o = LPK; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-                    if (sub == 0) hand.o[warp][i][(e / EPC * LPK + chunk) * EPC + e % EPC] = x;
-                }
-                if (lane == 0) {
-                    hand.m[warp][i] = m[g];
-                    hand.l[warp][i] = any_bad ? NAN : lsum;
-                }
-            }
+            for (int i = 0; i < HR; i++) give(g0 + i, hand.o[warp][i], &hand.m[warp][i], &hand.l[warp][i]);
             __syncthreads();
             finish_heads<GP, HR, D>(a, sg, hand, g0);
         }
@@ -228,8 +257,8 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
 template <typename T, int D, int GP> int launch_simt(AttnArgs &a, cudaStream_t st) {
     a.gp = GP;
     a.head_chunks = (a.group + GP - 1) / GP;
-    a.tile_shift = ilog2(Tile<T, D>::BLOCK);
-    a.cluster = cluster_of(a);
+    a.cluster = cluster_of(a, Tile<T, D>::KEYS);
+    a.tile_shift = ilog2(a.cluster == SOLO ? Tile<T, D>::KEYS : Tile<T, D>::BLOCK);
     return launch_attn(paged_attention_kernel<T, D, GP>, simt_smem<T, D, GP>(), a, st);
 }
 

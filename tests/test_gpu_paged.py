@@ -324,6 +324,46 @@ def test_attention_small_and_large_tables_agree(cuda, pool, group, dim, heads):
         assert bool(out[3].isnan().all()) and bool((out[1] == 0).all()) and bool(out[0].isfinite().all())
 
 
+@pytest.mark.parametrize("q_type,pool,group,dim", [
+    ("f32", "f32", 1, 128), ("f32", "f16", 7, 256), ("bf16", "bf16", 2, 64), ("bf16", "bf16", 5, 128),
+    ("f16", "f16", 20, 80), ("f32", "bf16", 16, 64), ("f32", "f32", 3, 20), ("bf16", "bf16", 6, 256),
+])
+def test_attention_many_short_rows(cuda, q_type, pool, group, dim):
+    """More (row, head)s than blocks and few positions each: a warp has one to itself.
+    Rows with nothing to see and rows that give NaN change none of their neighbours."""
+    from franken_ocr_b200 import paged
+
+    rows, heads = 450, 2
+    lens = [(7 * r) % 41 for r in range(rows)]
+    c = Cache(lens, heads, 8, dim, DTYPES[pool], seed=group)
+    q = torch.randn((rows, heads * group, dim), generator=torch.Generator().manual_seed(dim)).to(DTYPES[q_type])
+    good = check_attention(c, q, lens, weights=True)
+    assert same_bits(check_attention(c, q, lens), good)
+    check_attention(c, q, lens, refs=[r % 9 for r in range(rows)], window=6, weights=True)
+    kp, vp, table = c.cuda()
+    odd = torch.tensor(lens, dtype=torch.int32)
+    odd[3::10] = 1 << 20
+    odd[4::10] = -5
+    if lens[16] > 8:
+        table[16, 1] = -1
+    w = torch.zeros((rows, heads, 40), device="cuda")
+    out = paged.paged_attention(q.cuda(), kp, vp, table, odd.cuda(), weights=w).cpu()
+    nan = torch.zeros(rows, dtype=torch.bool)
+    nan[3::10] = True
+    nan[16] = lens[16] > 8
+    zero = odd <= 0
+    assert bool(out[nan].isnan().all()) and bool((out[zero] == 0).all())
+    rest = ~(nan | zero)
+    assert same_bits(out[rest], good.cpu()[rest])
+    assert bool((w.cpu()[~rest] == 0).all())
+    # an out that begins on no boundary of a wide store
+    flat = torch.full((out.numel() + 1,), 7.0, dtype=DTYPES[q_type], device="cuda")
+    view = flat[1:].view(out.shape)
+    paged.paged_attention(q.cuda(), kp, vp, table, odd.cuda(), out=view)
+    assert same_bits(view.cpu()[rest], good.cpu()[rest])
+    assert float(flat[0]) == 7
+
+
 @pytest.mark.parametrize("prefill,ring,more", [(1024, 128, 0), (1000, 37, 500), (1, 1, 300), (300, 128, 7)])
 def test_window_over_pages_equals_the_dense_caches(cuda, prefill, ring, more):
     """The R-SWA decode attention of the dense caches (reference block and ring) and the
