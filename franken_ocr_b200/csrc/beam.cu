@@ -313,7 +313,8 @@ __device__ __forceinline__ Cand no_cand() { return Cand{-INFINITY, -INFINITY, IN
 
 // A block per entry: the rows' sums, then the n best of all strips' candidates.
 // The n-th best score among the strips' first candidates (a thread takes the best
-// of those it sees) bounds the others; what reaches it is ranked by counting.
+// of those it sees), or among all where the strips are few, bounds the others; what
+// reaches it is ranked by counting.
 // Latency bounds it: 3 us for 1 x 4 beams, 6 for 32 x 8.
 __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
     __shared__ double row_m[MAX_N], row_s[MAX_N];
@@ -399,12 +400,23 @@ __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
         return d;
     };
     __syncthreads();
-    double best = t < lists ? made(t, 0, head_x, head_t).score : -INFINITY;
-    for (int l = t + ST; l < lists; l += ST) best = fmax(best, cand(l * a.n).score);
+    // neighbouring lists, and neighbours of a list, fall into different groups: one beam
+    // may be the only good one
+    const int groups = a.n <= 16 ? 32 : a.n <= 32 ? 64 : 128;
+    double best = -INFINITY;
+    if (lists >= groups) {
+        if (t < lists) best = made(t, 0, head_x, head_t).score;
+        for (int l = t + ST; l < lists; l += ST) best = fmax(best, cand(l * a.n).score);
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int j = t + u * ST, l = (int)a.by_n.div(j);
+            if (j < lists * a.n) best = fmax(best, made(l, j - l * a.n, early_x[u], early_t[u]).score);
+        }
+        for (int j = t + U * ST; j < lists * a.n; j += ST) best = fmax(best, cand(j).score);
+    }
     heads[t] = best;
     __syncthreads();
-    // lists of one beam, which may be the only good one, fall into different groups
-    const int groups = a.n <= 16 ? 32 : a.n <= 32 ? 64 : 128;
     if (t < groups) {
         for (int j = t + groups; j < ST; j += groups) best = fmax(best, heads[j]);
         tops[t] = best;
