@@ -321,7 +321,8 @@ __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
     __shared__ float row_cum[MAX_N];
     __shared__ uint8_t row_done[MAX_N];
     __shared__ __align__(16) char list_mem[LIST * sizeof(Cand)];
-    __shared__ double heads[ST], tops[ST / 2], bound;
+    __shared__ __align__(16) double heads[ST], tops[ST], list_score[LIST];
+    __shared__ double bound;
     __shared__ int count;
     Cand *list = reinterpret_cast<Cand *>(list_mem);
     pdl_wait();
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
     __syncthreads();
     // neighbouring lists, and neighbours of a list, fall into different groups: one beam
     // may be the only good one
-    const int groups = a.n <= 16 ? 32 : a.n <= 32 ? 64 : 128;
+    const int groups = a.n <= 8 ? 32 : a.n <= 16 ? 64 : a.n <= 32 ? 128 : 256;
     double best = -INFINITY;
     if (lists >= groups) {
         if (t < lists) best = made(t, 0, head_x, head_t).score;
@@ -429,22 +430,43 @@ __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
         if (rank == a.n - 1) bound = best;
     }
     __syncthreads();
-    const double low = bound;
+    double low = bound;
     auto enter = [&](const Cand &c) {
         if (c.beam != INT_MAX && c.score >= low) {
             const int i = atomicAdd(&count, 1);
-            if (i < LIST) list[i] = c;
+            if (i < LIST) {
+                list[i] = c;
+                list_score[i] = c.score;
+            }
         }
     };
+    int got;
+    for (;;) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int j = t + u * ST, l = (int)a.by_n.div(j);
-        if (j < lists * a.n) enter(made(l, j - l * a.n, early_x[u], early_t[u]));
-    }
+        for (int u = 0; u < U; u++) {
+            const int j = t + u * ST, l = (int)a.by_n.div(j);
+            if (j < lists * a.n) enter(made(l, j - l * a.n, early_x[u], early_t[u]));
+        }
 #pragma unroll 4
-    for (int j = t + U * ST; j < lists * a.n; j += ST) enter(cand(j));
-    __syncthreads();
-    const int got = count;
+        for (int j = t + U * ST; j < lists * a.n; j += ST) enter(cand(j));
+        __syncthreads();
+        got = count;
+        if (got <= LIST) break;
+        // One beam is far ahead: the n-th best of those that found a place is a nearer
+        // bound, unless it is tied.
+        for (int i = t; i < LIST; i += ST) {
+            const double mine = list_score[i];
+            int rank = 0;
+#pragma unroll 8
+            for (int j = 0; j < LIST; j++) rank += list_score[j] > mine || (list_score[j] == mine && j < i);
+            if (rank == a.n - 1) bound = mine;
+        }
+        __syncthreads();
+        if (bound == low) break;
+        low = bound;
+        if (t == 0) count = 0;
+        __syncthreads();
+    }
     const long long o = (long long)b * a.n;
     auto put = [&](int k, const Cand &c) {
         a.score_out[o + k] = c.beam == INT_MAX ? -INFINITY : (float)c.score;
@@ -452,11 +474,26 @@ __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
         a.token_out[o + k] = c.beam == INT_MAX ? -1 : c.token;
     };
     if (got <= LIST) {
-        for (int i = t; i < got; i += ST) {
+        int lanes = 1;   // that share the counting for one candidate
+        while (lanes < 32 && got * lanes * 2 <= ST) lanes <<= 1;
+        const int part = t & (lanes - 1);
+        for (int i0 = 0; i0 < got; i0 += ST / lanes) {
+            const int i = i0 + t / lanes;
+            const double mine = i < got ? list_score[i] : INFINITY;
+            int rank = 0, same = 0;
+#pragma unroll 8
+            for (int j = part; j < got; j += lanes) {
+                rank += list_score[j] > mine;
+                same += list_score[j] == mine;
+            }
+            for (int o = 1; o < lanes; o <<= 1) {
+                rank += __shfl_xor_sync(0xffffffffu, rank, o);
+                same += __shfl_xor_sync(0xffffffffu, same, o);
+            }
+            if (part || i >= got || rank >= a.n) continue;
             const Cand c = list[i];
-            int rank = 0;
-#pragma unroll 4
-            for (int j = 0; j < got; j++) rank += before(list[j], c);
+            if (same > 1)   // ties, rarely: by the rest of their order
+                for (int j = 0; j < got; j++) rank += list_score[j] == mine && before(list[j], c);
             if (rank < a.n) put(rank, c);
         }
         for (int k = got + t; k < a.n; k += ST) put(k, no_cand());

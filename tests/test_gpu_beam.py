@@ -97,6 +97,32 @@ def test_select_logits_far_from_zero(cuda, at):
     check_select(x, torch.randn((2, 3), generator=g), 6)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("kind", ["first", "last", "rising", "falling", "alone", "tied"])
+def test_select_beams_far_ahead_of_the_others(cuda, dtype, kind):
+    """The best lists hold nearly all that is chosen: more candidates reach the other
+    lists' best than are ranked at a time."""
+    beams, n = 64, 64
+    g = torch.Generator().manual_seed(21)
+    x = torch.randn((2, beams, 20000), generator=g).to(DTYPES[dtype])
+    cum = torch.full((2, beams), -40.0)
+    if kind == "first":
+        cum[:, 0] = -1.0
+    elif kind == "last":
+        cum[:, 60:] = torch.tensor([-3.0, -1.0, -2.0, -2.5])
+    elif kind == "rising":
+        cum = -70 + torch.arange(beams).float().expand(2, beams) * 0.25
+    elif kind == "falling":
+        cum = -torch.arange(beams).float().expand(2, beams) * 0.25
+    elif kind == "alone":
+        cum[:] = -math.inf
+        cum[0, 5] = cum[1, 63] = 0.0
+    else:
+        x[:] = x[:, :1]
+        x[:, :, 10:] = 0.0
+    check_select(x, cum.contiguous(), n)
+
+
 def test_select_probabilities_add_up(cuda):
     """Flat, steep and mixed rows: exp of the scores of a whole small vocabulary is 1."""
     from franken_ocr_b200 import beam
