@@ -491,12 +491,14 @@ template <typename K> int launch_attn(K kernel, int smem, const AttnArgs &a, cud
 // A cluster saves the prefix, the cuts and the join, and the hardware hands out the
 // rows; runs are even however long one row is.  So: as many blocks as fit the SMs at
 // once, 8 at most, where each has at most 128 KB of K to read, 256 KB where most SMs are
-// busy; and one block a (row, head) for up to four times as many as fit.  Clusters
-// against runs:
+// busy, twice that where 16 heads would be handed over in pieces; and one block a (row,
+// head) for up to four times as many as fit.  Clusters against runs:
 //   1 row, 10 heads of f32: 1024 positions 7.6 / 10.2 us, 2048 10.1 / 11.8, 4096 (256 KB
 //   on a quarter of the SMs) 15.3 / 13.5;
 //   8 rows x 8 heads of bf16: 256 positions 7.1 / 9.8, 2048 14.3 / 17.2; 32 x 8: 64 5.4 /
 //   7.5, 512 12.6 / 17.4, 1024 (256 KB) 25.5 / 30.4; all but one row short: 15.9 / 11.9;
+//   19 x 5 with 8 query heads: 1536 21.8 / 29.3, ragged 20.4 / 29.9, one long 18.7 / 15.5;
+//   80 of f32, 1024 positions: 3 blocks 16.2, 2 20.0, runs 18.6;
 //   64 x 10 of 1 to 512 positions 22.1 / 27.8, of 512 each 38.6 / 36.9; 4 query heads 26.5
 //   / 43.3 and 42.7 / 44.5; 256 x 16 of 128 each 79 / 64.
 // Where there are more (row, head)s than blocks fit, a warp takes one: nothing is joined
@@ -511,10 +513,11 @@ inline int cluster_of(const AttnArgs &a, int keys) {
     const size_t units = (size_t)a.rows * a.c.kv_heads * a.head_chunks, most = (size_t)attn_blocks();
     const size_t tiles = keys ? ((size_t)a.cap + keys - 1) / keys : SIZE_MAX;
     if (units > most && tiles <= 48 && tiles * 40 <= units) return SOLO;
-    size_t n = 8;
-    while (n > 1 && units * n > most) n >>= 1;
+    size_t n = 8;   // clusters of 5 and more leave gaps between them, those of 2 none
+    while (n > 1 && units * n * 16 > most * (n > 4 ? 13 : n > 2 ? 14 : 16)) n--;
     const size_t bytes = (size_t)a.cap * a.c.row_bytes;
-    if (units > most * 4 || bytes > n << (units * n * 4 >= most * 3 ? 18 : 17)) return RUNS;
+    const int shift = (units * n * 4 >= most * 3 ? 18 : 17) + (a.gp == 16);
+    if (units > most * 4 || bytes > n << shift) return RUNS;
     return (int)n;
 }
 
