@@ -8,13 +8,13 @@ namespace {
 constexpr int JT = 256;
 
 // Joins the pieces of the (row, kv head, chunk of query heads)s that block
-// boundaries cut: a block per boundary and query head of the chunk, of which the
-// one at a cut's first boundary does the work.  A long row of a small batch has
-// pieces of nearly every block, so the pieces' factors are found side by side
-// first, and the threads split the pieces as well as the columns.  Latency bounds
-// it: some 3 us behind the attention kernel, whose end it overlaps up to its lengths'
-// prefix.
-__global__ void __launch_bounds__(JT) paged_join_kernel(const AttnArgs a, int blocks) {
+// boundaries cut: a block per boundary, of which the one at a cut's first boundary
+// does the work, for `heads` query heads of the chunk.  Where a (row, head) can have few
+// pieces a warp joins a head.  A long row of a small batch has pieces of nearly every
+// block: there a block has one head, the pieces' factors are found side by side first,
+// and the threads split the pieces as well as the columns.  Latency bounds it: some 3 us
+// behind the attention kernel, whose end it overlaps up to its lengths' prefix.
+__global__ void __launch_bounds__(JT) paged_join_kernel(const AttnArgs a, int blocks, int heads) {
     extern __shared__ float factor[];   // [pieces]
     __shared__ int pre[ATTN_ROWS + 1];
     __shared__ float4 red[JT];
@@ -22,7 +22,7 @@ __global__ void __launch_bounds__(JT) paged_join_kernel(const AttnArgs a, int bl
     // the kernel before has waited for all that came before it: lengths may be
     // read while it still runs
     tile_prefix<JT>(a, pre);
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = blockIdx.y, HC = a.c.kv_heads * a.head_chunks;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, HC = a.c.kv_heads * a.head_chunks;
     const unsigned long long total = (unsigned long long)pre[a.rows] * HC, n = run_count(total, blocks);
     const unsigned long long b = blockIdx.x + 1;
     pdl_wait();
@@ -34,47 +34,75 @@ __global__ void __launch_bounds__(JT) paged_join_kernel(const AttnArgs a, int bl
     const unsigned long long u0 = (unsigned long long)pre[r] * HC + (unsigned long long)hc * tiles;
     if (u == u0 || before > u0) return;   // nothing is cut, or it was cut before
     const int kvh = hc / a.head_chunks, g0 = (hc - kvh * a.head_chunks) * a.gp;
-    if (g >= min(a.gp, a.group - g0)) return;
-    const int qh = kvh * a.group + g0 + g;
     // the last block whose run begins before the cut ends
     const int b0 = (int)b - 1, b1 = (int)quotient((u0 + tiles) * n - 1, total);
     const int pieces = b1 - b0 + 1, slot0 = 2 * b0 + (before == u0 ? 0 : 1);
     auto slot = [&](int p) { return p ? 2 * (b0 + p) : slot0; };
-    float M = -INFINITY, L = 0.0f;
-    for (int p = t; p < pieces; p += JT) M = fmaxf(M, a.ml[slot(p) * a.gp + g].x);
-    M = warp_max_f32(M);
-    if (lane == 0) warp_m[warp] = M;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < JT / 32; w++) M = fmaxf(M, warp_m[w]);
-    for (int p = t; p < pieces; p += JT) {
-        const float2 ml = a.ml[slot(p) * a.gp + g];
-        const float f = rescale(ml.x, M, a.c2);
-        factor[p] = f;
-        L = __fmaf_rn(ml.y, f, L);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    if (lane == 0) warp_l[warp] = L;
-    __syncthreads();
-    L = 0.0f;
-#pragma unroll
-    for (int w = 0; w < JT / 32; w++) L += warp_l[w];
-    if (a.stat && t == 0) a.stat[(int64_t)r * a.q_heads + qh] = make_float2(M, 1.0f / L);
     const int columns = a.dim / 4;   // at most 64
-    int ct = 8;
-    while (ct < columns) ct <<= 1;
-    const int splits = JT / ct, part = t / ct, c = t % ct;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (c < columns)
+    const int g_end = min(min(a.gp, a.group - g0), (int)(blockIdx.y + 1) * heads);
+    if (heads > 1 && pieces <= 32) {   // a warp a head
+        for (int g = blockIdx.y * heads + warp; g < g_end; g += JT / 32) {
+            const float2 ml = lane < pieces ? a.ml[slot(lane) * a.gp + g] : make_float2(-INFINITY, 0.0f);
+            const float M = warp_max_f32(ml.x), f = lane < pieces ? rescale(ml.x, M, a.c2) : 0.0f;
+            float L = ml.y * f;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+            if (a.stat && lane == 0) a.stat[(int64_t)r * a.q_heads + kvh * a.group + g0 + g] = make_float2(M, 1.0f / L);
+            float4 o[2] = {};
 #pragma unroll 4
-        for (int p = part; p < pieces; p += splits)
-            o = fma4(reinterpret_cast<const float4 *>(a.part + ((int64_t)slot(p) * a.gp + g) * a.dim)[c], factor[p], o);
-    red[t] = o;
-    __syncthreads();
-    if (part || c >= columns) return;
-    for (int s = 1; s < splits; s++) o = fma4(red[t + s * ct], 1.0f, o);
-    store4_as(a.out, a.q_type, r * a.out_stride + (long long)qh * a.dim + 4 * c, over4(o, L));
+            for (int p = 0; p < pieces; p++) {
+                const float fp = __shfl_sync(0xffffffffu, f, p);
+                const float4 *x = reinterpret_cast<const float4 *>(a.part + ((int64_t)slot(p) * a.gp + g) * a.dim);
+#pragma unroll
+                for (int y = 0; y < 2; y++)
+                    if (lane + y * 32 < columns) o[y] = fma4(x[lane + y * 32], fp, o[y]);
+            }
+#pragma unroll
+            for (int y = 0; y < 2; y++)
+                if (lane + y * 32 < columns)
+                    store4_as(a.out, a.q_type, r * a.out_stride + (long long)(kvh * a.group + g0 + g) * a.dim + 4 * (lane + y * 32),
+                              over4(o[y], L));
+        }
+        return;
+    }
+    for (int g = blockIdx.y * heads; g < g_end; g++) {
+        const int qh = kvh * a.group + g0 + g;
+        float M = -INFINITY, L = 0.0f;
+        for (int p = t; p < pieces; p += JT) M = fmaxf(M, a.ml[slot(p) * a.gp + g].x);
+        M = warp_max_f32(M);
+        if (lane == 0) warp_m[warp] = M;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < JT / 32; w++) M = fmaxf(M, warp_m[w]);
+        for (int p = t; p < pieces; p += JT) {
+            const float2 ml = a.ml[slot(p) * a.gp + g];
+            const float f = rescale(ml.x, M, a.c2);
+            factor[p] = f;
+            L = __fmaf_rn(ml.y, f, L);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        if (lane == 0) warp_l[warp] = L;
+        __syncthreads();
+        L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < JT / 32; w++) L += warp_l[w];
+        if (a.stat && t == 0) a.stat[(int64_t)r * a.q_heads + qh] = make_float2(M, 1.0f / L);
+        int ct = 8;
+        while (ct < columns) ct <<= 1;
+        const int splits = JT / ct, part = t / ct, c = t % ct;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (c < columns)
+#pragma unroll 4
+            for (int p = part; p < pieces; p += splits)
+                o = fma4(reinterpret_cast<const float4 *>(a.part + ((int64_t)slot(p) * a.gp + g) * a.dim)[c], factor[p], o);
+        red[t] = o;
+        __syncthreads();
+        if (!part && c < columns) {
+            for (int s = 1; s < splits; s++) o = fma4(red[t + s * ct], 1.0f, o);
+            store4_as(a.out, a.q_type, r * a.out_stride + (long long)qh * a.dim + 4 * c, over4(o, L));
+        }
+    }
 }
 
 // weights[r][kv head][j] += sum over the kv head's query heads of p_j, from the
@@ -147,8 +175,11 @@ int launch_attention(AttnArgs a, int dtype, float *weights, size_t w_row, size_t
                                        : launch_attention_bf16(a, st);
     if (rc) return rc;
     const int blocks = attn_blocks();
-    if (a.cluster == RUNS && blocks > 1)
-        FOCR_CUDA_TRY(launch_pdl(paged_join_kernel, dim3(blocks - 1, a.gp < a.group ? a.gp : a.group), JT, blocks * 4, st, a, blocks));
+    if (a.cluster == RUNS && blocks > 1) {
+        const int most = a.gp < a.group ? a.gp : a.group;
+        const int heads = most == 1 || (size_t)a.rows * a.c.kv_heads * a.head_chunks * 8 < (size_t)blocks ? 1 : 8;
+        FOCR_CUDA_TRY(launch_pdl(paged_join_kernel, dim3(blocks - 1, (most + heads - 1) / heads), JT, blocks * 4, st, a, blocks, heads));
+    }
     if (weights)
         FOCR_CUDA_TRY(launch_pdl(paged_weights_kernel, dim3((a.width + 1023) / 1024, a.c.kv_heads, a.rows), 256, 0, st,
                                  a, weights, (long long)w_row, (long long)w_head));

@@ -138,13 +138,24 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
         float unscale[2] = {1.0f, 1.0f};
         if constexpr (F32Q) {
             const float *qp = static_cast<const float *>(a.q) + r * a.q_stride + (long long)sg.qh0 * a.dim;
-            float scale[2] = {1.0f, 1.0f};
+            float qf[D / 16][4][2], scale[2] = {1.0f, 1.0f};
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ks++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int g = qr + (x & 1) * 8, d = ks * 16 + (x >> 1) * 8 + qc;
+                    const bool have = g < heads && d < a.dim;   // dim is even
+                    qf[ks][x][0] = have ? qp[g * a.dim + d] : 0.0f;
+                    qf[ks][x][1] = have ? qp[g * a.dim + d + 1] : 0.0f;
+                }
             if constexpr (HALF) {
 #pragma unroll
                 for (int y = 0; y < 2; y++) {
                     float top = 0.0f;
-                    if (qr + y * 8 < heads)
-                        for (int d = lane & 3; d < a.dim; d += 4) top = fmaxf(top, fabsf(qp[(qr + y * 8) * a.dim + d]));
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ks++)
+#pragma unroll
+                        for (int x = y; x < 4; x += 2) top = fmaxf(top, fmaxf(fabsf(qf[ks][x][0]), fabsf(qf[ks][x][1])));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                     // 2^(13 - exponent), between 2^-100 and 2^100; 0, inf and NaN as they are
@@ -160,10 +171,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
             for (int ks = 0; ks < D / 16; ks++)
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
-                    const int g = qr + (x & 1) * 8, d = ks * 16 + (x >> 1) * 8 + qc;
-                    const bool have = g < heads && d < a.dim;   // dim is even
-                    float q0 = have ? qp[g * a.dim + d] * scale[x & 1] : 0.0f;
-                    float q1 = have ? qp[g * a.dim + d + 1] * scale[x & 1] : 0.0f;
+                    float q0 = qf[ks][x][0] * scale[x & 1], q1 = qf[ks][x][1] * scale[x & 1];
 #pragma unroll
                     for (int p = 0; p < QP; p++) qa[p][ks][x] = take_pair<T>(&q0, &q1);
                 }
