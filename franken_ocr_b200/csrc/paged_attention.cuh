@@ -192,7 +192,7 @@ __device__ __forceinline__ unsigned long long quotient(unsigned long long n, uns
     return (n | d) >> 32 ? n / d : (uint32_t)n / (uint32_t)d;
 }
 
-struct Run {
+template <bool ALONE> struct Run {
     unsigned long long left;     // units to come
     int r, kvh, chunk, t, tiles; // where the next one lies: tile t of `tiles`
     int unit;                    // the next (row, head), counted, of a warp of its own
@@ -201,7 +201,7 @@ struct Run {
     // The run of this block; in a cluster its share of the cluster's (row, head),
     // which may be empty.
     __device__ Run(const AttnArgs &a, const int *pre) {
-        if (a.cluster == SOLO) {
+        if constexpr (ALONE) {
             unit = blockIdx.x * ATTN_WARPS + (threadIdx.x >> 5);
             return;
         }
@@ -236,7 +236,7 @@ struct Run {
         first = true;
     }
     __device__ bool next(const AttnArgs &a, const int *pre, Segment *s) {
-        if (a.cluster == SOLO) {
+        if constexpr (ALONE) {
             const int per_row = a.c.kv_heads * a.head_chunks;
             r = unit / per_row;
             if (r >= a.rows) return false;
@@ -284,26 +284,26 @@ struct Run {
 };
 
 // The first position of a warp's part of a tile.
-template <int KEYS> __device__ __forceinline__ int first_key(const AttnArgs &a, int tile, int warp) {
-    return (a.cluster == SOLO ? tile : tile * ATTN_WARPS + warp) * KEYS;
+template <int KEYS, bool ALONE> __device__ __forceinline__ int first_key(int tile, int warp) {
+    return (ALONE ? tile : tile * ATTN_WARPS + warp) * KEYS;
 }
 
 // The tiles of a block's run in order, across its segments, for the copies that run
 // ahead of the arithmetic.  A warp's lane `i` finds the place of the tile's i-th
 // position.
-template <int KEYS> struct Feed {
-    Run run;
+template <int KEYS, bool ALONE> struct Feed {
+    Run<ALONE> run;
     const int32_t *pages;
     int64_t head;          // the kv head's offset in a page
     RowView rv;
     int tile, end;
 
-    __device__ explicit Feed(const Run &r) : run(r), tile(0), end(0) {}
+    __device__ explicit Feed(const Run<ALONE> &r) : run(r), tile(0), end(0) {}
     // The byte offset of this lane's position of the next tile, -1 where there is
     // none; *bad if its page is not in the pool.
     __device__ int64_t next(const AttnArgs &a, const int *pre, int warp, int lane, bool *bad) {
         *bad = false;
-        while (tile == end) {   // a row may have no tiles
+        while (tile == end) {   // a row of a warp's own may have no tiles
             Segment s;
             if (!run.next(a, pre, &s)) return -1;
             pages = a.c.table + s.r * a.c.table_stride;
@@ -312,7 +312,7 @@ template <int KEYS> struct Feed {
             tile = s.t0;
             end = s.t1;
         }
-        const int i = first_key<KEYS>(a, tile++, warp) + lane;
+        const int i = first_key<KEYS, ALONE>(tile++, warp) + lane;
         if (lane >= KEYS || i >= rv.vis) return -1;
         const int64_t o = a.c.offset(pages, (uint32_t)(i < rv.ref ? i : i + rv.gap));
         *bad = o < 0;

@@ -77,7 +77,8 @@ template <typename T> __device__ __forceinline__ uint32_t take_pair(float *x, fl
 // PARTS: how many values of T a query element and a probability are split into.
 // A query of type T is one, and its probabilities two; an f32 query takes three
 // of both (24 bits of bf16, 33 of f16).
-template <typename T, int D, bool F32Q>
+// ALONE: a warp to each (row, head).
+template <typename T, int D, bool F32Q, bool ALONE>
 __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_attention_mma_kernel(const AttnArgs a) {
     using S = MmaTile<D>;
     constexpr int GP = 16, KEYS = S::KEYS, NT = KEYS / 8, ITS = S::HALF / 512, HR = mma_round<D>();
@@ -101,12 +102,12 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
 
     pdl_wait();
     pdl_trigger();
-    if (a.cluster == RUNS) tile_prefix<ATTN_WARPS * 32>(a, pre);
+    if (!ALONE && a.cluster == RUNS) tile_prefix<ATTN_WARPS * 32>(a, pre);
 
     const int qr = lane >> 2, qc = (lane & 3) * 2;   // this lane's row and columns of a tile
     const int mi = lane >> 3, rr = lane & 7;         // its matrix and row when loading one
-    Run run(a, pre);
-    Feed<KEYS> feed(run);
+    Run<ALONE> run(a, pre);
+    Feed<KEYS, ALONE> feed(run);
     uint32_t bad_stages = 0;   // of the stages in flight, those with a page outside the pool
     auto issue = [&](int stage, int64_t mine) {
         const uint32_t dst = ring_s + stage * 2 * S::HALF;
@@ -128,7 +129,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
         bad_stages |= (uint32_t)bad << s;
         cp_async_commit();
     }
-    finish_empty_rows(a, pre);
+    if constexpr (!ALONE) finish_empty_rows(a, pre);
 
     int stage = 0;
     Segment sg;
@@ -244,7 +245,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
                 for (int t = 0; t < NT; t++)
 #pragma unroll
                     for (int x = 0; x < 4; x++) s[t][x] *= unscale[x >> 1];
-            const int i0 = first_key<KEYS>(a, tile, warp) + qc;
+            const int i0 = first_key<KEYS, ALONE>(tile, warp) + qc;
             if (a.scores) {   // pairs: the stride is even, what lies behind vis is never read
                 float *sp = a.scores + ((int64_t)r * a.q_heads + sg.qh0 + qr) * a.score_stride + i0;
 #pragma unroll
@@ -327,7 +328,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
             l[y] += __shfl_xor_sync(0xffffffffu, l[y], 2);
             l[y] = any_bad ? NAN : l[y] * (1.0f / PS);
         }
-        if (a.cluster == SOLO) {
+        if constexpr (ALONE) {
 #pragma unroll
             for (int y = 0; y < 2; y++) {
                 const int g = qr + y * 8;
@@ -351,7 +352,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
                 *to_l = l[y];
             }
         };
-        if (a.cluster) {   // nothing is to come: all heads at once, where the rings were
+        if (HR < GP && a.cluster) {   // nothing is to come: all heads at once, where the rings were
             auto &all = *reinterpret_cast<Handover<GP, D> *>(smem);
             cp_async_wait<0>();
             __syncthreads();
@@ -379,9 +380,11 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
 template <typename T, int D, bool F32Q> int launch_mma(AttnArgs &a, cudaStream_t st) {
     a.gp = 16;
     a.head_chunks = (a.group + 15) / 16;
-    a.cluster = mma_q_bytes<D>() ? cluster_of(a, 0) : cluster_of(a, MmaTile<D>::KEYS);   // a query in shared memory is the block's
+    constexpr bool WARPS = mma_q_bytes<D>() == 0;   // a query in shared memory is the block's
+    a.cluster = cluster_of(a, WARPS ? MmaTile<D>::KEYS : 0);
     a.tile_shift = ilog2(a.cluster == SOLO ? MmaTile<D>::KEYS : MmaTile<D>::BLOCK);
-    return launch_attn(paged_attention_mma_kernel<T, D, F32Q>, mma_smem<D>(), a, st);
+    return launch_attn(a.cluster == SOLO ? paged_attention_mma_kernel<T, D, F32Q, WARPS> : paged_attention_mma_kernel<T, D, F32Q, false>,
+                       mma_smem<D>(), a, st);
 }
 // Whether this kernel takes the call.  16 rows x 8192 positions x 8 kv heads, bf16, this
 // kernel against the f32 units:

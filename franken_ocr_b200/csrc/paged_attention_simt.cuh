@@ -36,7 +36,8 @@ template <typename T, int D, int GP> constexpr int simt_smem() {
 // head against 512 bytes).  16 rows x 8192 positions x 8 kv heads of 128: bf16 90 us
 // with one query head (6.0 TB/s), 92 with two; f32 167 us (6.4 TB/s), 174 with four
 // query heads, 203 with eight, where 8 warps an SM leave the f32 units waiting.
-template <typename T, int D, int GP>
+// ALONE: a warp to each (row, head).
+template <typename T, int D, int GP, bool ALONE>
 __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(const AttnArgs a) {
     using S = Tile<T, D>;
     constexpr int LPK = S::LPK, KPI = S::KPI, ITS = S::ITS, KEYS = S::KEYS, NC = S::NC, EPL = S::EPL;
@@ -52,15 +53,15 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
 
     pdl_wait();
     pdl_trigger();
-    if (a.cluster == RUNS) tile_prefix<ATTN_WARPS * 32>(a, pre);
+    if (!ALONE && a.cluster == RUNS) tile_prefix<ATTN_WARPS * 32>(a, pre);
 
     const int sub = lane / LPK, chunk = lane % LPK;
     // the step whose score this lane holds after the transposing reduction
     const int my_it = (lane & (LPK / 2) ? 4 : 0) + (lane & (LPK / 4) ? 2 : 0) + (lane & (LPK / 8) ? 1 : 0);
     const int my_key = my_it * KPI + sub;
 
-    Run run(a, pre);
-    Feed<KEYS> feed(run);
+    Run<ALONE> run(a, pre);
+    Feed<KEYS, ALONE> feed(run);
     uint32_t bad_stages = 0;   // of the stages in flight, those with a page outside the pool
     auto issue = [&](int stage, int64_t mine) {
         const uint32_t dst = ring_s + stage * 2 * S::HALF + lane * 16;
@@ -84,7 +85,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
         bad_stages |= (uint32_t)bad << s;
         cp_async_commit();
     }
-    finish_empty_rows(a, pre);
+    if constexpr (!ALONE) finish_empty_rows(a, pre);
 
     int stage = 0;
     Segment sg;
@@ -130,7 +131,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
                     s[g][it] = d;
                 }
             }
-            const int i = first_key<KEYS>(a, tile, warp) + my_key;
+            const int i = first_key<KEYS, ALONE>(tile, warp) + my_key;
             const bool live = i < vis;
 #pragma unroll
             for (int g = 0; g < GP; g++) {
@@ -207,7 +208,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
 #pragma unroll
                 for (int o = LPK; o < 32; o <<= 1) acc[g][e] += __shfl_xor_sync(0xffffffffu, acc[g][e], o);
         }
-        if (a.cluster == SOLO) {
+        if constexpr (ALONE) {
 #pragma unroll
             for (int g = 0; g < GP; g++) {
                 if (g >= heads) break;
@@ -232,7 +233,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
                 *to_l = l[g];
             }
         };
-        if (a.cluster) {   // nothing is to come: all heads at once, where the rings were
+        if (HR < GP && a.cluster) {   // nothing is to come: all heads at once, where the rings were
             auto &all = *reinterpret_cast<Handover<GP, D> *>(smem);
             cp_async_wait<0>();
             __syncthreads();
@@ -259,7 +260,8 @@ template <typename T, int D, int GP> int launch_simt(AttnArgs &a, cudaStream_t s
     a.head_chunks = (a.group + GP - 1) / GP;
     a.cluster = cluster_of(a, Tile<T, D>::KEYS);
     a.tile_shift = ilog2(a.cluster == SOLO ? Tile<T, D>::KEYS : Tile<T, D>::BLOCK);
-    return launch_attn(paged_attention_kernel<T, D, GP>, simt_smem<T, D, GP>(), a, st);
+    return launch_attn(a.cluster == SOLO ? paged_attention_kernel<T, D, GP, true> : paged_attention_kernel<T, D, GP, false>,
+                       simt_smem<T, D, GP>(), a, st);
 }
 
 // 1, 2, 4 or 8 query heads a block: heads that a block does not have cost as much as
