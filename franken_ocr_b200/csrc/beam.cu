@@ -315,7 +315,7 @@ __device__ __forceinline__ Cand no_cand() { return Cand{-INFINITY, -INFINITY, IN
 // The n-th best score among the strips' first candidates (a thread takes the best
 // of those it sees), or among all where the strips are few, bounds the others; what
 // reaches it is ranked by counting.
-// Latency bounds it: 3 us for 1 x 4 beams, 6 for 32 x 8.
+// Latency bounds it: 3 us for 1 x 4 beams, 3 to 4 for 32 x 8.
 __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
     __shared__ double row_m[MAX_N], row_s[MAX_N];
     __shared__ float row_cum[MAX_N];
