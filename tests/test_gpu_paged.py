@@ -324,6 +324,17 @@ def test_attention_small_and_large_tables_agree(cuda, pool, group, dim, heads):
         assert bool(out[3].isnan().all()) and bool((out[1] == 0).all()) and bool(out[0].isfinite().all())
 
 
+@pytest.mark.parametrize("q_type,pool,group,dim", [("bf16", "bf16", 11, 64), ("f32", "f32", 6, 128), ("f32", "bf16", 2, 256)])
+def test_attention_one_long_row_among_many(cuda, q_type, pool, group, dim):
+    """A row cut into more pieces than a warp has lanes, with several heads to join."""
+    lens = [(3 * r) % 70 for r in range(50)]
+    lens[17] = 30000
+    c = Cache(lens, 1, 32, dim, DTYPES[pool], seed=31)
+    q = torch.randn((50, group, dim), generator=torch.Generator().manual_seed(32)).to(DTYPES[q_type])
+    got = check_attention(c, q, lens, weights=True)
+    assert same_bits(check_attention(c, q, lens), got)
+
+
 @pytest.mark.parametrize("q_type,pool,group,dim", [
     ("f32", "f32", 1, 128), ("f32", "f16", 7, 256), ("bf16", "bf16", 2, 64), ("bf16", "bf16", 5, 128),
     ("f16", "f16", 20, 80), ("f32", "bf16", 16, 64), ("f32", "f32", 3, 20), ("bf16", "bf16", 6, 256),
