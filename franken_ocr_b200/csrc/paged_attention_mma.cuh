@@ -11,8 +11,8 @@
 // are multiplied one after the other, so nothing is rounded to fewer bits than the
 // output has.
 //
-// Measured: 8 rows x 131072 positions, 64 / 8 heads of 128, bf16: 656 us, 6.5 TB/s;
-// 16 x 8192 x 8 heads: 93 us at 3 query heads each, 98 at 8, 109 at 16 (4.9 TB/s).
+// Measured: 8 rows x 131072 positions, 64 / 8 heads of 128, bf16: 657 us, 6.5 TB/s;
+// 16 x 8192 x 8 heads: 93 us at 3 query heads each, 96 at 8, 99 at 16 (5.4 TB/s).
 #pragma once
 
 #include "paged_attention.cuh"
@@ -39,15 +39,23 @@ template <int D> constexpr int mma_smem() {
            mma_q_bytes<D>() + (ATTN_ROWS + 1) * 4;
 }
 
-template <typename T> __device__ __forceinline__ void mma16816(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
+// c += a b; FIRST: c = a b.
+template <typename T, bool FIRST = false>
+__device__ __forceinline__ void mma16816(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
+    if constexpr (FIRST) c[0] = c[1] = c[2] = c[3] = 0.0f;
+    float d[4];
     if constexpr (std::is_same<T, __half>::value)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+    c[0] = d[0];
+    c[1] = d[1];
+    c[2] = d[2];
+    c[3] = d[3];
 }
 template <bool TRANS> __device__ __forceinline__ void ldmatrix4(uint32_t *r, uint32_t addr) {
     if constexpr (TRANS)
@@ -56,6 +64,11 @@ template <bool TRANS> __device__ __forceinline__ void ldmatrix4(uint32_t *r, uin
     else
         asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// Two f32 additions at a time.
+__device__ __forceinline__ void add_pair(float *a, const float *b) {
+    asm("{.reg .b64 a, b;\n mov.b64 a, {%0, %1};\n mov.b64 b, {%2, %3};\n add.rn.f32x2 a, a, b;\n mov.b64 {%0, %1}, a;}"
+        : "+f"(a[0]), "+f"(a[1]) : "f"(b[0]), "f"(b[1]));
 }
 // The pair (x, y) in T, and in *x, *y what it leaves of them.
 template <typename T> __device__ __forceinline__ uint32_t take_pair(float *x, float *y) {
@@ -212,8 +225,10 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
             __syncwarp();
             const uint32_t ks_s = ring_s + stage * 2 * S::HALF, vs_s = ks_s + S::HALF;
             // The tensor cores cut their sums off where f32 would round, always
-            // towards zero.  That is far below a 16-bit output, but not below an f32
-            // one: there the chains are kept short and joined by f32 additions.
+            // towards zero, so a long chain is off by a share that grows with its
+            // length (P V in one chain over 2^20 positions: 2^-9 of the output).  A
+            // chain of P V therefore ends with its tile and is joined by f32 additions;
+            // a score's is head_dim / 16 steps, of which an f32 query takes every other.
             constexpr int CHAINS = F32Q ? 3 : 1;   // even steps, odd steps, the query's lower parts
             float s[NT][4], sc[CHAINS][NT][4];
 #pragma unroll
@@ -304,16 +319,15 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
                     ldmatrix4<true>(b, vs_s + (kk * 16 + (mi & 1) * 8 + rr) * S::DB + (((jp * 2 + (mi >> 1)) ^ rr) << 4));
 #pragma unroll
                     for (int p = PP - 1; p >= 0; p--) {
-                        mma16816<T>(F32Q ? short_sum[0] : acc[2 * jp], pa[kk][p], b[0], b[1]);
-                        mma16816<T>(F32Q ? short_sum[1] : acc[2 * jp + 1], pa[kk][p], b[2], b[3]);
+                        mma16816<T>(short_sum[0], pa[kk][p], b[0], b[1]);
+                        mma16816<T>(short_sum[1], pa[kk][p], b[2], b[3]);
                     }
                 }
-                if constexpr (F32Q)
 #pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        acc[2 * jp][x] += short_sum[0][x];
-                        acc[2 * jp + 1][x] += short_sum[1][x];
-                    }
+                for (int x = 0; x < 4; x += 2) {
+                    add_pair(&acc[2 * jp][x], &short_sum[0][x]);
+                    add_pair(&acc[2 * jp + 1][x], &short_sum[1][x]);
+                }
             }
             __syncwarp();
             issue(stage, next);

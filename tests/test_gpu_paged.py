@@ -291,6 +291,36 @@ def test_attention_long_rows_stay_exact(cuda, pool, group, dim):
     assert rel < 2.0 ** -19.5, rel
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n", [1 << 17, 1 << 20])
+def test_attention_of_16_bit_queries_over_long_rows(cuda, dtype, dim, n):
+    """As many rows as blocks, so that one block sums a whole row of values of one sign:
+    no error that grows with the row."""
+    from franken_ocr_b200 import paged
+
+    dtype, page, group = DTYPES[dtype], 4096, 4
+    rows = 2 * torch.cuda.get_device_properties(0).multi_processor_count
+    g = torch.Generator(device="cuda").manual_seed(n + dim)
+    k = torch.randn((n // page, 1, page, dim), generator=g, device="cuda").to(dtype)
+    v = (1 + torch.randn(k.shape, generator=g, device="cuda").abs() / 2).to(dtype)
+    order = torch.randperm(n // page, generator=g, device="cuda")
+    q = torch.randn((4, group, dim), generator=g, device="cuda").to(dtype)
+    out = paged.paged_attention(q.repeat(rows // 4, 1, 1), k, v, order.int().repeat(rows, 1),
+                                torch.full((rows,), n, dtype=torch.int32, device="cuda"))
+    assert all(same_bits(out[r], out[r % 4]) for r in range(rows))
+    p = torch.softmax(q.view(-1, dim).double() @ k[order, 0].view(n, dim).double().T / math.sqrt(dim), -1)
+    want = (p @ v[order, 0].view(n, dim).double()).view(4, group, dim)
+    # One rounding to the output's type: half a step at the value. Below it f32 sums of
+    # n / 64 tiles a warp and their probabilities, whose roundings are of either sign:
+    # 2^-24 sqrt(n / 4) of the value, 2^-15 at 2^20; the probability's two parts leave
+    # 2^-17 of each, of either sign too, which the sum over n makes nothing.
+    step = torch.exp2(torch.floor(torch.log2(want))) * torch.finfo(dtype).eps
+    off = out[:4].double() - want
+    below = 2.0 ** -14 * want
+    assert bool((off.abs() <= step / 2 + below).all()), float(((off.abs() - step / 2) / want).max())
+
+
 @pytest.mark.parametrize("pool,group,dim", [("f32", 1, 128), ("bf16", 1, 64), ("bf16", 6, 128), ("f16", 20, 256)])
 @pytest.mark.parametrize("heads", [1, 3])
 def test_attention_small_and_large_tables_agree(cuda, pool, group, dim, heads):
