@@ -242,7 +242,8 @@ __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) 
     for (int i = t; i < (listed ? got : STRIP); i += listed ? 32 : ST) {
         float y = -INFINITY;
         if (listed) y = lx[i];
-        else if (first + i < a.vocab) y = fminf(to_f32<T>(x[first + i]), LARGEST);
+        else if (first + i < a.vocab) y = to_f32<T>(x[first + i]);   // NaN is not >= near
+        y = y == INFINITY ? LARGEST : y;
         if (y >= near) large += __double2ll_rn(exp((double)y - (double)m) * 0x1p48);
     }
     for (int o = 16; o > 0; o >>= 1) large += __shfl_xor_sync(0xffffffffu, large, o);

@@ -69,6 +69,21 @@ def test_select_ties_masks_and_values_that_are_no_numbers(cuda):
         check_select(x, scores, n)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_select_many_ties_beside_values_that_are_no_numbers(cuda, dtype):
+    """More equal logits in a strip than are listed, with NaN, -inf or +inf among them."""
+    x = torch.zeros((4, 2, 20000))
+    x[0, :, 5] = math.nan
+    x[1, :, ::3] = math.nan
+    x[2, 0, 7::2] = -math.inf
+    x[2, 1, 16000:] = math.nan
+    x[3, 0, 2000:9000] = math.inf
+    x[3, 0, 3] = math.nan
+    scores = torch.tensor([-1.0, -1.25]).expand(4, 2).contiguous()
+    for n in (1, 6):
+        check_select(x.to(DTYPES[dtype]), scores, n)
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_select_lowest_value_of_small_types(cuda, dtype):
     t = DTYPES[dtype]
