@@ -24,7 +24,8 @@ def beam_select(logits, scores, n: int | None = None, *, done=None, end_token: i
     token)``, each ``[batch, n]``, best first.
 
     A candidate's score is ``scores[b, i] + log_softmax(logits[b, i])[t]``, held
-    in 64 bits for the ranking; equal ones go to the lower beam, then the larger
+    in 64 bits for the ranking, of which a beam's log-sum is good to 2^-27 (the
+    same for the same logits); equal ones go to the lower beam, then the larger
     logit, then the lower token.  A beam with ``done[b, i]`` offers ``end_token``
     alone with its score unchanged; -inf and NaN logits and beams with a score
     that is not finite offer nothing.  Missing candidates: -inf, -1, -1."""

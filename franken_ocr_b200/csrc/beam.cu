@@ -4,9 +4,9 @@
 // A candidate (beam i, token t) scores
 //   cum_i + ((x_t - m_i) - log sum_u exp(x_u - m_i)),   m_i = max_u x_u,
 // and candidates are ranked by score, then lower beam, then larger logit, then
-// lower token.  The sum and the scores are held in 64 bits: candidates of
-// different beams often lie closer than f32 resolves, and a choice, unlike a
-// value, cannot be a little off.
+// lower token.  The scores are held in 64 bits, and a sum is good to 2^-27 of itself
+// (equal rows have equal ones): candidates of different beams often lie closer than f32
+// resolves, and a choice, unlike a value, cannot be a little off.
 //
 // Within one beam the ranking is the logits' own, so no sum is needed to
 // shorten the list: select_part_kernel reads each vocabulary strip once and
@@ -51,7 +51,7 @@ __device__ __forceinline__ float block_max_f32(float v, float *sh) {
 }
 
 constexpr float LARGEST = 3.402823466e38f;
-constexpr float SHIFT = 12582912.0f;   // 1.5 * 2^23: adding it rounds to an integer in the low bits
+constexpr float SHIFT = 786432.0f;   // 1.5 * 2^19: adding it rounds to sixteenths in the low bits
 
 // Two f32 operations at a time.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -68,21 +68,53 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
-// 2^(x log2 e - base) to about one rounding, for x / log2 e between base - 100 and
-// base + 1: Cody and Waite's reduction with log2 e in two parts, and the hardware's
-// 2^r for the rest, |r| <= 1/2.
-__device__ __forceinline__ float2 exp_below(float2 x, float base) {
-    const float2 high = make_float2(1.44269502f, 1.44269502f), low = make_float2(1.92596299e-8f, 1.92596299e-8f);
-    const float up = SHIFT - base;                     // base is an integer: exact
-    const float2 t = fma2(x, high, make_float2(up, up));
-    const float2 n = fma2(t, make_float2(-1.0f, -1.0f), make_float2(up, up));   // minus the nearest integer
-    const float2 r = fma2(x, low, fma2(x, high, n));
-    float2 p;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p.x) : "f"(r.x));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p.y) : "f"(r.y));
-    // t's low bits are n - base
-    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                       __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{.reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 d, a, b;\n"
+        " mov.b64 {%0, %1}, d;}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// 2^(i / 16), as the bits of a double.
+__constant__ unsigned long long POWER[16] = {
+    0x3ff0000000000000ull, 0x3ff0b5586cf9890full, 0x3ff172b83c7d517bull, 0x3ff2387a6e756238ull,
+    0x3ff306fe0a31b715ull, 0x3ff3dea64c123422ull, 0x3ff4bfdad5362a27ull, 0x3ff5ab07dd485429ull,
+    0x3ff6a09e667f3bcdull, 0x3ff7a11473eb0187ull, 0x3ff8ace5422aa0dbull, 0x3ff9c49182a3f090ull,
+    0x3ffae89f995ad3adull, 0x3ffc199bdd85529cull, 0x3ffd5818dcfba487ull, 0x3ffea4afa2a490daull};
+
+// Adds 2^(x log2 e - base) of four x between (base - 100) / log2 e and (base + 1) / log2 e
+// to *sum, each to 2^-27 of itself.  With n / 16 the nearest sixteenth to x log2 e, the
+// value is 2^(n / 16) (1 + p), p = 2^s - 1 with |s| <= 1/32 and |p| < 2^-5.5: the first
+// factor comes from a table and is summed in 64 bits; what is rounded to f32 lies 2^-5
+// below it.  s: two roundings of 2^-30; p: two of 2^-30; the four's sum: three of 2^-30.5;
+// together 2^-27.5.  log2 e is in two parts (Cody and Waite).
+// power: the table in shared memory, 16 entries over 32 banks, less i << 48, which the
+// shifted index adds again.
+__device__ __forceinline__ void add_exp4(float2 xa, float2 xb, float base, const uint2 *power, double *sum) {
+    const float up = SHIFT - base;   // base is an integer: exact
+    float2 rest = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const float2 x = i ? xb : xa;
+        const float2 t = fma2(x, both(1.44269502f), both(up));
+        const uint32_t t0 = __float_as_uint(t.x), t1 = __float_as_uint(t.y);   // low bits: n - 16 base
+        const float2 n = fma2(t, both(-1.0f), both(up));                       // -n / 16
+        const float2 s = fma2(x, both(1.92596299e-8f), fma2(x, both(1.44269502f), n));
+        float2 p = fma2(s, both(9.61812911e-3f), both(5.55041087e-2f));        // ln 2^k / k!
+        p = fma2(p, s, both(2.40226507e-1f));
+        p = fma2(p, s, both(6.93147181e-1f));
+        p = mul2(p, s);
+        const uint2 w0 = power[t0 & 15], w1 = power[t1 & 15];
+        const uint32_t h0 = (t0 << 16) + w0.y, h1 = (t1 << 16) + w1.y;
+        *sum += __hiloint2double((int)h0, (int)w0.x);
+        *sum += __hiloint2double((int)h1, (int)w1.x);
+        // the same as f32: 8 bits of exponent, its bias 896 less, and 23 of the fraction
+        const float2 f = make_float2(__uint_as_float(__funnelshift_l(w0.x, h0, 3) + 0x40000000u),
+                                     __uint_as_float(__funnelshift_l(w1.x, h1, 3) + 0x40000000u));
+        rest = fma2(p, f, rest);
+    }
+    *sum += rest.x + rest.y;
 }
 
 // One strip of one row's logits, held in registers (PER a thread, read once, 16
@@ -90,19 +122,20 @@ __device__ __forceinline__ float2 exp_below(float2 x, float base) {
 // its sum of exponentials and its n largest candidates.  A thread's logits do
 // not depend on the row's alignment, so equal rows give equal sums.
 //
-// The sum: terms above 1/e of the largest are few and go through the 64-bit
-// exponential; the others are rounded to f32, each by 2^-22 of itself at most and
-// not in one direction, which leaves some 1e-8 of the sum at worst and 1e-9 as a
-// rule.  All of them in 64 bits cost several times the strip's load.
+// The sum: every term to 2^-27 of itself (add_exp4), summed in 64 bits, so that equal
+// logits, whose errors all fall to one side, leave less than 2^-27 of it too (3e-9
+// measured; terms of 24 bits, summed in fours as f32, 1.1e-7 and 4.5 us less for 32 x 8
+// rows of 129280 logits).  The 64-bit exponential of every logit would cost several times
+// the strip's load.
 //
 // The n largest: at least n logits reach the n-th largest of the maxima of 2n or
 // more groups of threads, and hardly more do; these are collected and ranked by
 // counting.
 // Where too many reach it (a constant row), the n are taken one by one.
 //
-// Bound by instructions (860 a warp, half of them exponentials and list) and by the
-// three barriers of a short block: 32 x 8 rows of 129280 f32 logits, 132 MB, take
-// 46 us, 2.9 TB/s.
+// Bound by instructions, half of them the exponentials, and by the three barriers of a
+// short block: 32 x 8 rows of 129280 f32 logits, 132 MB, take 54 us with the join behind
+// them, 2.5 TB/s.
 template <typename T, int PER>
 __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) {
     constexpr int V = 16 / (int)sizeof(T), STRIP = ST * PER;
@@ -111,8 +144,9 @@ __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) 
     __shared__ int lt[LIST], count;
     __shared__ float bound;
     __shared__ double shd[ST / 32];
-    __shared__ long long shl[ST / 32];
+    __shared__ __align__(8) uint2 power[16];
     const int strip = blockIdx.x, row = blockIdx.y, t = threadIdx.x;
+    if (t < 16) power[t] = make_uint2((uint32_t)POWER[t], (uint32_t)(POWER[t] >> 32) - ((uint32_t)t << 16));
     pdl_wait();
     pdl_trigger();
     const T *x = static_cast<const T *>(a.x) + row * a.row_stride;
@@ -175,43 +209,34 @@ __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) 
     }
     // far from 0 the differences to the maximum are exact and stay small
     const float zero = fabsf(m) >= 1024.0f ? m : 0.0f, high = m - zero;
-    const float base = rintf(__fmul_rn(high, 1.44269502f)), near = m - 1.0f;
-    const float near0 = near - zero, none = high - 65.0f;   // e^-65 of the largest adds nothing
-    const float2 minus = make_float2(-zero, -zero);
+    const float base = rintf(__fmul_rn(high, 1.44269502f)), none = high - 65.0f;   // e^-65 of the largest adds nothing
+    const float2 minus = both(-zero);
     double sum = 0.0;
 #pragma unroll
     for (int g = 0; g < PER / 4; g++) {
         float2 y0 = add2(make_float2(v[4 * g], v[4 * g + 1]), minus), y1 = add2(make_float2(v[4 * g + 2], v[4 * g + 3]), minus);
-        y0 = make_float2(fmaxf(y0.x, none), fmaxf(y0.y, none));
+        y0 = make_float2(fmaxf(y0.x, none), fmaxf(y0.y, none));   // NaN too
         y1 = make_float2(fmaxf(y1.x, none), fmaxf(y1.y, none));
-        float2 x0 = exp_below(y0, base), x1 = exp_below(y1, base);
-        if (most[g] >= near) {   // rarely: those are summed in 64 bits below
-            x0.x = y0.x < near0 ? x0.x : 0.0f;
-            x0.y = y0.y < near0 ? x0.y : 0.0f;
-            x1.x = y1.x < near0 ? x1.x : 0.0f;
-            x1.y = y1.y < near0 ? x1.y : 0.0f;
-        }
-        x0 = add2(x0, x1);
-        sum += x0.x + x0.y;
+        add_exp4(y0, y1, base, power, &sum);
     }
     __syncthreads();
-    // the few that are large or candidates
-    const float low = bound, few = fminf(low, near);
+    // the candidates
+    const float low = bound;
     int c = 0;
 #pragma unroll
     for (int g = 0; g < PER / 4; g++)
-        if (most[g] >= few)
+        if (most[g] >= low)
 #pragma unroll
-            for (int i = 4 * g; i < 4 * g + 4; i++) c += v[i] >= few && v[i] > -INFINITY;
+            for (int i = 4 * g; i < 4 * g + 4; i++) c += v[i] >= low && v[i] > -INFINITY;
     if (c) {
         int k = atomicAdd(&count, c);
         if (k + c <= LIST)
 #pragma unroll
             for (int g = 0; g < PER / 4; g++)
-                if (most[g] >= few)
+                if (most[g] >= low)
 #pragma unroll
                     for (int i = 4 * g; i < 4 * g + 4; i++)
-                        if (v[i] >= few && v[i] > -INFINITY) {
+                        if (v[i] >= low && v[i] > -INFINITY) {
                             lx[k] = v[i];
                             lt[k++] = token(i);
                         }
@@ -225,7 +250,6 @@ __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) 
         for (int i = t - 32; i < got; i += ST - 32) {
             const float y = lx[i];
             const int c = lt[i];
-            if (y < low) continue;
             int rank = 0;
 #pragma unroll 8
             for (int j = 0; j < got; j++) rank += (lx[j] > y) | ((lx[j] == y) & (lt[j] < c));
@@ -237,26 +261,11 @@ __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) 
         for (int k = got + t - 32; k < a.n; k += ST - 32) a.ct[at * a.n + k] = -1;   // fewer than n: all are listed
         return;
     }
-    // the list's order is chance: a sum of whole multiples of 2^-48 has none
-    long long large = 0;
-    for (int i = t; i < (listed ? got : STRIP); i += listed ? 32 : ST) {
-        float y = -INFINITY;
-        if (listed) y = lx[i];
-        else if (first + i < a.vocab) y = to_f32<T>(x[first + i]);   // NaN is not >= near
-        y = y == INFINITY ? LARGEST : y;
-        if (y >= near) large += __double2ll_rn(exp((double)y - (double)m) * 0x1p48);
-    }
-    for (int o = 16; o > 0; o >>= 1) large += __shfl_xor_sync(0xffffffffu, large, o);
-    if (!listed) {
-        if ((t & 31) == 0) shl[t >> 5] = large;
-        __syncthreads();
-        for (int w = 1; t == 0 && w < ST / 32; w++) large += shl[w];
-    }
     if (t == 0) {
         for (int w = 1; w < ST / 32; w++) sum += shd[w];
         a.pm[at] = m;
-        // the small terms were taken relative to 2^base
-        a.ps[at] = sum * exp((double)base * 0.693147180559945309 - (double)high) + (double)large * 0x1p-48;
+        // the terms were taken relative to 2^base
+        a.ps[at] = sum * exp((double)base * 0.693147180559945309 - (double)high);
     }
     if (listed) return;
     float last = INFINITY;

@@ -138,6 +138,65 @@ def test_select_beams_far_ahead_of_the_others(cuda, dtype, kind):
     check_select(x, cum.contiguous(), n)
 
 
+def flat_beam(value, vocab):
+    """A logit 0 every thousand, all others `value`: their exponentials are all rounded
+    alike, and lie below the largest wherever a strip begins."""
+    x = torch.full((vocab,), value)
+    x[300::1000] = 0.0
+    return x
+
+
+def near_the_score(score, want):
+    """One rounding to f32, and what a term of the sum may be off by: of its 2^(s + k / 16),
+    |s| <= 1/32, s has two roundings of half a step, 2^-30, each ln 2 of that in the term;
+    2^s - 1 < 2^-5 has one of 2^-25 in its factor of s and one of 2^-30; four terms are
+    added up with three of 2^-25 of 2^-5.5: 2^-27.5 together."""
+    if math.isinf(want):
+        return float(score) == want
+    half = math.ldexp(1.0, math.frexp(want)[1] - 25) if want else 0.0
+    return abs(float(score) - want) <= half + 2.0 ** -27.5
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("value", [-0.03125, -0.99, -1.01, -1.3, -2.0, -2.71875, -3.0, -5.0, -9.5, -20.0])
+def test_select_sums_of_repeated_logits(cuda, dtype, value):
+    """A flat tail, as padding or masks by one value leave it, far from zero too."""
+    from franken_ocr_b200 import beam
+
+    for vocab, at in ((129280, 0.0), (40000, 0.0), (129280, 640.0), (5000, -1536.0)):
+        x = (flat_beam(value, vocab) + at).to(DTYPES[dtype])[None, None]
+        score, _, token = (t.cpu() for t in beam.beam_select(x.cuda(), torch.zeros((1, 1), device="cuda"), 3))
+        want = select(x, torch.zeros((1, 1)), 3)[0]
+        assert token[0].tolist() == [t for _, _, t in want]
+        for k in range(3):
+            assert near_the_score(score[0, k], want[k][0]), (vocab, at, float(score[0, k]) - want[k][0])
+
+
+@pytest.mark.parametrize("value", [-1.01, -1.3, -2.0, -2.71875, -3.0, -5.0, -9.5])
+def test_select_ranks_a_flat_beam_and_an_exact_one(cuda, value):
+    """Two beams whose scores differ by 1e-8 to 5e-8, either way: a flat tail of f32 terms
+    against a beam of equal logits, whose sum is a whole number."""
+    from franken_ocr_b200 import beam
+
+    vocab = 129280
+    x = torch.full((2, 2, vocab), -math.inf)
+    x[0, 0] = flat_beam(value, vocab)
+    x[0, 1, :max(1, round(float(x[0, 0].double().exp().sum())))] = 0.0
+    x[1] = x[0].flip(0)
+    norm = torch.logsumexp(x.double(), -1)
+    for gap in (-5e-8, -2e-8, -1e-8, 1e-8, 2e-8, 5e-8):
+        # the second beam's best score is `gap` above the first one's
+        scores = torch.zeros((2, 2))
+        scores[:, 1] = (norm[:, 1] - norm[:, 0] + gap).float()
+        best = scores.double() - norm
+        # scores below 0.05 in f32: the gap is met to 2^-29
+        assert bool(((best[:, 1] - best[:, 0] - gap).abs() < 2.0 ** -29).all()), best
+        got, parent, _ = beam.beam_select(x.cuda(), scores.cuda(), 1)
+        assert parent[:, 0].tolist() == [int(gap > 0)] * 2, gap
+        for b in range(2):
+            assert near_the_score(got[b, 0], float(best[b].max()))
+
+
 def test_select_probabilities_add_up(cuda):
     """Flat, steep and mixed rows: exp of the scores of a whole small vocabulary is 1."""
     from franken_ocr_b200 import beam
