@@ -172,6 +172,31 @@ def test_select_sums_of_repeated_logits(cuda, dtype, value):
             assert near_the_score(score[0, k], want[k][0]), (vocab, at, float(score[0, k]) - want[k][0])
 
 
+def test_select_scores_are_infinite_only_where_due(cuda):
+    """Masks by the lowest value, +inf logits and beams as good as dead: finite scores
+    stay finite, and what lies past f32 is -inf."""
+    from franken_ocr_b200 import beam
+
+    g = torch.Generator().manual_seed(12)
+    x = torch.randn((5, 3, 9000), generator=g)
+    low = float(torch.finfo(torch.float32).min)
+    x[0, 1, 4:] = low
+    x[1, 0, 17] = x[1, 2, 8500] = math.inf
+    x[2, 1] = -math.inf
+    x[2, 2, 1:] = -math.inf
+    x[3, :, 2:] = -math.inf
+    scores = torch.randn((5, 3), generator=g) - 5
+    scores[0, 0] = low
+    scores[4, 1] = -1e38
+    for n in (3, 40):
+        got, parent, token = (t.cpu() for t in beam.beam_select(x.cuda(), scores.cuda(), n))
+        for b, want in enumerate(select(x, scores, n)):
+            for k, (s, i, t) in enumerate(want):
+                assert (int(parent[b, k]), int(token[b, k])) == (i, t)
+                assert near_the_score(got[b, k], float(torch.tensor(s, dtype=torch.float64).float()) if abs(s) > 1e30 else s)
+            assert got[b, len(want):].tolist() == [-math.inf] * (n - len(want))
+
+
 @pytest.mark.parametrize("value", [-1.01, -1.3, -2.0, -2.71875, -3.0, -5.0, -9.5])
 def test_select_ranks_a_flat_beam_and_an_exact_one(cuda, value):
     """Two beams whose scores differ by 1e-8 to 5e-8, either way: a flat tail of f32 terms
