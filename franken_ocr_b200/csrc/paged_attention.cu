@@ -200,7 +200,7 @@ int focr_paged_attention_workspace(size_t rows, size_t q_heads, size_t head_dim,
         size_t n;
         if (!checked_mul(rows, q_heads, &n) || !checked_mul(n, weights_width, &n) || n > SIZE_MAX / 16)
             return fail(FOCR_E_SHAPE, "paged_attention_workspace: size overflow");
-        *bytes = attn_sizes(rows, q_heads, head_dim, weights_width).total;
+        *bytes = attn_sizes(rows < ATTN_ROWS ? rows : ATTN_ROWS, q_heads, head_dim, weights_width).total;
         return FOCR_OK;
     });
 }

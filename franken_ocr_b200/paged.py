@@ -181,10 +181,14 @@ def paged_attention(q, k_pages, v_pages, table, lens, *, scale: float | None = N
     ``[rows, kv_heads, width]`` f32 is added to: every seen position's
     probability, summed over the query heads of its kv head.
 
+    With ``weights`` the call's workspace holds 4 bytes for each of up to 1024 rows,
+    each query head and each position of the table or the weights, the narrower of
+    them, whatever the lengths.
+
     A row that sees nothing gives zeros.  A length past the table (or the
     weights), or a page id outside the pool, gives NaN for that row."""
     ctx = "paged_attention"
-    cache, index, kv_heads, dim, rows, _ = _cache(ctx, k_pages, v_pages, table)
+    cache, index, kv_heads, dim, rows, pages = _cache(ctx, k_pages, v_pages, table)
     if index != _device():
         return _elsewhere(paged_attention, index, q, k_pages, v_pages, table, lens, scale=scale, ref_lens=ref_lens,
                           window=window, weights=weights, out=out)
@@ -209,7 +213,7 @@ def paged_attention(q, k_pages, v_pages, table, lens, *, scale: float | None = N
         out = _empty((rows, heads, dim), (wide, dim, 1), q.dtype)
     else:
         _need(ctx, "out", out, q.dtype, shape, index)
-    need = _workspace("focr_paged_attention_workspace", rows, heads, dim, width)
+    need = _workspace("focr_paged_attention_workspace", rows, heads, dim, min(width, pages * k_pages.shape[2]))
     ws = _empty((need,), (1,), _U8)  # lives until the kernels are enqueued
     rc = lib.focr_paged_attention(cache, _pack_attention(
         q.data_ptr(), lens.data_ptr(), 0 if ref_lens is None else ref_lens.data_ptr(), out.data_ptr(),

@@ -551,7 +551,10 @@ int focr_paged_write(const focr_paged_cache *c, const focr_paged_write_args *a, 
  * elements: weights[r][h][j] += the probabilities of position j over the query
  * heads of h; entries of hidden positions, and of rows that give NaN, stay as
  * they were.  Two rows of a call must not share weights.
- * weights_width 0 for the workspace without weights. */
+ * The workspace keeps the scores of up to 1024 rows: with weights
+ * 4 * rows * q_heads * weights_width bytes, or max_pages * page_size where that is
+ * smaller, whatever the lengths and the window.  weights_width 0 for the workspace
+ * without weights. */
 int focr_paged_attention_workspace(size_t rows, size_t q_heads, size_t head_dim,
                                    size_t weights_width, size_t *bytes);
 typedef struct focr_paged_attention_args {

@@ -208,6 +208,26 @@ def test_attention_over_a_thousand_rows(cuda):
     check_attention(c, q, lens, weights=True)
 
 
+def test_attention_workspace_goes_by_the_narrower_of_table_and_weights(cuda):
+    """Weights far wider than the table ask for no more than the table's scores."""
+    from franken_ocr_b200 import paged
+
+    c = Cache([40] * 3, 2, 16, 64, torch.float32, seed=2)
+    kp, vp, table = c.cuda()
+    q = torch.randn((3, 4, 64), generator=torch.Generator().manual_seed(1)).cuda()
+    lens = torch.full((3,), 40, dtype=torch.int32, device="cuda")
+    w = torch.zeros((3, 2, 1 << 20), device="cuda")
+    paged.paged_attention(q, kp, vp, table, lens, weights=w)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = paged.paged_attention(q, kp, vp, table, lens, weights=w)
+    plain = paged.paged_attention(q, kp, vp, table, lens)
+    # the partial sums' part is there without weights too; scores of 48 positions beside it
+    assert torch.cuda.max_memory_allocated() - before < 4 << 20
+    assert same_bits(out, plain) and abs(float(w.sum()) - 3 * 2 * 2 * 2) < 1e-3
+
+
 def test_attention_peaks_and_scales(cuda):
     """Scores far apart, a maximum at either end, another scale."""
     n = 700

@@ -170,6 +170,16 @@ def test_workspaces_grow_with_their_calls():
         size("focr_paged_attention_workspace", 1 << 40, 1 << 20, 128, 1 << 20)
 
 
+def test_attention_workspace_holds_the_rows_of_one_launch():
+    """Rows past 1024 go in launches of their own, one behind the other."""
+    def size(rows):
+        n = C.c_size_t()
+        check(lib.focr_paged_attention_workspace(rows, 8, 128, 4096, C.byref(n)))
+        return n.value
+
+    assert size(1023) < size(1024) == size(1025) == size(100000)
+
+
 def test_python_checks_types_shapes_and_devices():
     import torch
 
