@@ -53,7 +53,7 @@ def beam_select(logits, scores, n: int | None = None, *, done=None, end_token: i
         raise ValueError(f"{ctx}: n must be positive")
     shape = (batch, n)
     out, parent, token = _empty(shape, (n, 1), _F32), _empty(shape, (n, 1), _I32), _empty(shape, (n, 1), _I32)
-    need = _workspace("focr_beam_select_workspace", batch, beams, vocab, n)
+    need = _workspace("focr_beam_select_workspace", index, batch, beams, vocab, n)
     ws = _empty((need,), (1,), _U8)  # lives until the kernels are enqueued
     row = stride[1] if beams > 1 else stride[0] if batch > 1 else vocab
     rc = lib.focr_beam_select(_pack_select(

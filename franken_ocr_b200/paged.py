@@ -121,8 +121,9 @@ def _elsewhere(fn, index: int, *args, **kw):
 
 
 @functools.lru_cache(maxsize=256)
-def _workspace(fn: str, *sizes) -> int:
-    """Bytes of a call's workspace, which go by its sizes alone."""
+def _workspace(fn: str, index: int, *sizes) -> int:
+    """Bytes of a call's workspace on device `index`, the current one, by whose number of
+    SMs they go beside the sizes."""
     need = C.c_size_t()
     check(getattr(lib, fn)(*sizes, C.byref(need)))
     return need.value
@@ -213,7 +214,7 @@ def paged_attention(q, k_pages, v_pages, table, lens, *, scale: float | None = N
         out = _empty((rows, heads, dim), (wide, dim, 1), q.dtype)
     else:
         _need(ctx, "out", out, q.dtype, shape, index)
-    need = _workspace("focr_paged_attention_workspace", rows, heads, dim, min(width, pages * k_pages.shape[2]))
+    need = _workspace("focr_paged_attention_workspace", index, rows, heads, dim, min(width, pages * k_pages.shape[2]))
     ws = _empty((need,), (1,), _U8)  # lives until the kernels are enqueued
     rc = lib.focr_paged_attention(cache, _pack_attention(
         q.data_ptr(), lens.data_ptr(), 0 if ref_lens is None else ref_lens.data_ptr(), out.data_ptr(),

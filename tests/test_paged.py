@@ -180,6 +180,29 @@ def test_attention_workspace_holds_the_rows_of_one_launch():
     assert size(1023) < size(1024) == size(1025) == size(100000)
 
 
+def test_workspace_sizes_are_kept_for_each_device(monkeypatch):
+    """They go by the device's SMs: one device's size is not another's."""
+    from types import SimpleNamespace
+
+    from franken_ocr_b200 import paged
+
+    current = 0
+
+    def query(rows, out):
+        out._obj.value = rows * (148 if current == 0 else 20)
+        return 0
+
+    monkeypatch.setattr(paged, "lib", SimpleNamespace(focr_query=query))
+    paged._workspace.cache_clear()
+    try:
+        assert paged._workspace("focr_query", 0, 3) == 3 * 148
+        current = 1
+        assert paged._workspace("focr_query", 1, 3) == 3 * 20
+        assert paged._workspace("focr_query", 0, 3) == 3 * 148
+    finally:
+        paged._workspace.cache_clear()
+
+
 def test_python_checks_types_shapes_and_devices():
     import torch
 
