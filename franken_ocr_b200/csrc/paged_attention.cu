@@ -279,9 +279,10 @@ int focr_paged_attention(const focr_paged_cache *cache, const focr_paged_attenti
         a.score_stride = (int)((width + 1) & ~(size_t)1);
         a.cap = weights ? (int)width : (int)cap;
         const size_t q_size = dtype_bytes(q_dtype);
-        for (size_t r0 = 0; r0 < rows; r0 += ATTN_ROWS) {
+        const size_t most = (size_t)attn_rows((size_t)a.cap);
+        for (size_t r0 = 0; r0 < rows; r0 += most) {
             AttnArgs b = a;
-            b.rows = (int)(rows - r0 < ATTN_ROWS ? rows - r0 : ATTN_ROWS);
+            b.rows = (int)(rows - r0 < most ? rows - r0 : most);
             b.c.table += r0 * cache->table_stride;
             b.q = (const char *)q + r0 * q_stride * q_size;
             b.out = (char *)out + r0 * out_stride * q_size;

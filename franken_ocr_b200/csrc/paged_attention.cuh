@@ -41,6 +41,15 @@ namespace cg = cooperative_groups;
 constexpr int ATTN_WARPS = 4, ATTN_ROWS = 1024;  // rows of one launch
 constexpr int ATTN_HEADS = 16;                   // most query heads a block takes together
 
+// Rows of one launch behind a table of `cap` positions: their tiles, of 32 positions or
+// more, are counted in 32 bits, however many rows share the pages.
+constexpr int attn_rows(size_t cap) {
+    const size_t tiles = (cap + 31) / 32, fit = tiles ? INT32_MAX / tiles : ATTN_ROWS;
+    return fit < ATTN_ROWS ? (int)fit : ATTN_ROWS;
+}
+static_assert(attn_rows(0) == ATTN_ROWS && attn_rows(1u << 25) == ATTN_ROWS && attn_rows(1u << 26) == ATTN_ROWS - 1 &&
+              attn_rows((size_t)INT32_MAX - 65535) == 32, "at least one row, at most 2^31 - 1 tiles");
+
 // How the work is shared out, where not by clusters: runs of block tiles, or a (row,
 // head) for each warp.
 constexpr int RUNS = 0, SOLO = -1;

@@ -27,6 +27,7 @@ template <int D> struct MmaTile {
     static constexpr int HALF = KEYS * DB;
     static constexpr int STAGES = HALF > 4096 ? 2 : 3;
     static constexpr int BLOCK = ATTN_WARPS * KEYS;
+    static_assert(BLOCK >= 32, "attn_rows counts on it");
 };
 // Heads that the warps hand over at a time: 2 KB a warp, or all where one block
 // fills an SM.

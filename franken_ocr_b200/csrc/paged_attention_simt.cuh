@@ -19,6 +19,7 @@ template <typename T, int D> struct Tile {
     static constexpr int HALF = KEYS * DB;      // bytes of K, and of V, in a stage
     static constexpr int STAGES = HALF > 4096 ? 2 : 3;
     static constexpr int BLOCK = ATTN_WARPS * KEYS;  // positions of a block tile
+    static_assert(BLOCK >= 32, "attn_rows counts on it");
     static constexpr int EPL = NC * 16 / (int)sizeof(T);  // dimensions of a lane
 };
 

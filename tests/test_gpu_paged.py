@@ -208,6 +208,25 @@ def test_attention_over_a_thousand_rows(cuda):
     check_attention(c, q, lens, weights=True)
 
 
+@pytest.mark.parametrize("q_type,pool,group,dim", [("f32", "f32", 1, 256), ("bf16", "bf16", 6, 64)])
+def test_attention_behind_a_table_of_all_the_positions_there_are(cuda, q_type, pool, group, dim):
+    """A row of such a table has up to 2^26 tiles: a launch takes only as many rows as
+    32 bits count tiles of, and the rows beyond follow."""
+    from franken_ocr_b200 import paged
+
+    page, rows = 1 << 12, 70
+    lens = [(13 * r) % 90 for r in range(rows)]
+    c = Cache(lens, 1, page, dim, DTYPES[pool], seed=3, capacity=1)
+    # short pages' contents, packed into pages that are long
+    pages, width = c.k.shape[0], (2**31 - 2**16) // page
+    kp, vp, _ = c.cuda()
+    table = torch.full((rows, width), -1, dtype=torch.int32, device="cuda")
+    table[:, :c.table.shape[1]] = c.table.cuda()
+    q = torch.randn((rows, group, dim), generator=torch.Generator().manual_seed(4)).to(DTYPES[q_type])
+    check_attention(c, q, lens, dev=(kp, vp, table))
+    check_attention(c, q, lens, refs=[r % 20 for r in range(rows)], window=30, dev=(kp, vp, table))
+
+
 def test_attention_workspace_goes_by_the_narrower_of_table_and_weights(cuda):
     """Weights far wider than the table ask for no more than the table's scores."""
     from franken_ocr_b200 import paged
