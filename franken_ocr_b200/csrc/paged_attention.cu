@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(JT) paged_join_kernel(const AttnArgs a, int bl
             for (int y = 0; y < 2; y++)
                 if (lane + y * 32 < columns)
                     store4_as(a.out, a.q_type, r * a.out_stride + (long long)(kvh * a.group + g0 + g) * a.dim + 4 * (lane + y * 32),
-                              over4(o[y], L));
+                              over4(o[y], L, true));
         }
         return;
     }
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(JT) paged_join_kernel(const AttnArgs a, int bl
         __syncthreads();
         if (!part && c < columns) {
             for (int s = 1; s < splits; s++) o = fma4(red[t + s * ct], 1.0f, o);
-            store4_as(a.out, a.q_type, r * a.out_stride + (long long)qh * a.dim + 4 * c, over4(o, L));
+            store4_as(a.out, a.q_type, r * a.out_stride + (long long)qh * a.dim + 4 * c, over4(o, L, true));
         }
     }
 }

@@ -379,8 +379,11 @@ __device__ __forceinline__ float4 fma4(float4 x, float f, float4 o) {
     return make_float4(__fmaf_rn(x.x, f, o.x), __fmaf_rn(x.y, f, o.y), __fmaf_rn(x.z, f, o.z),
                        __fmaf_rn(x.w, f, o.w));
 }
-__device__ __forceinline__ float4 over4(float4 x, float L) {
-    return L == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(x.x / L, x.y / L, x.z / L, x.w / L);
+// x / L; 0 where the row sees nothing, of whose sums L is 0 or, for a bad length, NaN.
+// Where it does see something, but all with scores of -inf, L is 0 too and 0 / 0 is right.
+__device__ __forceinline__ float4 over4(float4 x, float L, bool sees) {
+    if (!sees && L == 0.0f) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    return make_float4(x.x / L, x.y / L, x.z / L, x.w / L);
 }
 
 // What the warps of a block hand over at the end of a segment: HR heads at a time,
@@ -417,7 +420,7 @@ __device__ __forceinline__ void finish_heads(const AttnArgs &a, const Segment &s
                 h.o[1][i][1] = L;
             }
         } else if (s.whole) {
-            store4_as(a.out, a.q_type, s.r * a.out_stride + (long long)(s.qh0 + g) * a.dim + d, over4(o, L));
+            store4_as(a.out, a.q_type, s.r * a.out_stride + (long long)(s.qh0 + g) * a.dim + d, over4(o, L, s.rv.vis));
             if (a.stat && d == 0) a.stat[(int64_t)s.r * a.q_heads + s.qh0 + g] = make_float2(M, 1.0f / L);
         } else {
             *reinterpret_cast<float4 *>(a.part + ((int64_t)s.slot * GP + g) * a.dim + d) = o;
@@ -444,7 +447,7 @@ __device__ __forceinline__ void finish_heads(const AttnArgs &a, const Segment &s
             L = __fmaf_rn(ml.y, f, L);
             o = fma4(*reinterpret_cast<const float4 *>(&y->o[0][i][d]), f, o);
         }
-        store4_as(a.out, a.q_type, s.r * a.out_stride + (long long)(s.qh0 + g) * a.dim + d, over4(o, L));
+        store4_as(a.out, a.q_type, s.r * a.out_stride + (long long)(s.qh0 + g) * a.dim + d, over4(o, L, s.rv.vis));
         if (a.stat && d == 0) a.stat[(int64_t)s.r * a.q_heads + s.qh0 + g] = make_float2(M, 1.0f / L);
     }
     cluster.sync();   // nobody overwrites or leaves what another still reads

@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
             for (int y = 0; y < 2; y++) {
                 const int g = qr + y * 8;
                 if (g >= heads) break;
-                const float by = l[y] == 0.0f ? 0.0f : 1.0f / PS, L = l[y] == 0.0f ? 1.0f : l[y];
+                const float by = 1.0f / PS, L = !vis && l[y] == 0.0f ? 1.0f : l[y];   // as over4
                 const int64_t to = r * a.out_stride + (long long)(sg.qh0 + g) * a.dim + qc;
 #pragma unroll
                 for (int j = 0; j < D / 8; j++)

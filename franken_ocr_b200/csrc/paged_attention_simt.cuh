@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
                         const int d = (e / EPC * LPK + chunk) * EPC + e % EPC;
                         if (d < a.dim)
                             store4_as(a.out, a.q_type, r * a.out_stride + (long long)(qh0 + g) * a.dim + d,
-                                      over4(make_float4(acc[g][e], acc[g][e + 1], acc[g][e + 2], acc[g][e + 3]), l[g]));
+                                      over4(make_float4(acc[g][e], acc[g][e + 1], acc[g][e + 2], acc[g][e + 3]), l[g], vis));
                     }
                 if (a.stat && lane == 0) a.stat[(int64_t)r * a.q_heads + qh0 + g] = make_float2(m[g], 1.0f / l[g]);
             }

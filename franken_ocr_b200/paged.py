@@ -186,8 +186,9 @@ def paged_attention(q, k_pages, v_pages, table, lens, *, scale: float | None = N
     each query head and each position of the table or the weights, the narrower of
     them, whatever the lengths.
 
-    A row that sees nothing gives zeros.  A length past the table (or the
-    weights), or a page id outside the pool, gives NaN for that row."""
+    A row that sees nothing gives zeros.  Scores that are all -inf, a length past
+    the table (or the weights), or a page id outside the pool give NaN for that
+    row."""
     ctx = "paged_attention"
     cache, index, kv_heads, dim, rows, pages = _cache(ctx, k_pages, v_pages, table)
     if index != _device():

@@ -543,9 +543,9 @@ int focr_paged_write(const focr_paged_cache *c, const focr_paged_write_args *a, 
  * of its pages; out must not overlap q; with window > 0 only j < ref_lens[r] (NULL: 0) and
  * j >= lens[r] - window, which is the R-SWA rule of decode_attention
  * (rswa.rs:855-944).  out = softmax(scale * q.k) . v, all sums in f32, rounded
- * once.  A row that sees nothing gives zeros; a row whose length passes
- * max_pages * page_size (or weights_width), or one of whose pages is not in
- * the pool, gives NaN.  K and V behind a row's length are never read.
+ * once.  A row that sees nothing gives zeros; one whose visible scores are all
+ * -inf, whose length passes max_pages * page_size (or weights_width), or one of
+ * whose pages is not in the pool, gives NaN.  K and V behind a row's length are never read.
  *
  * weights (may be NULL) [rows][kv_heads][weights_width] f32, strides in
  * elements: weights[r][h][j] += the probabilities of position j over the query

@@ -280,6 +280,41 @@ def test_attention_unseen_nan_and_bad_pages(cuda):
     assert bool(out[0].isnan().all()) and bool((out[1:] == 0).all())
 
 
+# (query type, pool, query heads a kv head, head_dim): every kernel
+KINDS = [("f32", "f32", 1, 64), ("f16", "f16", 2, 128), ("bf16", "bf16", 3, 128), ("f16", "f16", 5, 64), ("f16", "f16", 4, 256),
+         ("bf16", "bf16", 17, 256), ("f32", "bf16", 6, 128), ("f32", "f16", 7, 64), ("f32", "f16", 5, 256)]
+
+
+def around_the_shares(c):
+    """The cache's tensors for each way of sharing the rows out: by its own table, by one
+    for long contexts, and among many short rows."""
+    kp, vp, table = c.cuda()
+    wide = torch.full((table.shape[0], 1 << 15), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    times = -(-1200 // table.shape[0])
+    return [(kp, vp, table, 1), (kp, vp, wide, 1), (kp, vp, table.repeat(times, 1), times)]
+
+
+@pytest.mark.parametrize("q_type,pool,group,dim", KINDS)
+def test_attention_where_every_score_is_minus_infinity(cuda, q_type, pool, group, dim):
+    """The softmax of nothing but -inf has no value: NaN, and the weights stay; a row
+    without positions gives zeros beside it."""
+    from franken_ocr_b200 import paged
+
+    lens = [50, 0, 50]
+    c = Cache(lens, 1, 16, dim, DTYPES[pool], seed=dim)
+    for j in range(50):
+        c.k[int(c.table[0, j // 16]), 0, j % 16, 3] = -math.inf
+    q = torch.randn((3, group, dim), generator=torch.Generator().manual_seed(group)).to(DTYPES[q_type])
+    q[:, :, 3] = q[:, :, 3].abs() + 0.25
+    for kp, vp, table, times in around_the_shares(c):
+        w = torch.zeros((3 * times, 1, 64), device="cuda")
+        out = paged.paged_attention(q.cuda().repeat(times, 1, 1), kp, vp, table, c.lens.cuda().repeat(times), weights=w).view(
+            times, 3, group, dim)
+        assert bool(out[:, 0].isnan().all()) and bool((out[:, 1] == 0).all()) and bool(out[:, 2].isfinite().all())
+        assert bool((w.view(times, 3, 64)[:, :2] == 0).all())
+
+
 def test_attention_strided_queries_and_out(cuda):
     from franken_ocr_b200 import paged
 
