@@ -254,8 +254,15 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int x = 0; x < 4; x++)
-                    s[t][x] = F32Q ? sc[0][t][x] + sc[CHAINS / 2][t][x] + sc[CHAINS - 1][t][x] : sc[0][t][x];
+                for (int x = 0; x < 4; x++) {
+                    s[t][x] = sc[0][t][x];
+                    if constexpr (F32Q) {
+                        // an infinite score is that of the query's upper part: the lower
+                        // ones have either sign, or are 0
+                        s[t][x] += sc[CHAINS / 2][t][x];
+                        if (fabsf(s[t][x]) != INFINITY) s[t][x] += sc[CHAINS - 1][t][x];
+                    }
+                }
             if constexpr (F32Q && HALF)
 #pragma unroll
                 for (int t = 0; t < NT; t++)

@@ -315,6 +315,42 @@ def test_attention_where_every_score_is_minus_infinity(cuda, q_type, pool, group
         assert bool((w.view(times, 3, 64)[:, :2] == 0).all())
 
 
+@pytest.mark.parametrize("q_type,pool,group,dim", KINDS)
+def test_attention_of_infinite_keys(cuda, q_type, pool, group, dim):
+    """A score of -inf has probability 0, whatever the kernel; one of +inf, or of both, has
+    none: NaN. Queries with an infinity of their own likewise."""
+    from franken_ocr_b200 import paged
+
+    n = 60
+    c = Cache([n, n, n], 1, 16, dim, DTYPES[pool], seed=dim)
+    q = torch.randn((3, group, dim), generator=torch.Generator().manual_seed(group)).to(DTYPES[q_type])
+    q[:, :, 5] = q[:, :, 5].abs() + 0.25
+    q[:, :, 9] = -q[:, :, 9].abs() - 0.25
+    for r in range(3):
+        for j in range(n):
+            at = c.k[int(c.table[r, j // 16]), 0, j % 16]
+            at[5], at[9] = at[5].abs() + 0.25, at[9].abs() + 0.25
+            if r == 0 and j % 3 == 1:      # -inf by either sign of the query
+                at[5 if j % 2 else 9] = math.inf * (-1 if j % 2 else 1)
+            if r == 1 and j == 30:
+                at[5] = math.inf
+    q[2, :, 9] = -math.inf                  # every score of the row
+    seen = [j for j in range(n) if j % 3 != 1]
+    p = torch.softmax(q[0].double() @ c.row(0, seen)[0].T / math.sqrt(dim), -1)
+    v = c.row(0, seen, "v")[0]
+    # (dim + 2) roundings of a score, the sums' and the exponential's, as in `attention`
+    rel = 2 * (dim + 2) * 2.0 ** -24 * float((q[0].double().abs() @ c.row(0, seen)[0].abs().T).max()) / math.sqrt(dim)
+    bound = (rel + 2.0 ** -13) * (p @ v.abs()) + (p @ v).abs() * HALF_STEP[q.dtype]
+    for kp, vp, table, times in around_the_shares(c):
+        w = torch.zeros((3 * times, 1, 64), device="cuda")
+        out = paged.paged_attention(q.cuda().repeat(times, 1, 1), kp, vp, table, c.lens.cuda().repeat(times), weights=w)
+        out = out.view(times, 3, group, dim).cpu()
+        assert bool(((out[:, 0].double() - p @ v).abs() <= bound).all())
+        assert bool(out[:, 1:].isnan().all())
+        w = w.view(times, 3, 64).cpu()
+        assert bool((w[:, 0, 1:n:3] == 0).all()) and bool((w[:, 1:] == 0).all())
+
+
 def test_attention_strided_queries_and_out(cuda):
     from franken_ocr_b200 import paged
 
