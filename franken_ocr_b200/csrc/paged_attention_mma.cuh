@@ -88,9 +88,45 @@ template <typename T> __device__ __forceinline__ uint32_t take_pair(float *x, fl
     }
 }
 
+// A pair of probabilities in N parts of T, whose sum they are.  Each part of one above 0
+// is above 0 too, as an infinite value times a negative part, or 0, would make NaN of it;
+// those of 0 are 0.  So all parts but the last are cut off, and a lower one has 2^-30 of
+// the probability added, or, in f16, which reaches no further down, is 2^-24 at least.
+template <typename T, int N> __device__ __forceinline__ void split_probs(float x, float y, uint32_t (*to)[4], int at) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const float fx = fminf(x * 0x1p127f, 0x1p-24f), fy = fminf(y * 0x1p127f, 0x1p-24f);   // 0 for 0
+#pragma unroll
+        for (int p = 0; p < N; p++) {
+            x = fmaxf(x, fx);
+            y = fmaxf(y, fy);
+            if (p == N - 1) {
+                to[p][at] = take_pair<T>(&x, &y);
+            } else {
+                asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(to[p][at]) : "f"(y), "f"(x));
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&to[p][at]));
+                x -= f.x;
+                y -= f.y;
+            }
+        }
+    } else {   // an f32's upper half is it cut off to bf16
+        const float x0 = x, y0 = y;
+#pragma unroll
+        for (int p = 0; p < N; p++) {
+            if (p == N - 1) {
+                to[p][at] = take_pair<T>(&x, &y);
+            } else {
+                const uint32_t bx = __float_as_uint(x), by = __float_as_uint(y);
+                to[p][at] = __byte_perm(bx, by, 0x7632);
+                x = __fmaf_rn(x0, 0x1p-30f, x - __uint_as_float(bx & 0xffff0000u));
+                y = __fmaf_rn(y0, 0x1p-30f, y - __uint_as_float(by & 0xffff0000u));
+            }
+        }
+    }
+}
+
 // PARTS: how many values of T a query element and a probability are split into.
-// A query of type T is one, and its probabilities two; an f32 query takes three
-// of both (24 bits of bf16, 33 of f16).
+// A query of type T is one, and its probabilities two (16 bits of bf16, 22 of f16, the
+// last rounded); an f32 query takes three of both (24 bits of bf16, 33 of f16).
 // ALONE: a warp to each (row, head).
 template <typename T, int D, bool F32Q, bool ALONE>
 __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_attention_mma_kernel(const AttnArgs a) {
@@ -102,7 +138,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
     constexpr bool HALF = std::is_same<T, __half>::value;
     // f16 holds nothing below 2^-24: probabilities, at most 1, are scaled up, and a
     // head's f32 query by the power of two that brings its largest value near 2^14
-    constexpr float PS = HALF ? 2048.0f : 1.0f;
+    constexpr float PS = HALF ? 16384.0f : 1.0f;
     constexpr int RINGS = ATTN_WARPS * S::STAGES * 2 * S::HALF;
     static_assert(sizeof(Handover<GP, D>) <= RINGS, "all heads fit the rings");
     extern __shared__ __align__(128) char smem[];
@@ -315,8 +351,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
                     const int t = 2 * kk + (x >> 1), y = x & 1;
                     float p0 = prob(s[t][2 * y], a.c2, mc[y]) * PS, p1 = prob(s[t][2 * y + 1], a.c2, mc[y]) * PS;
                     l[y] += p0 + p1;
-#pragma unroll
-                    for (int p = 0; p < PP; p++) pa[kk][p][x] = take_pair<T>(&p0, &p1);
+                    split_probs<T, PP>(p0, p1, pa[kk], x);
                 }
 #pragma unroll
             for (int jp = 0; jp < D / 16; jp++) {

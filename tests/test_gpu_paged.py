@@ -351,6 +351,42 @@ def test_attention_of_infinite_keys(cuda, q_type, pool, group, dim):
         assert bool((w[:, 0, 1:n:3] == 0).all()) and bool((w[:, 1:] == 0).all())
 
 
+@pytest.mark.parametrize("q_type,pool,group,dim", KINDS)
+def test_attention_of_infinite_values(cuda, q_type, pool, group, dim):
+    """A visible infinity in V is the output's, in its column alone and whatever the kernel;
+    with its opposite, or NaN, it has none."""
+    from franken_ocr_b200 import paged
+
+    n = 70
+    c = Cache([n, n], 1, 16, dim, DTYPES[pool], seed=dim)
+    q = torch.randn((2, group, dim), generator=torch.Generator().manual_seed(group)).to(DTYPES[q_type])
+
+    def put(j, d, x):
+        c.v[int(c.table[0, j // 16]), 0, j % 16, d] = x
+
+    # every position once, so every part of a probability meets one
+    for j in range(n):
+        put(j, j % 30, math.inf if j % 2 else -math.inf)
+    want = torch.full((dim,), math.nan)
+    want[30] = 0.0          # stands for any finite value
+    for d in range(30):
+        signs = {j % 2 for j in range(n) if j % 30 == d}
+        want[d] = math.nan if len(signs) == 2 else math.inf if 1 in signs else -math.inf
+    put(40, 31, math.inf)
+    put(41, 31, -math.inf)
+    put(69, 32, math.nan)
+    want[33:] = 0.0
+    plain, _, bound = attention(c, q, [n, n], 1 / math.sqrt(dim))
+    for kp, vp, table, times in around_the_shares(c):
+        out = paged.paged_attention(q.cuda().repeat(times, 1, 1), kp, vp, table, c.lens.cuda().repeat(times))
+        out = out.view(times, 2, group, dim).cpu()
+        got = torch.where(out[:, 0].isfinite(), torch.zeros(()), out[:, 0].float())
+        assert torch.equal(got.nan_to_num(nan=7.0, posinf=8.0, neginf=9.0),
+                           want.nan_to_num(nan=7.0, posinf=8.0, neginf=9.0).expand(got.shape))
+        assert bool(((out[:, 0, :, 33:].double() - plain[0, :, 33:]).abs() <= bound[0, :, 33:]).all())
+        assert bool(((out[:, 1].double() - plain[1]).abs() <= bound[1]).all())
+
+
 def test_attention_strided_queries_and_out(cuda):
     from franken_ocr_b200 import paged
 
