@@ -74,7 +74,8 @@ def beam_reorder(k_pages, v_pages, table, lens, parent, fresh, *, weights=None):
     f32 (without the first dimension for one layer) follow.
 
     Returns ``(table, lens, weights or None)``, new tensors.  A parent outside
-    ``[0, beams)`` leaves an empty row.  The fresh pages must differ from one
+    ``[0, beams)`` leaves an empty row, as does a length past the table; a partly
+    filled page outside the pool stays missing (-1).  The fresh pages must differ from one
     another and from every page the table uses."""
     ctx = "beam_reorder"
     layered = k_pages.dim() == 5

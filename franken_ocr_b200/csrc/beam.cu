@@ -591,9 +591,12 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(const ReorderArgs a) 
     const int32_t *pages = a.c.table + (int64_t)(src < 0 ? 0 : src) * a.c.table_stride;
     const int here = a.fresh[i];
     const int from = rest > 0 ? pages[full] : -1;
+    // a tail whose page is not in the pool stays without one, so that its row goes on
+    // giving NaN and not what the fresh page holds
+    const bool lost = rest > 0 && (uint32_t)from >= (uint32_t)a.c.n_pages;
     if (lh == 0) {
         for (int j = t; j < a.c.max_pages; j += 256)
-            a.table_out[(int64_t)i * a.c.max_pages + j] = j < full ? pages[j] : j == full ? here : -1;
+            a.table_out[(int64_t)i * a.c.max_pages + j] = j < full ? pages[j] : j == full && !lost ? here : -1;
         if (t == 0) a.lens_out[i] = n;
     }
     if ((uint32_t)from < (uint32_t)a.c.n_pages && (uint32_t)here < (uint32_t)a.c.n_pages) {

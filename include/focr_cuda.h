@@ -626,7 +626,8 @@ int focr_beam_select(const focr_beam_select_args *a, void *stream);
  * layer_stride elements behind layer l - 1's; one table for all).  Full pages
  * are shared through table_out [rows][max_pages]; the parent's partly filled
  * page is copied to page fresh[i], which also takes that place in table_out
- * where nothing is copied, so every beam can go on writing.  lens_out [rows].
+ * where nothing is copied, so every beam can go on writing; if it is not in the
+ * pool, that place becomes -1.  lens_out [rows].
  * Entries behind that page become -1.  weights [layers][rows][kv_heads][width]
  * (may be NULL) follow into weights_out, contiguous, with 0 from the new
  * length on.  A parent outside [0, beams) leaves an empty row, and a length past

@@ -405,6 +405,24 @@ def test_reorder_skips_pages_outside_the_pool(cuda):
     assert same_bits(kd, k) and same_bits(vd, v)
 
 
+def test_reorder_keeps_a_lost_tail_lost(cuda):
+    """A row whose tail page is not in the pool gives NaN before and after: the fresh page's
+    old contents are not its own."""
+    from franken_ocr_b200 import beam, paged
+
+    c, k, v, _, _ = reorder_case(1, 2, 2, [20, 32], 2, 16, 64, torch.float32, seed=6)
+    kd, vd = k[0].cuda().nan_to_num(1.0), v[0].cuda().nan_to_num(1.0)
+    table, fresh = c.table.cuda(), torch.tensor(c.spare, dtype=torch.int32, device="cuda")
+    table[1, 1] = c.k.shape[0]
+    parent = torch.tensor([[1, 0], [1, 1]], dtype=torch.int32, device="cuda")
+    new, lens, _ = beam.beam_reorder(kd, vd, table, c.lens.cuda(), parent, fresh)
+    assert new[:, 0].tolist() == table[[1, 0, 3, 3], 0].tolist()
+    assert new[:2, 1].tolist() == [-1, c.spare[1]]                  # 20 entries: the tail is the second page
+    assert new[2:, 1:3].tolist() == [[int(table[3, 1]), c.spare[2]], [int(table[3, 1]), c.spare[3]]]
+    out = paged.paged_attention(torch.ones((4, 2, 64), device="cuda"), kd, vd, new, lens)
+    assert bool(out[0].isnan().all()) and bool(out[1:].isfinite().all())
+
+
 # ---- together -------------------------------------------------------------------------
 
 def test_beams_over_a_paged_cache_as_they_are_used(cuda):
