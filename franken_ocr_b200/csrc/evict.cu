@@ -23,6 +23,7 @@ constexpr int HELD = 40;      // most keys of a thread that shared memory holds
 constexpr int BINS = 2048;
 constexpr int MOST = 8;       // blocks of a cluster
 constexpr uint32_t ZERO = 0x80000000u;   // the key of weight 0
+constexpr uint32_t LOST = 0x7fff7fffu;   // one NaN of f32, two of f16 or bf16
 
 // Unsigned integers that order like the weights: -0 equals 0, NaN lies below
 // every number.
@@ -283,19 +284,22 @@ __global__ void __launch_bounds__(256) evict_gather_kernel(const EvictArgs a) {
                 s[u] = a.c.offset(from, (uint32_t)pos[u]);
                 d[u] = a.c.offset(to, j);
             }
-            if (d[u] < 0) s[u] = -1;
             s[u] += s[u] < 0 ? 0 : (int64_t)(x - j * cpr) * 16;
-            d[u] += (int64_t)(x - j * cpr) * 16;
+            d[u] += d[u] < 0 ? 0 : (int64_t)(x - j * cpr) * 16;
         }
+        // an entry whose page is not in the pool is NaN (of every type), as it was, and
+        // not what the new page holds
 #pragma unroll
-        for (int u = 0; u < U; u++)
-            if (s[u] >= 0) {
+        for (int u = 0; u < U; u++) {
+            k[u] = v[u] = make_uint4(LOST, LOST, LOST, LOST);
+            if (s[u] >= 0 && d[u] >= 0) {
                 k[u] = *(const uint4 *)(kb + s[u]);
                 v[u] = *(const uint4 *)(vb + s[u]);
             }
+        }
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (s[u] >= 0) {
+            if (d[u] >= 0) {
                 *(uint4 *)(const_cast<char *>(kb) + d[u]) = k[u];
                 *(uint4 *)(const_cast<char *>(vb) + d[u]) = v[u];
             }

@@ -235,6 +235,10 @@ def paged_evict(k_pages, v_pages, table, lens, weights, new_table, budget: int, 
     pages of ``new_table`` ``[rows, pages]``, none of which may be a page that a
     row of this call reads; the old pages are not written.
 
+    A length below 0, past the table or past the weights (for which attention gives
+    NaN) counts as 0 and leaves an empty row; an entry on a page outside the pool
+    becomes NaN.
+
     Returns ``(kept, lens, weights)``: the old positions ``[rows, kv_heads,
     budget]`` (-1 behind the last), the new lengths, and the kept entries'
     weights in a tensor of ``weights``' shape, 0 behind them."""

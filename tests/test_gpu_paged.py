@@ -798,6 +798,43 @@ def test_evict_in_a_replayed_graph_and_beyond_32_bits(cuda):
         w.copy_(torch.rand(w.shape, generator=g, device="cuda"))
 
 
+@pytest.mark.parametrize("pool", ["f32", "f16", "bf16"])
+def test_evict_keeps_lost_entries_lost(cuda, pool):
+    """Entries on a page outside the pool give NaN before and after, not what the new page
+    held; a new page outside the pool is not written."""
+    from franken_ocr_b200 import paged
+
+    c = Cache([64] * 4, 2, 16, 64, DTYPES[pool], seed=3, spare=8)
+    kp, vp, table = c.cuda()
+    kp, vp = kp.nan_to_num(1.0), vp.nan_to_num(1.0)
+    before = kp.clone(), vp.clone()
+    table[1, 3], table[2, 2] = -1, kp.shape[0]
+    into = torch.tensor(c.spare, dtype=torch.int32, device="cuda").view(4, 2)
+    into[3, 1] = -5
+    w = torch.zeros((4, 2, 64), device="cuda")
+    w[2, 0, 32:48] = 1.0           # of row 2 one head keeps entries of the missing page
+    kept, lens, _ = paged.paged_evict(kp, vp, table, c.lens.cuda(), w, into, 20, recent=4)
+    assert lens.tolist() == [20] * 4
+    for r in range(4):
+        for h in range(2):
+            for j, p in enumerate(kept[r, h].tolist()):
+                at, src = int(into[r, j // 16]), int(table[r, p // 16])
+                for new, old in zip((kp, vp), before):
+                    if not 0 <= at < kp.shape[0]:
+                        continue
+                    if 0 <= src < kp.shape[0]:
+                        assert same_bits(new[at, h, j % 16], old[src, h, p % 16])
+                    else:
+                        assert bool(new[at, h, j % 16].isnan().all())
+    out = paged.paged_attention(torch.ones((4, 2, 64), device="cuda"), kp, vp, into, lens)
+    assert out.isnan().any(-1).tolist() == [[False, False], [True, True], [True, False], [True, True]]
+    # nothing else is touched
+    same = torch.ones(kp.shape[0], dtype=torch.bool)
+    same[[p for p in into.view(-1).tolist() if p >= 0]] = False
+    for new, old in zip((kp, vp), before):
+        assert same_bits(new.cpu()[same], old.cpu()[same])
+
+
 def test_evict_lengths_out_of_range_and_bad_pages(cuda):
     from franken_ocr_b200 import paged
 
