@@ -21,7 +21,7 @@ def beam_select(logits, scores, n: int | None = None, *, done=None, end_token: i
     """From ``logits`` ``[batch, beams, vocab]`` (f32, f16 or bf16) and the beams'
     cumulated log probabilities ``scores`` ``[batch, beams]`` f32: the ``n`` (by
     default ``beams``) best continuations of every entry as ``(scores, parent,
-    token)``, each ``[batch, n]``, best first.
+    token)``, each ``[batch, n]``, best first.  ``beams`` and ``n`` are at most 64.
 
     A candidate's score is ``scores[b, i] + log_softmax(logits[b, i])[t]``, held
     in 64 bits for the ranking, of which a beam's log-sum is good to 2^-27 (the

@@ -646,9 +646,11 @@ extern "C" {
 int focr_beam_select_workspace(size_t batch, size_t beams, size_t vocab, size_t n, size_t *bytes) {
     return guarded("beam_select_workspace", [&]() -> int {
         if (!bytes) return fail(FOCR_E_ARG, "beam_select_workspace: null pointer");
+        if (beams > MAX_N || n > MAX_N)
+            return fail(FOCR_E_UNSUPPORTED, "beam_select_workspace: beams and n are at most " + std::to_string(MAX_N) +
+                                                ", not " + std::to_string(beams) + " and " + std::to_string(n));
         size_t rows, x;
-        if (!checked_mul(batch, beams, &rows) || !checked_mul(rows, vocab / ST + 8, &x) || n > MAX_N ||
-            x > SIZE_MAX / 1024)
+        if (!checked_mul(batch, beams, &rows) || !checked_mul(rows, vocab / ST + 8, &x) || x > SIZE_MAX / 1024)
             return fail(FOCR_E_SHAPE, "beam_select_workspace: size out of range");
         *bytes = select_sizes(rows, vocab, n).total;
         return FOCR_OK;

@@ -170,6 +170,14 @@ def test_workspaces_grow_with_their_calls():
         size("focr_paged_attention_workspace", 1 << 40, 1 << 20, 128, 1 << 20)
 
 
+@pytest.mark.parametrize("beams,n", [(4, 65), (33, 66), (65, 4)])
+def test_select_workspace_names_the_limit(beams, n):
+    """It is what the Python call asks first."""
+    with pytest.raises(FocrError, match=f"at most 64, not {beams} and {n}") as e:
+        check(lib.focr_beam_select_workspace(1, beams, 1000, n, C.byref(C.c_size_t())))
+    assert e.value.code == -7
+
+
 def test_attention_workspace_holds_the_rows_of_one_launch():
     """Rows past 1024 go in launches of their own, one behind the other."""
     def size(rows):
