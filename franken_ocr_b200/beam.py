@@ -4,7 +4,8 @@
   lm-head's logits;
 * ``beam_reorder`` -- every beam gets its parent's paged cache.
 
-CUDA tensors on one device, torch's current stream; both can be captured.
+CUDA tensors on one device, torch's current stream; both can be captured, and
+no gradient passes through them.
 """
 from __future__ import annotations
 

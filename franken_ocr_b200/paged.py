@@ -13,7 +13,8 @@ A pool is ``[pages, kv_heads, page_size, head_dim]`` (f32, f16 or bf16), one for
 K and one for V with the same strides; a row's position ``p`` lies in page
 ``table[row, p // page_size]``, slot ``p % page_size``.  The calls take CUDA
 tensors on one device, enqueue work on torch's current stream of that device
-and can be captured into a CUDA graph.
+and can be captured into a CUDA graph.  They are for decoding: no gradient passes
+through them, and no output requires one.
 
 The checks are written for speed: a decode step makes these calls for every
 layer, and the smallest run 2 us on the device.
@@ -46,13 +47,22 @@ _pack_cache = _packer(PagedCache, "6N5Ii")
 _pack_write = _packer(PagedWriteArgs, "8Ni")
 _pack_attention = _packer(PagedAttentionArgs, "15Nif")
 _pack_evict = _packer(PagedEvictArgs, "15N")
-_device = torch._C._cuda_getDevice
-_stream = torch._C._cuda_getCurrentRawStream
+# torch's own short cuts where it has them, its public calls where not: the current
+# device, its stream, and an allocation on it without the dispatcher (half the time; the
+# calls work on addresses, so no dispatch mode could follow them either way)
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+try:
+    from torch._C._dynamo.guards import _empty_strided_cuda as _quick_empty
+except ImportError:
+    _quick_empty = None
 
-try:  # an allocation on the current device without the dispatcher: half the time
-    from torch._C._dynamo.guards import _empty_strided_cuda as _empty
-except ImportError:  # pragma: no cover
-    def _empty(shape, stride, dtype):
+
+def _empty(shape, stride, dtype):
+    try:
+        return _quick_empty(shape, stride, dtype)
+    except TypeError:  # there is none, or it takes something else
         return torch.empty_strided(shape, stride, dtype=dtype, device="cuda")
 
 

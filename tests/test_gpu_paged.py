@@ -666,6 +666,26 @@ def test_attention_is_the_same_every_time_and_in_a_graph(cuda):
     assert same_bits(outs[0], paged.paged_attention(qs[1], kp, vp, table, lens))
 
 
+def test_calls_without_torchs_internal_short_cuts(cuda, monkeypatch):
+    """The public calls in their place give the same; outputs never require a gradient."""
+    from franken_ocr_b200 import paged
+
+    c = Cache([70, 50], 2, 16, 64, torch.bfloat16, seed=16)
+    kp, vp, table = c.cuda()
+    q = torch.randn((2, 4, 64), generator=torch.Generator().manual_seed(1)).cuda().requires_grad_()
+    want = paged.paged_attention(q, kp, vp, table, c.lens.cuda())
+    assert not want.requires_grad
+    monkeypatch.setattr(paged, "_quick_empty", None)
+    monkeypatch.setattr(paged, "_device", torch.cuda.current_device)
+    monkeypatch.setattr(paged, "_stream", lambda index: torch.cuda.current_stream(index).cuda_stream)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = paged.paged_attention(q, kp, vp, table, c.lens.cuda())
+    torch.cuda.synchronize()
+    assert same_bits(got, want)
+
+
 def test_attention_offsets_past_32_bits(cuda):
     """A pool of over 4 GB whose last pages hold the row."""
     from franken_ocr_b200 import paged

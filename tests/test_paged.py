@@ -211,6 +211,32 @@ def test_workspace_sizes_are_kept_for_each_device(monkeypatch):
         paged._workspace.cache_clear()
 
 
+def test_public_torch_calls_stand_in_for_missing_short_cuts(monkeypatch):
+    """Without torch's internal calls, or with others of that name, the public ones serve."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    import torch
+
+    from franken_ocr_b200 import paged
+
+    code = ("import sys, types, torch\n"
+            "del torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream\n"
+            "sys.modules['torch._C._dynamo.guards'] = types.ModuleType('guards')\n"
+            "from franken_ocr_b200 import beam, paged\n"
+            "assert paged._device is torch.cuda.current_device and paged._quick_empty is None\n"
+            "torch.cuda.current_stream = lambda i: types.SimpleNamespace(cuda_stream=70 + i)\n"
+            "assert paged._stream(3) == 73\n")
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=Path(paged.__file__).parents[1])
+    seen = []
+    monkeypatch.setattr(torch, "empty_strided", lambda *a, **k: seen.append((a, k)))
+    for quick in (None, lambda shape: None):
+        monkeypatch.setattr(paged, "_quick_empty", quick)
+        paged._empty((2, 3), (3, 1), torch.float32)
+    assert seen == [(((2, 3), (3, 1)), dict(dtype=torch.float32, device="cuda"))] * 2
+
+
 def test_python_checks_types_shapes_and_devices():
     import torch
 
