@@ -9,10 +9,12 @@ no gradient passes through them.
 """
 from __future__ import annotations
 
+import struct
+
 import torch
 
 from ._lib import FOCR_OK, BeamReorderArgs, BeamSelectArgs, check, lib
-from .paged import _F32, _I32, _U8, _cache, _device, _dtype, _elsewhere, _empty, _need, _packer, _stream, _workspace
+from .paged import _F32, _I32, _U8, _cache, _device, _dtype, _elsewhere, _empty, _misfit, _need, _packer, _stream, _workspace
 
 _pack_select = _packer(BeamSelectArgs, "13Nii")
 _pack_reorder = _packer(BeamReorderArgs, "15N")
@@ -52,14 +54,18 @@ def beam_select(logits, scores, n: int | None = None, *, done=None, end_token: i
         n = beams
     if n < 1:
         raise ValueError(f"{ctx}: n must be positive")
+    need = _workspace("focr_beam_select_workspace", index, batch, beams, vocab, n)
     shape = (batch, n)
     out, parent, token = _empty(shape, (n, 1), _F32), _empty(shape, (n, 1), _I32), _empty(shape, (n, 1), _I32)
-    need = _workspace("focr_beam_select_workspace", index, batch, beams, vocab, n)
     ws = _empty((need,), (1,), _U8)  # lives until the kernels are enqueued
     row = stride[1] if beams > 1 else stride[0] if batch > 1 else vocab
-    rc = lib.focr_beam_select(_pack_select(
-        logits.data_ptr(), scores.data_ptr(), 0 if done is None else done.data_ptr(), out.data_ptr(), parent.data_ptr(),
-        token.data_ptr(), ws.data_ptr(), batch, beams, vocab, row, n, need, code, end_token), _stream(index))
+    try:
+        args = _pack_select(
+            logits.data_ptr(), scores.data_ptr(), 0 if done is None else done.data_ptr(), out.data_ptr(),
+            parent.data_ptr(), token.data_ptr(), ws.data_ptr(), batch, beams, vocab, row, n, need, code, end_token)
+    except (struct.error, OverflowError) as e:
+        raise _misfit(ctx, e) from e
+    rc = lib.focr_beam_select(args, _stream(index))
     if rc != FOCR_OK:
         check(rc)
     return out, parent, token

@@ -124,6 +124,11 @@ def _cache(ctx: str, k_pages, v_pages, table, dims: int = 4):
     return packed, index, heads, dim, rows, width
 
 
+def _misfit(ctx: str, e: Exception) -> ValueError:
+    """For a caller's number that its C type does not hold."""
+    return ValueError(f"{ctx}: an argument is out of range ({e})")
+
+
 def _elsewhere(fn, index: int, *args, **kw):
     """The same call with its tensors' device as the current one."""
     with torch.cuda.device(index):
@@ -227,10 +232,14 @@ def paged_attention(q, k_pages, v_pages, table, lens, *, scale: float | None = N
         _need(ctx, "out", out, q.dtype, shape, index)
     need = _workspace("focr_paged_attention_workspace", index, rows, heads, dim, min(width, pages * k_pages.shape[2]))
     ws = _empty((need,), (1,), _U8)  # lives until the kernels are enqueued
-    rc = lib.focr_paged_attention(cache, _pack_attention(
-        q.data_ptr(), lens.data_ptr(), 0 if ref_lens is None else ref_lens.data_ptr(), out.data_ptr(),
-        0 if weights is None else weights.data_ptr(), ws.data_ptr(), rows, heads, stride[0], wide, window, width, w_row,
-        w_head, need, code, 1.0 / math.sqrt(dim) if scale is None else scale), _stream(index))
+    try:
+        args = _pack_attention(
+            q.data_ptr(), lens.data_ptr(), 0 if ref_lens is None else ref_lens.data_ptr(), out.data_ptr(),
+            0 if weights is None else weights.data_ptr(), ws.data_ptr(), rows, heads, stride[0], wide, window, width,
+            w_row, w_head, need, code, 1.0 / math.sqrt(dim) if scale is None else scale)
+    except (struct.error, OverflowError) as e:
+        raise _misfit(ctx, e) from e
+    rc = lib.focr_paged_attention(cache, args, _stream(index))
     if rc != FOCR_OK:
         check(rc)
     return out
@@ -264,12 +273,18 @@ def paged_evict(k_pages, v_pages, table, lens, weights, new_table, budget: int, 
         raise ValueError(f"{ctx}: new_table has {new_rows} rows, table {rows}")
     if budget < 1 or sink < 0 or recent < 0:
         raise ValueError(f"{ctx}: budget must be positive, sink and recent not negative")
+    if budget > new_pages * k_pages.shape[2]:
+        raise ValueError(f"{ctx}: the new pages hold fewer entries than the budget")
     kept = _empty((rows, heads, budget), (heads * budget, budget, 1), _I32)
     new_lens = _empty((rows,), (1,), _I32)
     new_weights = _empty((rows, heads, width), (heads * width, width, 1), _F32)
-    rc = lib.focr_paged_evict(cache, _pack_evict(
-        lens.data_ptr(), weights.data_ptr(), new_table.data_ptr(), kept.data_ptr(), new_lens.data_ptr(),
-        new_weights.data_ptr(), rows, width, w_row, w_head, new_step, new_pages, budget, sink, recent), _stream(index))
+    try:
+        args = _pack_evict(
+            lens.data_ptr(), weights.data_ptr(), new_table.data_ptr(), kept.data_ptr(), new_lens.data_ptr(),
+            new_weights.data_ptr(), rows, width, w_row, w_head, new_step, new_pages, budget, sink, recent)
+    except (struct.error, OverflowError) as e:
+        raise _misfit(ctx, e) from e
+    rc = lib.focr_paged_evict(cache, args, _stream(index))
     if rc != FOCR_OK:
         check(rc)
     return kept, new_lens, new_weights

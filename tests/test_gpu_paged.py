@@ -686,6 +686,34 @@ def test_calls_without_torchs_internal_short_cuts(cuda, monkeypatch):
     assert same_bits(got, want)
 
 
+def test_numbers_that_no_c_type_holds_are_refused(cuda):
+    """As ValueErrors that name the call, before anything is allocated by them."""
+    from franken_ocr_b200 import beam, paged
+    from franken_ocr_b200._lib import FocrError
+
+    c = Cache([70, 50], 2, 16, 64, torch.float32, seed=16)
+    kp, vp, table = c.cuda()
+    q, lens = torch.zeros((2, 4, 64), device="cuda"), c.lens.cuda()
+    w = torch.zeros((2, 2, 80), device="cuda")
+    with pytest.raises(FocrError, match="scale must be positive and finite"):   # infinite as f32
+        paged.paged_attention(q, kp, vp, table, lens, scale=1e39)
+    for kw in (dict(window=1 << 70), dict(scale=10 ** 400)):
+        with pytest.raises(ValueError, match="paged_attention: an argument is out of range"):
+            paged.paged_attention(q, kp, vp, table, lens, **kw)
+    for budget in (1 << 40, 1 << 70, 81):
+        with pytest.raises(ValueError, match="paged_evict: the new pages hold fewer entries than the budget"):
+            paged.paged_evict(kp, vp, table, lens, w, table.clone(), budget)
+    with pytest.raises(ValueError, match="paged_evict: an argument is out of range"):
+        paged.paged_evict(kp, vp, table, lens, w, table.clone(), 8, sink=1 << 70)
+    x, scores = torch.zeros((1, 40, 9), device="cuda"), torch.zeros((1, 40), device="cuda")
+    with pytest.raises(ValueError, match="beam_select: an argument is out of range"):
+        beam.beam_select(x, scores, end_token=1 << 31)
+    for n in (65, 80, 1 << 40):
+        with pytest.raises(FocrError, match=f"beams and n are at most 64, not 40 and {n}"):
+            beam.beam_select(x, scores, n)
+    assert int(torch.zeros(1, device="cuda")) == 0
+
+
 def test_attention_offsets_past_32_bits(cuda):
     """A pool of over 4 GB whose last pages hold the row."""
     from franken_ocr_b200 import paged
