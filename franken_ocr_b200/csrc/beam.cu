@@ -564,7 +564,7 @@ struct ReorderArgs {
     float *w_out;
     int64_t layer_stride;   // bytes between two layers' pages
     long long w_layer, w_row, w_head, wo_layer;
-    int rows, beams, layers, width;
+    int beams, width;
 };
 
 __device__ __forceinline__ int reorder_source(const ReorderArgs &a, int i) {
@@ -783,9 +783,7 @@ int focr_beam_reorder(const focr_paged_cache *cache, const focr_beam_reorder_arg
         a.w_row = (long long)weights_row_stride;
         a.w_head = (long long)weights_head_stride;
         a.wo_layer = (long long)rows * cache->kv_heads * (long long)width;
-        a.rows = (int)rows;
         a.beams = (int)beams;
-        a.layers = (int)layers;
         a.width = (int)width;
         FOCR_CUDA_TRY(launch_pdl(beam_reorder_kernel, dim3((unsigned)lh, (unsigned)rows), 256, 0,
                                  (cudaStream_t)stream, a));

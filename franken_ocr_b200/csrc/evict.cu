@@ -41,7 +41,7 @@ struct EvictArgs {
     float *w_out;
     int32_t *kept, *lens_out;
     long long w_row, w_head, into_stride;
-    int rows, width, budget, sink, recent, into_pages;
+    int width, budget, sink, recent;
 };
 
 // The row's length; one that passes its weights or its pages counts as 0.
@@ -323,13 +323,13 @@ __global__ void __launch_bounds__(256) evict_gather_kernel(const EvictArgs a) {
 // have, 8 at most.  Clusters of up to 16 against 8, rows and heads of 131072 weights,
 // with the copy of the weights: one 15.8 / 18.3 us, 16 39 / 33, 64 112 / 80: they wait
 // for one another's place.
-int launch_select(const EvictArgs &a, cudaStream_t st) {
+int launch_select(const EvictArgs &a, unsigned rows, cudaStream_t st) {
     int size = 1;
     while (size < MOST && size * SEL * 16 < a.width) size <<= 1;
     const int most = (a.width + size * SEL - 1) / (size * SEL), held = most < HELD ? most : HELD;
     FOCR_CUDA_TRY(set_max_dynamic_smem((const void *)evict_select_kernel, HELD * SEL * 4));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(size, a.c.kv_heads, a.rows);
+    cfg.gridDim = dim3(size, a.c.kv_heads, rows);
     cfg.blockDim = SEL;
     cfg.dynamicSmemBytes = (size_t)held * SEL * 4;
     cfg.stream = st;
@@ -402,14 +402,12 @@ extern "C" int focr_paged_evict(const focr_paged_cache *cache, const focr_paged_
         a.w_row = (long long)weights_row_stride;
         a.w_head = (long long)weights_head_stride;
         a.into_stride = (long long)new_table_stride;
-        a.rows = (int)rows;
         a.width = (int)width;
         a.budget = (int)budget;
         a.sink = (int)sink;
         a.recent = (int)recent;
-        a.into_pages = (int)new_pages;
         cudaStream_t st = (cudaStream_t)stream;
-        if ((rc = launch_select(a, st))) return rc;
+        if ((rc = launch_select(a, (unsigned)rows, st))) return rc;
         const size_t n = budget * (a.c.row_bytes / 16), most = n > width ? n : width;
         const unsigned blocks = (unsigned)((most + 1023) / 1024);
         FOCR_CUDA_TRY(launch_pdl(evict_gather_kernel, dim3(blocks < 256 ? blocks : 256, cache->kv_heads, (unsigned)rows),
