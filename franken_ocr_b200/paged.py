@@ -251,8 +251,9 @@ def paged_evict(k_pages, v_pages, table, lens, weights, new_table, budget: int, 
     ``sink``, its last ``recent`` and, between them, the entries of the largest
     ``weights`` (``[rows, kv_heads, width]`` f32; equal ones: the lower
     position), each kv head for itself.  The kept entries go, in order, to the
-    pages of ``new_table`` ``[rows, pages]``, none of which may be a page that a
-    row of this call reads; the old pages are not written.
+    pages of ``new_table`` ``[rows, pages]``, which must differ from one another
+    and from every page that a row of this call reads; the old pages are not
+    written.
 
     A length below 0, past the table or past the weights (for which attention gives
     NaN) counts as 0 and leaves an empty row; an entry on a page outside the pool

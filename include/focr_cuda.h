@@ -581,7 +581,8 @@ int focr_paged_attention(const focr_paged_cache *c, const focr_paged_attention_a
  * page_size >= budget): kept [rows][kv_heads][budget] gets their old
  * positions (-1 behind the last), lens_out [rows] the new lengths, weights_out
  * [rows][kv_heads][width] their weights with 0 behind them.
- * The new pages must not be among the pages that any row of the call reads;
+ * The new pages must differ from one another and from the pages that any row of
+ * the call reads;
  * the old pages are left as they were.  A length below 0, or past `width` or
  * the table, counts as 0: the row is empty from then on.  A kept entry whose page
  * is not in the pool becomes NaN; one whose new page is not is not written. */

@@ -423,6 +423,79 @@ def test_reorder_keeps_a_lost_tail_lost(cuda):
     assert bool(out[0].isnan().all()) and bool(out[1:].isfinite().all())
 
 
+def test_calls_while_another_device_is_current(cuda, monkeypatch):
+    """Tensors elsewhere than on the current device: the same call, with theirs as the
+    current one, every argument handed on."""
+    from franken_ocr_b200 import beam, paged
+
+    real = paged._device
+    c, k, v, parent, w = reorder_case(2, 2, 2, [20, 33], 2, 16, 64, torch.float32, seed=7, width=64)
+    table, lens, fresh = c.table.cuda(), c.lens.cuda(), torch.tensor(c.spare, dtype=torch.int32).cuda()
+    g = torch.Generator().manual_seed(1)
+    q, x = torch.randn((4, 4, 64), generator=g).cuda(), torch.randn((2, 2, 500), generator=g).cuda()
+    done = torch.tensor([[True, False], [False, False]]).cuda()
+
+    def calls():
+        """Everything that the five calls return or change."""
+        kd, vd, wd = k.cuda(), v.cuda(), w.cuda()
+        add = torch.zeros((4, 2, 70), device="cuda")
+        out = torch.empty_like(q)
+        paged.paged_attention(q, kd[0], vd[0], table, lens, scale=0.3, ref_lens=lens // 4, window=7, weights=add, out=out)
+        new, n, ww = beam.beam_reorder(kd, vd, table, lens, parent.cuda(), fresh, weights=wd)
+        row = torch.tensor([3, -1, 0], dtype=torch.int32).cuda()
+        paged.paged_write(q[:3, :2].contiguous(), q[:3, 2:].contiguous(), kd[1], vd[1], new, n[[3, 0, 0]].contiguous(), row=row)
+        evicted = paged.paged_evict(kd[1], vd[1], table, lens, wd[1], fresh[:, None].contiguous(), 16, sink=2, recent=5)
+        chosen = beam.beam_select(x, torch.zeros((2, 2), device="cuda"), 5, done=done, end_token=9)
+        return [out, add, new, n, ww, kd, vd, *evicted, *chosen]
+
+    want = calls()
+    asked = []
+
+    def device():
+        asked.append(None)
+        return real() + len(asked) % 2      # every first question of a call: another one
+
+    for module in (paged, beam):
+        monkeypatch.setattr(module, "_device", device)
+    got = calls()
+    torch.cuda.synchronize()
+    assert len(asked) == 10
+    assert all(same_bits(a, b) for a, b in zip(got, want))
+
+
+def test_calls_at_once_on_two_streams(cuda):
+    """Selections, reorderings and evictions side by side do not see one another's
+    workspaces."""
+    from franken_ocr_b200 import beam, paged
+
+    g = torch.Generator().manual_seed(8)
+    work = []
+    for i in range(2):
+        c, k, v, parent, w = reorder_case(3, 2, 4, [200, 77], 2, 16, 64, torch.float16, seed=20 + i, width=220)
+        spare = torch.tensor(c.spare, dtype=torch.int32).cuda()
+        x, s = (torch.randn((3, 4, 30000), generator=g) * 2).cuda(), torch.randn((3, 4), generator=g).cuda()
+        work.append((c.table.cuda(), c.lens.cuda(), spare, k.cuda(), v.cuda(), parent.cuda(), w.cuda(), x, s))
+
+    def calls(table, lens, spare, k, v, parent, w, x, s):
+        first = beam.beam_select(x, s, 8)
+        new = beam.beam_reorder(k, v, table, lens, parent, spare, weights=w)
+        kept = paged.paged_evict(k[0], v[0], table, lens, w[0], spare[:, None].contiguous(), 16, sink=1, recent=3)
+        return [*first, *new, *kept]
+
+    want = [calls(*a) for a in work]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(calls(*work[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for one in got[i]:
+            assert all(same_bits(a, b) for a, b in zip(one, want[i]))
+
+
 # ---- together -------------------------------------------------------------------------
 
 def test_beams_over_a_paged_cache_as_they_are_used(cuda):
