@@ -531,9 +531,9 @@ __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
 }
 
 // Logits of a strip.  Where long ones would keep fewer than half the SMs busy: short
-// ones (over 129280 tokens of f32 one beam 6.0 us, long 6.6; 1 x 4 beams 6.6 and 7.2,
-// bf16 6.8 and 8.0).  Otherwise long ones, whose candidates are fewer to join (1 x 8
-// beams 9.1 us, short 11.3; 32 x 8 with 4096 logits 78, 8192 54, 16384 62).
+// ones (over 129280 tokens of f32 one beam 6.6 us, long 7.9; 1 x 4 beams 7.2 and 8.3,
+// bf16 7.8 and 9.1).  Otherwise long ones, whose candidates are fewer to join (1 x 8
+// beams 8.8 us, short 9.5; 32 x 8 54 and 72).
 int strip_of(size_t rows, size_t vocab) {
     return rows * ((vocab + ST * 32 - 1) / (ST * 32)) < (size_t)num_sms() / 2 ? ST * 16 : ST * 32;
 }

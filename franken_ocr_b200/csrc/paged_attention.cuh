@@ -501,26 +501,31 @@ template <typename K> int launch_attn(K kernel, int smem, const AttnArgs &a, cud
 // How a call is shared out.  The visible positions of a row are not known here, only
 // its table's capacity.
 // A cluster saves the prefix, the cuts and the join, and the hardware hands out the
-// rows; runs are even however long one row is.  So: as many blocks as fit the SMs at
-// once, 8 at most, where each has at most 128 KB of K to read, 256 KB where most SMs are
-// busy, twice that where 16 heads would be handed over in pieces; and one block a (row,
-// head) for up to four times as many as fit.  Clusters against runs:
-//   1 row, 10 heads of f32: 1024 positions 7.6 / 10.2 us, 2048 10.1 / 11.8, 4096 (256 KB
-//   on a quarter of the SMs) 15.3 / 13.5;
-//   8 rows x 8 heads of bf16: 256 positions 7.1 / 9.8, 2048 14.3 / 17.2; 32 x 8: 64 5.4 /
-//   7.5, 512 12.6 / 17.4, 1024 (256 KB) 25.5 / 30.4; all but one row short: 15.9 / 11.9;
-//   19 x 5 with 8 query heads: 1536 21.8 / 29.3, ragged 20.4 / 29.9, one long 18.7 / 15.5;
-//   80 of f32, 1024 positions: 3 blocks 16.2, 2 20.0, runs 18.6;
-//   64 x 10 of 1 to 512 positions 22.1 / 27.8, of 512 each 38.6 / 36.9; 4 query heads 26.5
-//   / 43.3 and 42.7 / 44.5; 256 x 16 of 128 each 79 / 64.
+// rows; runs are even however long one row is.  So: as many blocks as fit the SMs at two
+// each (at head_dim 256 the tensor cores' blocks, and those of an f32 cache, fit one an
+// SM: there the split was not measured apart), 8 at most, where each has at most 128 KB
+// of K to read, 256 KB where most SMs are busy, twice that where 16 heads would be handed
+// over in pieces; and one block a (row, head) for up to four times as many as fit.
+// Clusters against runs:
+//   1 row, 10 heads of f32: 1024 positions 7.7 / 10.5 us, 2048 10.4 / 11.7, 4096 (256 KB
+//   on a quarter of the SMs, not taken) 15.4 / 13.6;
+//   8 rows x 8 heads of bf16: 256 positions 7.2 / 9.7, 2048 14.0 / 17.3; 32 x 8: 64 5.6 /
+//   7.6, 512 12.5 / 17.2, 1024 (256 KB) 25.7 / 30.6; 512 in one row, the others short:
+//   10.4 / 11.4;
+//   19 x 5 with 8 query heads: 1536 23.3 / 24.5, ragged 21.3 / 24.9, one long 19.7 / 17.1;
+//   80 of f32, 1024 positions: 3 blocks 15.0, 2 18.5, runs 18.3;
+//   64 x 10 of 1 to 512 positions 22.9 / 29.1, of 512 each 39.0 / 37.4; 4 query heads 31.9
+//   / 44.0 and 47.5 / 42.5; 256 x 16 of 128 each (not taken) 84 / 64.
 // Where there are more (row, head)s than blocks fit, a warp takes one: nothing is joined
 // or waited for, but its tiles, about 0.9 us each, follow one another.  Up to a
 // fortieth of the (row, head)s, 48 at most, the longest row ends about when the others
-// do.  bf16, full tables, warps against the better of the above: 40 x 8: 64 positions (4
-// tiles) 8.1 / 11.0 us, 128 11.0 / 12.8, 256 (16 tiles, not taken) 16.9 / 17.1, ragged
-// 16.7 / 13.4; 128 x 8: 16 6.6 / 20.2, 256 26.2 / 40.5; 224 x 16: 16 16.0 / 44.2, 128
-// 51.1 / 66.4, 512 (32 tiles) 156 / 152, ragged 93.5 / 122.5.  `keys`: of a warp's tile,
-// 0 where the kernel's warps cannot work alone.
+// do.  bf16, full tables, warps against the better of the above, for one query head and
+// for four: 40 x 8: 64 positions (4 tiles) 7.0 / 9.2 us and 10.4 / 13.3, 128 9.7 / 11.0
+// and 13.5 / 15.1, 256 (16 tiles, not taken) 15.1 / 14.7 and 19.6 / 19.6, ragged 14.7 /
+// 10.9 and 19.2 / 15.2; 128 x 8: 16 5.4 / 14.6 and 8.8 / 21.0, 256 25.7 / 33.9 and 28.8 /
+// 40.9; 224 x 16: 16 13.5 / 34.5 and 26.2 / 54.4, 128 47.5 / 58.2 and 59.4 / 74.8, 512 (32
+// tiles) 152 / 148 and 168 / 164, ragged 88.4 / 103.5 and 101.8 / 140.1.  `keys`: of a
+// warp's tile, 0 where the kernel's warps cannot work alone.
 inline int cluster_of(const AttnArgs &a, int keys) {
     const size_t units = (size_t)a.rows * a.c.kv_heads * a.head_chunks, most = (size_t)attn_blocks();
     const size_t tiles = keys ? ((size_t)a.cap + keys - 1) / keys : SIZE_MAX;

@@ -11,8 +11,9 @@
 // are multiplied one after the other, so nothing is rounded to fewer bits than the
 // output has.
 //
-// Measured: 8 rows x 131072 positions, 64 / 8 heads of 128, bf16: 657 us, 6.5 TB/s;
-// 16 x 8192 x 8 heads: 93 us at 3 query heads each, 96 at 8, 99 at 16 (5.4 TB/s).
+// Measured: 8 rows x 131072 positions, 64 / 8 heads of 128, bf16: 650 to 690 us (where
+// the pages lie makes the difference), 6.2 to 6.6 TB/s; 16 x 8192 x 8 heads: 93 us at 3
+// query heads each, 97 at 8, 99 at 16 (5.4 TB/s).
 #pragma once
 
 #include "paged_attention.cuh"
@@ -446,11 +447,11 @@ template <typename T, int D, bool F32Q> int launch_mma(AttnArgs &a, cudaStream_t
 // Whether this kernel takes the call.  16 rows x 8192 positions x 8 kv heads, bf16, this
 // kernel against the f32 units:
 //   query of the cache's type, from 3 query heads a kv head on: head_dim 64: 2 heads
-//   53.8 / 53.5 us, 3 heads 52.5 / 62.6; 128: 92.9 / 91.3, 92.8 / 104.9; 256: 184 / 177,
-//   187.8 / 188.7, 6 heads 195 / 308;
+//   47.2 / 52.5 us, 3 heads 47.0 / 60.3; 128: 94.1 / 92.8, 93.0 / 102.7; 256: 179 / 176,
+//   186 / 191, 6 heads 187 / 317;
 //   f32 query, three times the products and short chains, from 5 heads on: head_dim 64:
-//   4 heads 61.7 / 61.1, 6 heads 64 / 100; 128: 4 heads 110 / 104, 6 heads 119 / 176; not
-//   at 256, where its parts do not fit the registers.
+//   4 heads 59.2 / 58.0, 5 heads 59.4 / 98.9; 128: 4 heads 107 / 101, 5 heads 110 / 172;
+//   not at 256, where its parts do not fit the registers.
 template <typename T> bool mma_takes(const AttnArgs &a) {
     constexpr int own = std::is_same<T, __half>::value ? FOCR_F16 : FOCR_BF16;
     if (a.q_type == own) return a.group >= 3;

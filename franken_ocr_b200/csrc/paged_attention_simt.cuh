@@ -34,9 +34,10 @@ template <typename T, int D, int GP> constexpr int simt_smem() {
 
 // The arithmetic runs on the f32 units: with few query heads a kv head the
 // loads bound it (a key of 128 16-bit values costs a warp ~25 instructions a
-// head against 512 bytes).  16 rows x 8192 positions x 8 kv heads of 128: bf16 90 us
-// with one query head (6.0 TB/s), 92 with two; f32 167 us (6.4 TB/s), 174 with four
-// query heads, 203 with eight, where 8 warps an SM leave the f32 units waiting.
+// head against 512 bytes).  16 rows x 8192 positions x 8 kv heads of 128: bf16 92 us
+// with one query head (5.8 TB/s), 94 with two; f32 166 us (6.5 TB/s), 178 with four
+// query heads, 203 with eight, where 8 warps an SM leave the f32 units waiting, and 402
+// with sixteen, in two chunks that each read the cache.
 // ALONE: a warp to each (row, head).
 template <typename T, int D, int GP, bool ALONE>
 __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(const AttnArgs a) {

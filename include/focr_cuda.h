@@ -540,21 +540,23 @@ int focr_paged_write(const focr_paged_cache *c, const focr_paged_write_args *a, 
 /* Attention of one new token per row: q, out [rows][q_heads][head_dim] of
  * `q_dtype` (rows q_stride / out_stride elements apart); query head h reads
  * kv head h / (q_heads / kv_heads).  Row r sees the positions j < lens[r]
- * of its pages; out must not overlap q; with window > 0 only j < ref_lens[r] (NULL: 0) and
+ * of its pages; with window > 0 only j < ref_lens[r] (NULL: 0) and
  * j >= lens[r] - window, which is the R-SWA rule of decode_attention
- * (rswa.rs:855-944).  out = softmax(scale * q.k) . v, all sums in f32, rounded
+ * (rswa.rs:855-944); out must not overlap q.  out = softmax(scale * q.k) . v, all sums in f32, rounded
  * once.  A row that sees nothing gives zeros; one whose visible scores are all
  * -inf, whose length passes max_pages * page_size (or weights_width), or one of
- * whose pages is not in the pool, gives NaN.  K and V behind a row's length are never read.
+ * whose pages is not in the pool, gives NaN.  An infinity in a visible V is its
+ * column's output, unless it meets its opposite or its probability is below f32's
+ * smallest (then NaN).  K and V behind a row's length are never read.
  *
  * weights (may be NULL) [rows][kv_heads][weights_width] f32, strides in
  * elements: weights[r][h][j] += the probabilities of position j over the query
- * heads of h; entries of hidden positions, and of rows that give NaN, stay as
- * they were.  Two rows of a call must not share weights.
- * The workspace keeps the scores of up to 1024 rows: with weights
- * 4 * rows * q_heads * weights_width bytes, or max_pages * page_size where that is
- * smaller, whatever the lengths and the window.  weights_width 0 for the workspace
- * without weights. */
+ * heads of h; entries of hidden positions, and of heads h one of whose query heads
+ * has no probabilities (all its outputs are NaN), stay as they were.  Two rows of a call must not share weights.
+ * With weights the workspace keeps the scores of up to 1024 rows: 4 bytes for each
+ * row, query head and position of weights_width, whatever the lengths and the window
+ * (max_pages * page_size will do where that is less).  weights_width 0 for the
+ * workspace without weights. */
 int focr_paged_attention_workspace(size_t rows, size_t q_heads, size_t head_dim,
                                    size_t weights_width, size_t *bytes);
 typedef struct focr_paged_attention_args {
