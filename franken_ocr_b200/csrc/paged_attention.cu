@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(JT) paged_join_kernel(const AttnArgs a, int bl
 }
 
 // weights[r][kv head][j] += sum over the kv head's query heads of p_j, from the
-// kept scores.  A row whose output is NaN leaves its weights as they were.  Bound by
+// kept scores.  Where one of them has no probabilities the weights stay as they were.  Bound by
 // the scores' bytes, most of them still in L2: 32 rows of 8300 positions on average,
 // 8 kv heads with 4 query heads each: 13.5 us for 51 MB (22.8 with one position a
 // thread).

@@ -41,10 +41,8 @@ template <int D> constexpr int mma_smem() {
            mma_q_bytes<D>() + (ATTN_ROWS + 1) * 4;
 }
 
-// c += a b; FIRST: c = a b.
-template <typename T, bool FIRST = false>
-__device__ __forceinline__ void mma16816(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
-    if constexpr (FIRST) c[0] = c[1] = c[2] = c[3] = 0.0f;
+// c += a b.  The addend has registers of its own, so that zeros need none.
+template <typename T> __device__ __forceinline__ void mma16816(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
     float d[4];
     if constexpr (std::is_same<T, __half>::value)
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
