@@ -131,9 +131,9 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(const AttnArgs a, fl
     for (int g0 = 0; g0 < a.group; g0 += 256) {
         const int heads = min(256, a.group - g0);
         __syncthreads();
-        if (t < heads) {   // (c M, 1 / L)
+        if (t < heads) {   // (M, 1 / L)
             const float2 x = a.stat[(int64_t)r * a.q_heads + kvh * a.group + g0 + t];
-            st[t] = make_float2(scaled_max(x.x, a.c2), x.y);
+            st[t] = make_float2(base_of(x.x), x.y);
         }
         __syncthreads();
         const float *s = a.scores + ((int64_t)r * a.q_heads + kvh * a.group + g0) * a.score_stride;

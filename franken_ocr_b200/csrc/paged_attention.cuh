@@ -103,17 +103,15 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// 2^(c (s - m)) with m's product rounded once, the same for every s of a row.
-__device__ __forceinline__ float prob(float s, float c, float mc) { return ex2(__fmaf_rn(s, c, -mc)); }
-__device__ __forceinline__ float scaled_max(float m, float c) {
-    return m == -INFINITY ? 0.0f : __fmul_rn(m, c);
-}
-// What takes sums relative to the maximum m over to the maximum top >= m: the
-// probabilities were formed with the rounded products, so the factor is too, and is
-// exactly 1 where the maximum stays.
-__device__ __forceinline__ float rescale(float m, float top, float c) {
-    return m == -INFINITY ? 0.0f : ex2(__fsub_rn(__fmul_rn(m, c), scaled_max(top, c)));
-}
+// The maximum that scores are taken relative to: 0 where all are -inf.
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f : m; }
+// 2^(c (s - m)), m from base_of.  The difference comes first: a product of m and c of its
+// own would be rounded by more than the exponential bears where it passes 2^24, as the
+// lowest finite values in all of a row's keys make it.
+__device__ __forceinline__ float prob(float s, float c, float m) { return ex2(__fmul_rn(__fsub_rn(s, m), c)); }
+// What takes sums relative to the maximum m over to the maximum top >= m; exactly 1 where
+// the maximum stays.
+__device__ __forceinline__ float rescale(float m, float top, float c) { return m == -INFINITY ? 0.0f : prob(m, c, top); }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {
     asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),

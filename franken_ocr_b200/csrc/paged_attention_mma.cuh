@@ -341,14 +341,14 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, D == 256 ? 1 : 2) paged_atten
                     }
                 }
             }
-            const float mc[2] = {scaled_max(m[0], a.c2), scaled_max(m[1], a.c2)};
+            const float base[2] = {base_of(m[0]), base_of(m[1])};
             uint32_t pa[KEYS / 16][PP][4];
 #pragma unroll
             for (int kk = 0; kk < KEYS / 16; kk++)
 #pragma unroll
                 for (int x = 0; x < 4; x++) {  // registers: (row, low keys), (row + 8, low), (row, high), (row + 8, high)
                     const int t = 2 * kk + (x >> 1), y = x & 1;
-                    float p0 = prob(s[t][2 * y], a.c2, mc[y]) * PS, p1 = prob(s[t][2 * y + 1], a.c2, mc[y]) * PS;
+                    float p0 = prob(s[t][2 * y], a.c2, base[y]) * PS, p1 = prob(s[t][2 * y + 1], a.c2, base[y]) * PS;
                     l[y] += p0 + p1;
                     split_probs<T, PP>(p0, p1, pa[kk], x);
                 }

@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32, 2) paged_attention_kernel(con
             }
 #pragma unroll
             for (int g = 0; g < GP; g++) {
-                const float p = prob(s[g][0], a.c2, scaled_max(m[g], a.c2));
+                const float p = prob(s[g][0], a.c2, base_of(m[g]));
                 l[g] += p;
                 probs[g * KEYS + sub * ITS + my_it] = p;
             }

@@ -316,6 +316,40 @@ def test_attention_where_every_score_is_minus_infinity(cuda, q_type, pool, group
 
 
 @pytest.mark.parametrize("q_type,pool,group,dim", KINDS)
+@pytest.mark.parametrize("size", [1e7, 3e8, 1e10, 1e20])
+def test_attention_of_scores_past_2_24(cuda, q_type, pool, group, dim, size):
+    """Scores whose products round by more than 1: the largest, a tied few, share the
+    probability, and the others, far behind, have none."""
+    from franken_ocr_b200 import paged
+
+    n = 50
+    c = Cache([n, n], 1, 16, dim, DTYPES[pool], seed=dim)
+    g = torch.Generator().manual_seed(group)
+    q = (1 + torch.rand((2, group, dim), generator=g)).to(DTYPES[q_type])
+    top = (1 + torch.rand((dim,), generator=g)).to(DTYPES[pool])
+    best = [3, 17, 40]
+    for r in range(2):
+        for j in range(n):
+            # a lower key has half of every product or less
+            c.k[int(c.table[r, j // 16]), 0, j % 16] = top if j in best else (top.float() * (j % 4) / 8).to(c.dtype)
+    want = c.row(0, best, "v")[0].mean(0), c.row(1, best, "v")[0].mean(0)
+    scale = size / float((q.double() @ top.double()).max())
+    for kp, vp, table, times in around_the_shares(c):
+        w = torch.zeros((2 * times, 1, 64), device="cuda")
+        out = paged.paged_attention(q.cuda().repeat(times, 1, 1), kp, vp, table, c.lens.cuda().repeat(times), scale=scale,
+                                    weights=w).view(times, 2, group, dim).cpu().double()
+        for r in range(2):
+            # three equal probabilities: a few roundings, and the output's own
+            off = (out[:, r] - want[r]).abs()
+            assert bool((off <= 2.0 ** -16 * 3 + want[r].abs() * HALF_STEP[q.dtype]).all())
+        # a third each for every query head, to a few roundings
+        got = w.view(times, 2, 64).cpu().double()
+        assert bool(((got[:, :, best] - group / 3).abs() <= group * 2.0 ** -20).all())
+        got[:, :, best] = 0
+        assert bool((got == 0).all())
+
+
+@pytest.mark.parametrize("q_type,pool,group,dim", KINDS)
 def test_attention_of_infinite_keys(cuda, q_type, pool, group, dim):
     """A score of -inf has probability 0, whatever the kernel; one of +inf, or of both, has
     none: NaN. Queries with an infinity of their own likewise."""
