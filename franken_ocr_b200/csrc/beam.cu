@@ -124,9 +124,10 @@ __device__ __forceinline__ void add_exp4(float2 xa, float2 xb, float base, const
 //
 // The sum: every term to 2^-27 of itself (add_exp4), summed in 64 bits, so that equal
 // logits, whose errors all fall to one side, leave less than 2^-27 of it too (3e-9
-// measured; terms of 24 bits, summed in fours as f32, 1.1e-7 and 4.5 us less for 32 x 8
-// rows of 129280 logits).  The 64-bit exponential of every logit would cost several times
-// the strip's load.
+// measured; terms of 24 bits, summed in fours as f32, 1.1e-7 and 7 us less for 32 x 8
+// rows of 129280 logits).  The largest logits count 1 each, exactly: rows that leave one
+// token, or equal ones, tie where their beams do.  The 64-bit exponential of every logit
+// would cost several times the strip's load.
 //
 // The n largest: at least n logits reach the n-th largest of the maxima of 2n or
 // more groups of threads, and hardly more do; these are collected and ranked by
@@ -134,8 +135,8 @@ __device__ __forceinline__ void add_exp4(float2 xa, float2 xb, float base, const
 // Where too many reach it (a constant row), the n are taken one by one.
 //
 // Bound by instructions, half of them the exponentials, and by the three barriers of a
-// short block: 32 x 8 rows of 129280 f32 logits, 132 MB, take 54 us with the join behind
-// them, 2.5 TB/s.
+// short block: 32 x 8 rows of 129280 f32 logits, 132 MB, take 56 us with the join behind
+// them, 2.4 TB/s.
 template <typename T, int PER>
 __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) {
     constexpr int V = 16 / (int)sizeof(T), STRIP = ST * PER;
@@ -144,6 +145,7 @@ __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) 
     __shared__ int lt[LIST], count;
     __shared__ float bound;
     __shared__ double shd[ST / 32];
+    __shared__ int shc[ST / 32];
     __shared__ __align__(8) uint2 power[16];
     const int strip = blockIdx.x, row = blockIdx.y, t = threadIdx.x;
     if (t < 16) power[t] = make_uint2((uint32_t)POWER[t], (uint32_t)(POWER[t] >> 32) - ((uint32_t)t << 16));
@@ -212,11 +214,18 @@ __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) 
     const float base = rintf(__fmul_rn(high, 1.44269502f)), none = high - 65.0f;   // e^-65 of the largest adds nothing
     const float2 minus = both(-zero);
     double sum = 0.0;
+    int ones = 0;
 #pragma unroll
     for (int g = 0; g < PER / 4; g++) {
         float2 y0 = add2(make_float2(v[4 * g], v[4 * g + 1]), minus), y1 = add2(make_float2(v[4 * g + 2], v[4 * g + 3]), minus);
         y0 = make_float2(fmaxf(y0.x, none), fmaxf(y0.y, none));   // NaN too
         y1 = make_float2(fmaxf(y1.x, none), fmaxf(y1.y, none));
+        if (most[g] == m) {   // rarely
+            if (v[4 * g] == m) ones++, y0.x = none;
+            if (v[4 * g + 1] == m) ones++, y0.y = none;
+            if (v[4 * g + 2] == m) ones++, y1.x = none;
+            if (v[4 * g + 3] == m) ones++, y1.y = none;
+        }
         add_exp4(y0, y1, base, power, &sum);
     }
     __syncthreads();
@@ -242,7 +251,11 @@ __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) 
                         }
     }
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if ((t & 31) == 0) shd[t >> 5] = sum;
+    ones = __reduce_add_sync(0xffffffffu, ones);
+    if ((t & 31) == 0) {
+        shd[t >> 5] = sum;
+        shc[t >> 5] = ones;
+    }
     __syncthreads();
     const int got = count;
     const bool listed = got <= LIST;
@@ -262,10 +275,13 @@ __global__ void __launch_bounds__(ST, 4) select_part_kernel(const SelectArgs a) 
         return;
     }
     if (t == 0) {
-        for (int w = 1; w < ST / 32; w++) sum += shd[w];
+        for (int w = 1; w < ST / 32; w++) {
+            sum += shd[w];
+            ones += shc[w];
+        }
         a.pm[at] = m;
-        // the terms were taken relative to 2^base
-        a.ps[at] = sum * exp((double)base * 0.693147180559945309 - (double)high);
+        // the other terms were taken relative to 2^base
+        a.ps[at] = ones + sum * exp((double)base * 0.693147180559945309 - (double)high);
     }
     if (listed) return;
     float last = INFINITY;
@@ -531,9 +547,9 @@ __global__ void __launch_bounds__(ST) select_join_kernel(const SelectArgs a) {
 }
 
 // Logits of a strip.  Where long ones would keep fewer than half the SMs busy: short
-// ones (over 129280 tokens of f32 one beam 6.6 us, long 7.9; 1 x 4 beams 7.2 and 8.3,
-// bf16 7.8 and 9.1).  Otherwise long ones, whose candidates are fewer to join (1 x 8
-// beams 8.8 us, short 9.5; 32 x 8 54 and 72).
+// ones (over 129280 tokens of f32 one beam 6.6 us, long 8.0; 1 x 4 beams 7.3 and 8.5,
+// bf16 7.4 and 8.9).  Otherwise long ones, whose candidates are fewer to join (1 x 8
+// beams 8.9 us, short 9.6; 32 x 8 56 and 74).
 int strip_of(size_t rows, size_t vocab) {
     return rows * ((vocab + ST * 32 - 1) / (ST * 32)) < (size_t)num_sms() / 2 ? ST * 16 : ST * 32;
 }

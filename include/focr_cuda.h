@@ -603,8 +603,9 @@ int focr_paged_evict(const focr_paged_cache *c, const focr_paged_evict_args *a, 
  * elements apart) and the beams' cumulated log probabilities scores
  * [batch][beams], the n best continuations of every entry, ranked by
  *   scores[b][i] + log softmax(logits[b][i])[t]
- * in 64 bits, of which a beam's log-sum is good to 2^-27 (two beams of the same
- * logits have the same one); equal scores go to the lower beam, then the larger logit, then
+ * in 64 bits, of which a beam's log-sum is good to 2^-27 (exact where all of its
+ * candidates are equal, and the same for two beams of the same logits); equal
+ * scores go to the lower beam, then the larger logit, then
  * the lower token.  scores_out (rounded to f32), parent_out (the beam) and
  * token_out are [batch][n].  NaN and -inf logits are no candidates and add
  * nothing to a sum; +inf counts as the largest finite f32.  A beam with

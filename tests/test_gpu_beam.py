@@ -138,6 +138,24 @@ def test_select_beams_far_ahead_of_the_others(cuda, dtype, kind):
     check_select(x, cum.contiguous(), n)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [1, 7, 5000, 20001])
+def test_select_ties_of_beams_whose_sums_are_whole_numbers(cuda, dtype, vocab):
+    """Beams that leave one token, or equal ones, wherever those logits lie: their scores
+    are equal, and equal ones go to the lower beam."""
+    beams = 16
+    g = torch.Generator().manual_seed(vocab)
+    at = (torch.randn((beams, 1), generator=g) * 20).to(DTYPES[dtype])
+    x = torch.full((4, beams, vocab), -math.inf, dtype=DTYPES[dtype])
+    x[0] = at                                           # all equal
+    x[1, :, vocab // 2] = at[:, 0]                      # one token
+    x[2, :, ::3] = at                                   # a third of them
+    x[3] = torch.finfo(DTYPES[dtype]).min               # masked by the lowest value
+    x[3, :, vocab // 2] = at[:, 0]
+    for n in (1, 5, 40):
+        check_select(x, torch.full((4, beams), -3.0), n)
+
+
 def flat_beam(value, vocab):
     """A logit 0 every thousand, all others `value`: their exponentials are all rounded
     alike, and lie below the largest wherever a strip begins."""
