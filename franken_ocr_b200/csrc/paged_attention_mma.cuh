@@ -11,9 +11,9 @@
 // are multiplied one after the other, so nothing is rounded to fewer bits than the
 // output has.
 //
-// Measured: 8 rows x 131072 positions, 64 / 8 heads of 128, bf16: 650 to 690 us (where
-// the pages lie makes the difference), 6.2 to 6.6 TB/s; 16 x 8192 x 8 heads: 93 us at 3
-// query heads each, 97 at 8, 99 at 16 (5.4 TB/s).
+// Measured: 8 rows x 131072 positions, 64 / 8 heads of 128, bf16: 645 to 665 us, call
+// after call under the power cap 625 to 685 by the GPU, 6.3 to 6.9 TB/s; 16 x 8192 x 8
+// heads: 93 us at 3 query heads each, 97 at 8, 99 at 16 (5.4 TB/s).
 #pragma once
 
 #include "paged_attention.cuh"
